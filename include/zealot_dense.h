@@ -43,6 +43,39 @@ int zk_add(const void *a, const void *b, void *out, int64_t n, zk_dtype dtype, v
 int zk_embedding(const int64_t *ids, const void *table, void *out, int64_t num_tokens, int64_t vocab,
                  int64_t dim, zk_dtype dtype, void *stream);
 
+/* Norms of the query and key heads and the rotary position embedding in one
+ * pass.  No reference counterpart (its runner applies neither between the
+ * projections and the KV write, cuda_runner.rs:331-461).  Every head row x of
+ * q [num_tokens, num_heads, head_dim] and k [num_tokens, num_kv_heads,
+ * head_dim]:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight       (weight NULL: y = x)
+ *   (y_a, y_b) -> (y_a c_i - y_b s_i, y_b c_i + y_a s_i),  i < rot_dim / 2,
+ * (a, b) = (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved; dimensions
+ * from rot_dim on keep y.  Row p of rope (f32 [max_positions, rot_dim]) holds
+ * the rot_dim / 2 cosines of position p, then its sines; rot_dim 0: no rotation
+ * (rope and positions may be NULL).  A token whose position lies outside [0,
+ * max_positions) gets zero rows.  Arithmetic in f32, one rounding.  Token rows
+ * are *_stride elements apart (0 = packed), so columns of a fused projection
+ * are read, and with q_out == q (k_out == k) and equal strides written, in
+ * place; any other overlap of an output is refused.  head_dim <= 1024,
+ * num_tokens < 2^24. */
+int zk_qk_norm_rope(const void *q, int64_t q_stride, const void *k, int64_t k_stride, zk_dtype dtype,
+                    int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim, const void *q_weight,
+                    const void *k_weight, float eps, const int32_t *positions, const float *rope,
+                    int64_t max_positions, int rot_dim, int interleaved, void *q_out, int64_t q_out_stride,
+                    void *k_out, int64_t k_out_stride, void *stream);
+/* zk_qk_norm_rope with zk_append of the resulting K rows and of v in the same
+ * launch: K is rounded once, to the pool's type (with an F32 or BF16 pool of the
+ * source's type, bit for bit the two calls).  Slots, pools, scales and token_row
+ * as for zk_append; a token without a slot still gets its q row. */
+int zk_qk_norm_rope_append(void *k_pool, void *v_pool, zk_dtype cache_dtype, const void *q, int64_t q_stride,
+                           const void *k, int64_t k_stride, const void *v, int64_t v_stride, zk_dtype dtype,
+                           int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim, const void *q_weight,
+                           const void *k_weight, float eps, const int32_t *positions, const float *rope,
+                           int64_t max_positions, int rot_dim, int interleaved, void *q_out, int64_t q_out_stride,
+                           const int64_t *slot_mapping, int block_size, int64_t num_blocks, const float *k_scales,
+                           const float *v_scales, const int32_t *token_row, void *stream);
+
 /* Projection y[m, n] = x[m, k] . w[n, k]^T (w in nn.Linear layout), the
  * product of every cublasSgemm_v2 site (attention/cublas.rs:72-114;
  * cuda_runner.rs:331-369, :483-495, :531-559, :577-589, :627-639), with

@@ -206,6 +206,79 @@ int zk_paged_decode_noalloc(const void *q, zk_dtype q_dtype, const void *k_pool,
                             float scale, zk_gqa_mapping mapping, const float *k_scales,
                             const float *v_scales, void *stream);
 
+/* ---- tables of a step from its request lengths, on the GPU.  The reference
+ * computes slots and tables on the host, token by token (kv_cache.rs:127-161,
+ * :229-256).  Sequence i holds seq_lens[i] tokens and receives new_lens[i]
+ * (device int32; negative counts as 0; 0 is allowed).  Its new tokens' blocks
+ * beyond the ceil(seq_lens[i] / block_size) it has come from new_blocks (device
+ * int32 [num_new_blocks], the blocks granted for the step, e.g. by
+ * zk_bm_allocate), taken in batch order from *cursor on (device int64; NULL: 0)
+ * and entered in block_tables [num_seqs, max_blocks_per_seq]; other entries are
+ * left as they are.  new_blocks NULL: the tables hold every block already.
+ * Outputs, num_rows token rows packed in batch order:
+ *   slot_mapping[r]  the append's slot of the token; -1 where it has no block
+ *                    (past the table, no block granted, a negative entry)
+ *   positions[r], token_row[r]  its position and its sequence's batch index
+ *   cu_seqlens[i]    first row of sequence i (int64, num_seqs + 1 entries)
+ *   kv_lens[i]       seq_lens + new_lens, at most the table's tokens
+ *   *cursor_out      the cursor behind the blocks the step takes: past
+ *                    num_new_blocks when too few were granted
+ * Rows behind the last token get -1 in all three; tokens behind row num_rows
+ * get no row and enter no block.  kv_lens and cursor_out must not be the
+ * inputs' memory. */
+int zk_step_tables(int32_t *block_tables, int num_seqs, int max_blocks_per_seq, const int32_t *seq_lens,
+                   const int32_t *new_lens, int block_size, const int32_t *new_blocks, int64_t num_new_blocks,
+                   const int64_t *cursor, int64_t *cursor_out, int64_t *slot_mapping, int32_t *positions,
+                   int32_t *token_row, int64_t num_rows, int64_t *cu_seqlens, int32_t *kv_lens, void *stream);
+
+/* ---- sparse decode attention over pages.  No reference counterpart (its
+ * decode reads every page, paged_attention.cu:65-131).
+ *
+ * Page bounds: bounds[b, h, 0, d] / [b, h, 1, d] = the smallest / largest
+ * K[.., d] over the tokens written to page (b, h) (pool type, [num_blocks, Hkv,
+ * 2, head_dim]; the values themselves, without an fp8 pool's scales).  This
+ * call brings the bounds up to date behind a write of K at slot_mapping (the
+ * write's own; negative slots are skipped): a page written from its first token
+ * on starts afresh, another one extends its bounds.  The rows of one page must
+ * be consecutive with consecutive slots, as the step tables give them (a page
+ * in two runs of one call gets the bounds of either, in no fixed order).  NaN
+ * keys make NaN bounds.  A copied block needs its bounds copied
+ * (zk_copy_blocks on the bounds as a pool). */
+int zk_page_bounds(const void *k_pool, zk_dtype kv_dtype, const int64_t *slot_mapping, int64_t num_tokens,
+                   int num_kv_heads, int head_dim, int block_size, int64_t num_blocks, void *bounds, void *stream);
+/* scores[n, h, p] (f32 [num_seqs, Hkv, max_blocks_per_seq]) = the maximum over
+ * the query heads g of kv-head h of sum_d min(q_d, 0) lo_d + max(q_d, 0) hi_d:
+ * no key of page p has a larger q . k (times the fp8 key scale, positive and the
+ * same for all pages of (n, h)).  -inf for pages behind the length and table
+ * entries outside the pool.  q [num_seqs, num_heads, head_dim], F32 or BF16.  A
+ * NaN score (NaN or infinite keys) ranks first in zk_select_pages. */
+int zk_page_scores(const void *q, zk_dtype q_dtype, const void *bounds, zk_dtype kv_dtype, const int32_t *block_tables,
+                   const int32_t *seq_lens, float *scores, int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                   int block_size, int max_blocks_per_seq, int64_t num_blocks, zk_gqa_mapping mapping, void *stream);
+/* pages[n, h, 0..num_pages) = the num_pages pages of the best scores among the
+ * ceil(seq_lens[n] / block_size) that sequence n holds, in ascending order; the
+ * first `sink` and the last `recent` of them are always among them (sink +
+ * recent <= num_pages); of equal scores the lower page.  Sequences that hold
+ * fewer pages list them all, then -1.  max_blocks_per_seq <= 65536. */
+int zk_select_pages(const float *scores, const int32_t *seq_lens, int num_seqs, int num_kv_heads,
+                    int max_blocks_per_seq, int block_size, int num_pages, int sink, int recent, int32_t *pages,
+                    void *stream);
+/* zk_paged_decode over the listed pages only: kv-head h of sequence n attends
+ * the tokens below seq_lens[n] of pages[n, h, 0..num_pages) (indices into the
+ * sequence's block table, int32, any order; a page listed twice counts twice).
+ * A negative entry, one past the table or the length and one whose block lies
+ * outside the pool add nothing; a row without tokens is zero.  Operands as in
+ * zk_paged_decode; head_dim <= 256, H / Hkv <= 16, num_seqs <= 65535.  workspace:
+ * zk_paged_decode_sparse_workspace_size bytes (0: none needed), 256-B aligned. */
+size_t zk_paged_decode_sparse_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                             int num_pages);
+int zk_paged_decode_sparse(const void *q, zk_dtype q_dtype, const void *k_pool, const void *v_pool, zk_dtype kv_dtype,
+                           void *out, const int32_t *block_tables, const int32_t *seq_lens, const int32_t *pages,
+                           int num_pages, int num_seqs, int num_heads, int num_kv_heads, int head_dim, int block_size,
+                           int max_blocks_per_seq, int64_t num_blocks, float scale, zk_gqa_mapping mapping,
+                           const float *k_scales, const float *v_scales, void *workspace, size_t workspace_bytes,
+                           void *stream);
+
 /* ======================================================= KVCache (stateful)
  * src/kv_cache.rs:51-356.  Owns per-layer K/V pools (one HBM slab) and
  * per-sequence device block tables.  Sequence ids are NUL-terminated strings. */
@@ -413,7 +486,9 @@ int zk_paged_prefill(const void *q, zk_dtype q_dtype, const void *k_pool, const 
  * "append", "fp8_scales", "gather", "copy_blocks", "decode_seq_info",
  * "decode_plan", "decode_partials", "decode_reduce", "prefill_plan",
  * "prefill_attention", "stream_copy", "stream_read", "rms_norm", "silu_mul",
- * "add", "embedding", "linear", "swap_out", "swap_in". */
+ * "add", "embedding", "linear", "swap_out", "swap_in", "step_tables",
+ * "qk_norm_rope", "page_bounds", "page_scores", "select_pages",
+ * "sparse_partials", "sparse_reduce". */
 int zk_timing_enable(int on);
 int zk_timing_reset(void);
 int zk_timing_query(const char *kernel, int64_t *launches, double *total_ms);

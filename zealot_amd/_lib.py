@@ -100,6 +100,13 @@ SIGNATURES = {
     "zk_paged_prefill_workspace_size": (_SZ, [_I, _I64, _I, _I]),
     "zk_paged_prefill": (_I, [_P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _I64, _I, _I, _I, _I, _I, _I64, _F, _I,
                               _I, _P, _P, _P, _SZ, _P]),
+    "zk_step_tables": (_I, [_P, _I, _I, _P, _P, _I, _P, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P]),
+    "zk_page_bounds": (_I, [_P, _I, _P, _I64, _I, _I, _I, _I64, _P, _P]),
+    "zk_page_scores": (_I, [_P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I64, _I, _P]),
+    "zk_select_pages": (_I, [_P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
+    "zk_paged_decode_sparse_workspace_size": (_SZ, [_I, _I, _I, _I, _I]),
+    "zk_paged_decode_sparse": (_I, [_P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I64, _F, _I,
+                                    _P, _P, _P, _SZ, _P]),
     "zk_cache_create": (_I, [_SZ, _SZ, _SZ, _SZ, _SZ, _I, _SZ, _SZ, _P, ctypes.POINTER(_P)]),
     "zk_cache_destroy": (None, [_P]),
     "zk_cache_register_seq": (_I, [_P, _CP, _SZ]),
@@ -138,6 +145,10 @@ SIGNATURES = {
     "zk_silu_mul": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _I, _P]),
     "zk_add": (_I, [_P, _P, _P, _I64, _I, _P]),
     "zk_embedding": (_I, [_P, _P, _P, _I64, _I64, _I64, _I, _P]),
+    "zk_qk_norm_rope": (_I, [_P, _I64, _P, _I64, _I, _I64, _I, _I, _I, _P, _P, _F, _P, _P, _I64, _I, _I, _P, _I64,
+                             _P, _I64, _P]),
+    "zk_qk_norm_rope_append": (_I, [_P, _P, _I, _P, _I64, _P, _I64, _P, _I64, _I, _I64, _I, _I, _I, _P, _P, _F, _P,
+                                    _P, _I64, _I, _I, _P, _I64, _P, _I, _I64, _P, _P, _P, _P]),
     "zk_linear": (_I, [_P, _P, _P, _I64, _I64, _I64, _I, _I, _P]),
     "zk_linear_rms_norm": (_I, [_P, _P, _I64, _I64, _I64, _P, _P, _F, _P, _P, _P]),
     "zk_linear_choice": (_I, [_I64, _I64, _I64, _I, _I, _P]),

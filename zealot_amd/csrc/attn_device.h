@@ -1,0 +1,40 @@
+// attn_device.h -- device helpers the decode attention kernels share.
+#pragma once
+
+#include <cmath>
+
+#include "zk_common.h"
+
+namespace zk {
+
+// Lane l ^ 16 / l ^ 32's value, on the VALU: v_permlane16_swap exchanges the
+// odd 16-lane rows of its first operand with the even rows of its second, and
+// v_permlane32_swap the upper half of the first with the lower half of the
+// second; with both operands v, a lane's partner value lands in the second
+// result on the even rows (lower half) and in the first elsewhere.  (Unlike
+// ds_swizzle / ds_bpermute they are not LDS instructions, so they never wait
+// behind outstanding LDS or scalar loads.)
+__device__ __forceinline__ float xor16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 16) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float xor32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Two f32 -> packed bf16, round to nearest even (v_cvt_pk_bf16_f32).
+__device__ __forceinline__ uint32_t bf16x2_rne(float lo, float hi) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2_t));
+}
+
+// scale / l for a row of maximum m: 0 where it saw no keys (m = -inf), NaN where
+// all their scores were -inf (l = 0 at the lowest finite m).
+__device__ __forceinline__ float inverse_sum(float l, float m, float scale = 1.0f) {
+    return l > 0.0f ? scale / l : m == -INFINITY ? 0.0f : NAN;
+}
+
+}  // namespace zk

@@ -1,0 +1,535 @@
+// sparse_ops.hip -- the selection side of sparse decode attention over pages:
+// bounds of each page's keys, an upper bound of a page's logits from them, and
+// the best pages of each (sequence, kv-head).  paged_sparse.hip attends them.
+// No reference counterpart (its decode reads every page,
+// src/attention/kernels/paged_attention.cu:65-131).
+//
+// bounds[b][h][0][d] = min, [1][d] = max over the page's tokens of K[.., d], in
+// the pool's type (exact: a bound is one of the keys' values).
+// For any key k of page p and query q:
+//   q . k = sum_d q_d k_d <= sum_d max(q_d lo_d, q_d hi_d)
+//         = sum_d min(q_d, 0) lo_d + max(q_d, 0) hi_d,
+// the last form a product of 2 D terms, which runs on the matrix cores.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "zk_common.h"
+
+using namespace zk;
+
+namespace {
+
+constexpr int kThreads = 256;
+
+int check_launch(const char *what) {
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+        return set_error(ZK_ERR_HIP, std::string("Internal error: ") + what + ": " + hipGetErrorString(e));
+    return ZK_OK;
+}
+
+// ------------------------------------------------------------ page bounds
+// One 16-byte piece of a row as f32 values (VEC), or one element.
+template <int KV, bool VEC> struct Piece;
+template <bool VEC> struct Piece<ZK_F32, VEC> {
+    static constexpr int N = VEC ? 4 : 1;
+    static __device__ __forceinline__ void load(const char *p, float *x) {
+        if constexpr (VEC) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = v[e];
+        } else {
+            x[0] = *(const float *)p;
+        }
+    }
+    static __device__ __forceinline__ void store(char *p, const float *x) {
+        if constexpr (VEC) *reinterpret_cast<f32x4 *>(p) = f32x4{x[0], x[1], x[2], x[3]};
+        else *(float *)p = x[0];
+    }
+};
+template <bool VEC> struct Piece<ZK_BF16, VEC> {
+    static constexpr int N = VEC ? 8 : 1;
+    static __device__ __forceinline__ void load(const char *p, float *x) {
+        if constexpr (VEC) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] = bf16lo(v[i]);
+                x[2 * i + 1] = bf16hi(v[i]);
+            }
+        } else {
+            x[0] = __uint_as_float((uint32_t) * (const uint16_t *)p << 16);
+        }
+    }
+    static __device__ __forceinline__ void store(char *p, const float *x) {  // (bf16 values: the high halves)
+        if constexpr (VEC) {
+            u32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]), 0x07060302u);
+            *reinterpret_cast<u32x4 *>(p) = v;
+        } else {
+            *(uint16_t *)p = (uint16_t)(__float_as_uint(x[0]) >> 16);
+        }
+    }
+};
+template <bool VEC> struct Piece<ZK_FP8_E4M3, VEC> {
+    static constexpr int N = VEC ? 16 : 1;
+    static __device__ __forceinline__ void load(const char *p, float *x) {
+        if constexpr (VEC) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e4m3x4_to_f32(v[i], x + 4 * i);
+        } else {
+            float t[4];
+            e4m3x4_to_f32(*(const uint8_t *)p, t);
+            x[0] = t[0];
+        }
+    }
+    static __device__ __forceinline__ void store(char *p, const float *x) {
+        if constexpr (VEC) {
+            u32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = e4m3x4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            *reinterpret_cast<u32x4 *>(p) = v;
+        } else {
+            *(uint8_t *)p = (uint8_t)e4m3x4(x[0], 0.f, 0.f, 0.f);
+        }
+    }
+};
+
+// NaN once seen stays: a page with such a key has NaN bounds.
+__device__ __forceinline__ float min_nan(float a, float b) { return b < a || b != b ? b : a; }
+__device__ __forceinline__ float max_nan(float a, float b) { return b > a || b != b ? b : a; }
+
+// A workgroup looks at `rows` rows of the slot map.  The row that is the first
+// of its page's run (consecutive rows with consecutive slots of one block)
+// folds the run's keys, and the page's bounds from before unless the run
+// begins the page.  Threads hold the pieces of a token's heads.  Bound by HBM
+// for prompts, by latency for a decode step's single tokens.
+template <int KV, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+page_bounds_kernel(const char *__restrict__ k_pool, const int64_t *__restrict__ slots, int64_t num_tokens, int rows,
+                   int hkv, int head_dim, int block_size, int64_t num_slots, char *__restrict__ bounds) {
+    typedef Piece<KV, VEC> P;
+    constexpr int N = P::N, ES = KV == ZK_F32 ? 4 : KV == ZK_BF16 ? 2 : 1;
+    const int lane = threadIdx.x & 63;
+    const int ppr = head_dim / N, pieces = hkv * ppr;
+    const int64_t t0 = (int64_t)blockIdx.x * rows, t1 = min(t0 + rows, num_tokens);
+    for (int64_t t = t0; t < t1; ++t) {
+        const int64_t slot = slots[t];
+        if (slot < 0 || slot >= num_slots) continue;
+        const int64_t blk = slot / block_size;
+        const int first = (int)(slot - blk * block_size);
+        if (first && t > 0 && slots[t - 1] == slot - 1) continue;  // inside a run
+        int run = 1;
+        while (run < block_size - first) {  // how far the run goes, 64 rows at a time
+            const int j = run + lane;
+            const bool on = j < block_size - first && t + j < num_tokens && slots[t + j] == slot + j;
+            const uint64_t off = ~__builtin_amdgcn_ballot_w64(on);
+            run += off ? (int)__builtin_ctzll(off) : 64;
+            if (off) break;
+        }
+        for (int i = threadIdx.x; i < pieces; i += kThreads) {
+            const int h = i / ppr, c = i - h * ppr;
+            const size_t row_bytes = (size_t)head_dim * ES;
+            const char *src = k_pool + (((size_t)blk * hkv + h) * block_size + first) * row_bytes + (size_t)c * N * ES;
+            char *dst = bounds + ((size_t)blk * hkv + h) * 2 * row_bytes + (size_t)c * N * ES;
+            float lo[N], hi[N];
+            int j = 0;
+            if (first) {
+                P::load(dst, lo);
+                P::load(dst + row_bytes, hi);
+            } else {
+                P::load(src, lo);
+#pragma unroll
+                for (int e = 0; e < N; ++e) hi[e] = lo[e];
+                j = 1;
+            }
+#pragma unroll 4
+            for (; j < run; ++j) {
+                float x[N];
+                P::load(src + (size_t)j * row_bytes, x);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    lo[e] = min_nan(lo[e], x[e]);
+                    hi[e] = max_nan(hi[e], x[e]);
+                }
+            }
+            P::store(dst, lo);
+            P::store(dst + row_bytes, hi);
+        }
+    }
+}
+
+// ------------------------------------------------------------ page scores
+struct ScoreArgs {
+    const void *q;
+    const char *bounds;
+    const int32_t *tables, *seq_lens;
+    float *scores;  // [N][Hkv][max_blocks]
+    int64_t num_blocks;
+    int num_heads, num_kv_heads, head_dim, block_size, max_blocks, grouped, q_f32;
+    int tiles;  // of 16 pages a wave
+};
+
+__device__ __forceinline__ int held_pages(const ScoreArgs &a, int n) {
+    const int64_t len = max(a.seq_lens[n], 0);
+    return (int)min((len + a.block_size - 1) / a.block_size, (int64_t)a.max_blocks);
+}
+__device__ __forceinline__ int qhead(const ScoreArgs &a, int kvh, int j, int G) {
+    return a.grouped ? kvh * G + j : kvh + j * a.num_kv_heads;
+}
+
+// bf16 queries, bf16 or fp8 bounds: A = 16 pages' [lo | hi] rows, B = the
+// query heads' [min(q, 0) | max(q, 0)], on v_mfma_f32_16x16x32_bf16 (both
+// exact in bf16, the sums in f32).  Lane (grp, col) loads dims 8 grp .. + 7 of
+// a 32-dim step of page col, so a page's four lanes read 64 contiguous bytes;
+// columns past the G heads repeat them, which leaves the maximum over the
+// heads as it is.  Bound by HBM: 2 D values a page and kv-head are read once.
+template <int KV, int D, int G>
+__global__ void __launch_bounds__(kThreads) page_scores_mfma_kernel(ScoreArgs a) {
+    constexpr int KK = 2 * D / 32, ES = KV == ZK_BF16 ? 2 : 1;
+    typedef typename std::conditional<KV == ZK_BF16, u32x4, u32x2>::type piece_t;
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, wave = threadIdx.x >> 6;
+    const int kvh = blockIdx.y, n = blockIdx.z;
+    const int held = held_pages(a, n);
+    const int32_t *row = a.tables + (size_t)n * a.max_blocks;
+    float *out = a.scores + ((size_t)n * a.num_kv_heads + kvh) * a.max_blocks;
+    const int per = 16 * a.tiles * (kThreads / 64);  // pages of a workgroup
+    const int p0 = blockIdx.x * per + wave * 16, step = 16 * (kThreads / 64), p1 = min((int)(blockIdx.x + 1) * per, a.max_blocks);
+    if (p0 >= p1) return;
+    bf16x8 qf[KK];
+    if (p0 < held) {
+        const uint16_t *q = (const uint16_t *)a.q + ((size_t)n * a.num_heads + qhead(a, kvh, col % G, G)) * D;
+#pragma unroll
+        for (int kk = 0; kk < KK / 2; ++kk) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(q + kk * 32 + grp * 8);
+            u32x4 neg, pos;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // by sign bit (a NaN's value goes into the half of its sign)
+                const uint32_t m = ((w[i] >> 15) & 0x10001u) * 0xffffu;  // 0xffff in negative halves
+                neg[i] = w[i] & m;
+                pos[i] = w[i] & ~m;
+            }
+            qf[kk] = __builtin_bit_cast(bf16x8, neg);
+            qf[kk + KK / 2] = __builtin_bit_cast(bf16x8, pos);
+        }
+    }
+    const size_t page_bytes = (size_t)2 * D * ES, block_bytes = page_bytes * a.num_kv_heads;
+    for (int p = p0; p < p1; p += step) {
+        const int page = p + col;
+        if (p >= held) {  // behind the context
+            if (grp == 0 && page < p1) out[page] = -INFINITY;
+            continue;
+        }
+        const int blk = page < held ? row[page] : 0;
+        const bool ok = blk >= 0 && blk < a.num_blocks;
+        const char *src = a.bounds + (size_t)(ok ? blk : 0) * block_bytes + (size_t)kvh * page_bytes + grp * 8 * ES;
+        piece_t w[KK];
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) w[kk] = *reinterpret_cast<const piece_t *>(src + kk * 32 * ES);
+        f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            bf16x8 f;
+            if constexpr (KV == ZK_BF16) {
+                f = __builtin_bit_cast(bf16x8, w[kk]);
+            } else {
+                const u32x2 lo = e4m3x4_to_bf16x4(w[kk][0]), hi = e4m3x4_to_bf16x4(w[kk][1]);
+                f = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+            }
+            acc[kk & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[kk], acc[kk & 1], 0, 0, 0);
+        }
+        f32x4 s = acc[0] + acc[1];  // head col's scores of pages p + 4 grp + i
+#pragma unroll
+        for (int o = 1; o < G; o <<= 1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = max_nan(s[i], __shfl_xor(s[i], o));
+        // lane col < 4 of each group writes page 4 grp + col
+        float v = s[0];
+        v = col == 1 ? s[1] : v;
+        v = col == 2 ? s[2] : v;
+        v = col == 3 ? s[3] : v;
+        const int dst = p + 4 * grp + col;
+        const int ok_dst = __shfl((int)(ok && page < held), 4 * grp + (col & 3));  // (lane c < 16 holds page p + c)
+        if (col < 4 && dst < p1) out[dst] = ok_dst ? v : -INFINITY;
+    }
+}
+
+// Any shape and type: one wave per (page, kv-head, sequence), lanes over the
+// dimensions.
+template <int KV>
+__global__ void __launch_bounds__(kThreads) page_scores_generic_kernel(ScoreArgs a) {
+    typedef Piece<KV, false> P;
+    constexpr int ES = KV == ZK_F32 ? 4 : KV == ZK_BF16 ? 2 : 1;
+    const int lane = threadIdx.x & 63;
+    const int page = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), kvh = blockIdx.y, n = blockIdx.z;
+    if (page >= a.max_blocks) return;
+    const int D = a.head_dim, G = a.num_heads / a.num_kv_heads;
+    float best = -INFINITY;
+    const int blk = page < held_pages(a, n) ? a.tables[(size_t)n * a.max_blocks + page] : -1;
+    if (blk >= 0 && blk < a.num_blocks) {
+        const char *lo = a.bounds + ((size_t)blk * a.num_kv_heads + kvh) * 2 * D * ES, *hi = lo + (size_t)D * ES;
+        for (int j = 0; j < G; ++j) {
+            const size_t qo = ((size_t)n * a.num_heads + qhead(a, kvh, j, G)) * D;
+            float s = 0.0f;
+            for (int d = lane; d < D; d += 64) {
+                const float q = a.q_f32 ? ((const float *)a.q)[qo + d]
+                                        : __uint_as_float((uint32_t)((const uint16_t *)a.q)[qo + d] << 16);
+                float l, u;
+                P::load(lo + (size_t)d * ES, &l);
+                P::load(hi + (size_t)d * ES, &u);
+                const bool neg = __float_as_uint(q) >> 31;
+                s = fmaf(neg ? q : 0.0f, l, s);
+                s = fmaf(neg ? 0.0f : q, u, s);
+            }
+            for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+            best = j == 0 ? s : max_nan(best, s);
+        }
+    }
+    if (lane == 0) a.scores[((size_t)n * a.num_kv_heads + kvh) * a.max_blocks + page] = best;
+}
+
+// ------------------------------------------------------------ selection
+// Order of the scores as unsigned numbers: greater score, greater key; -0 as
+// +0, every NaN above +inf, pages taken in any case above those.
+__device__ __forceinline__ uint32_t score_key(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    if (x != x) return 0xfffffffeu;
+    return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// One workgroup of W waves per (sequence, kv-head); a lane keeps the keys of R
+// pages: page (w R + r) 64 + lane.  The k-th largest key is found bit by bit
+// from the top (32 rounds of count(keys >= candidate), a ballot per register,
+// ending early when a candidate has exactly k), then pages above it and, in
+// page order, as many equal to it as are wanted are written at their rank.
+// No sort and no atomics: the list is in ascending order and the same every
+// time.  Bound by the rounds' instructions and, with W > 1, their barriers.
+template <int W, int R>
+__global__ void __launch_bounds__(64 * W)
+select_pages_kernel(const float *__restrict__ scores, const int32_t *__restrict__ seq_lens, int width, int block_size,
+                    int k, int sink, int recent, int32_t *__restrict__ pages) {
+    __shared__ int part[2][2][W];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int hkv = gridDim.x, n = blockIdx.y;
+    const size_t rowi = (size_t)n * hkv + blockIdx.x;
+    const int64_t len = max(seq_lens[n], 0);
+    const int held = (int)min((len + block_size - 1) / block_size, (int64_t)width);
+    int32_t *out = pages + rowi * (size_t)k;
+    if (held <= k) {  // all of them
+        for (int i = threadIdx.x; i < k; i += 64 * W) out[i] = i < held ? i : -1;
+        return;
+    }
+    const float *row = scores + rowi * (size_t)width;
+    uint32_t key[R];  // first the scores' bits: all loads before any use
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int p = (w * R + r) * 64 + lane;
+        key[r] = __float_as_uint(row[min(p, held - 1)]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int p = (w * R + r) * 64 + lane;
+        key[r] = p >= held ? 0u : p < sink || p >= held - recent ? 0xffffffffu : score_key(__uint_as_float(key[r]));
+    }
+    int flip = 0;
+    auto over_waves = [&](int a, int b, int &before_a, int &before_b, int &sum_a, int &sum_b) {
+        if constexpr (W == 1) {
+            before_a = before_b = 0;
+            sum_a = a;
+            sum_b = b;
+        } else {
+            if (lane == 0) {
+                part[flip][0][w] = a;
+                part[flip][1][w] = b;
+            }
+            __syncthreads();
+            before_a = before_b = sum_a = sum_b = 0;
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const int pa = part[flip][0][j], pb = part[flip][1][j];
+                before_a += j < w ? pa : 0;
+                before_b += j < w ? pb : 0;
+                sum_a += pa;
+                sum_b += pb;
+            }
+            flip ^= 1;  // (the other copy next time: one barrier a round)
+        }
+    };
+    uint32_t t = 0;  // the greatest value with at least k keys not below it
+    bool exact = false;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0 && !exact; --bit) {
+        const uint32_t cand = t | (1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] >= cand));
+        int b0, b1, all, none;
+        over_waves(c, 0, b0, b1, all, none);
+        if (all >= k) {
+            t = cand;
+            exact = all == k;
+        }
+    }
+    // counts of this wave's keys above t and equal to it (exact: every key >= t
+    // is taken, and there are k of them)
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] > t));
+        equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] == t));
+    }
+    int above_at, equal_at, all_above, all_equal;
+    over_waves(above, equal, above_at, equal_at, all_above, all_equal);
+    const int want = k - all_above;  // of the equal ones, the first
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const uint64_t gt = __builtin_amdgcn_ballot_w64(key[r] > t), eq = __builtin_amdgcn_ballot_w64(key[r] == t);
+        const int ga = above_at + __builtin_popcountll(gt & below), ea = equal_at + __builtin_popcountll(eq & below);
+        const bool take = key[r] > t || (key[r] == t && ea < want);
+        if (take) out[ga + min(ea, want)] = (w * R + r) * 64 + lane;
+        above_at += __builtin_popcountll(gt);
+        equal_at += __builtin_popcountll(eq);
+    }
+}
+
+constexpr int kSelectMost = 16 * 64 * 64;  // pages of the widest variant
+
+template <int KV, int D>
+void launch_scores_g(const ScoreArgs &a, dim3 grid, int G, hipStream_t s) {
+    switch (G) {
+        case 1: page_scores_mfma_kernel<KV, D, 1><<<grid, kThreads, 0, s>>>(a); break;
+        case 2: page_scores_mfma_kernel<KV, D, 2><<<grid, kThreads, 0, s>>>(a); break;
+        case 4: page_scores_mfma_kernel<KV, D, 4><<<grid, kThreads, 0, s>>>(a); break;
+        case 8: page_scores_mfma_kernel<KV, D, 8><<<grid, kThreads, 0, s>>>(a); break;
+        default: page_scores_mfma_kernel<KV, D, 16><<<grid, kThreads, 0, s>>>(a); break;
+    }
+}
+template <int KV>
+void launch_scores(const ScoreArgs &a, dim3 grid, int G, hipStream_t s) {
+    if (a.head_dim == 128) launch_scores_g<KV, 128>(a, grid, G, s);
+    else launch_scores_g<KV, 64>(a, grid, G, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int zk_page_bounds(const void *k_pool, zk_dtype kv_dtype, const int64_t *slot_mapping, int64_t num_tokens,
+                   int num_kv_heads, int head_dim, int block_size, int64_t num_blocks, void *bounds, void *stream) {
+    if (!valid_dtype(kv_dtype))
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_bounds: unsupported dtype");
+    if (num_tokens < 0 || num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0 || num_blocks <= 0 ||
+        (int64_t)num_kv_heads * head_dim > 0x7fffffff)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_bounds: bad shape");
+    if (num_tokens == 0) return ZK_OK;
+    if (!k_pool || !slot_mapping || !bounds)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_bounds: NULL pointer");
+    const bool vec = ((size_t)head_dim * elt_size(kv_dtype)) % 16 == 0 && (((uintptr_t)k_pool | (uintptr_t)bounds) & 15u) == 0;
+    // a row a workgroup while that fills the chip no more than a few times, then a block's worth
+    int64_t rows = num_tokens <= 4096 ? 1 : 16;
+    const int64_t grid_most = 1 << 24;
+    rows = std::max(rows, (num_tokens + grid_most - 1) / grid_most);
+    if (rows > 0x7fffffff)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_bounds: too many tokens for one launch");
+    const unsigned grid = (unsigned)((num_tokens + rows - 1) / rows);
+    hipStream_t s = (hipStream_t)stream;
+    KernelTimer timer("page_bounds", s);
+    auto go = [&](auto kernel) {
+        kernel<<<grid, kThreads, 0, s>>>((const char *)k_pool, slot_mapping, num_tokens, (int)rows, num_kv_heads, head_dim,
+                                         block_size, num_blocks * block_size, (char *)bounds);
+    };
+    if (kv_dtype == ZK_F32) vec ? go(page_bounds_kernel<ZK_F32, true>) : go(page_bounds_kernel<ZK_F32, false>);
+    else if (kv_dtype == ZK_BF16) vec ? go(page_bounds_kernel<ZK_BF16, true>) : go(page_bounds_kernel<ZK_BF16, false>);
+    else vec ? go(page_bounds_kernel<ZK_FP8_E4M3, true>) : go(page_bounds_kernel<ZK_FP8_E4M3, false>);
+    return check_launch("zk_page_bounds");
+}
+
+int zk_page_scores(const void *q, zk_dtype q_dtype, const void *bounds, zk_dtype kv_dtype, const int32_t *block_tables,
+                   const int32_t *seq_lens, float *scores, int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                   int block_size, int max_blocks_per_seq, int64_t num_blocks, zk_gqa_mapping mapping, void *stream) {
+    if ((q_dtype != ZK_F32 && q_dtype != ZK_BF16) || !valid_dtype(kv_dtype))
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_scores: unsupported dtype");
+    if (num_seqs < 0 || num_seqs > 65535 || num_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || head_dim <= 0 ||
+        block_size <= 0 || max_blocks_per_seq <= 0 || num_blocks <= 0 || num_heads % num_kv_heads != 0)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_scores: bad shape");
+    if (mapping != ZK_GQA_GROUPED && mapping != ZK_GQA_MODULO)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_scores: bad gqa mapping");
+    if (num_seqs == 0) return ZK_OK;
+    if (!q || !bounds || !block_tables || !seq_lens || !scores)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_scores: NULL pointer");
+    ScoreArgs a{};
+    a.q = q;
+    a.bounds = (const char *)bounds;
+    a.tables = block_tables;
+    a.seq_lens = seq_lens;
+    a.scores = scores;
+    a.num_blocks = num_blocks;
+    a.num_heads = num_heads;
+    a.num_kv_heads = num_kv_heads;
+    a.head_dim = head_dim;
+    a.block_size = block_size;
+    a.max_blocks = max_blocks_per_seq;
+    a.grouped = mapping == ZK_GQA_GROUPED;
+    a.q_f32 = q_dtype == ZK_F32;
+    const int G = num_heads / num_kv_heads;
+    hipStream_t s = (hipStream_t)stream;
+    KernelTimer timer("page_scores", s);
+    const bool mfma = q_dtype == ZK_BF16 && kv_dtype != ZK_F32 && (head_dim == 64 || head_dim == 128) &&
+                      (G == 1 || G == 2 || G == 4 || G == 8 || G == 16) && (((uintptr_t)q | (uintptr_t)bounds) & 15u) == 0;
+    if (mfma) {
+        // 8 tiles a wave (a workgroup then takes 512 pages) unless that leaves
+        // fewer than 1024 workgroups
+        a.tiles = 8;
+        auto groups = [&](int tiles) {
+            return (int64_t)num_seqs * num_kv_heads * ((max_blocks_per_seq + 64 * tiles - 1) / (64 * tiles));
+        };
+        while (a.tiles > 1 && groups(a.tiles) < 1024) a.tiles /= 2;
+        const dim3 grid((max_blocks_per_seq + 64 * a.tiles - 1) / (64 * a.tiles), num_kv_heads, num_seqs);
+        if (kv_dtype == ZK_BF16) launch_scores<ZK_BF16>(a, grid, G, s);
+        else launch_scores<ZK_FP8_E4M3>(a, grid, G, s);
+    } else {
+        const dim3 grid((max_blocks_per_seq + kThreads / 64 - 1) / (kThreads / 64), num_kv_heads, num_seqs);
+        if (kv_dtype == ZK_F32) page_scores_generic_kernel<ZK_F32><<<grid, kThreads, 0, s>>>(a);
+        else if (kv_dtype == ZK_BF16) page_scores_generic_kernel<ZK_BF16><<<grid, kThreads, 0, s>>>(a);
+        else page_scores_generic_kernel<ZK_FP8_E4M3><<<grid, kThreads, 0, s>>>(a);
+    }
+    return check_launch("zk_page_scores");
+}
+
+int zk_select_pages(const float *scores, const int32_t *seq_lens, int num_seqs, int num_kv_heads,
+                    int max_blocks_per_seq, int block_size, int num_pages, int sink, int recent, int32_t *pages,
+                    void *stream) {
+    if (num_seqs < 0 || num_seqs > 65535 || num_kv_heads <= 0 || max_blocks_per_seq <= 0 || block_size <= 0 ||
+        num_pages <= 0 || (int64_t)max_blocks_per_seq * block_size > 0x7fffffff)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_select_pages: bad shape");
+    if (sink < 0 || recent < 0 || (int64_t)sink + recent > num_pages)
+        return set_error(ZK_ERR_INVALID_ARGUMENT,
+                         "Internal error: zk_select_pages: sink + recent must not exceed num_pages");
+    if (max_blocks_per_seq > kSelectMost)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_select_pages: at most 65536 pages a sequence");
+    if (num_seqs == 0) return ZK_OK;
+    if (!scores || !seq_lens || !pages)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_select_pages: NULL pointer");
+    const dim3 grid(num_kv_heads, num_seqs);
+    hipStream_t s = (hipStream_t)stream;
+    const int width = max_blocks_per_seq;
+    KernelTimer timer("select_pages", s);
+    auto go = [&](auto kernel, int waves) {
+        kernel<<<grid, 64 * waves, 0, s>>>(scores, seq_lens, width, block_size, num_pages, sink, recent, pages);
+    };
+    if (width <= 64 * 8) go(select_pages_kernel<1, 8>, 1);
+    else if (width <= 64 * 4 * 8) go(select_pages_kernel<4, 8>, 4);
+    else if (width <= 64 * 16 * 8) go(select_pages_kernel<16, 8>, 16);
+    else go(select_pages_kernel<16, 64>, 16);
+    return check_launch("zk_select_pages");
+}
+
+}  // extern "C"

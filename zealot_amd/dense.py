@@ -1,15 +1,15 @@
 """Dense ops around the paged-KV path over the C ABI (include/zealot_dense.h):
-rms_norm (optionally fused with the residual add), silu_mul, add, embedding
-and linear (hipBLASLt or the weight-streaming kernel; TiledWeight for weights
+rms_norm (optionally fused with the residual add), silu_mul, add, embedding,
+qk_norm_rope (head norms and rotary embedding) and linear (hipBLASLt or the weight-streaming kernel; TiledWeight for weights
 kept in that kernel's tiled layout).  Torch device tensors in, launches on
 torch's current stream; the kernels are in zealot_amd/csrc/dense_ops.hip,
-gemm.cpp and skinny_gemm.hip."""
+rope_ops.hip, gemm.cpp and skinny_gemm.hip."""
 from __future__ import annotations
 
 import torch
 
 from . import _lib
-from .ops import _dev, _stream, zk_dtype
+from .ops import _dev, _empty, _here, _rope_operands, _rows, _stream, zk_dtype
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -93,6 +93,43 @@ def embedding(ids, table, out=None, stream=None):
     _lib.check(_lib.lib().zk_embedding(_dev(ids, "ids", torch.int64), _dev(table, "table"), _dev(out, "out"), n,
                                        table.shape[0], table.shape[1], _dt(table), _stream(stream)))
     return out
+
+
+def rope_table(max_positions: int, rot_dim: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
+    """The position table of qk_norm_rope (f32 [max_positions, rot_dim]): row p
+    holds cos(p theta^(-2 i / rot_dim)) for i < rot_dim / 2, then the sines.
+    Angles are formed in 64 bits, so far positions keep their phase."""
+    if max_positions <= 0 or rot_dim <= 0 or rot_dim % 2:
+        raise ValueError("rope_table needs positions and an even rot_dim")
+    freq = float(theta) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
+
+
+def qk_norm_rope(q, k, positions, rope, q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False,
+                 q_out=None, k_out=None, stream=None):
+    """RMSNorm of the query and key heads (q [T, H, D], k [T, Hkv, D]; weights
+    [D], None: no norm) and the rotary embedding of their first rot_dim dimensions
+    by the rows `positions` (int32 [T]) of `rope` (rope_table; None: no
+    rotation) in one pass: returns (q_out, k_out).  q and k may be columns of a
+    fused projection output, and q_out / k_out those columns themselves."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape[2] != q.shape[2]:
+        raise ValueError("q must be [T, H, D] and k [T, Hkv, D]")
+    t, h, d = q.shape
+    hkv = k.shape[1]
+    dt = _dt(q)
+    if q_out is None:
+        q_out = _empty((t, h, d), q.dtype, q.device, stream)
+    if k_out is None:
+        k_out = _empty((t, hkv, d), q.dtype, q.device, stream)
+    qs, ks = _rows(q, "q", h, d, q.dtype, t), _rows(k, "k", hkv, d, q.dtype, t)
+    qo, ko = _rows(q_out, "q_out", h, d, q.dtype, t), _rows(k_out, "k_out", hkv, d, q.dtype, t)
+    weights, table = _rope_operands(q, positions, rope, q_weight, k_weight)
+    _here(q, k, positions, rope, q_weight, k_weight, q_out, k_out, stream=stream)
+    _lib.check(_lib.lib().zk_qk_norm_rope(
+        q.data_ptr(), qs, k.data_ptr(), ks, dt, t, h, hkv, d, *weights, float(eps), *table, int(bool(interleaved)),
+        q_out.data_ptr(), qo, k_out.data_ptr(), ko, _stream(stream)))
+    return q_out, k_out
 
 
 class TiledWeight:

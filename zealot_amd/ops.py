@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -57,6 +58,25 @@ def _dev(t: torch.Tensor, name: str, dtype=None, contiguous=True) -> int:
 
 def _opt(t, name, dtype=None):
     return None if t is None else _dev(t, name, dtype)
+
+
+def _here(*operands, stream=None) -> None:
+    """Every operand (None: left out) is on torch's current device, whose stream
+    the launch goes to, and so is `stream`."""
+    cur = torch.cuda.current_device() if _get_device is None or not torch.cuda.is_initialized() else _get_device()
+    if stream is not None and stream.device_index != cur:
+        raise ValueError(f"stream is on device {stream.device_index}, the current device is {cur}")
+    for t in operands:
+        if t is not None and t.is_cuda and t.get_device() != cur:
+            raise ValueError(f"an operand is on {t.device}, the current device is {cur}")
+
+
+def _empty(shape, dtype, device, stream=None) -> torch.Tensor:
+    """A new tensor for a launch on `stream`: the allocator reuses its memory in that stream's order."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _pool_shape(k_pool: torch.Tensor, v_pool: torch.Tensor):
@@ -165,6 +185,230 @@ def paged_decode(q, k_pool, v_pool, block_tables, seq_lens, scale=None, mapping=
         _MAPPINGS[mapping], _opt(k_scales, "k_scales", torch.float32),
         _opt(v_scales, "v_scales", torch.float32), _dev(workspace, "workspace"),
         workspace.numel() * workspace.element_size(), _stream(stream)))
+    return out
+
+
+class StepTables(NamedTuple):
+    """What step_tables gives: rows are the step's tokens packed in batch order."""
+    slot_mapping: torch.Tensor  # int64 [num_rows]; -1: no block, or no token
+    positions: torch.Tensor     # int32 [num_rows]; -1: no token
+    token_row: torch.Tensor     # int32 [num_rows], the token's sequence; -1: no token
+    cu_seqlens: torch.Tensor    # int64 [N + 1]
+    kv_lens: torch.Tensor       # int32 [N], lengths after the step
+    cursor: torch.Tensor        # int64 [1], behind the granted blocks that the step takes
+
+
+def step_tables(block_tables, seq_lens, new_lens, block_size: int, num_rows: int, new_blocks=None, cursor=None, out=None,
+                stream=None) -> StepTables:
+    """Block tables, slots and offsets of a step from its request lengths, on the
+    GPU (zk_step_tables): sequence i holds seq_lens[i] tokens and receives
+    new_lens[i] (int32 [N]); blocks it lacks are taken from new_blocks (int32,
+    in batch order from cursor on, int64 [1]) and entered in block_tables (int32
+    [N, max_blocks], in place).  num_rows: rows of the batch, padding included.
+    out: a StepTables to write to; its kv_lens and cursor must not be inputs."""
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [N, max_blocks]")
+    n, mb = block_tables.shape
+    if seq_lens.shape != (n,) or new_lens.shape != (n,):
+        raise ValueError("seq_lens and new_lens must be [N]")
+    if new_blocks is not None and new_blocks.dim() != 1:
+        raise ValueError("new_blocks must be one list")
+    if cursor is not None and cursor.numel() != 1:
+        raise ValueError("cursor must hold one value")
+    if num_rows < 0:
+        raise ValueError("num_rows must not be negative")
+    dev = block_tables.device
+    if out is None:  # one buffer a type
+        wide = _empty(num_rows + n + 2, torch.int64, dev, stream)
+        narrow = _empty(2 * num_rows + n, torch.int32, dev, stream)
+        slots, cu, end = wide.split((num_rows, n + 1, 1))
+        pos, row, lens = narrow.split((num_rows, num_rows, n))
+        out = StepTables(slots, pos, row, cu, lens, end)
+    elif (out.slot_mapping.shape != (num_rows,) or out.positions.shape != (num_rows,) or out.token_row.shape != (num_rows,)
+          or out.cu_seqlens.shape != (n + 1,) or out.kv_lens.shape != (n,) or out.cursor.shape != (1,)):
+        raise ValueError("out does not match num_rows and the number of sequences")
+    _here(block_tables, seq_lens, new_lens, new_blocks, cursor, *out, stream=stream)
+    granted = 0 if new_blocks is None else new_blocks.shape[0]
+    blocks = _opt(new_blocks, "new_blocks", torch.int32)
+    if new_blocks is not None and granted == 0:  # none were granted (a NULL list would mean: none are needed)
+        blocks = block_tables.data_ptr()
+    _lib.check(_lib.lib().zk_step_tables(
+        _dev(block_tables, "block_tables", torch.int32), n, mb, _dev(seq_lens, "seq_lens", torch.int32),
+        _dev(new_lens, "new_lens", torch.int32), block_size, blocks, granted, _opt(cursor, "cursor", torch.int64),
+        _dev(out.cursor, "out.cursor", torch.int64), _dev(out.slot_mapping, "out.slot_mapping", torch.int64),
+        _dev(out.positions, "out.positions", torch.int32), _dev(out.token_row, "out.token_row", torch.int32), num_rows,
+        _dev(out.cu_seqlens, "out.cu_seqlens", torch.int64), _dev(out.kv_lens, "out.kv_lens", torch.int32),
+        _stream(stream)))
+    return out
+
+
+def _rows(t, name: str, heads: int, dim: int, dtype, rows: int) -> int:
+    """Elements from one token's row of `t` [rows, heads, dim] to the next: rows
+    may lie apart (columns of a fused projection), a row itself is packed."""
+    _dev(t, name, dtype, contiguous=False)
+    if t.dim() != 3 or tuple(t.shape) != (rows, heads, dim):
+        raise ValueError(f"{name} must be [{rows}, {heads}, {dim}], got {tuple(t.shape)}")
+    packed = heads * dim
+    st = t.stride()
+    if rows and ((dim > 1 and st[2] != 1) or (heads > 1 and st[1] != dim) or (rows > 1 and st[0] < packed)):
+        raise ValueError(f"{name} must have packed [heads, dim] rows that do not overlap")
+    return st[0] if rows > 1 else packed
+
+
+def _rope_operands(q, positions, rope, q_weight, k_weight):
+    """(pointer, ...) of the operands that both rope calls take besides q and k."""
+    t, _, d = q.shape
+    if rope is not None:
+        if rope.dim() != 2 or rope.shape[1] % 2 or rope.shape[1] > d or rope.shape[1] == 0 or rope.shape[0] == 0:
+            raise ValueError(f"rope must be [max_positions, rot_dim] with an even rot_dim of at most {d}")
+        if positions is None or positions.shape != (t,):
+            raise ValueError("positions must be [T]")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and w.shape != (d,):
+            raise ValueError(f"{name} must be [{d}]")
+    return (_opt(q_weight, "q_weight", q.dtype), _opt(k_weight, "k_weight", q.dtype)), (
+        _opt(positions, "positions", torch.int32) if rope is not None else None, _opt(rope, "rope", torch.float32),
+        0 if rope is None else rope.shape[0], 0 if rope is None else rope.shape[1])
+
+
+def qk_norm_rope_append(k_pool, v_pool, q, k, v, positions, slot_mapping, rope, q_weight=None, k_weight=None,
+                        eps: float = 1e-6, interleaved: bool = False, q_out=None, k_scales=None, v_scales=None,
+                        token_row=None, stream=None):
+    """dense.qk_norm_rope of q [T, H, D] and k [T, Hkv, D], and append of the
+    resulting K rows and of v at slot_mapping, in one launch: returns q_out
+    (which may be q).  q, k and v may be columns of one fused projection output;
+    K is rounded once, to the pool's type."""
+    nb, hkv, bs, d = _pool_shape(k_pool, v_pool)
+    if q.dim() != 3 or q.shape[2] != d:
+        raise ValueError(f"q must be [T, H, {d}]")
+    t, h, _ = q.shape
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("q must be float32 or bfloat16")
+    if slot_mapping.shape != (t,):
+        raise ValueError("slot_mapping must be [T]")
+    if token_row is not None and token_row.shape != (t,):
+        raise ValueError("token_row must be [T]")
+    for name, sc in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if sc is not None and (sc.dim() != 2 or sc.shape[1] != hkv):
+            raise ValueError(f"{name} must be [sequences, {hkv}]")
+    if q_out is None:
+        q_out = _empty((t, h, d), q.dtype, q.device, stream)
+    qs, ks, vs = _rows(q, "q", h, d, q.dtype, t), _rows(k, "k", hkv, d, q.dtype, t), _rows(v, "v", hkv, d, q.dtype, t)
+    os_ = _rows(q_out, "q_out", h, d, q.dtype, t)
+    weights, table = _rope_operands(q, positions, rope, q_weight, k_weight)
+    _here(k_pool, v_pool, q, k, v, positions, slot_mapping, rope, q_weight, k_weight, q_out, k_scales, v_scales, token_row,
+          stream=stream)
+    _lib.check(_lib.lib().zk_qk_norm_rope_append(
+        _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool"), zk_dtype(k_pool), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(),
+        vs, zk_dtype(q), t, h, hkv, d, *weights, float(eps), *table, int(bool(interleaved)), q_out.data_ptr(), os_,
+        _dev(slot_mapping, "slot_mapping", torch.int64), bs, nb, _opt(k_scales, "k_scales", torch.float32),
+        _opt(v_scales, "v_scales", torch.float32), _opt(token_row, "token_row", torch.int32), _stream(stream)))
+    return q_out
+
+
+def _bounds_shape(bounds):
+    if bounds.dim() != 4 or bounds.shape[2] != 2:
+        raise ValueError("bounds must be [num_blocks, Hkv, 2, D]")
+    nb, hkv, _, d = bounds.shape
+    return nb, hkv, d
+
+
+def page_bounds(k_pool, slot_mapping, bounds, stream=None) -> None:
+    """Bring the pages' key bounds ([num_blocks, Hkv, 2, D]: smallest, then
+    largest, of the pool's type) up to date behind a write of K at slot_mapping
+    (int64 [T]); the rows of one page are consecutive (zk_page_bounds)."""
+    if k_pool.dim() != 4:
+        raise ValueError("k_pool must be [num_blocks, Hkv, block_size, D]")
+    nb, hkv, bs, d = k_pool.shape
+    if tuple(bounds.shape) != (nb, hkv, 2, d) or zk_dtype(bounds) != zk_dtype(k_pool):
+        raise ValueError(f"bounds must be [{nb}, {hkv}, 2, {d}] of the pool's type")
+    if slot_mapping.dim() != 1:
+        raise ValueError("slot_mapping must be [T]")
+    _here(k_pool, slot_mapping, bounds, stream=stream)
+    _lib.check(_lib.lib().zk_page_bounds(
+        _dev(k_pool, "k_pool"), zk_dtype(k_pool), _dev(slot_mapping, "slot_mapping", torch.int64), slot_mapping.shape[0],
+        hkv, d, bs, nb, _dev(bounds, "bounds"), _stream(stream)))
+
+
+def page_scores(q, bounds, block_tables, seq_lens, block_size: int, mapping="grouped", out=None, stream=None):
+    """An upper bound of q . k over each page's keys and the heads of a kv-head
+    (zk_page_scores): q [N, H, D], scores f32 [N, Hkv, max_blocks], -inf behind
+    the length."""
+    nb, hkv, d = _bounds_shape(bounds)
+    if q.dim() != 3 or q.shape[2] != d:
+        raise ValueError(f"q must be [N, H, {d}]")
+    n, h, _ = q.shape
+    if block_tables.dim() != 2 or block_tables.shape[0] != n or seq_lens.shape != (n,):
+        raise ValueError("block_tables must be [N, max_blocks] and seq_lens [N]")
+    mb = block_tables.shape[1]
+    if out is None:
+        out = _empty((n, hkv, mb), torch.float32, q.device, stream)
+    elif tuple(out.shape) != (n, hkv, mb):
+        raise ValueError(f"out must be [{n}, {hkv}, {mb}]")
+    _here(q, bounds, block_tables, seq_lens, out, stream=stream)
+    _lib.check(_lib.lib().zk_page_scores(
+        _dev(q, "q"), zk_dtype(q), _dev(bounds, "bounds"), zk_dtype(bounds),
+        _dev(block_tables, "block_tables", torch.int32), _dev(seq_lens, "seq_lens", torch.int32),
+        _dev(out, "out", torch.float32), n, h, hkv, d, block_size, mb, nb, _MAPPINGS[mapping], _stream(stream)))
+    return out
+
+
+def select_pages(scores, seq_lens, block_size: int, num_pages: int, sink: int = 1, recent: int = 1, out=None, stream=None):
+    """The num_pages best pages of each (sequence, kv-head) in ascending order
+    (int32 [N, Hkv, num_pages], then -1), the first `sink` and last `recent` held
+    ones always among them; equal scores: the lower page (zk_select_pages)."""
+    if scores.dim() != 3 or seq_lens.shape != (scores.shape[0],):
+        raise ValueError("scores must be [N, Hkv, max_blocks] and seq_lens [N]")
+    n, hkv, mb = scores.shape
+    if out is None:
+        out = _empty((n, hkv, num_pages), torch.int32, scores.device, stream)
+    elif tuple(out.shape) != (n, hkv, num_pages):
+        raise ValueError(f"out must be [{n}, {hkv}, {num_pages}]")
+    _here(scores, seq_lens, out, stream=stream)
+    _lib.check(_lib.lib().zk_select_pages(
+        _dev(scores, "scores", torch.float32), _dev(seq_lens, "seq_lens", torch.int32), n, hkv, mb, block_size, num_pages,
+        sink, recent, _dev(out, "out", torch.int32), _stream(stream)))
+    return out
+
+
+def sparse_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_dim, num_pages) -> int:
+    return int(_lib.lib().zk_paged_decode_sparse_workspace_size(num_seqs, num_heads, num_kv_heads, head_dim, num_pages))
+
+
+def paged_decode_sparse(q, k_pool, v_pool, block_tables, seq_lens, pages, scale=None, mapping="grouped", k_scales=None,
+                        v_scales=None, out=None, workspace=None, stream=None):
+    """paged_decode over listed pages only: pages int32 [N, Hkv, K] holds indices
+    into each sequence's block table (negative: none), as select_pages gives
+    them; returns out [N, H, D] (zk_paged_decode_sparse)."""
+    nb, hkv, bs, d = _pool_shape(k_pool, v_pool)
+    if q.dim() != 3 or q.shape[2] != d:
+        raise ValueError(f"q must be [N, H, {d}]")
+    n, h, _ = q.shape
+    if block_tables.dim() != 2 or block_tables.shape[0] != n or seq_lens.shape != (n,):
+        raise ValueError("block_tables must be [N, max_blocks] and seq_lens [N]")
+    if pages.dim() != 3 or tuple(pages.shape[:2]) != (n, hkv):
+        raise ValueError(f"pages must be [N, {hkv}, num_pages]")
+    for name, sc in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if sc is not None and tuple(sc.shape) != (n, hkv):
+            raise ValueError(f"{name} must be [N, {hkv}]")
+    mb, np_ = block_tables.shape[1], pages.shape[2]
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    if out is None:
+        out = _empty(q.shape, q.dtype, q.device, stream)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must match q")
+    if workspace is None:
+        need = sparse_workspace_bytes(n, h, hkv, d, np_)
+        workspace = _empty(need, torch.uint8, q.device, stream) if need else None
+    _here(q, k_pool, v_pool, block_tables, seq_lens, pages, out, workspace, k_scales, v_scales, stream=stream)
+    _lib.check(_lib.lib().zk_paged_decode_sparse(
+        _dev(q, "q"), zk_dtype(q), _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool"), zk_dtype(k_pool), _dev(out, "out"),
+        _dev(block_tables, "block_tables", torch.int32), _dev(seq_lens, "seq_lens", torch.int32),
+        _dev(pages, "pages", torch.int32), np_, n, h, hkv, d, bs, mb, nb, float(scale), _MAPPINGS[mapping],
+        _opt(k_scales, "k_scales", torch.float32), _opt(v_scales, "v_scales", torch.float32),
+        None if workspace is None else _dev(workspace, "workspace"),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(stream)))
     return out
 
 
