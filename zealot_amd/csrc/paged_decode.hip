@@ -338,23 +338,6 @@ plan_kernel(Params p, int num_seqs) {
 }
 
 // ------------------------------------------------------------ MFMA kernel
-typedef __attribute__((address_space(3))) void lds_void;
-
-// 16 bytes per lane from global memory straight into LDS at lds + 16 * lane
-// (global_load_lds_dwordx4; no VGPRs, counted by vmcnt).  Cache policy NT
-// (nontemporal, aux bit 1): every K/V byte is read exactly once, and the
-// streaming hint measured ~9% faster than the default policy on C2.
-constexpr int kCachePolicyNT = 2;
-__device__ __forceinline__ void g2l16(const void *g, lds_void *l) {
-    __builtin_amdgcn_global_load_lds(g, l, 16, 0, kCachePolicyNT);
-}
-// s_waitcnt vmcnt(N) alone (gfx9 encoding: expcnt 7 and lgkmcnt 15 mean "no wait").
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-    static_assert(N >= 0 && N <= 63, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
-}
-__device__ __forceinline__ void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(0xc07f); }
 
 template <int BYTES>
 struct LdsVec;

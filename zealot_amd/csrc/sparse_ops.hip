@@ -174,8 +174,9 @@ struct ScoreArgs {
     float *scores;  // [N][Hkv][max_blocks]
     int64_t num_blocks;
     int num_heads, num_kv_heads, head_dim, block_size, max_blocks, grouped, q_f32;
-    int tiles;  // of 16 pages a wave
+    int tiles;  // of 16 pages a wave (at most kScoreTiles)
 };
+constexpr int kScoreTiles = 32, kScoreHeads = 2;  // most tiles a wave, waves (kv-heads) a workgroup
 
 __device__ __forceinline__ int held_pages(const ScoreArgs &a, int n) {
     const int64_t len = max(a.seq_lens[n], 0);
@@ -187,65 +188,90 @@ __device__ __forceinline__ int qhead(const ScoreArgs &a, int kvh, int j, int G) 
 
 // bf16 queries, bf16 or fp8 bounds: A = 16 pages' [lo | hi] rows, B = the
 // query heads' [min(q, 0) | max(q, 0)], on v_mfma_f32_16x16x32_bf16 (both
-// exact in bf16, the sums in f32).  Lane (grp, col) loads dims 8 grp .. + 7 of
-// a 32-dim step of page col, so a page's four lanes read 64 contiguous bytes;
-// columns past the G heads repeat them, which leaves the maximum over the
-// heads as it is.  Bound by HBM: 2 D values a page and kv-head are read once.
+// exact in bf16, the sums in f32).  One wave per (16 * tiles pages, kv-head,
+// sequence).  A page's row of 2 D values is contiguous, the rows of a tile lie
+// anywhere: the wave loads whole rows, one tile ahead, and turns them into
+// fragments through LDS, chunk c of row r at c ^ r so that 16 rows do not meet in
+// a bank.  (Loaded by the lanes that need them, 64 bytes of 16 rows an
+// instruction, the lines were fetched twice: 83 us for 271 MB.)  Columns past
+// the G heads repeat them, which leaves the maximum over the heads as it is.
+// Bound by HBM.
 template <int KV, int D, int G>
-__global__ void __launch_bounds__(kThreads) page_scores_mfma_kernel(ScoreArgs a) {
+__global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(ScoreArgs a) {
     constexpr int KK = 2 * D / 32, ES = KV == ZK_BF16 ? 2 : 1;
-    typedef typename std::conditional<KV == ZK_BF16, u32x4, u32x2>::type piece_t;
+    constexpr int RB = 2 * D * ES, CPR = RB / 16;  // bytes and 16-byte chunks of a page's row
+    constexpr int LPT = 16 * RB / 1024;            // loads a tile
+    constexpr int SW = CPR < 16 ? CPR : 16;        // chunk c of row r lies at c ^ (r % SW)
+    extern __shared__ __attribute__((aligned(16))) char dyn[];  // a tile a wave
+    __shared__ int32_t ids[16 * kScoreTiles];
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, wave = threadIdx.x >> 6;
-    const int kvh = blockIdx.y, n = blockIdx.z;
+    // (chunks last: consecutive workgroups go to the XCDs in turn, and a sequence's
+    // later chunks are often behind its context)
+    const int kvh = blockIdx.y * (blockDim.x >> 6) + wave, n = blockIdx.x;
     const int held = held_pages(a, n);
     const int32_t *row = a.tables + (size_t)n * a.max_blocks;
-    float *out = a.scores + ((size_t)n * a.num_kv_heads + kvh) * a.max_blocks;
-    const int per = 16 * a.tiles * (kThreads / 64);  // pages of a workgroup
-    const int p0 = blockIdx.x * per + wave * 16, step = 16 * (kThreads / 64), p1 = min((int)(blockIdx.x + 1) * per, a.max_blocks);
-    if (p0 >= p1) return;
-    bf16x8 qf[KK];
-    if (p0 < held) {
-        const uint16_t *q = (const uint16_t *)a.q + ((size_t)n * a.num_heads + qhead(a, kvh, col % G, G)) * D;
-#pragma unroll
-        for (int kk = 0; kk < KK / 2; ++kk) {
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(q + kk * 32 + grp * 8);
-            u32x4 neg, pos;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {  // by sign bit (a NaN's value goes into the half of its sign)
-                const uint32_t m = ((w[i] >> 15) & 0x10001u) * 0xffffu;  // 0xffff in negative halves
-                neg[i] = w[i] & m;
-                pos[i] = w[i] & ~m;
-            }
-            qf[kk] = __builtin_bit_cast(bf16x8, neg);
-            qf[kk + KK / 2] = __builtin_bit_cast(bf16x8, pos);
-        }
+    const int p0 = blockIdx.z * 16 * a.tiles, p1 = min(p0 + 16 * a.tiles, a.max_blocks);
+    const int live = min(p1, held) - p0;  // pages here that the sequence holds
+    for (int i = threadIdx.x; i < 16 * a.tiles; i += blockDim.x) {
+        const int id = i < live ? row[p0 + i] : -1;
+        ids[i] = id < a.num_blocks ? id : -1;
     }
-    const size_t page_bytes = (size_t)2 * D * ES, block_bytes = page_bytes * a.num_kv_heads;
-    for (int p = p0; p < p1; p += step) {
-        const int page = p + col;
-        if (p >= held) {  // behind the context
-            if (grp == 0 && page < p1) out[page] = -INFINITY;
-            continue;
-        }
-        const int blk = page < held ? row[page] : 0;
-        const bool ok = blk >= 0 && blk < a.num_blocks;
-        const char *src = a.bounds + (size_t)(ok ? blk : 0) * block_bytes + (size_t)kvh * page_bytes + grp * 8 * ES;
-        piece_t w[KK];
+    __syncthreads();
+    if (kvh >= a.num_kv_heads) return;
+    float *out = a.scores + ((size_t)n * a.num_kv_heads + kvh) * a.max_blocks + p0;
+    for (int p = max(live, 0) + lane; p < p1 - p0; p += 64) out[p] = -INFINITY;  // behind the context
+    if (live <= 0) return;
+    bf16x8 qf[KK];
+    const uint16_t *q = (const uint16_t *)a.q + ((size_t)n * a.num_heads + qhead(a, kvh, col % G, G)) * D;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) w[kk] = *reinterpret_cast<const piece_t *>(src + kk * 32 * ES);
+    for (int kk = 0; kk < KK / 2; ++kk) {
+        // a k-step's dims of lane group grp: 8 of 32 in turn; of fp8 rows the
+        // halves of 16 bytes go to two steps
+        const int d0 = KV == ZK_BF16 ? 32 * kk + 8 * grp : 64 * (kk / 2) + 16 * grp + 8 * (kk % 2);
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(q + d0);
+        u32x4 neg, pos;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // by sign bit (a NaN's value goes into the half of its sign)
+            const uint32_t m = ((w[i] >> 15) & 0x10001u) * 0xffffu;  // 0xffff in negative halves
+            neg[i] = w[i] & m;
+            pos[i] = w[i] & ~m;
+        }
+        qf[kk] = __builtin_bit_cast(bf16x8, neg);
+        qf[kk + KK / 2] = __builtin_bit_cast(bf16x8, pos);
+    }
+    char *lds = dyn + wave * 16 * RB;
+    const size_t block_bytes = (size_t)RB * a.num_kv_heads;
+    const char *base = a.bounds + (size_t)kvh * RB;
+    auto load = [&](int tile, u32x4 (&in)[LPT]) {
+#pragma unroll
+        for (int j = 0; j < LPT; ++j) {
+            const int slot = 64 * j + lane, r = slot / CPR, c = slot % CPR;
+            const size_t blk = (size_t)max(ids[16 * tile + r], 0);
+            in[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(base + blk * block_bytes + c * 16));
+        }
+    };
+    auto tile = [&](int t, const u32x4 (&in)[LPT]) {
+#pragma unroll
+        for (int j = 0; j < LPT; ++j) {
+            const int slot = 64 * j + lane, r = slot / CPR, c = slot % CPR;
+            *reinterpret_cast<u32x4 *>(lds + (r * CPR + (c ^ (r % SW))) * 16) = in[j];
+        }
         f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            bf16x8 f;
+        for (int c = 0; c < CPR / 4; ++c) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(lds + (col * CPR + ((4 * c + grp) ^ (col % SW))) * 16);
             if constexpr (KV == ZK_BF16) {
-                f = __builtin_bit_cast(bf16x8, w[kk]);
+                acc[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), qf[c], acc[c & 1], 0, 0, 0);
             } else {
-                const u32x2 lo = e4m3x4_to_bf16x4(w[kk][0]), hi = e4m3x4_to_bf16x4(w[kk][1]);
-                f = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const u32x2 lo = e4m3x4_to_bf16x4(w[2 * h]), hi = e4m3x4_to_bf16x4(w[2 * h + 1]);
+                    acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]}),
+                                                                     qf[2 * c + h], acc[h], 0, 0, 0);
+                }
             }
-            acc[kk & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[kk], acc[kk & 1], 0, 0, 0);
         }
-        f32x4 s = acc[0] + acc[1];  // head col's scores of pages p + 4 grp + i
+        f32x4 s = acc[0] + acc[1];  // head col's scores of the tile's pages 4 grp + i
 #pragma unroll
         for (int o = 1; o < G; o <<= 1)
 #pragma unroll
@@ -255,10 +281,20 @@ __global__ void __launch_bounds__(kThreads) page_scores_mfma_kernel(ScoreArgs a)
         v = col == 1 ? s[1] : v;
         v = col == 2 ? s[2] : v;
         v = col == 3 ? s[3] : v;
-        const int dst = p + 4 * grp + col;
-        const int ok_dst = __shfl((int)(ok && page < held), 4 * grp + (col & 3));  // (lane c < 16 holds page p + c)
-        if (col < 4 && dst < p1) out[dst] = ok_dst ? v : -INFINITY;
+        const int p = 16 * t + 4 * grp + col;
+        if (col < 4 && p < live) out[p] = ids[p] >= 0 ? v : -INFINITY;
+    };
+    const int tiles = (live + 15) / 16;
+    u32x4 in0[LPT], in1[LPT];
+    load(0, in0);
+    int t = 0;
+    for (; t + 1 < tiles; t += 2) {
+        load(t + 1, in1);
+        tile(t, in0);
+        load(min(t + 2, tiles - 1), in0);
+        tile(t + 1, in1);
     }
+    if (t < tiles) tile(t, in0);
 }
 
 // Any shape and type: one wave per (page, kv-head, sequence), lanes over the
@@ -404,12 +440,13 @@ constexpr int kSelectMost = 16 * 64 * 64;  // pages of the widest variant
 
 template <int KV, int D>
 void launch_scores_g(const ScoreArgs &a, dim3 grid, int G, hipStream_t s) {
+    const int waves = std::min(a.num_kv_heads, kScoreHeads), lds = waves * 16 * 2 * D * (KV == ZK_BF16 ? 2 : 1);
     switch (G) {
-        case 1: page_scores_mfma_kernel<KV, D, 1><<<grid, kThreads, 0, s>>>(a); break;
-        case 2: page_scores_mfma_kernel<KV, D, 2><<<grid, kThreads, 0, s>>>(a); break;
-        case 4: page_scores_mfma_kernel<KV, D, 4><<<grid, kThreads, 0, s>>>(a); break;
-        case 8: page_scores_mfma_kernel<KV, D, 8><<<grid, kThreads, 0, s>>>(a); break;
-        default: page_scores_mfma_kernel<KV, D, 16><<<grid, kThreads, 0, s>>>(a); break;
+        case 1: page_scores_mfma_kernel<KV, D, 1><<<grid, 64 * waves, lds, s>>>(a); break;
+        case 2: page_scores_mfma_kernel<KV, D, 2><<<grid, 64 * waves, lds, s>>>(a); break;
+        case 4: page_scores_mfma_kernel<KV, D, 4><<<grid, 64 * waves, lds, s>>>(a); break;
+        case 8: page_scores_mfma_kernel<KV, D, 8><<<grid, 64 * waves, lds, s>>>(a); break;
+        default: page_scores_mfma_kernel<KV, D, 16><<<grid, 64 * waves, lds, s>>>(a); break;
     }
 }
 template <int KV>
@@ -482,17 +519,17 @@ int zk_page_scores(const void *q, zk_dtype q_dtype, const void *bounds, zk_dtype
     const int G = num_heads / num_kv_heads;
     hipStream_t s = (hipStream_t)stream;
     KernelTimer timer("page_scores", s);
-    const bool mfma = q_dtype == ZK_BF16 && kv_dtype != ZK_F32 && (head_dim == 64 || head_dim == 128) &&
+    const bool mfma = q_dtype == ZK_BF16 && kv_dtype != ZK_F32 && max_blocks_per_seq <= 65535 * 16 * kScoreTiles && (head_dim == 64 || head_dim == 128) &&
                       (G == 1 || G == 2 || G == 4 || G == 8 || G == 16) && (((uintptr_t)q | (uintptr_t)bounds) & 15u) == 0;
     if (mfma) {
-        // 8 tiles a wave (a workgroup then takes 512 pages) unless that leaves
-        // fewer than 1024 workgroups
         a.tiles = 8;
         auto groups = [&](int tiles) {
-            return (int64_t)num_seqs * num_kv_heads * ((max_blocks_per_seq + 64 * tiles - 1) / (64 * tiles));
+            return (int64_t)num_seqs * num_kv_heads * ((max_blocks_per_seq + 16 * tiles - 1) / (16 * tiles));  // of a wave
         };
-        while (a.tiles > 1 && groups(a.tiles) < 1024) a.tiles /= 2;
-        const dim3 grid((max_blocks_per_seq + 64 * a.tiles - 1) / (64 * a.tiles), num_kv_heads, num_seqs);
+        while (a.tiles > 1 && groups(a.tiles) < 2048) a.tiles /= 2;
+        while ((max_blocks_per_seq + 16 * a.tiles - 1) / (16 * a.tiles) > 65535 && a.tiles < kScoreTiles) a.tiles *= 2;
+        const dim3 grid(num_seqs, (num_kv_heads + kScoreHeads - 1) / kScoreHeads,
+                        (max_blocks_per_seq + 16 * a.tiles - 1) / (16 * a.tiles));
         if (kv_dtype == ZK_BF16) launch_scores<ZK_BF16>(a, grid, G, s);
         else launch_scores<ZK_FP8_E4M3>(a, grid, G, s);
     } else {
