@@ -28,7 +28,8 @@ struct RopeArgs {
     int64_t num_blocks, num_slots;
     const float *k_scales, *v_scales;
     const int32_t *token_row;
-    int lanes;  // of a head in the vector kernel
+    int lanes;      // of a head in the vector kernel
+    float inv_dim;  // 1 / head_dim
 };
 int qk_norm_rope(const RopeArgs &a, hipStream_t s);
 

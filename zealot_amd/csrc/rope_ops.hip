@@ -19,6 +19,7 @@
 #include <cstdint>
 #include <string>
 
+#include "attn_device.h"
 #include "rope_ops.h"
 #include "zk_common.h"
 
@@ -32,30 +33,43 @@ constexpr int kMaxDim = 1024;  // of the generic kernel's LDS row
 template <typename T> struct Elt;
 template <> struct Elt<float> {
     static constexpr int V = 4;  // of a 16-byte vector
-    static __device__ __forceinline__ void load(const float *p, float *x) {
-        const f32x4 v = *reinterpret_cast<const f32x4 *>(p);
+    static __device__ __forceinline__ void unpack(u32x4 v, float *x) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = v[e];
+        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(v[e]);
     }
-    static __device__ __forceinline__ void store(float *p, const float *x) {
-        *reinterpret_cast<f32x4 *>(p) = f32x4{x[0], x[1], x[2], x[3]};
+    static __device__ __forceinline__ u32x4 pack(const float *x) {
+        return u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+    }
+    static __device__ __forceinline__ float squares(u32x4 v) {
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += __uint_as_float(v[e]) * __uint_as_float(v[e]);
+        return s;
     }
     static __device__ __forceinline__ float get(const float *p) { return *p; }
     static __device__ __forceinline__ void put(float *p, float x) { *p = x; }
 };
 template <> struct Elt<uint16_t> {  // bf16 bits
     static constexpr int V = 8;
-    static __device__ __forceinline__ void load(const uint16_t *p, float *x) {
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
+    static __device__ __forceinline__ void unpack(u32x4 v, float *x) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[2 * i] = bf16lo(v[i]);
             x[2 * i + 1] = bf16hi(v[i]);
         }
     }
-    static __device__ __forceinline__ void store(uint16_t *p, const float *x) {
-        *reinterpret_cast<u32x4 *>(p) = u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                                              pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+    static __device__ __forceinline__ u32x4 pack(const float *x) {
+        return u32x4{bf16x2_rne(x[0], x[1]), bf16x2_rne(x[2], x[3]), bf16x2_rne(x[4], x[5]), bf16x2_rne(x[6], x[7])};
+    }
+    static __device__ __forceinline__ float squares(u32x4 v) {  // exact products, f32 sums
+        typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = v[i];
+            s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), __builtin_bit_cast(bf16x2_t, w), s, false);
+        }
+        return s;
     }
     static __device__ __forceinline__ float get(const uint16_t *p) { return __uint_as_float((uint32_t)*p << 16); }
     static __device__ __forceinline__ void put(uint16_t *p, float x) { *p = (uint16_t)f32_to_bf16_bits(x); }
@@ -65,10 +79,11 @@ template <> struct Elt<uint16_t> {  // bf16 bits
 template <int V>
 __device__ __forceinline__ void store_pool(void *pool, int dt, size_t at, const float *x, float inv) {
     if (dt == ZK_BF16) {
-#pragma unroll
-        for (int j = 0; j < V / 4; ++j) {
-            const u32x2 w = {pack_bf16x2(x[4 * j], x[4 * j + 1]), pack_bf16x2(x[4 * j + 2], x[4 * j + 3])};
-            reinterpret_cast<u32x2 *>((uint16_t *)pool + at)[j] = w;
+        if constexpr (V == 8) {
+            __builtin_nontemporal_store(Elt<uint16_t>::pack(x), reinterpret_cast<u32x4 *>((uint16_t *)pool + at));
+        } else {
+            const u32x2 w = {bf16x2_rne(x[0], x[1]), bf16x2_rne(x[2], x[3])};
+            *reinterpret_cast<u32x2 *>((uint16_t *)pool + at) = w;
         }
     } else if (dt == ZK_F32) {
 #pragma unroll
@@ -87,127 +102,211 @@ __device__ __forceinline__ void put_pool(void *pool, int dt, size_t at, float x,
     else ((uint8_t *)pool)[at] = (uint8_t)(e4m3x4(x * inv, 0.f, 0.f, 0.f) & 0xffu);
 }
 
-// Where a token's K and V rows go: the row index in the pools (of head 0,
-// heads are block_size rows apart), or -1.
-__device__ __forceinline__ int64_t pool_row(const RopeArgs &a, int64_t t) {
-    const int64_t slot = a.slots[t];
+// Row index in the pools of a slot's token (of head 0; heads are block_size
+// rows apart), or -1.
+__device__ __forceinline__ int64_t pool_row(const RopeArgs &a, int64_t slot) {
     if (slot < 0 || slot >= a.num_slots) return -1;
     const int64_t blk = slot / a.block_size;
     return blk * a.num_kv_heads * a.block_size + (slot - blk * a.block_size);
 }
 
-// One workgroup per token (gridDim.y workgroups when there are few): `lanes`
-// lanes (a power of two) hold one head, V values in one 16-byte vector each,
-// the cosines, sines and weights of a lane's dimensions stay in registers over
-// its heads.  The sum of squares and the partner's half of a rotation cross
-// lanes by shuffles; a lane writes what it read, so outputs may be the inputs.
-// Bound by HBM.
-template <typename T>
+// Sum over aligned groups of `lanes` lanes, in every lane of a group: within 16
+// by the VALU's lane permutations (pairs, pairs of pairs, then mirrored halves,
+// whose lanes agree by then).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane_sum(float x, int lanes) {
+    if (lanes > 1) x += dpp<0xb1>(x);   // lane ^ 1
+    if (lanes > 2) x += dpp<0x4e>(x);   // lane ^ 2
+    if (lanes > 4) x += dpp<0x141>(x);  // mirrored in 8
+    if (lanes > 8) x += dpp<0x140>(x);  // mirrored in 16
+    if (lanes > 16) x += xor16(x);
+    if (lanes > 32) x += xor32(x);
+    return x;
+}
+
+// One workgroup per token (gridDim.y of them share its heads when tokens are
+// few or heads many); `lanes` lanes (a power of two) hold one head, V values in
+// one 16-byte vector each, NP heads a lane, all loaded before any is used.  A
+// lane writes what it read, so outputs may be the inputs.
+//
+// 32768 tokens, 32 + 2 x 8 heads of 128 bf16 (810 MB): 137 us, 5.9 TB/s (a copy
+// reaches 6.7).  Between HBM and the VALU (busy 104 us of it), so what a head
+// needs is kept small: cosines and sines times the weights once a token, the
+// norm's factor applied to the rotated value, sums of squares by dot products of
+// packed pairs, partners exchanged packed, V copied (before: 187 us, and 233 with
+// plain loads and stores).  And its waves must be many (82 registers, six a
+// SIMD): workgroups that walk the tokens and load the next one ahead hold 180-200
+// registers, two waves a SIMD, and took 178-217 us.
+template <typename T, int NP, bool INTER>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
-    constexpr int V = Elt<T>::V;
-    const int64_t t = blockIdx.x;
+    constexpr int V = Elt<T>::V, TV = INTER ? V / 2 : V;  // cosines of a lane
+    // read only: scalar loads, apart from the vector loads' order
+    typedef const __attribute__((address_space(4))) int32_t *cint_t;
+    typedef const __attribute__((address_space(4))) int64_t *clong_t;
     const int D = a.head_dim, half = a.rot_dim / 2;
     const int lanes = a.lanes, l = threadIdx.x & (lanes - 1), d0 = l * V;
-    const int group = threadIdx.x / lanes, groups = kThreads / lanes;
-    const bool live = d0 < D;
-    const bool pool = a.k_pool != nullptr;
+    const int groups = kThreads / lanes, step = groups * gridDim.y;
+    const int hg = blockIdx.y * groups + threadIdx.x / lanes;  // this lane's heads: hg + j * step
+    const bool live = d0 < D, pool = a.k_pool != nullptr;
     const int heads = a.num_heads + (pool ? 2 : 1) * a.num_kv_heads;
-    const int64_t pos = a.rot_dim ? a.positions[t] : 0;
-    const bool zero = a.rot_dim && (pos < 0 || pos >= a.max_positions);
-    const int64_t prow = pool ? pool_row(a, t) : 0;
-    const bool rotated = live && d0 < a.rot_dim;
-    const bool second = !a.interleaved && d0 >= half;  // holds the y_b of its pairs
-    const int partner = a.interleaved ? threadIdx.x : second ? threadIdx.x - half / V : threadIdx.x + half / V;
-    float c[V], s[V], wq[V], wk[V];
+    const bool rot = a.rot_dim > 0, part = a.rot_dim < D, rotated = live && d0 < a.rot_dim;
+    const bool second = !INTER && d0 >= half;  // holds the y_b of its pairs
+    const int away = !rotated || INTER ? 0 : second ? -(half / V) : half / V;  // the partner's lane
+    const int partner = ((int)threadIdx.x + away) & 63;
+    const int at_table = !rotated ? 0 : INTER ? d0 / 2 : second ? d0 - half : d0;
+
+    // weights of this lane's dimensions and (rotate-half) its partner's, packed
+    u32x4 wq, wk, uq, uk;
+    {
+        float one[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        c[e] = 1.0f;
-        s[e] = 0.0f;
-        wq[e] = wk[e] = 1.0f;
-    }
-    if (rotated && !zero) {
-        const float *row = a.rope + (size_t)pos * a.rot_dim;
-        if (a.interleaved) {
-#pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                c[e] = c[e + 1] = row[(d0 + e) / 2];
-                s[e] = s[e + 1] = row[half + (d0 + e) / 2];
-            }
-        } else {
-            const int i = second ? d0 - half : d0;
-#pragma unroll
-            for (int e = 0; e < V; e += 4) {
-                const f32x4 cv = *reinterpret_cast<const f32x4 *>(row + i + e);
-                const f32x4 sv = *reinterpret_cast<const f32x4 *>(row + half + i + e);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    c[e + j] = cv[j];
-                    s[e + j] = sv[j];
-                }
-            }
+        for (int e = 0; e < V; ++e) one[e] = 1.0f;
+        wq = wk = uq = uk = Elt<T>::pack(one);
+        if (live && a.q_weight) {
+            wq = *reinterpret_cast<const u32x4 *>((const T *)a.q_weight + d0);
+            uq = *reinterpret_cast<const u32x4 *>((const T *)a.q_weight + d0 + away * V);
+        }
+        if (live && a.k_weight) {
+            wk = *reinterpret_cast<const u32x4 *>((const T *)a.k_weight + d0);
+            uk = *reinterpret_cast<const u32x4 *>((const T *)a.k_weight + d0 + away * V);
         }
     }
-    if (live && a.q_weight) Elt<T>::load((const T *)a.q_weight + d0, wq);
-    if (live && a.k_weight) Elt<T>::load((const T *)a.k_weight + d0, wk);
-    const int step = groups * gridDim.y;
-    for (int h0 = blockIdx.y * groups; h0 < heads; h0 += step) {
-        const int h = h0 + group;
-        const bool is_q = h < a.num_heads, is_v = h >= a.num_heads + a.num_kv_heads;
-        const int kh = is_v ? h - a.num_heads - a.num_kv_heads : h - a.num_heads;
-        const bool on = live && h < heads;
+    const int t = blockIdx.x;
+    u32x4 raw[NP];                      // this lane's values of its heads
+    bool has_q = false, has_k = false;  // whether query or key heads are among them
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int h = hg + j * step, kh = h - a.num_heads, vh = kh - a.num_kv_heads;
+        // (a lane without a head loads the row's start, not used: no branch around a load)
+        const bool q_row = kh < 0 || h >= heads || !live;
+        const int64_t stride = q_row ? a.q_stride : vh < 0 ? a.k_stride : a.v_stride;
+        const T *p = q_row ? (const T *)a.q : vh < 0 ? (const T *)a.k : (const T *)a.v;
+        if (live && h < heads) p += (size_t)(kh < 0 ? h : vh < 0 ? kh : vh) * D + d0;
+        raw[j] = __builtin_nontemporal_load(
+            reinterpret_cast<const u32x4 *>((const char *)p + (uint64_t)(uint32_t)t * (uint32_t)(sizeof(T) * stride)));
+        has_q = has_q || kh < 0;
+        has_k = has_k || (kh >= 0 && vh < 0);
+    }
+    const int64_t pos = rot ? ((cint_t)a.positions)[t] : 0;
+    const bool zero = rot && (pos < 0 || pos >= a.max_positions);
+    f32x4 cs[V / 4], sn[V / 4];  // cosines and sines of this lane's pairs
+    if (rot) {
+        const float *row = a.rope + (zero ? 0 : (size_t)pos * a.rot_dim) + at_table;
+        if constexpr (TV >= 4) {
+#pragma unroll
+            for (int e = 0; e < TV / 4; ++e) {
+                cs[e] = *reinterpret_cast<const f32x4 *>(row + 4 * e);
+                sn[e] = *reinterpret_cast<const f32x4 *>(row + half + 4 * e);
+            }
+        } else {
+            const f32x2 cv = *reinterpret_cast<const f32x2 *>(row), sv = *reinterpret_cast<const f32x2 *>(row + half);
+            cs[0] = f32x4{cv[0], cv[1], 0.f, 0.f};
+            sn[0] = f32x4{sv[0], sv[1], 0.f, 0.f};
+        }
+    }
+    // cosines times this lane's weights, sines times those of what they meet (and its sign)
+    struct Turn {
+        float c[V], s[V];
+    };
+    auto make = [&](u32x4 w_, u32x4 u_, Turn &m) {
+        float w[V], u[V];
+        Elt<T>::unpack(w_, w);
+        Elt<T>::unpack(u_, u);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const int i = INTER ? e / 2 : e;
+            const bool minus = INTER ? !(e & 1) : !second;
+            const float c = rotated ? cs[i / 4][i % 4] : 1.0f, s = rotated ? sn[i / 4][i % 4] : 0.0f;
+            m.c[e] = c * w[e];
+            m.s[e] = (minus ? -s : s) * (INTER ? w[e ^ 1] : u[e]);
+        }
+    };
+    // y = (x * c + its partner * s) * the norm's factor
+    auto turn = [&](u32x4 v, const Turn &m, bool norm, float *y) {
         float x[V];
-        if (on) {
-            const T *src = is_q   ? (const T *)a.q + t * a.q_stride + (size_t)h * D
-                           : is_v ? (const T *)a.v + t * a.v_stride + (size_t)kh * D
-                                  : (const T *)a.k + t * a.k_stride + (size_t)kh * D;
-            Elt<T>::load(src + d0, x);
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[e] = 0.0f;
-        }
-        float y[V];
-        const bool norm = is_q ? a.q_weight != nullptr : a.k_weight != nullptr;
+        Elt<T>::unpack(v, x);
         float inv = 1.0f;
-        if (a.q_weight || a.k_weight) {  // (all lanes: the shuffles need their partners)
-            float ss = 0.0f;
-#pragma unroll
-            for (int e = 0; e < V; ++e) ss += x[e] * x[e];
-            for (int o = lanes / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-            inv = rsqrtf(ss / (float)D + a.eps);
+        if (norm) {
+            const float ss = Elt<T>::squares(v);
+            inv = rsqrtf(lane_sum(live ? ss : 0.0f, lanes) * a.inv_dim + a.eps);
         }
+        if (!rot) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) y[e] = !norm || is_v ? x[e] : x[e] * inv * (is_q ? wq[e] : wk[e]);
-        if (a.rot_dim && !is_v) {  // (is_v is the same for a head's lanes)
-            float z[V];
-            if (a.interleaved) {
-#pragma unroll
-                for (int e = 0; e < V; e += 2) {
-                    z[e] = y[e] * c[e] - y[e + 1] * s[e];
-                    z[e + 1] = y[e + 1] * c[e] + y[e] * s[e];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float p = __shfl(y[e], partner & 63);
-                    z[e] = second ? y[e] * c[e] + p * s[e] : y[e] * c[e] - p * s[e];
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = zero ? 0.0f : rotated ? z[e] : y[e];
+            for (int e = 0; e < V; ++e) y[e] = x[e] * m.c[e] * inv;
+            return;
         }
-        if (!on) continue;
-        if (is_q) {
-            Elt<T>::store((T *)a.q_out + t * a.q_out_stride + (size_t)h * D + d0, y);
-        } else if (!pool) {
-            Elt<T>::store((T *)a.k_out + t * a.k_out_stride + (size_t)kh * D + d0, y);
-        } else if (prow >= 0) {
-            float f = 1.0f;
-            if (a.cache_dtype == ZK_FP8_E4M3)
-                f = 1.0f / (is_v ? a.v_scales : a.k_scales)[(size_t)a.token_row[t] * a.num_kv_heads + kh];
-            const size_t at = ((size_t)prow + (size_t)kh * a.block_size) * D + d0;
-            store_pool<V>(is_v ? a.v_pool : a.k_pool, a.cache_dtype, at, y, f);
+        float p[V];
+        if constexpr (INTER) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) p[e] = x[e ^ 1];
+        } else {
+            u32x4 other;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) other[i] = (uint32_t)__shfl((int)v[i], partner);
+            Elt<T>::unpack(other, p);
+        }
+        if (part)  // behind rot_dim an infinity times the sine of 0 must not count
+#pragma unroll
+            for (int e = 0; e < V; ++e) p[e] = rotated ? p[e] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = (x[e] * m.c[e] + p[e] * m.s[e]) * inv;
+    };
+    const int64_t prow = pool ? pool_row(a, ((clong_t)a.slots)[t]) : 0;
+    auto to_pool = [&](bool is_v, int hd, const float *y) {
+        if (prow < 0) return;
+        float f = 1.0f;
+        if (a.cache_dtype == ZK_FP8_E4M3)
+            f = 1.0f / (is_v ? a.v_scales : a.k_scales)[(size_t)((cint_t)a.token_row)[t] * a.num_kv_heads + hd];
+        store_pool<V>(is_v ? a.v_pool : a.k_pool, a.cache_dtype, ((size_t)prow + (size_t)hd * a.block_size) * D + d0, y, f);
+    };
+    // queries, keys, values: a wave skips what none of its lanes holds
+    if (has_q) {
+        Turn m;
+        make(wq, uq, m);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int h = hg + j * step;
+            if (h >= a.num_heads) continue;
+            float y[V];
+            turn(raw[j], m, a.q_weight != nullptr, y);
+            u32x4 w = Elt<T>::pack(y);
+            if (zero) w = u32x4{0u, 0u, 0u, 0u};
+            if (live)
+                __builtin_nontemporal_store(
+                    w, reinterpret_cast<u32x4 *>((T *)a.q_out + t * a.q_out_stride + (size_t)h * D + d0));
         }
     }
+    if (has_k) {
+        Turn m;
+        make(wk, uk, m);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int kh = hg + j * step - a.num_heads;
+            if (kh < 0 || kh >= a.num_kv_heads) continue;
+            float y[V];
+            turn(raw[j], m, a.k_weight != nullptr, y);
+            if (zero)
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = 0.0f;
+            if (!live) continue;
+            if (pool) to_pool(false, kh, y);
+            else
+                __builtin_nontemporal_store(
+                    Elt<T>::pack(y), reinterpret_cast<u32x4 *>((T *)a.k_out + t * a.k_out_stride + (size_t)kh * D + d0));
+        }
+    }
+    if (pool)
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int vh = hg + j * step - a.num_heads - a.num_kv_heads;
+            if (vh < 0 || vh >= a.num_kv_heads || !live) continue;
+            float y[V];
+            Elt<T>::unpack(raw[j], y);
+            to_pool(true, vh, y);
+        }
 }
 
 // Any shape and alignment up to kMaxDim: one wave per (token, head), the row
@@ -238,7 +337,7 @@ __global__ void __launch_bounds__(64) qk_norm_rope_generic_kernel(RopeArgs a) {
     const int64_t pos = a.rot_dim ? a.positions[t] : 0;
     const bool zero = !is_v && a.rot_dim && (pos < 0 || pos >= a.max_positions);
     const float *cs = a.rope + (zero || is_v ? 0 : (size_t)pos * a.rot_dim);
-    const int64_t prow = pool && !is_q ? pool_row(a, t) : 0;
+    const int64_t prow = pool && !is_q ? pool_row(a, a.slots[t]) : 0;
     if (prow < 0) return;
     float f = 1.0f;
     if (pool && !is_q && a.cache_dtype == ZK_FP8_E4M3)
@@ -278,15 +377,22 @@ bool rows_overlap(const void *a, int64_t a_stride, int64_t a_width, const void *
 
 template <typename T>
 void launch(const RopeArgs &a, bool vec, int heads, hipStream_t s) {
-    if (vec) {
-        // Few tokens: the heads of a token over several workgroups, down to one
-        // pass of 256 / lanes heads each.
-        const int passes = (heads * a.lanes + kThreads - 1) / kThreads;
-        const int y = (int)std::max<int64_t>(1, std::min<int64_t>(passes, 2048 / std::max<int64_t>(1, a.num_tokens)));
-        qk_norm_rope_kernel<T><<<dim3((unsigned)a.num_tokens, y), kThreads, 0, s>>>(a);
-    } else {
+    if (!vec) {
         qk_norm_rope_generic_kernel<T><<<dim3((unsigned)a.num_tokens, heads), 64, 0, s>>>(a);
+        return;
     }
+    // Few tokens: the heads of a token over several workgroups, down to one
+    // pass of 256 / lanes heads each; many heads: at most four passes.
+    const int passes = (heads * a.lanes + kThreads - 1) / kThreads;
+    const int64_t fill = 2048 / std::max<int64_t>(1, a.num_tokens);
+    const int y = std::max((passes + 3) / 4, (int)std::max<int64_t>(1, std::min<int64_t>(passes, fill)));
+    const int np = (passes + y - 1) / y;
+    const dim3 grid((unsigned)a.num_tokens, y);
+    auto go = [&](auto rotate_half, auto inter) { (a.interleaved ? inter : rotate_half)<<<grid, kThreads, 0, s>>>(a); };
+    if (np <= 1) go(qk_norm_rope_kernel<T, 1, false>, qk_norm_rope_kernel<T, 1, true>);
+    else if (np <= 2) go(qk_norm_rope_kernel<T, 2, false>, qk_norm_rope_kernel<T, 2, true>);
+    else if (np <= 3) go(qk_norm_rope_kernel<T, 3, false>, qk_norm_rope_kernel<T, 3, true>);
+    else go(qk_norm_rope_kernel<T, 4, false>, qk_norm_rope_kernel<T, 4, true>);
 }
 
 }  // namespace
@@ -342,9 +448,11 @@ int zk::qk_norm_rope(const RopeArgs &in, hipStream_t s) {
                al(a.k_weight) && (!a.rot_dim || al(a.rope));
     if (pool) vec = vec && mult(a.v_stride) && al(a.v) && al(a.k_pool) && al(a.v_pool);
     else vec = vec && mult(a.k_out_stride) && al(a.k_out);
+    vec = vec && std::max({a.q_stride, a.k_stride, pool ? a.v_stride : 0}) * e < (1ll << 32);  // (32-bit steps)
     int lanes = 1;
     while (lanes * V < D) lanes *= 2;
     a.lanes = lanes;
+    a.inv_dim = 1.0f / (float)D;
     const int heads = a.num_heads + (pool ? 2 : 1) * a.num_kv_heads;
     KernelTimer timer("qk_norm_rope", s);
     if (a.dtype == ZK_BF16) launch<uint16_t>(a, vec, heads, s);

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _dev, _empty, _here, _rope_operands, _rows, _stream, zk_dtype
+from .ops import _current, _dev, _dims, _empty, _rope_operands, _rows, _stream, zk_dtype
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -113,22 +113,25 @@ def qk_norm_rope(q, k, positions, rope, q_weight=None, k_weight=None, eps: float
     by the rows `positions` (int32 [T]) of `rope` (rope_table; None: no
     rotation) in one pass: returns (q_out, k_out).  q and k may be columns of a
     fused projection output, and q_out / k_out those columns themselves."""
-    if q.dim() != 3 or k.dim() != 3 or k.shape[2] != q.shape[2]:
-        raise ValueError("q must be [T, H, D] and k [T, Hkv, D]")
-    t, h, d = q.shape
-    hkv = k.shape[1]
-    dt = _dt(q)
+    t, h, d = _dims(q, "q", "[T, H, D]")
+    _, hkv, _ = _dims(k, "k", "[T, Hkv, D]")
+    dt = q.dtype
+    code = _dt(q)
+    cur = _current(stream)
+    qs, ks = _rows(q, "q", t, h, d, dt, cur), _rows(k, "k", t, hkv, d, dt, cur)
+    qo = ko = 0
     if q_out is None:
-        q_out = _empty((t, h, d), q.dtype, q.device, stream)
+        q_out = _empty(q, (t, h, d), dt, stream)
+    else:
+        qo = _rows(q_out, "q_out", t, h, d, dt, cur)
     if k_out is None:
-        k_out = _empty((t, hkv, d), q.dtype, q.device, stream)
-    qs, ks = _rows(q, "q", h, d, q.dtype, t), _rows(k, "k", hkv, d, q.dtype, t)
-    qo, ko = _rows(q_out, "q_out", h, d, q.dtype, t), _rows(k_out, "k_out", hkv, d, q.dtype, t)
-    weights, table = _rope_operands(q, positions, rope, q_weight, k_weight)
-    _here(q, k, positions, rope, q_weight, k_weight, q_out, k_out, stream=stream)
+        k_out = _empty(k, (t, hkv, d), dt, stream)
+    else:
+        ko = _rows(k_out, "k_out", t, hkv, d, dt, cur)
+    weights, table = _rope_operands(positions, rope, q_weight, k_weight, t, d, dt, cur)
     _lib.check(_lib.lib().zk_qk_norm_rope(
-        q.data_ptr(), qs, k.data_ptr(), ks, dt, t, h, hkv, d, *weights, float(eps), *table, int(bool(interleaved)),
-        q_out.data_ptr(), qo, k_out.data_ptr(), ko, _stream(stream)))
+        q.data_ptr(), qs, k.data_ptr(), ks, code, t, h, hkv, d, *weights, eps, *table, interleaved, q_out.data_ptr(), qo,
+        k_out.data_ptr(), ko, _stream(stream)))
     return q_out, k_out
 
 

@@ -60,23 +60,77 @@ def _opt(t, name, dtype=None):
     return None if t is None else _dev(t, name, dtype)
 
 
-def _here(*operands, stream=None) -> None:
-    """Every operand (None: left out) is on torch's current device, whose stream
-    the launch goes to, and so is `stream`."""
-    cur = torch.cuda.current_device() if _get_device is None or not torch.cuda.is_initialized() else _get_device()
+# Operands of the calls below _need: one expression a tensor on the way through
+# (0.5 us; a fused norm + rotation + append names 14 of them), the reasons apart.
+
+def _current(stream=None) -> int:
+    """torch's current device, which the launch goes to; `stream` belongs to it."""
+    if _get_device is None or not torch.cuda.is_initialized():
+        cur = torch.cuda.current_device() if torch.cuda.is_available() else -2  # (-1 is a host tensor's)
+    else:
+        cur = _get_device()
     if stream is not None and stream.device_index != cur:
         raise ValueError(f"stream is on device {stream.device_index}, the current device is {cur}")
-    for t in operands:
-        if t is not None and t.is_cuda and t.get_device() != cur:
-            raise ValueError(f"an operand is on {t.device}, the current device is {cur}")
+    return cur
 
 
-def _empty(shape, dtype, device, stream=None) -> torch.Tensor:
+def _refuse(t, name: str, shape, dtype, cur: int):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a GPU (got {t.device})")
+    if t.get_device() != cur:
+        raise ValueError(f"{name} is on {t.device}, the current device is {cur}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    raise ValueError(f"{name} must be contiguous")
+
+
+def _need(t, name: str, shape, dtype, cur: int) -> int:
+    """The address of a contiguous operand of this shape and type (None: any) on the current device."""
+    try:
+        ok = t.get_device() == cur and (dtype is None or t.dtype is dtype) and t.shape == shape and t.is_contiguous()
+    except AttributeError:
+        ok = False
+    if not ok:
+        _refuse(t, name, shape, dtype, cur)
+    return t.data_ptr()
+
+
+def _need_opt(t, name: str, shape, dtype, cur: int):
+    return None if t is None else _need(t, name, shape, dtype, cur)
+
+
+def _rows(t, name: str, rows: int, heads: int, dim: int, dtype, cur: int) -> int:
+    """Elements from one token's row of an operand [rows, heads, dim] to the
+    next: rows may lie apart (columns of a fused projection), a row is packed."""
+    shape = (rows, heads, dim)
+    if not isinstance(t, torch.Tensor) or t.get_device() != cur or t.dtype is not dtype or t.shape != shape:
+        _refuse(t, name, shape, dtype, cur)
+    st = t.stride()
+    if rows and ((st[2] != 1 and dim > 1) or (st[1] != dim and heads > 1) or (st[0] < heads * dim and rows > 1)):
+        raise ValueError(f"{name} must have packed [heads, dim] rows that do not overlap")
+    return st[0] if rows > 1 else heads * dim
+
+
+def _dims(t, name: str, dims: str):
+    """The shape of an operand of as many dimensions as `dims` names."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    shape = t.shape
+    if len(shape) != dims.count(",") + 1:
+        raise ValueError(f"{name} must be {dims}, got {list(shape)}")
+    return shape
+
+
+def _empty(like: torch.Tensor, shape, dtype, stream=None) -> torch.Tensor:
     """A new tensor for a launch on `stream`: the allocator reuses its memory in that stream's order."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _pool_shape(k_pool: torch.Tensor, v_pool: torch.Tensor):
@@ -206,69 +260,50 @@ def step_tables(block_tables, seq_lens, new_lens, block_size: int, num_rows: int
     in batch order from cursor on, int64 [1]) and entered in block_tables (int32
     [N, max_blocks], in place).  num_rows: rows of the batch, padding included.
     out: a StepTables to write to; its kv_lens and cursor must not be inputs."""
-    if block_tables.dim() != 2:
-        raise ValueError("block_tables must be [N, max_blocks]")
-    n, mb = block_tables.shape
-    if seq_lens.shape != (n,) or new_lens.shape != (n,):
-        raise ValueError("seq_lens and new_lens must be [N]")
-    if new_blocks is not None and new_blocks.dim() != 1:
-        raise ValueError("new_blocks must be one list")
-    if cursor is not None and cursor.numel() != 1:
-        raise ValueError("cursor must hold one value")
+    n, mb = _dims(block_tables, "block_tables", "[N, max_blocks]")
+    cur = _current(stream)
+    i32, i64 = torch.int32, torch.int64
+    tables = _need(block_tables, "block_tables", (n, mb), i32, cur)
+    lens, new = _need(seq_lens, "seq_lens", (n,), i32, cur), _need(new_lens, "new_lens", (n,), i32, cur)
+    at = _need_opt(cursor, "cursor", (1,), i64, cur)
+    granted, blocks = 0, None
+    if new_blocks is not None:
+        granted, = _dims(new_blocks, "new_blocks", "[blocks]")
+        blocks = _need(new_blocks, "new_blocks", (granted,), i32, cur)
+        if granted == 0:  # none were granted (a NULL list would mean that none are needed)
+            blocks = tables
     if num_rows < 0:
         raise ValueError("num_rows must not be negative")
-    dev = block_tables.device
     if out is None:  # one buffer a type
-        wide = _empty(num_rows + n + 2, torch.int64, dev, stream)
-        narrow = _empty(2 * num_rows + n, torch.int32, dev, stream)
-        slots, cu, end = wide.split((num_rows, n + 1, 1))
-        pos, row, lens = narrow.split((num_rows, num_rows, n))
-        out = StepTables(slots, pos, row, cu, lens, end)
-    elif (out.slot_mapping.shape != (num_rows,) or out.positions.shape != (num_rows,) or out.token_row.shape != (num_rows,)
-          or out.cu_seqlens.shape != (n + 1,) or out.kv_lens.shape != (n,) or out.cursor.shape != (1,)):
-        raise ValueError("out does not match num_rows and the number of sequences")
-    _here(block_tables, seq_lens, new_lens, new_blocks, cursor, *out, stream=stream)
-    granted = 0 if new_blocks is None else new_blocks.shape[0]
-    blocks = _opt(new_blocks, "new_blocks", torch.int32)
-    if new_blocks is not None and granted == 0:  # none were granted (a NULL list would mean: none are needed)
-        blocks = block_tables.data_ptr()
-    _lib.check(_lib.lib().zk_step_tables(
-        _dev(block_tables, "block_tables", torch.int32), n, mb, _dev(seq_lens, "seq_lens", torch.int32),
-        _dev(new_lens, "new_lens", torch.int32), block_size, blocks, granted, _opt(cursor, "cursor", torch.int64),
-        _dev(out.cursor, "out.cursor", torch.int64), _dev(out.slot_mapping, "out.slot_mapping", torch.int64),
-        _dev(out.positions, "out.positions", torch.int32), _dev(out.token_row, "out.token_row", torch.int32), num_rows,
-        _dev(out.cu_seqlens, "out.cu_seqlens", torch.int64), _dev(out.kv_lens, "out.kv_lens", torch.int32),
-        _stream(stream)))
+        # (the views are of memory that nothing else names)
+        slots, cu, end = _empty(block_tables, num_rows + n + 2, i64, stream).unsafe_split_with_sizes((num_rows, n + 1, 1))
+        pos, row, kv = _empty(block_tables, 2 * num_rows + n, i32, stream).unsafe_split_with_sizes((num_rows, num_rows, n))
+        out = StepTables(slots, pos, row, cu, kv, end)
+        p_slots, p_pos, p_row, p_cu, p_kv, p_end = [t.data_ptr() for t in out[:3]] + [cu.data_ptr(), kv.data_ptr(), end.data_ptr()]
+    else:
+        p_slots = _need(out.slot_mapping, "out.slot_mapping", (num_rows,), i64, cur)
+        p_pos, p_row = [_need(t, name, (num_rows,), i32, cur)
+                        for t, name in ((out.positions, "out.positions"), (out.token_row, "out.token_row"))]
+        p_cu, p_kv = _need(out.cu_seqlens, "out.cu_seqlens", (n + 1,), i64, cur), _need(out.kv_lens, "out.kv_lens", (n,), i32, cur)
+        p_end = _need(out.cursor, "out.cursor", (1,), i64, cur)
+    _lib.check(_lib.lib().zk_step_tables(tables, n, mb, lens, new, block_size, blocks, granted, at, p_end, p_slots, p_pos,
+                                         p_row, num_rows, p_cu, p_kv, _stream(stream)))
     return out
 
 
-def _rows(t, name: str, heads: int, dim: int, dtype, rows: int) -> int:
-    """Elements from one token's row of `t` [rows, heads, dim] to the next: rows
-    may lie apart (columns of a fused projection), a row itself is packed."""
-    _dev(t, name, dtype, contiguous=False)
-    if t.dim() != 3 or tuple(t.shape) != (rows, heads, dim):
-        raise ValueError(f"{name} must be [{rows}, {heads}, {dim}], got {tuple(t.shape)}")
-    packed = heads * dim
-    st = t.stride()
-    if rows and ((dim > 1 and st[2] != 1) or (heads > 1 and st[1] != dim) or (rows > 1 and st[0] < packed)):
-        raise ValueError(f"{name} must have packed [heads, dim] rows that do not overlap")
-    return st[0] if rows > 1 else packed
+_FLOAT = (torch.float32, torch.bfloat16)
 
 
-def _rope_operands(q, positions, rope, q_weight, k_weight):
-    """(pointer, ...) of the operands that both rope calls take besides q and k."""
-    t, _, d = q.shape
-    if rope is not None:
-        if rope.dim() != 2 or rope.shape[1] % 2 or rope.shape[1] > d or rope.shape[1] == 0 or rope.shape[0] == 0:
-            raise ValueError(f"rope must be [max_positions, rot_dim] with an even rot_dim of at most {d}")
-        if positions is None or positions.shape != (t,):
-            raise ValueError("positions must be [T]")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and w.shape != (d,):
-            raise ValueError(f"{name} must be [{d}]")
-    return (_opt(q_weight, "q_weight", q.dtype), _opt(k_weight, "k_weight", q.dtype)), (
-        _opt(positions, "positions", torch.int32) if rope is not None else None, _opt(rope, "rope", torch.float32),
-        0 if rope is None else rope.shape[0], 0 if rope is None else rope.shape[1])
+def _rope_operands(positions, rope, q_weight, k_weight, tokens: int, dim: int, dtype, cur: int):
+    """What both rope calls take besides q, k and v: ((weights), (positions, table, its rows, rot_dim))."""
+    weights = (_need_opt(q_weight, "q_weight", (dim,), dtype, cur), _need_opt(k_weight, "k_weight", (dim,), dtype, cur))
+    if rope is None:
+        return weights, (None, None, 0, 0)
+    most, rot = _dims(rope, "rope", "[max_positions, rot_dim]")
+    if rot % 2 or rot > dim or rot == 0 or most == 0:
+        raise ValueError(f"rope must be [max_positions, rot_dim] with an even rot_dim of at most {dim}")
+    return weights, (_need(positions, "positions", (tokens,), torch.int32, cur),
+                     _need(rope, "rope", (most, rot), torch.float32, cur), most, rot)
 
 
 def qk_norm_rope_append(k_pool, v_pool, q, k, v, positions, slot_mapping, rope, q_weight=None, k_weight=None,
@@ -278,78 +313,67 @@ def qk_norm_rope_append(k_pool, v_pool, q, k, v, positions, slot_mapping, rope, 
     resulting K rows and of v at slot_mapping, in one launch: returns q_out
     (which may be q).  q, k and v may be columns of one fused projection output;
     K is rounded once, to the pool's type."""
-    nb, hkv, bs, d = _pool_shape(k_pool, v_pool)
-    if q.dim() != 3 or q.shape[2] != d:
-        raise ValueError(f"q must be [T, H, {d}]")
-    t, h, _ = q.shape
-    if q.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError("q must be float32 or bfloat16")
-    if slot_mapping.shape != (t,):
-        raise ValueError("slot_mapping must be [T]")
-    if token_row is not None and token_row.shape != (t,):
-        raise ValueError("token_row must be [T]")
-    for name, sc in (("k_scales", k_scales), ("v_scales", v_scales)):
-        if sc is not None and (sc.dim() != 2 or sc.shape[1] != hkv):
-            raise ValueError(f"{name} must be [sequences, {hkv}]")
+    nb, hkv, bs, d = pool = _dims(k_pool, "k_pool", "[num_blocks, Hkv, block_size, D]")
+    t, h, _ = _dims(q, "q", "[T, H, D]")
+    dt = q.dtype
+    if dt not in _FLOAT:
+        raise TypeError(f"q must be float32 or bfloat16, got {dt}")
+    cur = _current(stream)
+    qs, ks, vs = _rows(q, "q", t, h, d, dt, cur), _rows(k, "k", t, hkv, d, dt, cur), _rows(v, "v", t, hkv, d, dt, cur)
     if q_out is None:
-        q_out = _empty((t, h, d), q.dtype, q.device, stream)
-    qs, ks, vs = _rows(q, "q", h, d, q.dtype, t), _rows(k, "k", hkv, d, q.dtype, t), _rows(v, "v", hkv, d, q.dtype, t)
-    os_ = _rows(q_out, "q_out", h, d, q.dtype, t)
-    weights, table = _rope_operands(q, positions, rope, q_weight, k_weight)
-    _here(k_pool, v_pool, q, k, v, positions, slot_mapping, rope, q_weight, k_weight, q_out, k_scales, v_scales, token_row,
-          stream=stream)
+        q_out, os_ = _empty(q, (t, h, d), dt, stream), 0
+    else:
+        os_ = _rows(q_out, "q_out", t, h, d, dt, cur)
+    weights, table = _rope_operands(positions, rope, q_weight, k_weight, t, d, dt, cur)
+    scales = (None, None, None)
+    if k_scales is not None or v_scales is not None or token_row is not None:
+        seqs, _ = _dims(k_scales, "k_scales", "[sequences, Hkv]")
+        scales = (_need(k_scales, "k_scales", (seqs, hkv), torch.float32, cur),
+                  _need(v_scales, "v_scales", (seqs, hkv), torch.float32, cur),
+                  _need(token_row, "token_row", (t,), torch.int32, cur))
+    kind = k_pool.dtype
     _lib.check(_lib.lib().zk_qk_norm_rope_append(
-        _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool"), zk_dtype(k_pool), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(),
-        vs, zk_dtype(q), t, h, hkv, d, *weights, float(eps), *table, int(bool(interleaved)), q_out.data_ptr(), os_,
-        _dev(slot_mapping, "slot_mapping", torch.int64), bs, nb, _opt(k_scales, "k_scales", torch.float32),
-        _opt(v_scales, "v_scales", torch.float32), _opt(token_row, "token_row", torch.int32), _stream(stream)))
+        _need(k_pool, "k_pool", pool, kind, cur), _need(v_pool, "v_pool", pool, kind, cur), zk_dtype(k_pool), q.data_ptr(),
+        qs, k.data_ptr(), ks, v.data_ptr(), vs, _ZK_DTYPES[dt], t, h, hkv, d, *weights, eps, *table, interleaved,
+        q_out.data_ptr(), os_, _need(slot_mapping, "slot_mapping", (t,), torch.int64, cur), bs, nb, *scales,
+        _stream(stream)))
     return q_out
-
-
-def _bounds_shape(bounds):
-    if bounds.dim() != 4 or bounds.shape[2] != 2:
-        raise ValueError("bounds must be [num_blocks, Hkv, 2, D]")
-    nb, hkv, _, d = bounds.shape
-    return nb, hkv, d
 
 
 def page_bounds(k_pool, slot_mapping, bounds, stream=None) -> None:
     """Bring the pages' key bounds ([num_blocks, Hkv, 2, D]: smallest, then
     largest, of the pool's type) up to date behind a write of K at slot_mapping
     (int64 [T]); the rows of one page are consecutive (zk_page_bounds)."""
-    if k_pool.dim() != 4:
-        raise ValueError("k_pool must be [num_blocks, Hkv, block_size, D]")
-    nb, hkv, bs, d = k_pool.shape
-    if tuple(bounds.shape) != (nb, hkv, 2, d) or zk_dtype(bounds) != zk_dtype(k_pool):
-        raise ValueError(f"bounds must be [{nb}, {hkv}, 2, {d}] of the pool's type")
-    if slot_mapping.dim() != 1:
-        raise ValueError("slot_mapping must be [T]")
-    _here(k_pool, slot_mapping, bounds, stream=stream)
+    nb, hkv, bs, d = pool = _dims(k_pool, "k_pool", "[num_blocks, Hkv, block_size, D]")
+    rows, = _dims(slot_mapping, "slot_mapping", "[T]")
+    cur = _current(stream)
+    kind = k_pool.dtype
     _lib.check(_lib.lib().zk_page_bounds(
-        _dev(k_pool, "k_pool"), zk_dtype(k_pool), _dev(slot_mapping, "slot_mapping", torch.int64), slot_mapping.shape[0],
-        hkv, d, bs, nb, _dev(bounds, "bounds"), _stream(stream)))
+        _need(k_pool, "k_pool", pool, kind, cur), zk_dtype(k_pool),
+        _need(slot_mapping, "slot_mapping", (rows,), torch.int64, cur), rows, hkv, d, bs, nb,
+        _need(bounds, "bounds", (nb, hkv, 2, d), kind, cur), _stream(stream)))
 
 
 def page_scores(q, bounds, block_tables, seq_lens, block_size: int, mapping="grouped", out=None, stream=None):
     """An upper bound of q . k over each page's keys and the heads of a kv-head
     (zk_page_scores): q [N, H, D], scores f32 [N, Hkv, max_blocks], -inf behind
     the length."""
-    nb, hkv, d = _bounds_shape(bounds)
-    if q.dim() != 3 or q.shape[2] != d:
-        raise ValueError(f"q must be [N, H, {d}]")
-    n, h, _ = q.shape
-    if block_tables.dim() != 2 or block_tables.shape[0] != n or seq_lens.shape != (n,):
-        raise ValueError("block_tables must be [N, max_blocks] and seq_lens [N]")
-    mb = block_tables.shape[1]
+    shape = _dims(bounds, "bounds", "[num_blocks, Hkv, 2, D]")
+    nb, hkv, two, d = shape
+    if two != 2:
+        raise ValueError("bounds must be [num_blocks, Hkv, 2, D]")
+    n, h, _ = _dims(q, "q", "[N, H, D]")
+    _, mb = _dims(block_tables, "block_tables", "[N, max_blocks]")
+    cur = _current(stream)
     if out is None:
-        out = _empty((n, hkv, mb), torch.float32, q.device, stream)
-    elif tuple(out.shape) != (n, hkv, mb):
-        raise ValueError(f"out must be [{n}, {hkv}, {mb}]")
-    _here(q, bounds, block_tables, seq_lens, out, stream=stream)
+        out = _empty(q, (n, hkv, mb), torch.float32, stream)
+        scores = out.data_ptr()
+    else:
+        scores = _need(out, "out", (n, hkv, mb), torch.float32, cur)
     _lib.check(_lib.lib().zk_page_scores(
-        _dev(q, "q"), zk_dtype(q), _dev(bounds, "bounds"), zk_dtype(bounds),
-        _dev(block_tables, "block_tables", torch.int32), _dev(seq_lens, "seq_lens", torch.int32),
-        _dev(out, "out", torch.float32), n, h, hkv, d, block_size, mb, nb, _MAPPINGS[mapping], _stream(stream)))
+        _need(q, "q", (n, h, d), None, cur), zk_dtype(q), _need(bounds, "bounds", shape, None, cur), zk_dtype(bounds),
+        _need(block_tables, "block_tables", (n, mb), torch.int32, cur), _need(seq_lens, "seq_lens", (n,), torch.int32, cur),
+        scores, n, h, hkv, d, block_size, mb, nb, _MAPPINGS[mapping], _stream(stream)))
     return out
 
 
@@ -357,17 +381,18 @@ def select_pages(scores, seq_lens, block_size: int, num_pages: int, sink: int = 
     """The num_pages best pages of each (sequence, kv-head) in ascending order
     (int32 [N, Hkv, num_pages], then -1), the first `sink` and last `recent` held
     ones always among them; equal scores: the lower page (zk_select_pages)."""
-    if scores.dim() != 3 or seq_lens.shape != (scores.shape[0],):
-        raise ValueError("scores must be [N, Hkv, max_blocks] and seq_lens [N]")
-    n, hkv, mb = scores.shape
+    n, hkv, mb = shape = _dims(scores, "scores", "[N, Hkv, max_blocks]")
+    if num_pages <= 0:
+        raise ValueError("num_pages must be positive")
+    cur = _current(stream)
     if out is None:
-        out = _empty((n, hkv, num_pages), torch.int32, scores.device, stream)
-    elif tuple(out.shape) != (n, hkv, num_pages):
-        raise ValueError(f"out must be [{n}, {hkv}, {num_pages}]")
-    _here(scores, seq_lens, out, stream=stream)
+        out = _empty(scores, (n, hkv, num_pages), torch.int32, stream)
+        pages = out.data_ptr()
+    else:
+        pages = _need(out, "out", (n, hkv, num_pages), torch.int32, cur)
     _lib.check(_lib.lib().zk_select_pages(
-        _dev(scores, "scores", torch.float32), _dev(seq_lens, "seq_lens", torch.int32), n, hkv, mb, block_size, num_pages,
-        sink, recent, _dev(out, "out", torch.int32), _stream(stream)))
+        _need(scores, "scores", shape, torch.float32, cur), _need(seq_lens, "seq_lens", (n,), torch.int32, cur), n, hkv, mb,
+        block_size, num_pages, sink, recent, pages, _stream(stream)))
     return out
 
 
@@ -380,35 +405,33 @@ def paged_decode_sparse(q, k_pool, v_pool, block_tables, seq_lens, pages, scale=
     """paged_decode over listed pages only: pages int32 [N, Hkv, K] holds indices
     into each sequence's block table (negative: none), as select_pages gives
     them; returns out [N, H, D] (zk_paged_decode_sparse)."""
-    nb, hkv, bs, d = _pool_shape(k_pool, v_pool)
-    if q.dim() != 3 or q.shape[2] != d:
-        raise ValueError(f"q must be [N, H, {d}]")
-    n, h, _ = q.shape
-    if block_tables.dim() != 2 or block_tables.shape[0] != n or seq_lens.shape != (n,):
-        raise ValueError("block_tables must be [N, max_blocks] and seq_lens [N]")
-    if pages.dim() != 3 or tuple(pages.shape[:2]) != (n, hkv):
-        raise ValueError(f"pages must be [N, {hkv}, num_pages]")
-    for name, sc in (("k_scales", k_scales), ("v_scales", v_scales)):
-        if sc is not None and tuple(sc.shape) != (n, hkv):
-            raise ValueError(f"{name} must be [N, {hkv}]")
-    mb, np_ = block_tables.shape[1], pages.shape[2]
+    nb, hkv, bs, d = pool = _dims(k_pool, "k_pool", "[num_blocks, Hkv, block_size, D]")
+    n, h, _ = _dims(q, "q", "[N, H, D]")
+    _, mb = _dims(block_tables, "block_tables", "[N, max_blocks]")
+    _, _, np_ = _dims(pages, "pages", "[N, Hkv, num_pages]")
+    cur = _current(stream)
     if scale is None:
         scale = 1.0 / math.sqrt(d)
+    dt = q.dtype
     if out is None:
-        out = _empty(q.shape, q.dtype, q.device, stream)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError("out must match q")
-    if workspace is None:
-        need = sparse_workspace_bytes(n, h, hkv, d, np_)
-        workspace = _empty(need, torch.uint8, q.device, stream) if need else None
-    _here(q, k_pool, v_pool, block_tables, seq_lens, pages, out, workspace, k_scales, v_scales, stream=stream)
+        out = _empty(q, (n, h, d), dt, stream)
+        dst = out.data_ptr()
+    else:
+        dst = _need(out, "out", (n, h, d), dt, cur)
+    need = _lib.lib().zk_paged_decode_sparse_workspace_size(n, h, hkv, d, np_) if workspace is None else 0
+    if need:
+        workspace = _empty(q, need, torch.uint8, stream)
+    ws = (None, 0)
+    if workspace is not None:  # (its size is checked by the call)
+        ws = (_need(workspace, "workspace", workspace.shape, None, cur), workspace.numel() * workspace.element_size())
+    kind = k_pool.dtype
     _lib.check(_lib.lib().zk_paged_decode_sparse(
-        _dev(q, "q"), zk_dtype(q), _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool"), zk_dtype(k_pool), _dev(out, "out"),
-        _dev(block_tables, "block_tables", torch.int32), _dev(seq_lens, "seq_lens", torch.int32),
-        _dev(pages, "pages", torch.int32), np_, n, h, hkv, d, bs, mb, nb, float(scale), _MAPPINGS[mapping],
-        _opt(k_scales, "k_scales", torch.float32), _opt(v_scales, "v_scales", torch.float32),
-        None if workspace is None else _dev(workspace, "workspace"),
-        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(stream)))
+        _need(q, "q", (n, h, d), dt, cur), zk_dtype(q), _need(k_pool, "k_pool", pool, kind, cur),
+        _need(v_pool, "v_pool", pool, kind, cur), zk_dtype(k_pool), dst,
+        _need(block_tables, "block_tables", (n, mb), torch.int32, cur), _need(seq_lens, "seq_lens", (n,), torch.int32, cur),
+        _need(pages, "pages", (n, hkv, np_), torch.int32, cur), np_, n, h, hkv, d, bs, mb, nb, scale, _MAPPINGS[mapping],
+        _need_opt(k_scales, "k_scales", (n, hkv), torch.float32, cur),
+        _need_opt(v_scales, "v_scales", (n, hkv), torch.float32, cur), *ws, _stream(stream)))
     return out
 
 
