@@ -54,6 +54,11 @@ __device__ __forceinline__ float load_q(const SparseArgs &a, size_t i) {
     return a.q_f32 ? ((const float *)a.q)[i] : __uint_as_float((uint32_t)((const uint16_t *)a.q)[i] << 16);
 }
 
+__device__ __forceinline__ void store_out(const SparseArgs &a, size_t i, float x) {
+    if (a.q_f32) ((float *)a.out)[i] = x;
+    else ((uint16_t *)a.out)[i] = (uint16_t)f32_to_bf16_bits(x);
+}
+
 // The entries of this workgroup's part of list (n, kvh) that add something, in
 // list order: their blocks and how many of a page's tokens lie below the
 // length.  Returns their number.  All threads of the workgroup.
@@ -100,10 +105,11 @@ __device__ __forceinline__ int stage_list(const SparseArgs &a, int n, int kvh, i
 }
 
 // ------------------------------------------------------------ MFMA kernel
-// bf16 and fp8 pools, 16-token pages, D in {64, 128}, G in {1, 2, 4, 8, 16}: one
-// workgroup of four waves per (kv-head, sequence, split).  A wave takes every
-// fourth pair of the staged pages; K and V go from memory straight into the
-// lanes that feed the matrix cores, one pair ahead of the one being computed:
+// 16-token pages, D in {64, 96, 128, 256}, up to 16 heads a kv-head: one workgroup
+// of four waves per (kv-head, sequence, split).  A wave takes every fourth step of the
+// staged pages (a step is a pair of bf16 or fp8 pages, one f32 page); K and V go
+// from memory straight into the lanes that feed the matrix cores, no LDS in the
+// loop:
 //   QK^T  v_mfma_f32_16x16x32_bf16, A = 16 K rows, B = the query heads; lane
 //         (grp, col) reads 16 bytes of row col a k-step (any order of the dims
 //         will do as long as the query's is the same) and gets tokens
@@ -113,36 +119,79 @@ __device__ __forceinline__ int stage_list(const SparseArgs &a, int n, int kvh, i
 //         token 4 grp + e % 4 of page e / 4), and lane (grp, col) reads D / 16
 //         consecutive dims of tokens 4 grp + i, whole rows by 16 lanes, which
 //         v_perm transposes into the D / 16 A operands.
-// No LDS in the loop.  The reference maximum of a head is moved only when a
-// score exceeds it by kSlack.  The waves' results are merged in LDS.
+// f32 pools: v_mfma_f32_16x16x4_f32, four k-steps a 16-byte chunk of K, one a
+// token of PV.
+// The reference maximum of a head is moved only when a score exceeds it by
+// kSlack.  The waves' results are merged in LDS.
+//
+// 256 contexts, 64 pages of each, 32 / 8 heads of 128 bf16 (1048 MB): 169 us, 6.2
+// TB/s (a read of one piece reaches 7.5, one of shuffled 4 KB pieces 7 % less).
+// One step ahead in registers needs 208 of them, two waves a SIMD, and took 179; the
+// 128 registers of four waves a SIMD spill, 215.
 constexpr int kWaves = 4;
 constexpr float kSlack = 8.0f;
 
-template <int KV, int D, int G>
+// The `BYTES` bytes at p (nontemporal), in the widest pieces that their number allows.
+template <int BYTES>
+__device__ __forceinline__ void load_words(const char *p, uint32_t *w) {
+    if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+        for (int j = 0; j < BYTES / 16; ++j) {
+            const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 16 * j));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[4 * j + e] = v[e];
+        }
+    } else if constexpr (BYTES % 8 == 0) {
+#pragma unroll
+        for (int j = 0; j < BYTES / 8; ++j) {
+            const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(p + 8 * j));
+            w[2 * j] = v[0];
+            w[2 * j + 1] = v[1];
+        }
+    } else if constexpr (BYTES % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < BYTES / 4; ++j) w[j] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p + 4 * j));
+    } else {
+        static_assert(BYTES == 6, "6 bytes: fp8 rows of 96");
+        const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+        w[0] = (uint32_t)__builtin_nontemporal_load(h) | (uint32_t)__builtin_nontemporal_load(h + 1) << 16;
+        w[1] = __builtin_nontemporal_load(h + 2);
+    }
+}
+
+template <int KV, int D>
 __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) {
-    constexpr int BS = 16, ELT = KV == ZK_BF16 ? 2 : 1, RB = D * ELT;
-    constexpr int KK = D / 32;                 // MFMA k-steps
-    constexpr int KC = RB / 64;                // 16-byte chunks of a K row a lane
+    constexpr bool F32 = KV == ZK_F32;
+    constexpr int BS = 16, ELT = F32 ? 4 : KV == ZK_BF16 ? 2 : 1, RB = D * ELT;
+    constexpr int PG = F32 ? 1 : 2;            // pages a step
+    constexpr int CB = RB % 64 ? 8 : 16;       // bytes of a K row that a lane reads at once
+    constexpr int KC = RB / (4 * CB);          // ... and how often
+    constexpr int KK = F32 ? KC : D / 32;      // query pieces: 4 f32, 8 bf16 dims
     constexpr int DT = D / 16, VB = DT * ELT;  // dims and bytes of a V row a lane
-    constexpr int VW = VB / 4;
+    constexpr int VW = (VB + 3) / 4;
+    static_assert(DT % 2 == 0 && (CB == 16 || KV == ZK_FP8_E4M3), "row shape");
     constexpr size_t PAGE = (size_t)BS * RB;
     __shared__ int32_t blk[kMaxList], cnt[kMaxList];
     __shared__ int wave_sum[kWaves];
-    __shared__ float mo[kWaves][G][D + 4], mm[kWaves][G], mlsum[kWaves][G];
+    __shared__ float mo[kWaves][kMaxG * (D + 4)], mm[kWaves][kMaxG], mlsum[kWaves][kMaxG];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
     const int kvh = blockIdx.x, split = blockIdx.y, n = blockIdx.z;
     const int np = stage_list<kWaves>(a, n, kvh, split, blk, cnt, wave_sum);
-    const int H = a.num_heads;
-    // query fragments: k-step kk of bf16 rows holds dims 32 kk + 8 grp .. + 7,
-    // of fp8 rows (16 dims in 16 bytes) dims 64 (kk / 2) + 16 grp + 8 (kk % 2) .. + 7
-    bf16x8 qf[KK];
+    const int H = a.num_heads, G = H / a.num_kv_heads;
+    // query pieces, as the lanes read K: bf16 rows (and fp8 ones read 8 bytes at
+    // once): dims 32 kk + 8 grp .. + 7; fp8 rows (16 dims in 16 bytes): 64 (kk / 2) +
+    // 16 grp + 8 (kk % 2) .. + 7; f32 rows: 16 kk + 4 grp .. + 3
+    u32x4 qf[KK];
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-        const int d0 = KV == ZK_BF16 ? 32 * kk + 8 * grp : 64 * (kk / 2) + 16 * grp + 8 * (kk % 2);
+        const int d0 = F32 ? 16 * kk + 4 * grp : KV == ZK_BF16 || CB == 8 ? 32 * kk + 8 * grp : 64 * (kk / 2) + 16 * grp + 8 * (kk % 2);
         u32x4 w = {0u, 0u, 0u, 0u};
         if (col < G) {
             const size_t at = ((size_t)n * H + qhead_of(a, kvh, col, G)) * D + d0;
-            if (a.q_f32) {
+            if constexpr (F32) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(load_q(a, at + j));
+            } else if (a.q_f32) {
                 const float *p = (const float *)a.q + at;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[j] = bf16x2_rne(p[2 * j], p[2 * j + 1]);
@@ -150,74 +199,72 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
                 w = *reinterpret_cast<const u32x4 *>((const uint16_t *)a.q + at);
             }
         }
-        qf[kk] = __builtin_bit_cast(bf16x8, w);
+        qf[kk] = w;
     }
     float sl2 = a.scale_log2, vscale = 1.0f;
     if constexpr (KV == ZK_FP8_E4M3) {
         sl2 *= a.k_scales[(size_t)n * a.num_kv_heads + kvh];
         vscale = a.v_scales[(size_t)n * a.num_kv_heads + kvh];
     }
-    const char *kbase = a.k_pool + (size_t)kvh * PAGE + (size_t)col * RB + grp * 16;
+    const char *kbase = a.k_pool + (size_t)kvh * PAGE + (size_t)col * RB + grp * CB;
     const char *vbase = a.v_pool + (size_t)kvh * PAGE + (size_t)(4 * grp) * RB + col * VB;
     const size_t block_bytes = PAGE * a.num_kv_heads;
 
-    struct Pair {
-        u32x4 k[2][KC];
-        uint32_t v[2][4][VW];
-        int cnt[2];
-    };
-    auto load = [&](int pair, Pair &r) {  // pair: of this list; past its end the last page again, with no tokens
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int i = min(2 * pair + h, np - 1);
-            const int b = __builtin_amdgcn_readfirstlane(blk[i]);
-            r.cnt[h] = 2 * pair + h < np ? __builtin_amdgcn_readfirstlane(cnt[i]) : 0;
-            const char *kp = kbase + (size_t)b * block_bytes, *vp = vbase + (size_t)b * block_bytes;
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-                r.k[h][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kp + 64 * c));
-#pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) {
-                if constexpr (VB == 16) {
-                    const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vp + i2 * RB));
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) r.v[h][i2][j] = w[j];
-                } else if constexpr (VB == 8) {
-                    const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(vp + i2 * RB));
-                    r.v[h][i2][0] = w[0];
-                    r.v[h][i2][1] = w[1];
-                } else {
-                    r.v[h][i2][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(vp + i2 * RB));
-                }
-            }
-        }
-    };
     f32x4 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -FLT_MAX, l = 0.0f;
-    auto compute = [&](const Pair &r) {
-        float sc[2][4];
+    const int steps = (np + PG - 1) / PG;
+    for (int step = wave; step < steps; step += kWaves) {
+        uint32_t kw[PG][KC][CB / 4];
+        uint32_t vw[PG][4][VW];
+        int tokens[PG];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < PG; ++h) {  // (an odd list's last page again, without tokens)
+            const int i = min(PG * step + h, np - 1);
+            const int b = __builtin_amdgcn_readfirstlane(blk[i]);
+            tokens[h] = PG * step + h < np ? __builtin_amdgcn_readfirstlane(cnt[i]) : 0;
+            const char *kp = kbase + (size_t)b * block_bytes, *vp = vbase + (size_t)b * block_bytes;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) load_words<CB>(kp + 4 * CB * c, kw[h][c]);
+#pragma unroll
+            for (int i2 = 0; i2 < 4; ++i2) load_words<VB>(vp + i2 * RB, vw[h][i2]);
+        }
+        float sc[PG][4];
+#pragma unroll
+        for (int h = 0; h < PG; ++h) {
             f32x4 s = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (F32) {
+                f32x4 s2 = s;  // two chains
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                u32x4 w;
-                if constexpr (KV == ZK_BF16) {
-                    w = r.k[h][kk];
-                } else {
-                    const u32x2 lo = e4m3x4_to_bf16x4(r.k[h][kk / 2][2 * (kk % 2)]),
-                                hi = e4m3x4_to_bf16x4(r.k[h][kk / 2][2 * (kk % 2) + 1]);
-                    w = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        f32x4 &t = e & 1 ? s2 : s;
+                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[h][c][e]), __uint_as_float(qf[c][e]), t, 0, 0, 0);
+                    }
+                s += s2;
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    u32x4 w;
+                    if constexpr (KV == ZK_BF16) {
+                        w = u32x4{kw[h][kk][0], kw[h][kk][1], kw[h][kk][2], kw[h][kk][3]};
+                    } else {
+                        const uint32_t *c8 = CB == 8 ? kw[h][kk] : kw[h][kk / 2] + 2 * (kk % 2);
+                        const u32x2 lo = e4m3x4_to_bf16x4(c8[0]), hi = e4m3x4_to_bf16x4(c8[1]);
+                        w = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                    }
+                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w),
+                                                                __builtin_bit_cast(bf16x8, qf[kk]), s, 0, 0, 0);
                 }
-                s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), qf[kk], s, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[h][i] = 4 * grp + i < r.cnt[h] ? s[i] * sl2 : -INFINITY;
+            for (int i = 0; i < 4; ++i) sc[h][i] = 4 * grp + i < tokens[h] ? s[i] * sl2 : -INFINITY;
         }
-        const float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                               fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+        float mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < PG; ++h) mx = fmaxf(mx, fmaxf(fmaxf(sc[h][0], sc[h][1]), fmaxf(sc[h][2], sc[h][3])));
         if (__builtin_amdgcn_ballot_w64(mx > m + kSlack)) {
             float cm = fmaxf(mx, xor16(mx));
             cm = fmaxf(cm, xor32(cm));
@@ -228,70 +275,66 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
             for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
             m = m_new;
         }
-        u32x4 pw;
+        float pr[PG][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float p[4];
+        for (int h = 0; h < PG; ++h) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = exp2_fast(sc[h][i] - m);
-            l += (p[0] + p[1]) + (p[2] + p[3]);
-            pw[2 * h] = bf16x2_rne(p[0], p[1]);
-            pw[2 * h + 1] = bf16x2_rne(p[2], p[3]);
-        }
-        // V rows as bf16 pairs: vw[h][i][j] = dims (2 j, 2 j + 1) of token 4 grp + i
-        uint32_t vw[2][4][DT / 2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (KV == ZK_BF16) {
-#pragma unroll
-                    for (int j = 0; j < DT / 2; ++j) vw[h][i][j] = r.v[h][i][j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < DT / 4; ++j) {
-                        const u32x2 c2 = e4m3x4_to_bf16x4(r.v[h][i][j]);
-                        vw[h][i][2 * j] = c2[0];
-                        vw[h][i][2 * j + 1] = c2[1];
-                    }
-                }
-            }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (r.cnt[h] < BS) {  // what lies behind the length must not reach O
+            for (int i = 0; i < 4; ++i) pr[h][i] = exp2_fast(sc[h][i] - m);
+            l += (pr[h][0] + pr[h][1]) + (pr[h][2] + pr[h][3]);
+            if (tokens[h] < BS) {  // what lies behind the length must not reach O
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (4 * grp + i >= r.cnt[h])
+                    if (4 * grp + i >= tokens[h])
 #pragma unroll
-                        for (int j = 0; j < DT / 2; ++j) vw[h][i][j] = 0u;
+                        for (int j = 0; j < VW; ++j) vw[h][i][j] = 0u;
             }
-        const bf16x8 pb = __builtin_bit_cast(bf16x8, pw);
+        }
+        if constexpr (F32) {
 #pragma unroll
-        for (int j = 0; j < DT / 2; ++j) {
-            u32x4 ev, od;
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                ev[2 * h] = __builtin_amdgcn_perm(vw[h][1][j], vw[h][0][j], 0x05040100u);
-                ev[2 * h + 1] = __builtin_amdgcn_perm(vw[h][3][j], vw[h][2][j], 0x05040100u);
-                od[2 * h] = __builtin_amdgcn_perm(vw[h][1][j], vw[h][0][j], 0x07060302u);
-                od[2 * h + 1] = __builtin_amdgcn_perm(vw[h][3][j], vw[h][2][j], 0x07060302u);
+                for (int dt = 0; dt < DT; ++dt)
+                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vw[0][i][dt]), pr[0][i], o[dt], 0, 0, 0);
+        } else {
+            // V rows as bf16 pairs: vb[h][i][j] = dims (2 j, 2 j + 1) of token 4 grp + i
+            uint32_t vb[PG][4][DT / 2];
+#pragma unroll
+            for (int h = 0; h < PG; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < VW; ++j) {
+                        if constexpr (KV == ZK_BF16) {
+                            vb[h][i][j] = vw[h][i][j];
+                        } else {
+                            const u32x2 c2 = e4m3x4_to_bf16x4(vw[h][i][j]);
+                            vb[h][i][2 * j] = c2[0];
+                            if (2 * j + 1 < DT / 2) vb[h][i][2 * j + 1] = c2[1];
+                        }
+                    }
+            u32x4 pw;
+#pragma unroll
+            for (int h = 0; h < PG; ++h) {
+                pw[2 * h] = bf16x2_rne(pr[h][0], pr[h][1]);
+                pw[2 * h + 1] = bf16x2_rne(pr[h][2], pr[h][3]);
             }
-            o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ev), pb, o[2 * j], 0, 0, 0);
-            o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, od), pb, o[2 * j + 1], 0, 0, 0);
+            const bf16x8 pb = __builtin_bit_cast(bf16x8, pw);
+#pragma unroll
+            for (int j = 0; j < DT / 2; ++j) {
+                u32x4 ev, od;
+#pragma unroll
+                for (int h = 0; h < PG; ++h) {
+                    ev[2 * h] = __builtin_amdgcn_perm(vb[h][1][j], vb[h][0][j], 0x05040100u);
+                    ev[2 * h + 1] = __builtin_amdgcn_perm(vb[h][3][j], vb[h][2][j], 0x05040100u);
+                    od[2 * h] = __builtin_amdgcn_perm(vb[h][1][j], vb[h][0][j], 0x07060302u);
+                    od[2 * h + 1] = __builtin_amdgcn_perm(vb[h][3][j], vb[h][2][j], 0x07060302u);
+                }
+                o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ev), pb, o[2 * j], 0, 0, 0);
+                o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, od), pb, o[2 * j + 1], 0, 0, 0);
+            }
         }
-    };
-    const int pairs = (np + 1) / 2;
-    if (wave < pairs) {
-        Pair r0, r1;
-        load(wave, r0);
-        int j = wave;
-        for (; j + kWaves < pairs; j += 2 * kWaves) {
-            load(j + kWaves, r1);
-            compute(r0);
-            load(min(j + 2 * kWaves, pairs), r0);  // (pair `pairs`: the last page again)
-            compute(r1);
-        }
-        if (j < pairs) compute(r0);
+    }
+    if (wave < steps) {
         l += xor16(l);
         l += xor32(l);
     } else {
@@ -301,7 +344,8 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) mo[wave][col][DT * (4 * grp + i) + dt] = o[dt][i];
+            for (int dt = 0; dt < DT; ++dt)
+                mo[wave][col * (D + 4) + DT * (4 * grp + i) + dt] = o[dt][i];
         if (grp == 0) {
             mm[wave][col] = m;
             mlsum[wave][col] = l;
@@ -318,13 +362,11 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
         for (int w = 0; w < kWaves; ++w) {
             const float f = mm[w][j] == -INFINITY ? 0.0f : exp2_fast(mm[w][j] - M);
             L += mlsum[w][j] * f;
-            v += mm[w][j] == -INFINITY ? 0.0f : mo[w][j][d] * f;
+            v += mm[w][j] == -INFINITY ? 0.0f : mo[w][j * (D + 4) + d] * f;
         }
         const size_t row = (size_t)n * H + qhead_of(a, kvh, j, G);
         if (a.splits == 1) {
-            const float r = v * inverse_sum(L, M, vscale);
-            if (a.q_f32) ((float *)a.out)[row * D + d] = r;
-            else ((uint16_t *)a.out)[row * D + d] = (uint16_t)f32_to_bf16_bits(r);
+            store_out(a, row * D + d, v * inverse_sum(L, M, vscale));
         } else {
             const size_t slot = row * a.splits + split;
             a.po[slot * D + d] = v * vscale;
@@ -336,7 +378,7 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
 // ------------------------------------------------------------ generic kernel
 // Any pool type and block size, D <= 256, G <= 16: one wave per (kv-head,
 // sequence, split), a token a lane for the scores, a dimension a lane for the
-// sums.
+// sums; GM: the kv-head's heads rounded up to 4, 8 or 16.
 constexpr int kDimSlots = 4;
 
 template <int KV>
@@ -349,24 +391,26 @@ __device__ __forceinline__ float load_kv(const char *pool, size_t i) {
     }
 }
 
-template <int KV>
+template <int KV, int GM>
 __global__ void __launch_bounds__(64) sparse_generic_kernel(SparseArgs a) {
     __shared__ int32_t blk[kMaxList], cnt[kMaxList];
-    __shared__ float q_s[kMaxG * 256], p_s[kMaxG][64];
+    __shared__ float q_s[256][GM], p_s[64][GM];  // a dimension's (token's) heads side by side
     const int lane = threadIdx.x;
     const int kvh = blockIdx.x, split = blockIdx.y, n = blockIdx.z;
     const int D = a.head_dim, G = a.num_heads / a.num_kv_heads, H = a.num_heads;
-    for (int i = lane; i < G * D; i += 64)
-        q_s[i] = load_q(a, ((size_t)n * H + qhead_of(a, kvh, i / D, G)) * D + i % D);
+    for (int i = lane; i < GM * D; i += 64) {  // (heads past G: zeros)
+        const int j = i / D, d = i - j * D;
+        q_s[d][j] = j < G ? load_q(a, ((size_t)n * H + qhead_of(a, kvh, j, G)) * D + d) : 0.0f;
+    }
     const int np = stage_list<1>(a, n, kvh, split, blk, cnt, nullptr);
     float sl2 = a.scale_log2, vs = 1.0f;
     if constexpr (KV == ZK_FP8_E4M3) {
         sl2 *= a.k_scales[(size_t)n * a.num_kv_heads + kvh];
         vs = a.v_scales[(size_t)n * a.num_kv_heads + kvh];
     }
-    float m[kMaxG], l[kMaxG], o[kMaxG][kDimSlots];
+    float m[GM], l[GM], o[GM][kDimSlots];
 #pragma unroll
-    for (int j = 0; j < kMaxG; ++j) {
+    for (int j = 0; j < GM; ++j) {
         m[j] = np ? -FLT_MAX : -INFINITY;
         l[j] = 0.0f;
 #pragma unroll
@@ -379,19 +423,17 @@ __global__ void __launch_bounds__(64) sparse_generic_kernel(SparseArgs a) {
         for (int t0 = 0; t0 < tokens; t0 += 64) {
             const int here = min(64, tokens - t0);
             const bool valid = lane < here;
-            float s[kMaxG];
+            const size_t row = (row0 + t0 + (valid ? lane : 0)) * D;
+            float s[GM];
 #pragma unroll
-            for (int j = 0; j < kMaxG; ++j) s[j] = 0.0f;
-            if (valid)
-                for (int d = 0; d < D; ++d) {
-                    const float kd = load_kv<KV>(a.k_pool, (row0 + t0 + lane) * D + d);
+            for (int j = 0; j < GM; ++j) s[j] = 0.0f;
+            for (int d = 0; d < D; ++d) {
+                const float kd = load_kv<KV>(a.k_pool, row + d);
 #pragma unroll
-                    for (int j = 0; j < kMaxG; ++j)
-                        if (j < G) s[j] = fmaf(q_s[j * D + d], kd, s[j]);
-                }
+                for (int j = 0; j < GM; ++j) s[j] = fmaf(q_s[d][j], kd, s[j]);
+            }
 #pragma unroll
-            for (int j = 0; j < kMaxG; ++j) {
-                if (j >= G) break;
+            for (int j = 0; j < GM; ++j) {
                 const float sj = valid ? s[j] * sl2 : -INFINITY;
                 float mx = sj;
                 for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
@@ -403,77 +445,114 @@ __global__ void __launch_bounds__(64) sparse_generic_kernel(SparseArgs a) {
                 m[j] = m_new;
 #pragma unroll
                 for (int c = 0; c < kDimSlots; ++c) o[j][c] *= alpha;
-                p_s[j][lane] = p;
+                p_s[lane][j] = p;
             }
             __syncthreads();
             for (int i = 0; i < here; ++i) {
-                float vd[kDimSlots];
 #pragma unroll
                 for (int c = 0; c < kDimSlots; ++c) {
                     const int d = lane + c * 64;
-                    vd[c] = d < D ? load_kv<KV>(a.v_pool, (row0 + t0 + i) * D + d) : 0.0f;
-                }
+                    const float v = d < D ? load_kv<KV>(a.v_pool, (row0 + t0 + i) * D + d) : 0.0f;
 #pragma unroll
-                for (int j = 0; j < kMaxG; ++j) {
-                    if (j >= G) break;
-#pragma unroll
-                    for (int c = 0; c < kDimSlots; ++c) o[j][c] = fmaf(p_s[j][i], vd[c], o[j][c]);
+                    for (int j = 0; j < GM; ++j) o[j][c] = fmaf(p_s[i][j], v, o[j][c]);
                 }
             }
             __syncthreads();
         }
     }
 #pragma unroll
-    for (int j = 0; j < kMaxG; ++j) {
-        if (j >= G) break;
-        const size_t row = (size_t)n * H + qhead_of(a, kvh, j, G);
-        const float inv = inverse_sum(l[j], m[j], vs);
+    for (int j = 0; j < GM; ++j) {
+        if (j < G) {
+            const size_t row = (size_t)n * H + qhead_of(a, kvh, j, G);
+            const float inv = inverse_sum(l[j], m[j], vs);
 #pragma unroll
-        for (int c = 0; c < kDimSlots; ++c) {
-            const int d = lane + c * 64;
-            if (d >= D) break;
-            if (a.splits == 1) {
-                const float r = o[j][c] * inv;
-                if (a.q_f32) ((float *)a.out)[row * D + d] = r;
-                else ((uint16_t *)a.out)[row * D + d] = (uint16_t)f32_to_bf16_bits(r);
-            } else {
-                a.po[(row * a.splits + split) * D + d] = o[j][c] * vs;
+            for (int c = 0; c < kDimSlots; ++c) {
+                const int d = lane + c * 64;
+                if (d < D) {
+                    if (a.splits == 1) store_out(a, row * D + d, o[j][c] * inv);
+                    else a.po[(row * a.splits + split) * D + d] = o[j][c] * vs;
+                }
             }
+            if (a.splits > 1 && lane == 0) a.ml[row * a.splits + split] = make_float2(m[j], l[j]);
         }
-        if (a.splits > 1 && lane == 0) a.ml[row * a.splits + split] = make_float2(m[j], l[j]);
     }
 }
 
-// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, in split order: a thread a
-// dimension, the splits' statistics read by all.
-__global__ void sparse_reduce_kernel(SparseArgs a) {
-    const int h = blockIdx.x, n = blockIdx.y, d = threadIdx.x, D = a.head_dim;
+// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s: one workgroup per (head,
+// sequence).  A lane holds a split's statistics (chunks of 64 splits); a thread
+// four dimensions of every (256 / (D / 4))-th split, whose values are loaded
+// before the statistics are used; the parts are added in order.
+constexpr int kReduceThreads = 256;
+__global__ void __launch_bounds__(kReduceThreads) sparse_reduce_kernel(SparseArgs a) {
+    constexpr int U = 4;
+    __shared__ float part[kReduceThreads][5];
+    const int h = blockIdx.x, n = blockIdx.y, D = a.head_dim, S = a.splits, lane = threadIdx.x & 63;
     const size_t row = (size_t)n * a.num_heads + h;
-    const float2 *ml = a.ml + row * a.splits;
-    float M = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[s].x);
-    float L = 0.0f, v = 0.0f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 x = ml[s];
-        if (x.x == -INFINITY) continue;
-        const float f = exp2_fast(x.x - M);
-        L += x.y * f;
-        if (d < D) v += a.po[(row * a.splits + s) * D + d] * f;
+    const float2 *ml = a.ml + row * S;
+    const int quads = (D + 3) / 4, every = kReduceThreads / quads;  // D <= 256
+    const int quad = threadIdx.x % quads, first = threadIdx.x / quads;
+    const bool on = first < every, whole = D % 4 == 0;
+    float M = -INFINITY, L = 0.0f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < S; s0 += 64) {
+        const int here = min(64, S - s0);
+        const float2 x = lane < here ? ml[s0 + lane] : make_float2(-INFINITY, 0.0f);
+        f32x4 p[U];
+        auto load = [&](int s) -> f32x4 {
+            const float *src = a.po + (row * S + s0 + s) * D + 4 * quad;
+            if (whole) return *reinterpret_cast<const f32x4 *>(src);
+            f32x4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (4 * quad + e < D) r[e] = src[e];
+            return r;
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (on && first + u * every < here) p[u] = load(first + u * every);
+        float c = x.x;
+        for (int o = 32; o > 0; o >>= 1) c = fmaxf(c, __shfl_xor(c, o));
+        const float m_new = fmaxf(M, c), alpha = M == -INFINITY ? 0.0f : exp2_fast(M - m_new);
+        const float w = x.x == -INFINITY ? 0.0f : exp2_fast(x.x - m_new);
+        float ls = x.y * w;
+        for (int o = 32; o > 0; o >>= 1) ls += __shfl_xor(ls, o);
+        L = L * alpha + (c == -INFINITY ? 0.0f : ls);
+        M = m_new;
+        v *= alpha;
+        for (int u = 0; u * every < here; ++u) {  // (the same for the workgroup: the shuffle needs every lane)
+            const int s = first + u * every;
+            const float ws = __shfl(w, min(s, 63));
+            if (!on || s >= here || ws == 0.0f) continue;
+            v += ws * (u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2] : u == 3 ? p[3] : load(s));
+        }
     }
-    if (d >= D) return;
-    const float r = v * inverse_sum(L, M);
-    if (a.q_f32) ((float *)a.out)[row * D + d] = r;
-    else ((uint16_t *)a.out)[row * D + d] = (uint16_t)f32_to_bf16_bits(r);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[threadIdx.x][e] = v[e];
+    __syncthreads();
+    if (first == 0) {
+        for (int f = 1; f < every; ++f)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += part[f * quads + quad][e];
+        const float inv = inverse_sum(L, M);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (4 * quad + e < D) store_out(a, row * D + 4 * quad + e, v[e] * inv);
+    }
 }
 
-// Parts of a list: enough workgroups to fill the CUs twice, of at least 16
-// pages each (a wave then has two pairs), at most kMaxList.
-int splits_for(int num_seqs, int num_kv_heads, int num_pages) {
+bool mfma_dim(int head_dim) { return head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256; }
+
+// Parts of a list: enough workgroups to fill the CUs twice (one-wave ones of
+// the generic kernel: four waves a SIMD), of at least 8 (4) pages each and, from 16
+// parts on, 16, at most kMaxList.  us with parts of 8, 16 and 32 pages: 8 lists of
+// 64 bf16 pages 9.6, 10.8, 13.3; 16 of 256 fp8 pages 13.3 (32 parts), 12.0, 13.7.
+int splits_for(int num_seqs, int num_kv_heads, int head_dim, int num_pages) {
     const int64_t rows = (int64_t)num_seqs * num_kv_heads;
-    const int64_t want = (512 + rows - 1) / rows;
-    int64_t s = std::max<int64_t>(1, std::min<int64_t>(want, num_pages / 16));
-    s = std::max<int64_t>(s, (num_pages + kMaxList - 1) / kMaxList);
-    return (int)s;
+    const bool mfma = mfma_dim(head_dim);
+    const int64_t want = ((mfma ? 512 : 4096) + rows - 1) / rows;
+    int64_t s = std::min<int64_t>(want, num_pages / (mfma ? 8 : 4));
+    if (mfma) s = std::min<int64_t>(s, std::max(16, num_pages / 16));
+    return (int)std::max<int64_t>(std::max<int64_t>(s, 1), (num_pages + kMaxList - 1) / kMaxList);
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -488,20 +567,15 @@ int check_launch(const char *what) {
     return ZK_OK;
 }
 
-template <int KV, int D>
-void launch_g(const SparseArgs &a, dim3 grid, int G, hipStream_t s) {
-    switch (G) {
-        case 1: sparse_mfma_kernel<KV, D, 1><<<grid, 64 * kWaves, 0, s>>>(a); break;
-        case 2: sparse_mfma_kernel<KV, D, 2><<<grid, 64 * kWaves, 0, s>>>(a); break;
-        case 4: sparse_mfma_kernel<KV, D, 4><<<grid, 64 * kWaves, 0, s>>>(a); break;
-        case 8: sparse_mfma_kernel<KV, D, 8><<<grid, 64 * kWaves, 0, s>>>(a); break;
-        default: sparse_mfma_kernel<KV, D, 16><<<grid, 64 * kWaves, 0, s>>>(a); break;
-    }
-}
 template <int KV>
-void launch_d(const SparseArgs &a, dim3 grid, int G, hipStream_t s) {
-    if (a.head_dim == 128) launch_g<KV, 128>(a, grid, G, s);
-    else launch_g<KV, 64>(a, grid, G, s);
+void launch(const SparseArgs &a, dim3 grid, int G, bool mfma, hipStream_t s) {
+    if (mfma && a.head_dim == 64) sparse_mfma_kernel<KV, 64><<<grid, 64 * kWaves, 0, s>>>(a);
+    else if (mfma && a.head_dim == 96) sparse_mfma_kernel<KV, 96><<<grid, 64 * kWaves, 0, s>>>(a);
+    else if (mfma && a.head_dim == 128) sparse_mfma_kernel<KV, 128><<<grid, 64 * kWaves, 0, s>>>(a);
+    else if (mfma) sparse_mfma_kernel<KV, 256><<<grid, 64 * kWaves, 0, s>>>(a);
+    else if (G <= 4) sparse_generic_kernel<KV, 4><<<grid, 64, 0, s>>>(a);
+    else if (G <= 8) sparse_generic_kernel<KV, 8><<<grid, 64, 0, s>>>(a);
+    else sparse_generic_kernel<KV, 16><<<grid, 64, 0, s>>>(a);
 }
 
 }  // namespace
@@ -511,7 +585,7 @@ extern "C" {
 size_t zk_paged_decode_sparse_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
                                              int num_pages) {
     if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_pages <= 0) return 0;
-    const int splits = splits_for(num_seqs, num_kv_heads, num_pages);
+    const int splits = splits_for(num_seqs, num_kv_heads, head_dim, num_pages);
     if (splits == 1) return 0;
     const size_t slots = (size_t)num_seqs * num_heads * splits;
     return align256(sizeof(float2) * slots) + sizeof(float) * slots * head_dim;
@@ -532,7 +606,7 @@ int zk_paged_decode_sparse(const void *q, zk_dtype q_dtype, const void *k_pool, 
     if (mapping != ZK_GQA_GROUPED && mapping != ZK_GQA_MODULO) return bad("bad gqa mapping");
     if (head_dim > 256 || num_heads / num_kv_heads > kMaxG) return bad("head_dim <= 256 and H/Hkv <= 16 required");
     if ((int64_t)max_blocks_per_seq * block_size > 0x7fffffff) return bad("context too long");
-    const int splits = num_seqs > 0 ? splits_for(num_seqs, num_kv_heads, num_pages) : 1;
+    const int splits = num_seqs > 0 ? splits_for(num_seqs, num_kv_heads, head_dim, num_pages) : 1;
     if (splits > 65535) return bad("too many pages a list");
     if (num_seqs == 0) return ZK_OK;
     if (!q || !k_pool || !v_pool || !out || !block_tables || !seq_lens || !pages) return bad("NULL pointer");
@@ -573,26 +647,18 @@ int zk_paged_decode_sparse(const void *q, zk_dtype q_dtype, const void *k_pool, 
     a.q_f32 = q_dtype == ZK_F32;
     hipStream_t s = (hipStream_t)stream;
     const dim3 grid(num_kv_heads, splits, num_seqs);
-    const bool mfma = kv_dtype != ZK_F32 && block_size == 16 && (head_dim == 64 || head_dim == 128) &&
-                      (G == 1 || G == 2 || G == 4 || G == 8 || G == 16) &&
+    const bool mfma = block_size == 16 && mfma_dim(head_dim) &&
                       (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15u) == 0;
     {
         KernelTimer timer("sparse_partials", s);
-        if (mfma) {
-            if (kv_dtype == ZK_BF16) launch_d<ZK_BF16>(a, grid, G, s);
-            else launch_d<ZK_FP8_E4M3>(a, grid, G, s);
-        } else if (kv_dtype == ZK_F32) {
-            sparse_generic_kernel<ZK_F32><<<grid, 64, 0, s>>>(a);
-        } else if (kv_dtype == ZK_BF16) {
-            sparse_generic_kernel<ZK_BF16><<<grid, 64, 0, s>>>(a);
-        } else {
-            sparse_generic_kernel<ZK_FP8_E4M3><<<grid, 64, 0, s>>>(a);
-        }
+        if (kv_dtype == ZK_F32) launch<ZK_F32>(a, grid, G, mfma, s);
+        else if (kv_dtype == ZK_BF16) launch<ZK_BF16>(a, grid, G, mfma, s);
+        else launch<ZK_FP8_E4M3>(a, grid, G, mfma, s);
     }
     if (int rc = check_launch("zk_paged_decode_sparse")) return rc;
     if (splits == 1) return ZK_OK;
     KernelTimer timer("sparse_reduce", s);
-    sparse_reduce_kernel<<<dim3(num_heads, num_seqs), (head_dim + 63) / 64 * 64, 0, s>>>(a);
+    sparse_reduce_kernel<<<dim3(num_heads, num_seqs), kReduceThreads, 0, s>>>(a);
     return check_launch("zk_paged_decode_sparse reduce");
 }
 
