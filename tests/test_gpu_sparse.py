@@ -225,7 +225,7 @@ def _select_ref(scores, lens, bs, k, sink, recent):
     return torch.tensor(out)
 
 
-@pytest.mark.parametrize("width", [1, 7, 64, 500, 512, 513, 2048, 2049, 8192, 8193])
+@pytest.mark.parametrize("width", [1, 7, 64, 500, 512, 513, 2048, 2049, 8192, 8193, 33000])
 @pytest.mark.parametrize("k,sink,recent", [(1, 0, 1), (1, 0, 0), (8, 2, 3), (64, 1, 2), (600, 1, 1)])
 def test_selection(width, k, sink, recent):
     from zealot_amd import ops
