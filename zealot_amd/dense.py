@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _current, _dev, _dims, _empty, _rope_operands, _rows, _stream, zk_dtype
+from .ops import _dev, _dims, _empty, _rope_operands, _rows, _stream, _target, zk_dtype
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -117,7 +117,7 @@ def qk_norm_rope(q, k, positions, rope, q_weight=None, k_weight=None, eps: float
     _, hkv, _ = _dims(k, "k", "[T, Hkv, D]")
     dt = q.dtype
     code = _dt(q)
-    cur = _current(stream)
+    cur, at_stream = _target(stream)
     qs, ks = _rows(q, "q", t, h, d, dt, cur), _rows(k, "k", t, hkv, d, dt, cur)
     qo = ko = 0
     if q_out is None:
@@ -131,7 +131,7 @@ def qk_norm_rope(q, k, positions, rope, q_weight=None, k_weight=None, eps: float
     weights, table = _rope_operands(positions, rope, q_weight, k_weight, t, d, dt, cur)
     _lib.check(_lib.lib().zk_qk_norm_rope(
         q.data_ptr(), qs, k.data_ptr(), ks, code, t, h, hkv, d, *weights, eps, *table, interleaved, q_out.data_ptr(), qo,
-        k_out.data_ptr(), ko, _stream(stream)))
+        k_out.data_ptr(), ko, at_stream))
     return q_out, k_out
 
 

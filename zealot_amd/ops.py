@@ -63,15 +63,17 @@ def _opt(t, name, dtype=None):
 # Operands of the calls below _need: one expression a tensor on the way through
 # (0.5 us; a fused norm + rotation + append names 14 of them), the reasons apart.
 
-def _current(stream=None) -> int:
-    """torch's current device, which the launch goes to; `stream` belongs to it."""
-    if _get_device is None or not torch.cuda.is_initialized():
-        cur = torch.cuda.current_device() if torch.cuda.is_available() else -2  # (-1 is a host tensor's)
-    else:
+def _target(stream=None):
+    """(torch's current device, which a launch goes to; the address of its stream, or of `stream`, which belongs to it)."""
+    if stream is None and _raw_stream is not None and _get_device is not None and torch.cuda.is_initialized():
         cur = _get_device()
+        return cur, _raw_stream(cur)
+    if not torch.cuda.is_available():
+        return -2, None  # (-1 is a host tensor's device: every operand is refused)
+    cur = torch.cuda.current_device()
     if stream is not None and stream.device_index != cur:
         raise ValueError(f"stream is on device {stream.device_index}, the current device is {cur}")
-    return cur
+    return cur, _stream(stream)
 
 
 def _refuse(t, name: str, shape, dtype, cur: int):
@@ -107,7 +109,11 @@ def _rows(t, name: str, rows: int, heads: int, dim: int, dtype, cur: int) -> int
     """Elements from one token's row of an operand [rows, heads, dim] to the
     next: rows may lie apart (columns of a fused projection), a row is packed."""
     shape = (rows, heads, dim)
-    if not isinstance(t, torch.Tensor) or t.get_device() != cur or t.dtype is not dtype or t.shape != shape:
+    try:
+        ok = t.get_device() == cur and t.dtype is dtype and t.shape == shape
+    except AttributeError:
+        ok = False
+    if not ok:
         _refuse(t, name, shape, dtype, cur)
     st = t.stride()
     if rows and ((st[2] != 1 and dim > 1) or (st[1] != dim and heads > 1) or (st[0] < heads * dim and rows > 1)):
@@ -261,7 +267,7 @@ def step_tables(block_tables, seq_lens, new_lens, block_size: int, num_rows: int
     [N, max_blocks], in place).  num_rows: rows of the batch, padding included.
     out: a StepTables to write to; its kv_lens and cursor must not be inputs."""
     n, mb = _dims(block_tables, "block_tables", "[N, max_blocks]")
-    cur = _current(stream)
+    cur, at_stream = _target(stream)
     i32, i64 = torch.int32, torch.int64
     tables = _need(block_tables, "block_tables", (n, mb), i32, cur)
     lens, new = _need(seq_lens, "seq_lens", (n,), i32, cur), _need(new_lens, "new_lens", (n,), i32, cur)
@@ -276,10 +282,14 @@ def step_tables(block_tables, seq_lens, new_lens, block_size: int, num_rows: int
         raise ValueError("num_rows must not be negative")
     if out is None:  # one buffer a type
         # (the views are of memory that nothing else names)
-        slots, cu, end = _empty(block_tables, num_rows + n + 2, i64, stream).unsafe_split_with_sizes((num_rows, n + 1, 1))
-        pos, row, kv = _empty(block_tables, 2 * num_rows + n, i32, stream).unsafe_split_with_sizes((num_rows, num_rows, n))
+        wide = _empty(block_tables, num_rows + n + 2, i64, stream)
+        narrow = _empty(block_tables, 2 * num_rows + n, i32, stream)
+        slots, cu, end = wide.unsafe_split_with_sizes((num_rows, n + 1, 1))
+        pos, row, kv = narrow.unsafe_split_with_sizes((num_rows, num_rows, n))
         out = StepTables(slots, pos, row, cu, kv, end)
-        p_slots, p_pos, p_row, p_cu, p_kv, p_end = [t.data_ptr() for t in out[:3]] + [cu.data_ptr(), kv.data_ptr(), end.data_ptr()]
+        p_slots, p_pos = wide.data_ptr(), narrow.data_ptr()
+        p_cu, p_end = p_slots + 8 * num_rows, p_slots + 8 * (num_rows + n + 1)
+        p_row, p_kv = p_pos + 4 * num_rows, p_pos + 8 * num_rows
     else:
         p_slots = _need(out.slot_mapping, "out.slot_mapping", (num_rows,), i64, cur)
         p_pos, p_row = [_need(t, name, (num_rows,), i32, cur)
@@ -287,7 +297,7 @@ def step_tables(block_tables, seq_lens, new_lens, block_size: int, num_rows: int
         p_cu, p_kv = _need(out.cu_seqlens, "out.cu_seqlens", (n + 1,), i64, cur), _need(out.kv_lens, "out.kv_lens", (n,), i32, cur)
         p_end = _need(out.cursor, "out.cursor", (1,), i64, cur)
     _lib.check(_lib.lib().zk_step_tables(tables, n, mb, lens, new, block_size, blocks, granted, at, p_end, p_slots, p_pos,
-                                         p_row, num_rows, p_cu, p_kv, _stream(stream)))
+                                         p_row, num_rows, p_cu, p_kv, at_stream))
     return out
 
 
@@ -318,7 +328,7 @@ def qk_norm_rope_append(k_pool, v_pool, q, k, v, positions, slot_mapping, rope, 
     dt = q.dtype
     if dt not in _FLOAT:
         raise TypeError(f"q must be float32 or bfloat16, got {dt}")
-    cur = _current(stream)
+    cur, at_stream = _target(stream)
     qs, ks, vs = _rows(q, "q", t, h, d, dt, cur), _rows(k, "k", t, hkv, d, dt, cur), _rows(v, "v", t, hkv, d, dt, cur)
     if q_out is None:
         q_out, os_ = _empty(q, (t, h, d), dt, stream), 0
@@ -336,7 +346,7 @@ def qk_norm_rope_append(k_pool, v_pool, q, k, v, positions, slot_mapping, rope, 
         _need(k_pool, "k_pool", pool, kind, cur), _need(v_pool, "v_pool", pool, kind, cur), zk_dtype(k_pool), q.data_ptr(),
         qs, k.data_ptr(), ks, v.data_ptr(), vs, _ZK_DTYPES[dt], t, h, hkv, d, *weights, eps, *table, interleaved,
         q_out.data_ptr(), os_, _need(slot_mapping, "slot_mapping", (t,), torch.int64, cur), bs, nb, *scales,
-        _stream(stream)))
+        at_stream))
     return q_out
 
 
@@ -346,12 +356,12 @@ def page_bounds(k_pool, slot_mapping, bounds, stream=None) -> None:
     (int64 [T]); the rows of one page are consecutive (zk_page_bounds)."""
     nb, hkv, bs, d = pool = _dims(k_pool, "k_pool", "[num_blocks, Hkv, block_size, D]")
     rows, = _dims(slot_mapping, "slot_mapping", "[T]")
-    cur = _current(stream)
+    cur, at_stream = _target(stream)
     kind = k_pool.dtype
     _lib.check(_lib.lib().zk_page_bounds(
         _need(k_pool, "k_pool", pool, kind, cur), zk_dtype(k_pool),
         _need(slot_mapping, "slot_mapping", (rows,), torch.int64, cur), rows, hkv, d, bs, nb,
-        _need(bounds, "bounds", (nb, hkv, 2, d), kind, cur), _stream(stream)))
+        _need(bounds, "bounds", (nb, hkv, 2, d), kind, cur), at_stream))
 
 
 def page_scores(q, bounds, block_tables, seq_lens, block_size: int, mapping="grouped", out=None, stream=None):
@@ -364,7 +374,7 @@ def page_scores(q, bounds, block_tables, seq_lens, block_size: int, mapping="gro
         raise ValueError("bounds must be [num_blocks, Hkv, 2, D]")
     n, h, _ = _dims(q, "q", "[N, H, D]")
     _, mb = _dims(block_tables, "block_tables", "[N, max_blocks]")
-    cur = _current(stream)
+    cur, at_stream = _target(stream)
     if out is None:
         out = _empty(q, (n, hkv, mb), torch.float32, stream)
         scores = out.data_ptr()
@@ -373,7 +383,7 @@ def page_scores(q, bounds, block_tables, seq_lens, block_size: int, mapping="gro
     _lib.check(_lib.lib().zk_page_scores(
         _need(q, "q", (n, h, d), None, cur), zk_dtype(q), _need(bounds, "bounds", shape, None, cur), zk_dtype(bounds),
         _need(block_tables, "block_tables", (n, mb), torch.int32, cur), _need(seq_lens, "seq_lens", (n,), torch.int32, cur),
-        scores, n, h, hkv, d, block_size, mb, nb, _MAPPINGS[mapping], _stream(stream)))
+        scores, n, h, hkv, d, block_size, mb, nb, _MAPPINGS[mapping], at_stream))
     return out
 
 
@@ -384,7 +394,7 @@ def select_pages(scores, seq_lens, block_size: int, num_pages: int, sink: int = 
     n, hkv, mb = shape = _dims(scores, "scores", "[N, Hkv, max_blocks]")
     if num_pages <= 0:
         raise ValueError("num_pages must be positive")
-    cur = _current(stream)
+    cur, at_stream = _target(stream)
     if out is None:
         out = _empty(scores, (n, hkv, num_pages), torch.int32, stream)
         pages = out.data_ptr()
@@ -392,7 +402,7 @@ def select_pages(scores, seq_lens, block_size: int, num_pages: int, sink: int = 
         pages = _need(out, "out", (n, hkv, num_pages), torch.int32, cur)
     _lib.check(_lib.lib().zk_select_pages(
         _need(scores, "scores", shape, torch.float32, cur), _need(seq_lens, "seq_lens", (n,), torch.int32, cur), n, hkv, mb,
-        block_size, num_pages, sink, recent, pages, _stream(stream)))
+        block_size, num_pages, sink, recent, pages, at_stream))
     return out
 
 
@@ -409,7 +419,7 @@ def paged_decode_sparse(q, k_pool, v_pool, block_tables, seq_lens, pages, scale=
     n, h, _ = _dims(q, "q", "[N, H, D]")
     _, mb = _dims(block_tables, "block_tables", "[N, max_blocks]")
     _, _, np_ = _dims(pages, "pages", "[N, Hkv, num_pages]")
-    cur = _current(stream)
+    cur, at_stream = _target(stream)
     if scale is None:
         scale = 1.0 / math.sqrt(d)
     dt = q.dtype
@@ -431,7 +441,7 @@ def paged_decode_sparse(q, k_pool, v_pool, block_tables, seq_lens, pages, scale=
         _need(block_tables, "block_tables", (n, mb), torch.int32, cur), _need(seq_lens, "seq_lens", (n,), torch.int32, cur),
         _need(pages, "pages", (n, hkv, np_), torch.int32, cur), np_, n, h, hkv, d, bs, mb, nb, scale, _MAPPINGS[mapping],
         _need_opt(k_scales, "k_scales", (n, hkv), torch.float32, cur),
-        _need_opt(v_scales, "v_scales", (n, hkv), torch.float32, cur), *ws, _stream(stream)))
+        _need_opt(v_scales, "v_scales", (n, hkv), torch.float32, cur), *ws, at_stream))
     return out
 
 
