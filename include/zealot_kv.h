@@ -355,6 +355,19 @@ int zk_cache_write_batch(zk_kv_cache *c, size_t layer, const char *const *ids,
 int zk_cache_write_batch_qkv(zk_kv_cache *c, size_t layer, const char *const *ids,
                              const int32_t *num_tokens, int n, const void *x, const void *w_qkv,
                              int64_t hidden, int num_heads, void *qkv);
+/* zk_cache_write_batch of rotated keys: head norms and rotary embedding of the
+ * step's q [T, num_heads, D] and k [T, Hkv, D] (zk_qk_norm_rope in
+ * zealot_dense.h: weights, eps, rope table, rot_dim, interleaved, token strides
+ * and overlaps as there) at each token's own position, K and v [T, Hkv, D] into
+ * the pages (copy-on-write first, fp8 scales as set), q into q_out, in one launch.
+ * rot_dim 0: norms alone.  A sequence that would pass max_positions fails with
+ * SequenceTooLong; every check runs before anything is written.  No counterpart
+ * in the reference (cuda_runner.rs:373-406 writes K as projected). */
+int zk_cache_write_batch_rope(zk_kv_cache *c, size_t layer, const char *const *ids, const int32_t *num_tokens, int n,
+                              const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
+                              int64_t v_stride, zk_dtype src_dtype, int num_heads, const void *q_weight,
+                              const void *k_weight, float eps, const float *rope, int64_t max_positions, int rot_dim,
+                              int interleaved, void *q_out, int64_t q_out_stride);
 /* Block tables from the caller's handles: sequence ids[i]'s table becomes
  * blocks[o_i .. o_i + num_blocks[i]) (packed in batch order), registering the
  * sequence on first use.  This is how a scheduler that shares `bm` with the

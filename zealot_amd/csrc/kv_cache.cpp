@@ -34,6 +34,7 @@
 #include <vector>
 
 #include "../../include/zealot_dense.h"
+#include "rope_ops.h"
 #include "zk_common.h"
 
 using zk::set_error;
@@ -521,10 +522,12 @@ struct WritePrep {
     const int64_t *d_slots = nullptr;
     const int32_t *d_rows = nullptr;
     const float *d_ks = nullptr, *d_vs = nullptr;
+    const int32_t *d_pos = nullptr;  // the tokens' positions, where asked for
 };
 
+// max_positions >= 0: the positions are uploaded too, and none reaches max_positions.
 int prepare_write(zk_kv_cache *c, size_t layer, const char *const *ids, const int32_t *num_tokens, int n,
-                  bool have_src, WritePrep &w, bool upload_slots = true) {
+                  bool have_src, WritePrep &w, bool upload_slots = true, int64_t max_positions = -1) {
     if (!c || (n > 0 && (!ids || !num_tokens)))
         return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: KVCache write batch: NULL argument");
     if (layer >= c->num_layers)
@@ -559,6 +562,9 @@ int prepare_write(zk_kv_cache *c, size_t layer, const char *const *ids, const in
         if (fp8 && s.k_scales.empty())
             return set_error(ZK_ERR_FAILED_PRECONDITION,
                              std::string("Failed precondition: fp8 scales not set for seq ") + ids[i]);
+        if (max_positions >= 0 && s.cached_tokens + (size_t)num_tokens[i] > (size_t)max_positions)
+            return set_error_typed(ZK_ERR_SEQUENCE_TOO_LONG, zk::ErrorKind::SequenceTooLong,
+                                   s.cached_tokens + (size_t)num_tokens[i], (uint64_t)max_positions);
         T += (size_t)num_tokens[i];
     }
     if (T == 0) return ZK_OK;
@@ -576,9 +582,11 @@ int prepare_write(zk_kv_cache *c, size_t layer, const char *const *ids, const in
     const size_t slots_bytes = T * sizeof(int64_t);
     const size_t rows_bytes = fp8 ? T * sizeof(int32_t) : 0;
     const size_t scale_bytes = fp8 ? 2 * (size_t)n * H * sizeof(float) : 0;
-    std::vector<char> host(slots_bytes + rows_bytes + scale_bytes);
+    const size_t pos_bytes = max_positions >= 0 ? T * sizeof(int32_t) : 0;
+    std::vector<char> host(slots_bytes + rows_bytes + scale_bytes + pos_bytes);
     int64_t *slots = (int64_t *)host.data();
     int32_t *rows = fp8 ? (int32_t *)(host.data() + slots_bytes) : nullptr;
+    int32_t *positions = pos_bytes ? (int32_t *)(host.data() + slots_bytes + rows_bytes + scale_bytes) : nullptr;
     size_t t = 0;
     for (int i = 0; i < n; ++i) {
         const SeqState &s = *seqs[i];
@@ -586,6 +594,7 @@ int prepare_write(zk_kv_cache *c, size_t layer, const char *const *ids, const in
             const size_t pos = s.cached_tokens + (size_t)j;
             slots[t] = (int64_t)s.handles[pos / bs].block_id * (int64_t)bs + (int64_t)(pos % bs);
             if (fp8) rows[t] = i;
+            if (positions) positions[t] = (int32_t)pos;
         }
     }
     if (fp8) {
@@ -602,6 +611,7 @@ int prepare_write(zk_kv_cache *c, size_t layer, const char *const *ids, const in
     w.d_rows = fp8 ? (const int32_t *)(d + slots_bytes) : nullptr;
     w.d_ks = fp8 ? (const float *)(d + slots_bytes + rows_bytes) : nullptr;
     w.d_vs = fp8 ? w.d_ks + (size_t)n * H : nullptr;
+    w.d_pos = pos_bytes ? (const int32_t *)(d + slots_bytes + rows_bytes + scale_bytes) : nullptr;
     return ZK_OK;
 }
 
@@ -862,6 +872,60 @@ int zk_cache_write_batch_qkv(zk_kv_cache *c, size_t layer, const char *const *id
                                 w.d_ks, w.d_vs, w.d_rows, c->stream))
             return rc;
     }
+    finish_write(c, layer, num_tokens, n, w);
+    return ZK_OK;
+}
+
+int zk_cache_write_batch_rope(zk_kv_cache *c, size_t layer, const char *const *ids, const int32_t *num_tokens, int n,
+                              const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
+                              int64_t v_stride, zk_dtype src_dtype, int num_heads, const void *q_weight,
+                              const void *k_weight, float eps, const float *rope, int64_t max_positions, int rot_dim,
+                              int interleaved, void *q_out, int64_t q_out_stride) {
+    if (!c) return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: KVCache write rope: NULL cache");
+    zk::RopeArgs a{};
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.dtype = src_dtype;
+    a.num_heads = num_heads;
+    a.num_kv_heads = (int)c->num_kv_heads;
+    a.head_dim = (int)c->head_dim;
+    a.q_weight = q_weight;
+    a.k_weight = k_weight;
+    a.eps = eps;
+    a.rope = rope;
+    a.max_positions = max_positions;
+    a.rot_dim = rot_dim;
+    a.interleaved = interleaved != 0;
+    a.q_out = q_out;
+    a.q_out_stride = q_out_stride;
+    a.k_pool = layer < c->num_layers ? c->k_pool(layer) : nullptr;  // (a layer out of range is refused below)
+    a.v_pool = layer < c->num_layers ? c->v_pool(layer) : nullptr;
+    a.cache_dtype = (zk_dtype)c->dtype;
+    a.block_size = (int)c->block_size;
+    a.num_blocks = (int64_t)c->num_blocks;
+    // all refusals come before prepare_write, whose copies on write change the tables
+    if (num_tokens && n > 0) {
+        int64_t T = 0;
+        for (int i = 0; i < n; ++i) T += num_tokens[i] > 0 ? num_tokens[i] : 0;
+        a.num_tokens = T;
+        if (layer < c->num_layers)
+            if (int rc = zk::check_qk_norm_rope(a, /*by_cache=*/true)) return rc;
+    }
+    WritePrep w;
+    if (int rc = prepare_write(c, layer, ids, num_tokens, n, q && k && v && q_out, w, true,
+                               rot_dim > 0 ? max_positions : INT64_MAX))
+        return rc;
+    if (w.T == 0) return ZK_OK;
+    a.slots = w.d_slots;
+    a.positions = w.d_pos;
+    a.k_scales = w.d_ks;
+    a.v_scales = w.d_vs;
+    a.token_row = w.d_rows;
+    if (int rc = zk::qk_norm_rope(a, c->stream)) return rc;
     finish_write(c, layer, num_tokens, n, w);
     return ZK_OK;
 }

@@ -32,5 +32,8 @@ struct RopeArgs {
     float inv_dim;  // 1 / head_dim
 };
 int qk_norm_rope(const RopeArgs &a, hipStream_t s);
+// Its checks of arguments alone.  by_cache: slots, positions, scales and
+// token_row are the cache's and not yet known.
+int check_qk_norm_rope(const RopeArgs &a, bool by_cache);
 
 }  // namespace zk

@@ -397,21 +397,30 @@ void launch(const RopeArgs &a, bool vec, int heads, hipStream_t s) {
 
 }  // namespace
 
-int zk::qk_norm_rope(const RopeArgs &in, hipStream_t s) {
-    RopeArgs a = in;
-    if (a.dtype != ZK_F32 && a.dtype != ZK_BF16) return bad("dtype must be f32 or bf16");
+namespace {
+
+void default_strides(RopeArgs &a) {
     const int64_t qw = (int64_t)a.num_heads * a.head_dim, kw = (int64_t)a.num_kv_heads * a.head_dim;
-    if (a.num_tokens < 0 || a.num_tokens > 0xffffff || a.num_heads <= 0 || a.num_kv_heads <= 0 || a.head_dim <= 0 ||
-        (int64_t)a.num_heads + 2 * (int64_t)a.num_kv_heads > 65535)
-        return bad("bad shape");
-    if (a.head_dim > kMaxDim) return bad("head_dim above 1024");
-    if (a.rot_dim < 0 || a.rot_dim > a.head_dim || a.rot_dim % 2) return bad("rot_dim must be even and at most head_dim");
-    const bool pool = a.k_pool || a.v_pool;
     if (a.q_stride == 0) a.q_stride = qw;
     if (a.k_stride == 0) a.k_stride = kw;
     if (a.v_stride == 0) a.v_stride = kw;
     if (a.q_out_stride == 0) a.q_out_stride = qw;
     if (a.k_out_stride == 0) a.k_out_stride = kw;
+}
+
+}  // namespace
+
+int zk::check_qk_norm_rope(const RopeArgs &in, bool by_cache) {
+    RopeArgs a = in;
+    if (a.dtype != ZK_F32 && a.dtype != ZK_BF16) return bad("dtype must be f32 or bf16");
+    if (a.num_tokens < 0 || a.num_tokens > 0xffffff || a.num_heads <= 0 || a.num_kv_heads <= 0 || a.head_dim <= 0 ||
+        (int64_t)a.num_heads + 2 * (int64_t)a.num_kv_heads > 65535)
+        return bad("bad shape");
+    if (a.head_dim > kMaxDim) return bad("head_dim above 1024");
+    if (a.rot_dim < 0 || a.rot_dim > a.head_dim || a.rot_dim % 2) return bad("rot_dim must be even and at most head_dim");
+    const int64_t qw = (int64_t)a.num_heads * a.head_dim, kw = (int64_t)a.num_kv_heads * a.head_dim;
+    const bool pool = a.k_pool || a.v_pool;
+    default_strides(a);
     if (a.q_stride < qw || a.k_stride < kw || a.q_out_stride < qw || (pool && a.v_stride < kw) ||
         (!pool && a.k_out_stride < kw))
         return bad("token stride below the row's width");
@@ -419,13 +428,13 @@ int zk::qk_norm_rope(const RopeArgs &in, hipStream_t s) {
         if (!valid_dtype(a.cache_dtype)) return bad("unsupported cache dtype");
         if (a.block_size <= 0 || a.num_blocks <= 0) return bad("bad pool shape");
         const bool fp8 = a.cache_dtype == ZK_FP8_E4M3;
-        if (fp8 && (!a.k_scales || !a.v_scales || !a.token_row)) return bad("fp8 pool needs scales and token_row");
+        if (!by_cache && fp8 && (!a.k_scales || !a.v_scales || !a.token_row))
+            return bad("fp8 pool needs scales and token_row");
         if (!fp8 && (a.k_scales || a.v_scales || a.token_row)) return bad("scales given for a non-fp8 pool");
-        a.num_slots = a.num_blocks * a.block_size;
     }
     if (a.num_tokens == 0) return ZK_OK;
-    if (!a.q || !a.k || !a.q_out || (pool ? !a.v || !a.k_pool || !a.v_pool || !a.slots : !a.k_out) ||
-        (a.rot_dim && (!a.positions || !a.rope)))
+    if (!a.q || !a.k || !a.q_out || (pool ? !a.v || !a.k_pool || !a.v_pool || (!by_cache && !a.slots) : !a.k_out) ||
+        (a.rot_dim && ((!by_cache && !a.positions) || !a.rope)))
         return bad("NULL pointer");
     if (a.rot_dim && a.max_positions <= 0) return bad("empty position table");
     const int e = elt_size(a.dtype);
@@ -440,6 +449,17 @@ int zk::qk_norm_rope(const RopeArgs &in, hipStream_t s) {
                    !apart(a.k_out, a.k_out_stride, kw, a.q, a.q_stride, qw, false) ||
                    !apart(a.k_out, a.k_out_stride, kw, a.q_out, a.q_out_stride, qw, false))))
         return bad("an output overlaps another operand (only the input of the same name, in its own layout, may be it)");
+    return ZK_OK;
+}
+
+int zk::qk_norm_rope(const RopeArgs &in, hipStream_t s) {
+    if (int rc = check_qk_norm_rope(in, false)) return rc;
+    if (in.num_tokens == 0) return ZK_OK;
+    RopeArgs a = in;
+    default_strides(a);
+    const bool pool = a.k_pool != nullptr;
+    if (pool) a.num_slots = a.num_blocks * a.block_size;
+    const int e = elt_size(a.dtype);
     const int V = 16 / e, D = a.head_dim, half = a.rot_dim / 2;
     auto mult = [&](int64_t stride) { return stride % V == 0; };
     auto al = [](const void *p) { return ((uintptr_t)p & 15u) == 0; };

@@ -237,6 +237,40 @@ class KVCache:
                                                        _dev(out, "out")))
         return out
 
+    def write_batch_rope(self, layer: int, ids, num_tokens, q, k, v, rope, q_weight=None, k_weight=None,
+                         eps: float = 1e-6, interleaved: bool = False, q_out=None):
+        """write_batch of keys that are normalised and rotated on the way, and
+        the step's queries with them (zk_cache_write_batch_rope): q [T, H, D], k
+        and v [T, Hkv, D] may be columns of a fused projection output; rope is a
+        dense.rope_table (None: norms alone), rows taken at the tokens' own
+        positions.  Returns q_out (by default new; it may be q)."""
+        b = _batch(ids)
+        nt = _counts(num_tokens, len(b))
+        rows = int(sum(nt))
+        h, d = q.shape[1], self.head_dim
+        if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+            raise TypeError("q, k and v must all be float32 or bfloat16")
+        qs = _token_stride(q, "q", rows, h, d)
+        ks = _token_stride(k, "k", rows, self.num_kv_heads, d)
+        vs = _token_stride(v, "v", rows, self.num_kv_heads, d)
+        if q_out is None:
+            q_out = torch.empty((rows, h, d), dtype=q.dtype, device=q.device)
+        elif q_out.dtype != q.dtype:
+            raise TypeError("q_out must have q's dtype")
+        os_ = _token_stride(q_out, "q_out", rows, h, d)
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None and (tuple(w.shape) != (d,) or w.dtype != q.dtype):
+                raise ValueError(f"{name} must be [{d}] of q's dtype")
+        if rope is not None and (rope.dim() != 2 or rope.dtype != torch.float32):
+            raise ValueError("rope must be a float32 [max_positions, rot_dim] table")
+        most, rot = (0, 0) if rope is None else rope.shape
+        _lib.check(_lib.lib().zk_cache_write_batch_rope(
+            self._h, layer, b.arr, ctypes.addressof(nt), len(b), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+            zk_dtype(q), h, None if q_weight is None else _dev(q_weight, "q_weight"),
+            None if k_weight is None else _dev(k_weight, "k_weight"), float(eps),
+            None if rope is None else _dev(rope, "rope"), most, rot, int(bool(interleaved)), q_out.data_ptr(), os_))
+        return q_out
+
     # -- decode --------------------------------------------------------------
     def paged_decode(self, layer: int, ids, q, out=None, scale=None, mapping="grouped"):
         """Decode attention for registered sequences `ids` (batch order; a list

@@ -6,8 +6,10 @@ Same math as the reference runner's step (src/cuda_runner.rs:271-660):
 embedding -> per layer [RMSNorm -> q/k/v projections -> KV store -> paged
 attention -> o_proj -> residual add -> RMSNorm -> gate/up projections ->
 SiLU(gate) * up -> down projection -> residual add] -> final RMSNorm of each
-sequence's last token -> lm_head logits (no rotary embedding, as in the
-reference).  What differs is the shape of the work:
+sequence's last token -> lm_head logits.  The reference has no rotary
+embedding and no norms of the heads, and neither has a model by default; with
+rope_theta or qk_norm set, both run in the KV write's launch
+(PagedKVRunner.write_rope).  What differs is the shape of the work:
   - one launch per op for all sequences of the batch (the reference loops
     over sequences, cuda_runner.rs:274);
   - q/k/v come from ONE projection against a fused [(H + 2 Hkv) D, hidden]
@@ -52,6 +54,10 @@ class LlamaConfig:
     num_kv_heads: int
     head_dim: int
     rms_eps: float = 1e-6
+    rope_theta: float = 0.0       # base of the rotary embedding's frequencies; 0: none
+    max_positions: int = 0        # rows of its table
+    rope_interleaved: bool = False  # pairs (2 i, 2 i + 1) instead of (i, i + head_dim / 2)
+    qk_norm: bool = False         # RMSNorm of every query and key head
 
     @staticmethod
     def llama3_8b(num_layers: int = 32) -> "LlamaConfig":
@@ -67,6 +73,8 @@ class LayerWeights:
     gate_up: object          # [2 I, hidden]: gate and up rows interleaved in blocks of 16 (dense.interleave_gate_up);
                              # a dense.TiledWeight of it for bf16 models
     down: object             # [hidden, I] (a dense.TiledWeight for bf16 models)
+    q_norm: torch.Tensor | None = None  # [head_dim], of models with qk_norm
+    k_norm: torch.Tensor | None = None
 
 
 @dataclass
@@ -98,6 +106,9 @@ class LlamaWeights:
         layers = [LayerWeights(norm(hid), lin((H + 2 * Hkv) * D, hid), lin(hid, H * D), norm(hid),
                                tile(dense.interleave_gate_up(lin(I, hid), lin(I, hid))), tile(lin(hid, I)))
                   for _ in range(cfg.num_layers)]
+        if cfg.qk_norm:
+            for lw in layers:
+                lw.q_norm, lw.k_norm = norm(D), norm(D)
         emb = torch.randn((cfg.vocab_size, hid), generator=g, device=device).to(dtype)
         return LlamaWeights(emb, layers, norm(hid), tile(lin(cfg.vocab_size, hid)))
 
@@ -111,6 +122,11 @@ class HipModelRunner:
         if (c.num_layers, c.num_kv_heads, c.head_dim) != (cfg.num_layers, cfg.num_kv_heads, cfg.head_dim):
             raise ValueError("KV cache shape does not match the model")
         self.cfg, self.w, self.kv = cfg, weights, kv
+        self.rope = None
+        if cfg.rope_theta > 0:
+            self.rope = dense.rope_table(cfg.max_positions, cfg.head_dim, cfg.rope_theta, weights.embedding.device)
+        if cfg.qk_norm and any(lw.q_norm is None or lw.k_norm is None for lw in weights.layers):
+            raise ValueError("a model with qk_norm needs the layers' q_norm and k_norm")
 
     def drop_state(self, request_id: str) -> None:
         self.kv.drop_state(request_id)
@@ -139,7 +155,13 @@ class HipModelRunner:
         dense.rms_norm(resid, w.layers[0].attn_norm, cfg.rms_eps, out=normed)
         last = len(w.layers) - 1
         for layer, lw in enumerate(w.layers):
-            if normed.dtype == torch.bfloat16:  # projection and KV write in one call
+            if self.rope is not None or cfg.qk_norm:  # heads normalised and rotated on the way to the pages
+                qkv = dense.linear(normed, lw.qkv)
+                q = qkv[:, :qd].view(T, H, D)
+                self.kv.write_rope(layer, plan, q, qkv[:, qd:qd + kd].view(T, Hkv, D), qkv[:, qd + kd:].view(T, Hkv, D),
+                                   self.rope, lw.q_norm if cfg.qk_norm else None, lw.k_norm if cfg.qk_norm else None,
+                                   cfg.rms_eps, cfg.rope_interleaved, q_out=q)
+            elif normed.dtype == torch.bfloat16:  # projection and KV write in one call
                 qkv = self.kv.write_qkv(layer, plan, normed, lw.qkv, H)
             else:
                 qkv = dense.linear(normed, lw.qkv)

@@ -77,6 +77,13 @@ class PagedKVRunner:
         the projection buffer (its q columns feed attention)."""
         return self.cache.write_batch_qkv(layer, plan.ids, plan.num_tokens, x, w_qkv, num_heads, out=out)
 
+    def write_rope(self, layer: int, plan: StepPlan, q, k, v, rope, q_weight=None, k_weight=None, eps: float = 1e-6,
+                   interleaved: bool = False, q_out=None):
+        """write of keys that are normalised and rotated on the way, with the
+        step's queries: returns the queries for attention."""
+        return self.cache.write_batch_rope(layer, plan.ids, plan.num_tokens, q, k, v, rope, q_weight, k_weight, eps,
+                                           interleaved, q_out)
+
     def attention(self, layer: int, plan: StepPlan, q, out=None, scale=None, mapping="grouped"):
         return self.cache.attention_batch(layer, plan.ids, plan.num_tokens, q, out=out, scale=scale,
                                           mapping=mapping)
