@@ -11,8 +11,8 @@
 //
 // Bound by HBM: every listed page's K and V are read once for the G = H / Hkv
 // heads that share them.  Softmax in the log2 domain, statistics and sums in
-// f32; the weights are rounded to bf16 for PV on bf16 and fp8 pools, whose
-// values have no more bits.
+// f32; f32 queries are rounded to bf16 for the matrix cores on bf16 and fp8 pools,
+// as the decode over all pages does.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -312,13 +312,18 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
                             if (2 * j + 1 < DT / 2) vb[h][i][2 * j + 1] = c2[1];
                         }
                     }
-            u32x4 pw;
+            // weights as two bf16 each, the second what the first leaves of it (17
+            // bits in all): the matrix cores wait for memory anyway
+            u32x4 pw, rw;
 #pragma unroll
-            for (int h = 0; h < PG; ++h) {
-                pw[2 * h] = bf16x2_rne(pr[h][0], pr[h][1]);
-                pw[2 * h + 1] = bf16x2_rne(pr[h][2], pr[h][3]);
-            }
-            const bf16x8 pb = __builtin_bit_cast(bf16x8, pw);
+            for (int h = 0; h < PG; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const uint32_t w = bf16x2_rne(pr[h][i], pr[h][i + 1]);
+                    pw[2 * h + i / 2] = w;
+                    rw[2 * h + i / 2] = bf16x2_rne(pr[h][i] - bf16lo(w), pr[h][i + 1] - bf16hi(w));
+                }
+            const bf16x8 pb = __builtin_bit_cast(bf16x8, pw), rb = __builtin_bit_cast(bf16x8, rw);
 #pragma unroll
             for (int j = 0; j < DT / 2; ++j) {
                 u32x4 ev, od;
@@ -329,8 +334,11 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
                     od[2 * h] = __builtin_amdgcn_perm(vb[h][1][j], vb[h][0][j], 0x07060302u);
                     od[2 * h + 1] = __builtin_amdgcn_perm(vb[h][3][j], vb[h][2][j], 0x07060302u);
                 }
-                o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ev), pb, o[2 * j], 0, 0, 0);
-                o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, od), pb, o[2 * j + 1], 0, 0, 0);
+                const bf16x8 e8 = __builtin_bit_cast(bf16x8, ev), o8 = __builtin_bit_cast(bf16x8, od);
+                o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e8, pb, o[2 * j], 0, 0, 0);
+                o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(o8, pb, o[2 * j + 1], 0, 0, 0);
+                o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e8, rb, o[2 * j], 0, 0, 0);
+                o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(o8, rb, o[2 * j + 1], 0, 0, 0);
             }
         }
     }
