@@ -149,7 +149,7 @@ def _scores_ref(q, bounds, table, lens, bs, mapping):
 
 
 SCORE_SHAPES = [(32, 8, 128, 16), (4, 4, 64, 16), (16, 8, 64, 16), (64, 8, 128, 16), (16, 1, 128, 16), (20, 4, 96, 16), (5, 1, 17, 16), (8, 2, 128, 37),
-                (48, 2, 64, 16)]
+                (48, 2, 64, 16), (8, 2, 256, 16), (10, 2, 128, 16), (33, 3, 96, 16)]
 
 
 @pytest.mark.parametrize("q_kind,kind", [("bf16", "bf16"), ("bf16", "fp8"), ("f32", "f32"), ("f32", "bf16"), ("bf16", "f32")])
@@ -322,12 +322,20 @@ def _attend(q, kp, vp, table, lens, pages, mapping="grouped", ks=None, vs=None, 
 
 
 SHAPES = [(32, 8, 128, 16), (8, 8, 128, 16), (16, 8, 64, 16), (64, 8, 128, 16), (16, 1, 64, 16), (20, 4, 96, 16), (3, 1, 40, 16), (8, 2, 256, 8),
-          (8, 4, 128, 80)]
+          (8, 4, 128, 80), (8, 2, 256, 16), (10, 2, 128, 16), (64, 4, 64, 16), (26, 2, 96, 16), (17, 1, 64, 16)]
 
 
 @pytest.mark.parametrize("q_kind,kind", [("bf16", "bf16"), ("bf16", "fp8"), ("f32", "f32"), ("f32", "bf16"), ("bf16", "f32")])
 @pytest.mark.parametrize("H,Hkv,D,bs", SHAPES)
 def test_sparse_decode(H, Hkv, D, bs, q_kind, kind):
+    if H // Hkv > 16:  # refused, as the decode over all pages refuses it
+        from zealot_amd import ZealotError, ops
+        z = torch.zeros(2, Hkv, bs, D, dtype=T_OF[kind], device="cuda")
+        with pytest.raises(ZealotError):
+            ops.paged_decode_sparse(_randn(1, (1, H, D), q_kind), z, z, _ints([[0]]), _ints([1]), _ints([[[0]] * Hkv]),
+                                    k_scales=None if kind != "fp8" else torch.ones(1, Hkv, device="cuda"),
+                                    v_scales=None if kind != "fp8" else torch.ones(1, Hkv, device="cuda"))
+        return
     lens = [0, 1, bs, bs + 1, 5 * bs - 1, 40 * bs + 3]
     table, nb = _tables(H + D, lens, bs, slack=2)
     kp, vp, q = _randn(1, (nb, Hkv, bs, D), kind), _randn(2, (nb, Hkv, bs, D), kind), _randn(3, (len(lens), H, D), q_kind)

@@ -23,6 +23,13 @@ __device__ __forceinline__ float xor32(float v) {
     return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// Another lane's value of the same 16 by the VALU's lane permutations: 0xb1 lane ^
+// 1, 0x4e lane ^ 2, 0x141 / 0x140 mirrored in 8 / 16 lanes, 0x120 + n rotated by n.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Two f32 -> packed bf16, round to nearest even (v_cvt_pk_bf16_f32).

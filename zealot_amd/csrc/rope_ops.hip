@@ -113,10 +113,6 @@ __device__ __forceinline__ int64_t pool_row(const RopeArgs &a, int64_t slot) {
 // Sum over aligned groups of `lanes` lanes, in every lane of a group: within 16
 // by the VALU's lane permutations (pairs, pairs of pairs, then mirrored halves,
 // whose lanes agree by then).
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
-}
 __device__ __forceinline__ float lane_sum(float x, int lanes) {
     if (lanes > 1) x += dpp<0xb1>(x);   // lane ^ 1
     if (lanes > 2) x += dpp<0x4e>(x);   // lane ^ 2

@@ -18,6 +18,7 @@
 #include <string>
 #include <type_traits>
 
+#include "attn_device.h"
 #include "zk_common.h"
 
 using namespace zk;
@@ -216,22 +217,27 @@ __device__ __forceinline__ int qhead(const ScoreArgs &a, int kvh, int j, int G) 
     return a.grouped ? kvh * G + j : kvh + j * a.num_kv_heads;
 }
 
-// bf16 queries, bf16 or fp8 bounds: A = 16 pages' [lo | hi] rows, B = the
-// query heads' [min(q, 0) | max(q, 0)], on v_mfma_f32_16x16x32_bf16 (both
-// exact in bf16, the sums in f32).  One wave per (16 * tiles pages, kv-head,
-// sequence).  A page's row of 2 D values is contiguous, the rows of a tile lie
-// anywhere: the wave loads whole rows, one tile ahead, and turns them into
-// fragments through LDS, chunk c of row r at c ^ r so that 16 rows do not meet in
-// a bank.  (Loaded by the lanes that need them, 64 bytes of 16 rows an
-// instruction, the lines were fetched twice: 83 us for 271 MB.)  Columns past
+// A = 16 pages' [lo | hi] rows, B = the query heads' [min(q, 0) | max(q, 0)], on
+// v_mfma_f32_16x16x32_bf16 (bf16 queries on bf16 or fp8 bounds: both exact in bf16,
+// the sums in f32) or v_mfma_f32_16x16x4_f32 (f32 bounds).  One wave per (16 *
+// tiles pages, kv-head, sequence).  A page's row of 2 D values is contiguous, the
+// rows of a tile lie anywhere: the wave loads whole rows, one tile ahead where its
+// registers allow, and turns them into fragments through LDS, rows 16 bytes
+// longer than they are so that 16 of them do not meet in a bank.  Columns past
 // the G heads repeat them, which leaves the maximum over the heads as it is.
-// Bound by HBM.
-template <int KV, int D, int G>
+//
+// 256 contexts of 512 to 8192 tokens, 32 / 8 heads of 128 bf16 (271 MB): 58 us, 4.7
+// TB/s; on contexts of one length 5.5 TB/s, 6.1 with the pages in order.  Loaded by
+// the lanes that need them, 64 bytes of 16 rows an instruction, the lines were
+// fetched twice: 83 us.
+template <int KV, int D>
 __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(ScoreArgs a) {
-    constexpr int KK = 2 * D / 32, ES = KV == ZK_BF16 ? 2 : 1;
-    constexpr int RB = 2 * D * ES, CPR = RB / 16;  // bytes and 16-byte chunks of a page's row
-    constexpr int LPT = 16 * RB / 1024;            // loads a tile
-    constexpr int SW = CPR < 16 ? CPR : 16;        // chunk c of row r lies at c ^ (r % SW)
+    constexpr bool F32 = KV == ZK_F32;
+    constexpr int ES = F32 ? 4 : KV == ZK_BF16 ? 2 : 1, RB = 2 * D * ES;
+    constexpr int CPR = RB / 16, LDR = RB + 16;     // 16-byte chunks of a row, its bytes in LDS
+    constexpr int LPT = 16 * RB / 1024;             // loads a tile
+    constexpr int QN = F32 ? CPR / 4 : 2 * D / 32;  // query pieces: 4 f32, 8 bf16 dims
+    static_assert(16 * RB % 1024 == 0 && CPR % 4 == 0, "row shape");
     extern __shared__ __attribute__((aligned(16))) char dyn[];  // a tile a wave
     __shared__ int32_t ids[16 * kScoreTiles];
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, wave = threadIdx.x >> 6;
@@ -251,25 +257,35 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
     float *out = a.scores + ((size_t)n * a.num_kv_heads + kvh) * a.max_blocks + p0;
     for (int p = max(live, 0) + lane; p < p1 - p0; p += 64) out[p] = -INFINITY;  // behind the context
     if (live <= 0) return;
-    bf16x8 qf[KK];
-    const uint16_t *q = (const uint16_t *)a.q + ((size_t)n * a.num_heads + qhead(a, kvh, col % G, G)) * D;
+    // The query's piece i meets dims d .. of the row [lo | hi]: the negative
+    // values (by sign bit; a NaN goes into the half of its sign) of dims d .. below D,
+    // the others of d - D .. from there.
+    const int G = a.num_heads / a.num_kv_heads;
+    const size_t q0 = ((size_t)n * a.num_heads + qhead(a, kvh, col % G, G)) * D;
+    u32x4 qf[QN];
 #pragma unroll
-    for (int kk = 0; kk < KK / 2; ++kk) {
-        // a k-step's dims of lane group grp: 8 of 32 in turn; of fp8 rows the
-        // halves of 16 bytes go to two steps
-        const int d0 = KV == ZK_BF16 ? 32 * kk + 8 * grp : 64 * (kk / 2) + 16 * grp + 8 * (kk % 2);
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(q + d0);
-        u32x4 neg, pos;
+    for (int i = 0; i < QN; ++i) {
+        const int d = F32 ? 16 * i + 4 * grp : KV == ZK_BF16 ? 32 * i + 8 * grp : 64 * (i / 2) + 16 * grp + 8 * (i % 2);
+        const bool hi = d >= D;
+        const size_t at = q0 + (hi ? d - D : d);
+        u32x4 w;
+        if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // by sign bit (a NaN's value goes into the half of its sign)
-            const uint32_t m = ((w[i] >> 15) & 0x10001u) * 0xffffu;  // 0xffff in negative halves
-            neg[i] = w[i] & m;
-            pos[i] = w[i] & ~m;
+            for (int e = 0; e < 4; ++e) {
+                w[e] = a.q_f32 ? __float_as_uint(((const float *)a.q)[at + e]) : (uint32_t)((const uint16_t *)a.q)[at + e] << 16;
+                w[e] = (w[e] >> 31 != 0) == hi ? 0u : w[e];
+            }
+        } else {
+            w = *reinterpret_cast<const u32x4 *>((const uint16_t *)a.q + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t m = ((w[e] >> 15) & 0x10001u) * 0xffffu;  // 0xffff in negative halves
+                w[e] &= hi ? ~m : m;
+            }
         }
-        qf[kk] = __builtin_bit_cast(bf16x8, neg);
-        qf[kk + KK / 2] = __builtin_bit_cast(bf16x8, pos);
+        qf[i] = w;
     }
-    char *lds = dyn + wave * 16 * RB;
+    char *lds = dyn + wave * 16 * LDR;
     const size_t block_bytes = (size_t)RB * a.num_kv_heads;
     const char *base = a.bounds + (size_t)kvh * RB;
     auto load = [&](int tile, u32x4 (&in)[LPT]) {
@@ -284,28 +300,36 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
 #pragma unroll
         for (int j = 0; j < LPT; ++j) {
             const int slot = 64 * j + lane, r = slot / CPR, c = slot % CPR;
-            *reinterpret_cast<u32x4 *>(lds + (r * CPR + (c ^ (r % SW))) * 16) = in[j];
+            *reinterpret_cast<u32x4 *>(lds + r * LDR + c * 16) = in[j];
         }
         f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int c = 0; c < CPR / 4; ++c) {
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(lds + (col * CPR + ((4 * c + grp) ^ (col % SW))) * 16);
-            if constexpr (KV == ZK_BF16) {
-                acc[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), qf[c], acc[c & 1], 0, 0, 0);
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(lds + col * LDR + (4 * c + grp) * 16);
+            if constexpr (F32) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[e]), __uint_as_float(qf[c][e]), acc[e & 1], 0, 0, 0);
+            } else if constexpr (KV == ZK_BF16) {
+                acc[c & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, qf[c]),
+                                                                     acc[c & 1], 0, 0, 0);
             } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const u32x2 lo = e4m3x4_to_bf16x4(w[2 * h]), hi = e4m3x4_to_bf16x4(w[2 * h + 1]);
                     acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]}),
-                                                                     qf[2 * c + h], acc[h], 0, 0, 0);
+                                                                     __builtin_bit_cast(bf16x8, qf[2 * c + h]), acc[h], 0, 0, 0);
                 }
             }
         }
-        f32x4 s = acc[0] + acc[1];  // head col's scores of the tile's pages 4 grp + i
+        f32x4 s = acc[0] + acc[1];  // column col's scores of the tile's pages 4 grp + i
 #pragma unroll
-        for (int o = 1; o < G; o <<= 1)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = max_nan(s[i], __shfl_xor(s[i], o));
+        for (int i = 0; i < 4; ++i) {  // maximum over the 16 columns
+            s[i] = max_nan(s[i], dpp<0x121>(s[i]));
+            s[i] = max_nan(s[i], dpp<0x122>(s[i]));
+            s[i] = max_nan(s[i], dpp<0x124>(s[i]));
+            s[i] = max_nan(s[i], dpp<0x128>(s[i]));
+        }
         // lane col < 4 of each group writes page 4 grp + col
         float v = s[0];
         v = col == 1 ? s[1] : v;
@@ -315,16 +339,24 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
         if (col < 4 && p < live) out[p] = ids[p] >= 0 ? v : -INFINITY;
     };
     const int tiles = (live + 15) / 16;
-    u32x4 in0[LPT], in1[LPT];
+    u32x4 in0[LPT];
     load(0, in0);
-    int t = 0;
-    for (; t + 1 < tiles; t += 2) {
-        load(t + 1, in1);
-        tile(t, in0);
-        load(min(t + 2, tiles - 1), in0);
-        tile(t + 1, in1);
+    if constexpr (LPT <= 8) {
+        u32x4 in1[LPT];
+        int t = 0;
+        for (; t + 1 < tiles; t += 2) {
+            load(t + 1, in1);
+            tile(t, in0);
+            load(min(t + 2, tiles - 1), in0);
+            tile(t + 1, in1);
+        }
+        if (t < tiles) tile(t, in0);
+    } else {
+        for (int t = 0; t < tiles; ++t) {
+            tile(t, in0);
+            if (t + 1 < tiles) load(t + 1, in0);
+        }
     }
-    if (t < tiles) tile(t, in0);
 }
 
 // Any shape and type: one wave per (page, kv-head, sequence), lanes over the
@@ -489,20 +521,21 @@ select_pages_kernel(const float *__restrict__ scores, const int32_t *__restrict_
 constexpr int kSelectMost = 16 * 64 * 64;  // pages of the widest variant
 
 template <int KV, int D>
-void launch_scores_g(const ScoreArgs &a, dim3 grid, int G, hipStream_t s) {
-    const int waves = std::min(a.num_kv_heads, kScoreHeads), lds = waves * 16 * 2 * D * (KV == ZK_BF16 ? 2 : 1);
-    switch (G) {
-        case 1: page_scores_mfma_kernel<KV, D, 1><<<grid, 64 * waves, lds, s>>>(a); break;
-        case 2: page_scores_mfma_kernel<KV, D, 2><<<grid, 64 * waves, lds, s>>>(a); break;
-        case 4: page_scores_mfma_kernel<KV, D, 4><<<grid, 64 * waves, lds, s>>>(a); break;
-        case 8: page_scores_mfma_kernel<KV, D, 8><<<grid, 64 * waves, lds, s>>>(a); break;
-        default: page_scores_mfma_kernel<KV, D, 16><<<grid, 64 * waves, lds, s>>>(a); break;
-    }
+void launch_scores_d(const ScoreArgs &a, dim3 grid, hipStream_t s) {
+    const int waves = std::min(a.num_kv_heads, kScoreHeads);
+    const int lds = waves * 16 * (2 * D * (KV == ZK_F32 ? 4 : KV == ZK_BF16 ? 2 : 1) + 16);
+    page_scores_mfma_kernel<KV, D><<<grid, 64 * waves, lds, s>>>(a);
 }
 template <int KV>
-void launch_scores(const ScoreArgs &a, dim3 grid, int G, hipStream_t s) {
-    if (a.head_dim == 128) launch_scores_g<KV, 128>(a, grid, G, s);
-    else launch_scores_g<KV, 64>(a, grid, G, s);
+void launch_scores(const ScoreArgs &a, dim3 grid, hipStream_t s) {
+    if (a.head_dim == 64) launch_scores_d<KV, 64>(a, grid, s);
+    else if (a.head_dim == 96) launch_scores_d<KV, 96>(a, grid, s);
+    else if (a.head_dim == 128) launch_scores_d<KV, 128>(a, grid, s);
+    else if constexpr (KV != ZK_F32) launch_scores_d<KV, 256>(a, grid, s);
+}
+bool scores_mfma(int q_dtype, int kv_dtype, int head_dim, int G) {
+    if (G > 16 || (q_dtype == ZK_F32 && kv_dtype != ZK_F32)) return false;  // (f32 queries are not rounded)
+    return head_dim == 64 || head_dim == 96 || head_dim == 128 || (head_dim == 256 && kv_dtype != ZK_F32);
 }
 
 }  // namespace
@@ -571,8 +604,8 @@ int zk_page_scores(const void *q, zk_dtype q_dtype, const void *bounds, zk_dtype
     const int G = num_heads / num_kv_heads;
     hipStream_t s = (hipStream_t)stream;
     KernelTimer timer("page_scores", s);
-    const bool mfma = q_dtype == ZK_BF16 && kv_dtype != ZK_F32 && max_blocks_per_seq <= 65535 * 16 * kScoreTiles && (head_dim == 64 || head_dim == 128) &&
-                      (G == 1 || G == 2 || G == 4 || G == 8 || G == 16) && (((uintptr_t)q | (uintptr_t)bounds) & 15u) == 0;
+    const bool mfma = scores_mfma(q_dtype, kv_dtype, head_dim, G) && max_blocks_per_seq <= 65535 * 16 * kScoreTiles &&
+                      (((uintptr_t)q | (uintptr_t)bounds) & 15u) == 0;
     if (mfma) {
         a.tiles = 8;
         auto groups = [&](int tiles) {
@@ -582,8 +615,9 @@ int zk_page_scores(const void *q, zk_dtype q_dtype, const void *bounds, zk_dtype
         while ((max_blocks_per_seq + 16 * a.tiles - 1) / (16 * a.tiles) > 65535 && a.tiles < kScoreTiles) a.tiles *= 2;
         const dim3 grid(num_seqs, (num_kv_heads + kScoreHeads - 1) / kScoreHeads,
                         (max_blocks_per_seq + 16 * a.tiles - 1) / (16 * a.tiles));
-        if (kv_dtype == ZK_BF16) launch_scores<ZK_BF16>(a, grid, G, s);
-        else launch_scores<ZK_FP8_E4M3>(a, grid, G, s);
+        if (kv_dtype == ZK_F32) launch_scores<ZK_F32>(a, grid, s);
+        else if (kv_dtype == ZK_BF16) launch_scores<ZK_BF16>(a, grid, s);
+        else launch_scores<ZK_FP8_E4M3>(a, grid, s);
     } else {
         const dim3 grid((max_blocks_per_seq + kThreads / 64 - 1) / (kThreads / 64), num_kv_heads, num_seqs);
         if (kv_dtype == ZK_F32) page_scores_generic_kernel<ZK_F32><<<grid, kThreads, 0, s>>>(a);
