@@ -411,6 +411,24 @@ def test_scores_of_minus_infinity_and_nan(kind, D):
     assert float((got[0].double().cpu() - want).abs().max()) <= 2.0 ** -7 * float(v.abs().max())
 
 
+@pytest.mark.parametrize("kind,D", [("bf16", 128), ("f32", 128), ("bf16", 96)])
+def test_values_of_infinity_stay_infinite(kind, D):
+    """Every weight is positive here (scores within a few units), 1 exactly in the first two rows."""
+    from zealot_amd import ops
+    lens = [1, 40, 40]
+    table, nb = _tables(13, lens)
+    kp, vp, q = _randn(1, (nb, 1, 16, D), kind), _randn(2, (nb, 1, 16, D), kind), _randn(3, (3, 4, D), "f32" if kind == "f32" else "bf16")
+    for p in range(3):
+        kp[int(table[1, p]), 0] = 0
+    for i in range(3):
+        vp[int(table[i, 0]), 0, 0, 3], vp[int(table[i, 0]), 0, 0, 6] = float("inf"), float("-inf")
+    got = ops.paged_decode_sparse(q, kp, vp, table, _ints(lens), _ints([[[0, 1, 2]]] * 3)).float().cpu()
+    assert bool((got[:, :, 3] == float("inf")).all()) and bool((got[:, :, 6] == float("-inf")).all())
+    rest = [d for d in range(D) if d not in (3, 6)]
+    assert bool(torch.isfinite(got[:, :, rest]).all())
+    assert torch.equal(got[0, :, rest], vp[int(table[0, 0]), 0, 0].float().cpu()[rest].expand(4, -1))
+
+
 def test_all_pages_are_the_dense_decode():
     from zealot_amd import ops
     lens = [100, 1, 700, 64]

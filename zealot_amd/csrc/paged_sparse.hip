@@ -312,16 +312,19 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
                             if (2 * j + 1 < DT / 2) vb[h][i][2 * j + 1] = c2[1];
                         }
                     }
-            // weights as two bf16 each, the second what the first leaves of it (17
-            // bits in all): the matrix cores wait for memory anyway
+            // weights as two bf16 each, the leading 8 bits and what they leave (16 bits in
+            // all): the matrix cores wait for memory anyway.  2^-20 of the weight is added
+            // to the second, which is then never zero nor of the other sign: an infinity
+            // in V stays one.
             u32x4 pw, rw;
 #pragma unroll
             for (int h = 0; h < PG; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
-                    const uint32_t w = bf16x2_rne(pr[h][i], pr[h][i + 1]);
+                    const uint32_t w = __builtin_amdgcn_perm(__float_as_uint(pr[h][i + 1]), __float_as_uint(pr[h][i]), 0x07060302u);
+                    constexpr float kAll = 1.0f + 0x1p-20f;
                     pw[2 * h + i / 2] = w;
-                    rw[2 * h + i / 2] = bf16x2_rne(pr[h][i] - bf16lo(w), pr[h][i + 1] - bf16hi(w));
+                    rw[2 * h + i / 2] = bf16x2_rne(fmaf(pr[h][i], kAll, -bf16lo(w)), fmaf(pr[h][i + 1], kAll, -bf16hi(w)));
                 }
             const bf16x8 pb = __builtin_bit_cast(bf16x8, pw), rb = __builtin_bit_cast(bf16x8, rw);
 #pragma unroll
