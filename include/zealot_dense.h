@@ -57,8 +57,8 @@ int zk_embedding(const int64_t *ids, const void *table, void *out, int64_t num_t
  * max_positions) gets zero rows.  Arithmetic in f32, one rounding.  Token rows
  * are *_stride elements apart (0 = packed), so columns of a fused projection
  * are read, and with q_out == q (k_out == k) and equal strides written, in
- * place; any other overlap of an output is refused.  head_dim <= 1024,
- * num_tokens < 2^24. */
+ * place; an output that otherwise overlaps q, k, v or the other one is refused.
+ * head_dim <= 1024, num_tokens < 2^24. */
 int zk_qk_norm_rope(const void *q, int64_t q_stride, const void *k, int64_t k_stride, zk_dtype dtype,
                     int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim, const void *q_weight,
                     const void *k_weight, float eps, const int32_t *positions, const float *rope,

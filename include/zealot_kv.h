@@ -224,8 +224,8 @@ int zk_paged_decode_noalloc(const void *q, zk_dtype q_dtype, const void *k_pool,
  *   *cursor_out      the cursor behind the blocks the step takes: past
  *                    num_new_blocks when too few were granted
  * Rows behind the last token get -1 in all three; tokens behind row num_rows
- * get no row and enter no block.  kv_lens and cursor_out must not be the
- * inputs' memory. */
+ * get no row and enter no block.  What is written must not overlap another
+ * operand. */
 int zk_step_tables(int32_t *block_tables, int num_seqs, int max_blocks_per_seq, const int32_t *seq_lens,
                    const int32_t *new_lens, int block_size, const int32_t *new_blocks, int64_t num_new_blocks,
                    const int64_t *cursor, int64_t *cursor_out, int64_t *slot_mapping, int32_t *positions,
@@ -248,7 +248,7 @@ int zk_page_bounds(const void *k_pool, zk_dtype kv_dtype, const int64_t *slot_ma
                    int num_kv_heads, int head_dim, int block_size, int64_t num_blocks, void *bounds, void *stream);
 /* scores[n, h, p] (f32 [num_seqs, Hkv, max_blocks_per_seq]) = the maximum over
  * the query heads g of kv-head h of sum_d min(q_d, 0) lo_d + max(q_d, 0) hi_d:
- * no key of page p has a larger q . k (times the fp8 key scale, positive and the
+ * no key of page p has a larger q . k, up to the sum's f32 roundings (times the fp8 key scale, positive and the
  * same for all pages of (n, h)).  -inf for pages behind the length and table
  * entries outside the pool.  q [num_seqs, num_heads, head_dim], F32 or BF16.  A
  * NaN score (NaN or infinite keys) ranks first in zk_select_pages. */

@@ -37,6 +37,14 @@ def test_step_tables():
         assert rc == BAD and "must not be inputs" in msg, kw
 
 
+def test_step_tables_outputs_apart():
+    for kw in (dict(slots=_at(0)), dict(pos=_at(0x2000)), dict(row=_at(0x3010)), dict(cu=_at(0x4000)), dict(row=_at(0x7008)),
+               dict(end=_at(0x9010)), dict(kv=_at(0x7c)), dict(pos=_at(0x6040)), dict(slots=_at(0xff8))):
+        rc, msg = _tables(**kw)
+        assert rc == BAD and "must not be inputs" in msg, kw
+    assert _tables(rows=1 << 31)[0] == BAD and _tables(cnt=1 << 31)[0] == BAD
+
+
 def _rope(append=False, **kw):
     T, H, Hkv, d = 10, 8, 2, 64
     row = (H + 2 * Hkv) * d
@@ -121,6 +129,18 @@ def test_paged_decode_sparse():
     size = _lib.lib().zk_paged_decode_sparse_workspace_size
     assert size(256, 32, 8, 128, 64) == 0  # one part a list: no merge
     assert size(1, 32, 8, 128, 1024) > 0 and size(0, 32, 8, 128, 64) == 0 and size(1, 32, 8, 128, 0) == 0
+
+
+def test_sizes_past_the_grids():
+    lib, n = _lib.lib(), (1 << 31) - 1
+    assert _rc(lib.zk_page_scores(D, _lib.BF16, D, _lib.BF16, D, D, D, 4, 32, 8, 128, 16, n, 10, 0, None))[0] == BAD
+    assert _rc(lib.zk_page_scores(D, _lib.F32, D, _lib.BF16, D, D, D, 4, 32, 8, 100, 16, 1 << 26, 10, 0, None))[0] == BAD
+    assert _rc(lib.zk_select_pages(D, D, 4, 8, 20, 16, n, 1, 1, D, None))[0] == BAD
+    for pages in (n, 65535 * 1024 + 1):
+        rc, msg = _rc(lib.zk_paged_decode_sparse(D, _lib.BF16, D, D, _lib.BF16, D, D, D, D, pages, 4, 32, 8, 128, 16, 100, 50, 0.1, 0, None,
+                                                 None, D, 1 << 62, None))
+        assert rc == BAD and "too many pages" in msg
+        assert lib.zk_paged_decode_sparse_workspace_size(4, 32, 8, 128, pages) == 0
 
 
 def test_python_entry_points_refuse_host_tensors_and_wrong_shapes():

@@ -595,7 +595,9 @@ extern "C" {
 
 size_t zk_paged_decode_sparse_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
                                              int num_pages) {
-    if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_pages <= 0) return 0;
+    if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_pages <= 0 ||
+        num_pages > 65535 * kMaxList)
+        return 0;
     const int splits = splits_for(num_seqs, num_kv_heads, head_dim, num_pages);
     if (splits == 1) return 0;
     const size_t slots = (size_t)num_seqs * num_heads * splits;
@@ -617,8 +619,8 @@ int zk_paged_decode_sparse(const void *q, zk_dtype q_dtype, const void *k_pool, 
     if (mapping != ZK_GQA_GROUPED && mapping != ZK_GQA_MODULO) return bad("bad gqa mapping");
     if (head_dim > 256 || num_heads / num_kv_heads > kMaxG) return bad("head_dim <= 256 and H/Hkv <= 16 required");
     if ((int64_t)max_blocks_per_seq * block_size > 0x7fffffff) return bad("context too long");
+    if (num_pages > 65535 * kMaxList) return bad("too many pages a list");
     const int splits = num_seqs > 0 ? splits_for(num_seqs, num_kv_heads, head_dim, num_pages) : 1;
-    if (splits > 65535) return bad("too many pages a list");
     if (num_seqs == 0) return ZK_OK;
     if (!q || !k_pool || !v_pool || !out || !block_tables || !seq_lens || !pages) return bad("NULL pointer");
     if ((kv_dtype == ZK_FP8_E4M3) != (k_scales != nullptr && v_scales != nullptr) || !k_scales != !v_scales)

@@ -208,6 +208,7 @@ struct ScoreArgs {
     int tiles;  // of 16 pages a wave (at most kScoreTiles)
 };
 constexpr int kScoreTiles = 32, kScoreHeads = 2;  // most tiles a wave, waves (kv-heads) a workgroup
+constexpr int kMostPages = 65535 * 16 * kScoreTiles;  // of a context, by the grid
 
 __device__ __forceinline__ int held_pages(const ScoreArgs &a, int n) {
     const int64_t len = max(a.seq_lens[n], 0);
@@ -580,7 +581,8 @@ int zk_page_scores(const void *q, zk_dtype q_dtype, const void *bounds, zk_dtype
     if ((q_dtype != ZK_F32 && q_dtype != ZK_BF16) || !valid_dtype(kv_dtype))
         return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_scores: unsupported dtype");
     if (num_seqs < 0 || num_seqs > 65535 || num_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || head_dim <= 0 ||
-        block_size <= 0 || max_blocks_per_seq <= 0 || num_blocks <= 0 || num_heads % num_kv_heads != 0)
+        block_size <= 0 || max_blocks_per_seq <= 0 || max_blocks_per_seq > kMostPages || num_blocks <= 0 ||
+        num_heads % num_kv_heads != 0)
         return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_scores: bad shape");
     if (mapping != ZK_GQA_GROUPED && mapping != ZK_GQA_MODULO)
         return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_scores: bad gqa mapping");
@@ -604,8 +606,7 @@ int zk_page_scores(const void *q, zk_dtype q_dtype, const void *bounds, zk_dtype
     const int G = num_heads / num_kv_heads;
     hipStream_t s = (hipStream_t)stream;
     KernelTimer timer("page_scores", s);
-    const bool mfma = scores_mfma(q_dtype, kv_dtype, head_dim, G) && max_blocks_per_seq <= 65535 * 16 * kScoreTiles &&
-                      (((uintptr_t)q | (uintptr_t)bounds) & 15u) == 0;
+    const bool mfma = scores_mfma(q_dtype, kv_dtype, head_dim, G) && (((uintptr_t)q | (uintptr_t)bounds) & 15u) == 0;
     if (mfma) {
         a.tiles = 8;
         auto groups = [&](int tiles) {
@@ -631,7 +632,7 @@ int zk_select_pages(const float *scores, const int32_t *seq_lens, int num_seqs, 
                     int max_blocks_per_seq, int block_size, int num_pages, int sink, int recent, int32_t *pages,
                     void *stream) {
     if (num_seqs < 0 || num_seqs > 65535 || num_kv_heads <= 0 || max_blocks_per_seq <= 0 || block_size <= 0 ||
-        num_pages <= 0 || (int64_t)max_blocks_per_seq * block_size > 0x7fffffff)
+        num_pages <= 0 || num_pages > kMostPages || (int64_t)max_blocks_per_seq * block_size > 0x7fffffff)
         return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_select_pages: bad shape");
     if (sink < 0 || recent < 0 || (int64_t)sink + recent > num_pages)
         return set_error(ZK_ERR_INVALID_ARGUMENT,

@@ -151,19 +151,34 @@ extern "C" int zk_step_tables(int32_t *block_tables, int num_seqs, int max_block
                               int64_t *slot_mapping, int32_t *positions, int32_t *token_row, int64_t num_rows,
                               int64_t *cu_seqlens, int32_t *kv_lens, void *stream) {
     if (num_seqs < 0 || max_blocks_per_seq <= 0 || block_size <= 0 || num_new_blocks < 0 || num_rows < 0 ||
+        num_new_blocks > 0x7fffffff || num_rows > 0x7fffffff ||
         (int64_t)max_blocks_per_seq * block_size > 0x7fffffff)
         return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_step_tables: bad shape");
     if (!cursor_out || !cu_seqlens || (num_seqs > 0 && (!block_tables || !seq_lens || !new_lens || !kv_lens)) ||
         (num_rows > 0 && (!slot_mapping || !positions || !token_row)) || (num_new_blocks > 0 && !new_blocks))
         return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_step_tables: NULL pointer");
-    // other workgroups read the inputs while the first writes these
-    auto meet = [&](const int32_t *x) {
-        const uintptr_t u = (uintptr_t)x, v = (uintptr_t)kv_lens, bytes = sizeof(int32_t) * (uintptr_t)num_seqs;
-        return u < v + bytes && v < u + bytes;
-    };
-    if (cursor == cursor_out || (num_seqs > 0 && (meet(seq_lens) || meet(new_lens))))
-        return set_error(ZK_ERR_INVALID_ARGUMENT,
-                         "Internal error: zk_step_tables: kv_lens and cursor_out must not be inputs");
+    // workgroups read the inputs while others write: what is written meets nothing else
+    const struct {
+        const void *p;
+        int64_t bytes;
+    } all[] = {{block_tables, 4 * (int64_t)num_seqs * max_blocks_per_seq},
+               {cursor_out, 8},
+               {slot_mapping, 8 * num_rows},
+               {positions, 4 * num_rows},
+               {token_row, 4 * num_rows},
+               {cu_seqlens, 8 * ((int64_t)num_seqs + 1)},
+               {kv_lens, 4 * (int64_t)num_seqs},
+               {seq_lens, 4 * (int64_t)num_seqs},
+               {new_lens, 4 * (int64_t)num_seqs},
+               {new_blocks, 4 * num_new_blocks},
+               {cursor, cursor ? 8 : 0}};
+    for (int i = 0; i < 7; ++i)
+        for (int j = i + 1; j < 11; ++j) {
+            const uintptr_t u = (uintptr_t)all[i].p, v = (uintptr_t)all[j].p;
+            if (all[i].bytes > 0 && all[j].bytes > 0 && u < v + all[j].bytes && v < u + all[i].bytes)
+                return set_error(ZK_ERR_INVALID_ARGUMENT,
+                                 "Internal error: zk_step_tables: outputs must not be inputs, the tables or each other");
+        }
     StepArgs a{};
     a.tables = block_tables;
     a.seq_lens = seq_lens;

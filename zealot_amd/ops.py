@@ -265,7 +265,7 @@ def step_tables(block_tables, seq_lens, new_lens, block_size: int, num_rows: int
     new_lens[i] (int32 [N]); blocks it lacks are taken from new_blocks (int32,
     in batch order from cursor on, int64 [1]) and entered in block_tables (int32
     [N, max_blocks], in place).  num_rows: rows of the batch, padding included.
-    out: a StepTables to write to; its kv_lens and cursor must not be inputs."""
+    out: a StepTables to write to; none of it may overlap an input."""
     n, mb = _dims(block_tables, "block_tables", "[N, max_blocks]")
     cur, at_stream = _target(stream)
     i32, i64 = torch.int32, torch.int64
