@@ -206,6 +206,34 @@ def test_scores_of_a_long_context_and_a_nan_page():
     assert bool(((got - want).abs()[fin] <= 258 * 2.0 ** -23 * mag[fin]).all())
 
 
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "f32"])
+@pytest.mark.parametrize("N", [60, 300])
+def test_scores_of_batches(N, kind):
+    """Waves of several tiles: lengths anywhere in them, blocks outside the pool."""
+    from zealot_amd import ops
+    Hkv, G, D, width = 8, 2, 64, 200
+    rng = np.random.default_rng(N)
+    lens = rng.integers(0, width * 16 + 1, N)
+    lens[:5] = [0, 1, width * 16, 192 * 16, 192 * 16 + 1]
+    nb = 5000
+    table = _ints(rng.integers(-1, nb + 1, (N, width)))
+    q = _randn(1, (N, Hkv * G, D), "f32" if kind == "f32" else "bf16")
+    keys = torch.stack([_randn(s, (nb, Hkv, D)) for s in (1, 2)])
+    bounds = torch.stack([keys.amin(0), keys.amax(0)], 2).to(T_OF[kind])
+    got = ops.page_scores(q, bounds, table, _ints(lens), 16).double()
+    ok = (table >= 0) & (table < nb) & (torch.arange(width, device="cuda") * 16 < _ints(lens)[:, None])
+    b = bounds.double()[table.long().clamp(0, nb - 1)]  # [N, width, Hkv, 2, D]
+    want, mag = torch.full((N, Hkv, width), -math.inf, dtype=torch.float64, device="cuda"), torch.zeros(N, Hkv, width, dtype=torch.float64, device="cuda")
+    for g in range(G):
+        x = q.view(N, 1, Hkv, G, D)[:, :, :, g].double()
+        lo, hi = x.clamp(max=0) * b[..., 0, :], x.clamp(min=0) * b[..., 1, :]
+        want = torch.maximum(want, (lo + hi).sum(-1).transpose(1, 2))
+        mag = torch.maximum(mag, (lo.abs() + hi.abs()).sum(-1).transpose(1, 2))
+    ok = ok[:, None].expand(N, Hkv, width)
+    assert bool((got[~ok] == -math.inf).all())
+    assert bool(((got - want).abs()[ok] <= (2 * D + 2) * 2.0 ** -23 * mag[ok] + 1e-37).all())
+
+
 # ------------------------------------------------------------------ selection
 
 def _select_ref(scores, lens, bs, k, sink, recent):

@@ -207,7 +207,7 @@ struct ScoreArgs {
     int num_heads, num_kv_heads, head_dim, block_size, max_blocks, grouped, q_f32;
     int tiles;  // of 16 pages a wave (at most kScoreTiles)
 };
-constexpr int kScoreTiles = 32, kScoreHeads = 2;  // most tiles a wave, waves (kv-heads) a workgroup
+constexpr int kScoreTiles = 24, kScoreHeads = 2;  // most tiles a wave, waves (kv-heads) a workgroup
 constexpr int kMostPages = 65535 * 16 * kScoreTiles;  // of a context, by the grid
 
 __device__ __forceinline__ int held_pages(const ScoreArgs &a, int n) {
@@ -227,7 +227,7 @@ __device__ __forceinline__ int qhead(const ScoreArgs &a, int kvh, int j, int G) 
 // longer than they are so that 16 of them do not meet in a bank.  Columns past
 // the G heads repeat them, which leaves the maximum over the heads as it is.
 //
-// 256 contexts of 512 to 8192 tokens, 32 / 8 heads of 128 bf16 (271 MB): 58 us, 4.7
+// 256 contexts of 512 to 8192 tokens, 32 / 8 heads of 128 bf16 (271 MB): 56 us, 4.8
 // TB/s; on contexts of one length 5.5 TB/s, 6.1 with the pages in order.  Loaded by
 // the lanes that need them, 64 bytes of 16 rows an instruction, the lines were
 // fetched twice: 83 us.
@@ -608,7 +608,11 @@ int zk_page_scores(const void *q, zk_dtype q_dtype, const void *bounds, zk_dtype
     KernelTimer timer("page_scores", s);
     const bool mfma = scores_mfma(q_dtype, kv_dtype, head_dim, G) && (((uintptr_t)q | (uintptr_t)bounds) & 15u) == 0;
     if (mfma) {
-        a.tiles = 8;
+        // Long stretches a wave as long as there are enough of them; us with 8, 12 and 16
+        // tiles to begin with: 256 contexts of 512 to 8192 tokens 57.8, 56.1, 61.1; 256 of
+        // 8192 100.6, 99.6, 95.2; 2 of 100000 and more (fp8) 8.5, 7.7, 8.5; 64 of f32 38.1,
+        // 39.3, 38.1
+        a.tiles = 12;
         auto groups = [&](int tiles) {
             return (int64_t)num_seqs * num_kv_heads * ((max_blocks_per_seq + 16 * tiles - 1) / (16 * tiles));  // of a wave
         };
