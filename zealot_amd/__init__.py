@@ -13,6 +13,11 @@ zealot_amd/csrc with `python -m zealot_amd.build`):
                               (src/cuda_runner.rs:271-461)
   ops.append / gather / copy_blocks / paged_decode / paged_prefill / fp8_scales
                               stateless launches over caller-owned tensors
+  ops.step_tables             a step's block tables and slots from its lengths
+  ops.qk_norm_rope_append, dense.qk_norm_rope, KVCache.write_batch_rope
+                              head norms and rotary embedding, with the KV write
+  ops.page_bounds / page_scores / select_pages / paged_decode_sparse
+                              decode over the pages that bounds of their keys select
 """
 from ._lib import ZealotError, lib  # noqa: F401
 from .block_manager import BlockHandle, BlockManager  # noqa: F401

@@ -124,7 +124,7 @@ __device__ __forceinline__ int stage_list(const SparseArgs &a, int n, int kvh, i
 // The reference maximum of a head is moved only when a score exceeds it by
 // kSlack.  The waves' results are merged in LDS.
 //
-// 256 contexts, 64 pages of each, 32 / 8 heads of 128 bf16 (1048 MB): 169 us, 6.2
+// 256 contexts, 64 pages of each, 32 / 8 heads of 128 bf16 (1048 MB): 166 us, 6.3
 // TB/s (a read of one piece reaches 7.5, one of shuffled 4 KB pieces 7 % less).
 // One step ahead in registers needs 208 of them, two waves a SIMD, and took 179; the
 // 128 registers of four waves a SIMD spill, 215.

@@ -128,7 +128,7 @@ __device__ __forceinline__ float lane_sum(float x, int lanes) {
 // one 16-byte vector each, NP heads a lane, all loaded before any is used.  A
 // lane writes what it read, so outputs may be the inputs.
 //
-// 32768 tokens, 32 + 2 x 8 heads of 128 bf16 (810 MB): 137 us, 5.9 TB/s (a copy
+// 32768 tokens, 32 + 2 x 8 heads of 128 bf16 (810 MB): 134 us, 6.0 TB/s (a copy
 // reaches 6.7).  Between HBM and the VALU (busy 104 us of it), so what a head
 // needs is kept small: cosines and sines times the weights once a token, the
 // norm's factor applied to the rotated value, sums of squares by dot products of
