@@ -565,3 +565,82 @@ def test_another_stream_and_two_at_once():
     got = [ops.paged_decode_sparse(q, kp, vp, table, n, pages, stream=s) for _ in range(5) for s in streams]
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for x in got)
+
+
+@pytest.mark.parametrize("D", [128, 80])
+def test_pools_past_32_bits(D):
+    """The same step on a small pool and on one whose last blocks lie more than 2^32 elements in: equal results."""
+    from zealot_amd import dense, ops
+    H, Hkv, bs, small = 32, 8, 16, 40
+    nb = 2 ** 32 // (Hkv * bs * D) + 100
+    lens = [200, 33, 290]
+    table, used = _tables(21, lens)
+    assert used <= small
+    x = _randn(22, (sum(lens), (H + 2 * Hkv) * D), "bf16")
+    q, k, v = [y.unflatten(1, (-1, D)) for y in x.split((H * D, Hkv * D, Hkv * D), 1)]
+    rope, qd, results = dense.rope_table(300, D), _randn(23, (3, H, D), "bf16"), []
+    for blocks in (small, nb):
+        far = torch.where((table >= 0) & (table % 2 == 0), table + blocks - small, table)
+        kp, vp = [torch.empty(blocks, Hkv, bs, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        bounds = torch.empty(blocks, Hkv, 2, D, dtype=torch.bfloat16, device="cuda")
+        t = ops.step_tables(far, _ints([0] * 3), _ints(lens), bs, sum(lens))
+        qo = ops.qk_norm_rope_append(kp, vp, q, k, v, t.positions, t.slot_mapping, rope)
+        ops.page_bounds(kp, t.slot_mapping, bounds)
+        s = ops.page_scores(qd, bounds, far, t.kv_lens, bs)
+        pages = ops.select_pages(s, t.kv_lens, bs, 6)
+        results.append((qo, s, pages, ops.paged_decode_sparse(qd, kp, vp, far, t.kv_lens, pages)))
+        assert blocks == small or int(t.slot_mapping.max()) * Hkv * D > 2 ** 32 - 2 ** 24
+        del kp, vp, bounds
+    torch.cuda.empty_cache()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def _off(x):
+    """A copy of x whose first element lies one element behind an aligned address."""
+    y = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].view(x.shape)
+    return y.copy_(x)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "fp8"])
+def test_operands_off_their_alignment(kind):
+    from zealot_amd import ops
+    lens = [100, 1, 700, 64]
+    table, nb = _tables(15, lens)
+    kp, vp, q = [_off(_randn(s, sh, t)) for s, sh, t in ((1, (nb, 2, 16, 128), kind), (2, (nb, 2, 16, 128), kind), (3, (4, 8, 128), "bf16"))]
+    ks, vs = [(0.5 + torch.rand(4, 2, generator=torch.Generator().manual_seed(s))).cuda() if kind == "fp8" else None for s in (4, 5)]
+    _attend(q, kp, vp, table, lens, _lists(1, lens, 2, 9), "grouped", ks, vs, out=_off(torch.zeros(4, 8, 128, dtype=torch.bfloat16)))
+    slots = torch.cat([table[i].repeat_interleave(16).long()[:n] * 16 + torch.arange(n, device="cuda") % 16 for i, n in enumerate(lens)])
+    bounds = _off(torch.zeros(nb, 2, 2, 128, dtype=T_OF[kind], device="cuda"))
+    want = _bounds_ref(kp, slots, bounds)
+    ops.page_bounds(kp, slots, bounds)
+    _same(bounds, want)
+    got = ops.page_scores(q, bounds, table, _ints(lens), 16).double().cpu()
+    want, mag = _scores_ref(q, bounds, table, lens, 16, "grouped")
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isinf(got), ~fin) and bool(((got - want).abs()[fin] <= 258 * 2.0 ** -23 * mag[fin] + 1e-37).all())
+
+
+def test_two_graphs_over_one_workspace():
+    """Parts of a list are written before they are read within each call, so graphs that run in turn may share it."""
+    from zealot_amd import ops
+    sets = []
+    for seed, lens in ((30, [3000, 2000]), (31, [900, 5000])):
+        table, nb = _tables(seed, lens)
+        sets.append((_randn(seed, (2, 8, 128), "bf16"), _randn(1, (nb, 2, 16, 128), "bf16"), _randn(2, (nb, 2, 16, 128), "bf16"), table, _ints(lens),
+                     _lists(seed, lens, 2, 64)))
+    ws = torch.empty(ops.sparse_workspace_bytes(2, 8, 2, 128, 64), dtype=torch.uint8, device="cuda")
+    want = [ops.paged_decode_sparse(*s) for s in sets]
+    outs, graphs = [torch.empty_like(w) for w in want], []
+    torch.cuda.synchronize()
+    for s, out in zip(sets, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.paged_decode_sparse(*s, out=out, workspace=ws)
+        graphs.append(g)
+    for _ in range(4):
+        for g, out, w in zip(graphs, outs, want):
+            out.zero_()
+            g.replay()
+            ws.add_(1)
+            torch.cuda.synchronize()
+            assert torch.equal(out, w)
