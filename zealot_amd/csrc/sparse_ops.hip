@@ -210,9 +210,9 @@ struct ScoreArgs {
 constexpr int kScoreTiles = 24, kScoreHeads = 2;  // most tiles a wave, waves (kv-heads) a workgroup
 constexpr int kMostPages = 65535 * 16 * kScoreTiles;  // of a context, by the grid
 
-__device__ __forceinline__ int held_pages(const ScoreArgs &a, int n) {
-    const int64_t len = max(a.seq_lens[n], 0);
-    return (int)min((len + a.block_size - 1) / a.block_size, (int64_t)a.max_blocks);
+// Pages that a length holds, at most `most`.
+__device__ __forceinline__ int held_pages(int len, int block_size, int most) {
+    return len <= 0 ? 0 : (int)min((uint32_t)(len - 1) / (uint32_t)block_size + 1u, (uint32_t)most);
 }
 __device__ __forceinline__ int qhead(const ScoreArgs &a, int kvh, int j, int G) {
     return a.grouped ? kvh * G + j : kvh + j * a.num_kv_heads;
@@ -227,8 +227,8 @@ __device__ __forceinline__ int qhead(const ScoreArgs &a, int kvh, int j, int G) 
 // longer than they are so that 16 of them do not meet in a bank.  Columns past
 // the G heads repeat them, which leaves the maximum over the heads as it is.
 //
-// 256 contexts of 512 to 8192 tokens, 32 / 8 heads of 128 bf16 (271 MB): 56 us, 4.8
-// TB/s; on contexts of one length 5.5 TB/s, 6.1 with the pages in order.  Loaded by
+// 256 contexts of 512 to 8192 tokens, 32 / 8 heads of 128 bf16 (271 MB): 54 us, 5.0
+// TB/s; on contexts of one length 5.7 TB/s (a plain read of such rows: 6.6).  Loaded by
 // the lanes that need them, 64 bytes of 16 rows an instruction, the lines were
 // fetched twice: 83 us.
 template <int KV, int D>
@@ -241,11 +241,14 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
     static_assert(16 * RB % 1024 == 0 && CPR % 4 == 0, "row shape");
     extern __shared__ __attribute__((aligned(16))) char dyn[];  // a tile a wave
     __shared__ int32_t ids[16 * kScoreTiles];
+    __shared__ float found[kScoreHeads][16 * kScoreTiles];
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, wave = threadIdx.x >> 6;
-    // (chunks last: consecutive workgroups go to the XCDs in turn, and a sequence's
-    // later chunks are often behind its context)
-    const int kvh = blockIdx.y * (blockDim.x >> 6) + wave, n = blockIdx.x;
-    const int held = held_pages(a, n);
+    // Consecutive workgroups go to the XCDs in turn: the kv-heads first, so that a block's
+    // rows are not asked for by one XCD at a time (256 contexts 56 us with the sequences
+    // first, 54; 64 of f32 39, 34), chunks last, as a sequence's later ones are often
+    // behind its context
+    const int kvh = blockIdx.x * (blockDim.x >> 6) + wave, n = blockIdx.y;
+    const int held = held_pages(a.seq_lens[n], a.block_size, a.max_blocks);
     const int32_t *row = a.tables + (size_t)n * a.max_blocks;
     const int p0 = blockIdx.z * 16 * a.tiles, p1 = min(p0 + 16 * a.tiles, a.max_blocks);
     const int live = min(p1, held) - p0;  // pages here that the sequence holds
@@ -337,7 +340,7 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
         v = col == 2 ? s[2] : v;
         v = col == 3 ? s[3] : v;
         const int p = 16 * t + 4 * grp + col;
-        if (col < 4 && p < live) out[p] = ids[p] >= 0 ? v : -INFINITY;
+        if (col < 4) found[wave][p] = ids[p] >= 0 ? v : -INFINITY;
     };
     const int tiles = (live + 15) / 16;
     u32x4 in0[LPT];
@@ -358,6 +361,8 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
             if (t + 1 < tiles) load(t + 1, in0);
         }
     }
+    // in whole lines at the end: 64 bytes a tile as they come cost 2 us of 256 contexts' 54
+    for (int p = lane; p < live; p += 64) out[p] = found[wave][p];
 }
 
 // Any shape and type: one wave per (page, kv-head, sequence), lanes over the
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(kThreads) page_scores_generic_kernel(ScoreArgs
     if (page >= a.max_blocks) return;
     const int D = a.head_dim, G = a.num_heads / a.num_kv_heads;
     float best = -INFINITY;
-    const int blk = page < held_pages(a, n) ? a.tables[(size_t)n * a.max_blocks + page] : -1;
+    const int blk = page < held_pages(a.seq_lens[n], a.block_size, a.max_blocks) ? a.tables[(size_t)n * a.max_blocks + page] : -1;
     if (blk >= 0 && blk < a.num_blocks) {
         const char *lo = a.bounds + ((size_t)blk * a.num_kv_heads + kvh) * 2 * D * ES, *hi = lo + (size_t)D * ES;
         for (int j = 0; j < G; ++j) {
@@ -424,25 +429,29 @@ select_pages_kernel(const float *__restrict__ scores, const int32_t *__restrict_
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int hkv = gridDim.x, n = blockIdx.y;
     const size_t rowi = (size_t)n * hkv + blockIdx.x;
-    const int64_t len = max(seq_lens[n], 0);
-    const int held = (int)min((len + block_size - 1) / block_size, (int64_t)width);
+    const float *row = scores + rowi * (size_t)width;
+    const int len = seq_lens[n];
+    uint32_t key[R];  // first the scores' bits: all loads before any use
+    if constexpr (W == 1) {  // (narrow rows: not behind the length's load, though it may leave few of them)
+#pragma unroll
+        for (int r = 0; r < R; ++r) key[r] = __float_as_uint(row[min(r * 64 + lane, width - 1)]);
+    }
+    const float first = row[min(sink, width - 1)];
+    const int held = held_pages(len, block_size, width);
     int32_t *out = pages + rowi * (size_t)k;
     if (held <= k) {  // all of them
         for (int i = threadIdx.x; i < k; i += 64 * W) out[i] = i < held ? i : -1;
         return;
     }
-    const float *row = scores + rowi * (size_t)width;
     const int free0 = sink, free1 = held - recent;  // pages that compete (at least one: held > k >= sink + recent)
     if constexpr (W > 1) {
         if (threadIdx.x < 32) count_s[threadIdx.x] = 0;
         if (threadIdx.x == 0) diff_s = 0;
     }
-    uint32_t key[R];  // first the scores' bits: all loads before any use
-    const uint32_t base = score_key(row[free0]);
+    const uint32_t base = score_key(first);
+    if constexpr (W > 1) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int p = (w * R + r) * 64 + lane;
-        key[r] = __float_as_uint(row[min(p, held - 1)]);
+        for (int r = 0; r < R; ++r) key[r] = __float_as_uint(row[min((w * R + r) * 64 + lane, held - 1)]);
     }
     uint32_t diff = 0;  // bits in which competing keys differ from the first one
 #pragma unroll
@@ -609,16 +618,16 @@ int zk_page_scores(const void *q, zk_dtype q_dtype, const void *bounds, zk_dtype
     const bool mfma = scores_mfma(q_dtype, kv_dtype, head_dim, G) && (((uintptr_t)q | (uintptr_t)bounds) & 15u) == 0;
     if (mfma) {
         // Long stretches a wave as long as there are enough of them; us with 8, 12 and 16
-        // tiles to begin with: 256 contexts of 512 to 8192 tokens 57.8, 56.1, 61.1; 256 of
-        // 8192 100.6, 99.6, 95.2; 2 of 100000 and more (fp8) 8.5, 7.7, 8.5; 64 of f32 38.1,
-        // 39.3, 38.1
+        // tiles to begin with: 256 contexts of 512 to 8192 tokens 53.4, 53.8, 58.6; 256 of
+        // 8192 98.0, 96.1, 92.1; 2 of 100000 and more (fp8) 8.6, 7.7, 8.6; 64 of f32 38.2,
+        // 34.4, 38.1
         a.tiles = 12;
         auto groups = [&](int tiles) {
             return (int64_t)num_seqs * num_kv_heads * ((max_blocks_per_seq + 16 * tiles - 1) / (16 * tiles));  // of a wave
         };
         while (a.tiles > 1 && groups(a.tiles) < 2048) a.tiles /= 2;
         while ((max_blocks_per_seq + 16 * a.tiles - 1) / (16 * a.tiles) > 65535 && a.tiles < kScoreTiles) a.tiles *= 2;
-        const dim3 grid(num_seqs, (num_kv_heads + kScoreHeads - 1) / kScoreHeads,
+        const dim3 grid((num_kv_heads + kScoreHeads - 1) / kScoreHeads, num_seqs,
                         (max_blocks_per_seq + 16 * a.tiles - 1) / (16 * a.tiles));
         if (kv_dtype == ZK_F32) launch_scores<ZK_F32>(a, grid, s);
         else if (kv_dtype == ZK_BF16) launch_scores<ZK_BF16>(a, grid, s);
