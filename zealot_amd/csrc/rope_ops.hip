@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
     typedef const __attribute__((address_space(4))) int64_t *clong_t;
     const int D = a.head_dim, half = a.rot_dim / 2;
     const int lanes = a.lanes, l = threadIdx.x & (lanes - 1), d0 = l * V;
-    const int groups = kThreads / lanes, step = groups * gridDim.y;
+    const int groups = (int)blockDim.x / lanes, step = groups * gridDim.y;
     const int hg = blockIdx.y * groups + threadIdx.x / lanes;  // this lane's heads: hg + j * step
     const bool live = d0 < D, pool = a.k_pool != nullptr;
     const int heads = a.num_heads + (pool ? 2 : 1) * a.num_kv_heads;
@@ -379,14 +379,19 @@ void launch(const RopeArgs &a, bool vec, int heads, hipStream_t s) {
         qk_norm_rope_generic_kernel<T><<<dim3((unsigned)a.num_tokens, heads), 64, 0, s>>>(a);
         return;
     }
+    // What a wave does once a token is shared by its heads, so a token gets as few
+    // waves as four passes over them allow (8000 tokens of 20 + 2 x 4 heads of 96: 26 us
+    // with four waves a token, 22 with two).
+    int threads = kThreads;
+    while (threads > 64 && heads * a.lanes <= threads / 2 * 4) threads /= 2;
     // Few tokens: the heads of a token over several workgroups, down to one
-    // pass of 256 / lanes heads each; many heads: at most four passes.
-    const int passes = (heads * a.lanes + kThreads - 1) / kThreads;
+    // pass of threads / lanes heads each; many heads: at most four passes.
+    const int passes = (heads * a.lanes + threads - 1) / threads;
     const int64_t fill = 2048 / std::max<int64_t>(1, a.num_tokens);
     const int y = std::max((passes + 3) / 4, (int)std::max<int64_t>(1, std::min<int64_t>(passes, fill)));
     const int np = (passes + y - 1) / y;
     const dim3 grid((unsigned)a.num_tokens, y);
-    auto go = [&](auto rotate_half, auto inter) { (a.interleaved ? inter : rotate_half)<<<grid, kThreads, 0, s>>>(a); };
+    auto go = [&](auto rotate_half, auto inter) { (a.interleaved ? inter : rotate_half)<<<grid, threads, 0, s>>>(a); };
     if (np <= 1) go(qk_norm_rope_kernel<T, 1, false>, qk_norm_rope_kernel<T, 1, true>);
     else if (np <= 2) go(qk_norm_rope_kernel<T, 2, false>, qk_norm_rope_kernel<T, 2, true>);
     else if (np <= 3) go(qk_norm_rope_kernel<T, 3, false>, qk_norm_rope_kernel<T, 3, true>);
