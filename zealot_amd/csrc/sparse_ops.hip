@@ -362,6 +362,7 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
         }
     }
     // in whole lines at the end: 64 bytes a tile as they come cost 2 us of 256 contexts' 54
+    __builtin_amdgcn_wave_barrier();
     for (int p = lane; p < live; p += 64) out[p] = found[wave][p];
 }
 
