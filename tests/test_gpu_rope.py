@@ -204,6 +204,27 @@ def test_with_the_kv_write(T, H, Hkv, D, bs, dtype, kind):
         assert bool((rows[other] == 3.0).all())
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,Hkv,D", [(20, 4, 96), (64, 8, 128), (32, 32, 128), (16, 8, 64), (40, 2, 256)])
+def test_many_tokens_of_many_heads(H, Hkv, D, dtype, interleaved):
+    """Every number of heads a lane and of waves a token, past the last whole group of tokens."""
+    from zealot_amd import dense, ops
+    T = 2100
+    q, k, v, (wq, wk) = _inputs(T + D, T, H, Hkv, D, dtype)
+    table, pos = dense.rope_table(500, D), _positions(5, T, 500)
+    kp, vp = _pools(140, Hkv, 16, D, "f32" if dtype == torch.float32 else "bf16")
+    slots = torch.randperm(140 * 16, generator=torch.Generator().manual_seed(3))[:T]
+    qo = ops.qk_norm_rope_append(kp, vp, q, k, v, pos, slots.cuda(), table, wq, wk, interleaved=interleaved)
+    _close(qo, *_reference(q, wq, pos, table, interleaved), dtype)
+    rows = [p.transpose(1, 2).reshape(-1, Hkv, D)[slots.cuda()] for p in (kp, vp)]
+    _close(rows[0], *_reference(k, wk, pos, table, interleaved), dtype)
+    assert torch.equal(rows[1], v)
+    q2, k2 = dense.qk_norm_rope(q, k, pos, table, wq, wk, interleaved=interleaved)
+    _close(q2, *_reference(q, wq, pos, table, interleaved), dtype)
+    _close(k2, *_reference(k, wk, pos, table, interleaved), dtype)
+
+
 @pytest.mark.parametrize("dtype,kind", [(torch.float32, "f32"), (torch.bfloat16, "bf16")])
 def test_the_fused_call_is_the_two_calls(dtype, kind):
     """Bit for bit where the pool has the source's type."""
