@@ -663,9 +663,13 @@ int zk_select_pages(const float *scores, const int32_t *seq_lens, int num_seqs, 
     auto go = [&](auto kernel, int waves) {
         kernel<<<grid, 64 * waves, 0, s>>>(scores, seq_lens, width, block_size, num_pages, sink, recent, pages);
     };
+    // the fewest waves that hold a row in a few registers a lane (2048 rows of up to 8192
+    // pages with 16 waves of 8 registers 55 us, 8 of 16 43; 32 rows of 16250 with 16 of 32
+    // 24.5, 8 of 32 16.8, 16 of 16 15.1; 32 of 62000 with 8 of 128 114, 16 of 64 64)
     if (width <= 64 * 8) go(select_pages_kernel<1, 8>, 1);
     else if (width <= 64 * 4 * 8) go(select_pages_kernel<4, 8>, 4);
-    else if (width <= 64 * 16 * 8) go(select_pages_kernel<16, 8>, 16);
+    else if (width <= 64 * 8 * 16) go(select_pages_kernel<8, 16>, 8);
+    else if (width <= 64 * 16 * 16) go(select_pages_kernel<16, 16>, 16);
     else if (width <= 64 * 16 * 32) go(select_pages_kernel<16, 32>, 16);
     else go(select_pages_kernel<16, 64>, 16);
     return check_launch("zk_select_pages");
