@@ -141,8 +141,6 @@ def test_sizes_past_the_grids():
                                                  None, D, 1 << 62, None))
         assert rc == BAD and "too many pages" in msg
         assert lib.zk_paged_decode_sparse_workspace_size(4, 32, 8, 128, pages) == 0
-    assert _rc(lib.zk_paged_decode_sparse(D, _lib.BF16, D, D, _lib.BF16, D, D, D, D, 64, 4, 1 << 17, 1 << 17, 128, 16, 100, 50, 0.1, 0, None,
-                                          None, D, 1 << 62, None))[0] == BAD
 
 
 def test_python_entry_points_refuse_host_tensors_and_wrong_shapes():

@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
     __shared__ int wave_sum[kWaves];
     __shared__ float mo[kWaves][kMaxG * (D + 4)], mm[kWaves][kMaxG], mlsum[kWaves][kMaxG];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
-    const int kvh = blockIdx.z, split = blockIdx.y, n = blockIdx.x;
+    const int kvh = blockIdx.x, split = blockIdx.y, n = blockIdx.z;
     const int np = stage_list<kWaves>(a, n, kvh, split, blk, cnt, wave_sum);
     const int H = a.num_heads, G = H / a.num_kv_heads;
     // query pieces, as the lanes read K: bf16 rows (and fp8 ones read 8 bytes at
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(64) sparse_generic_kernel(SparseArgs a) {
     __shared__ int32_t blk[kMaxList], cnt[kMaxList];
     __shared__ float q_s[256][GM], p_s[64][GM];  // a dimension's (token's) heads side by side
     const int lane = threadIdx.x;
-    const int kvh = blockIdx.z, split = blockIdx.y, n = blockIdx.x;
+    const int kvh = blockIdx.x, split = blockIdx.y, n = blockIdx.z;
     const int D = a.head_dim, G = a.num_heads / a.num_kv_heads, H = a.num_heads;
     for (int i = lane; i < GM * D; i += 64) {  // (heads past G: zeros)
         const int j = i / D, d = i - j * D;
@@ -612,7 +612,7 @@ int zk_paged_decode_sparse(const void *q, zk_dtype q_dtype, const void *k_pool, 
                            void *stream) {
     if (q_dtype != ZK_F32 && q_dtype != ZK_BF16) return bad("q dtype must be f32 or bf16");
     if (!valid_dtype(kv_dtype)) return bad("unsupported kv dtype");
-    if (num_seqs < 0 || num_seqs > 65535 || num_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || head_dim <= 0 ||
+    if (num_seqs < 0 || num_seqs > 65535 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
         block_size <= 0 || max_blocks_per_seq <= 0 || num_blocks <= 0 || num_pages <= 0)
         return bad("bad shape");
     if (num_heads % num_kv_heads != 0) return bad("num_heads must be a multiple of num_kv_heads");
@@ -659,9 +659,9 @@ int zk_paged_decode_sparse(const void *q, zk_dtype q_dtype, const void *k_pool, 
     a.grouped = mapping == ZK_GQA_GROUPED;
     a.q_f32 = q_dtype == ZK_F32;
     hipStream_t s = (hipStream_t)stream;
-    // sequences first: 1 % less time on large batches than with the kv-heads first, where
-    // an XCD has one kv-head's pages
-    const dim3 grid(num_seqs, splits, num_kv_heads);
+    // Workgroups go to the 8 XCDs in turn: a sequence's are on all of them this way (with the
+    // sequences first, 1 % less time on 256 lists, a long one among 8 has one XCD alone)
+    const dim3 grid(num_kv_heads, splits, num_seqs);
     const bool mfma = block_size == 16 && mfma_dim(head_dim) &&
                       (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15u) == 0;
     {
