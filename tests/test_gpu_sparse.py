@@ -109,6 +109,20 @@ def test_bounds_of_a_large_batch_of_chunks():
     _same(bounds, want)
 
 
+@pytest.mark.parametrize("lens", [[513], [2000, 97], [1] * 700, [300, 1, 0, 17, 16, 15, 900, 64], [4096], [4097, 3]])
+def test_bounds_of_prompts_of_any_size(lens):
+    """Rows past the last whole group of workgroups, runs that begin anywhere."""
+    from zealot_amd import ops
+    table, nb = _tables(len(lens), [n + 5 for n in lens])
+    flat = table.cpu().numpy()
+    slots = torch.tensor([int(flat[i, x // 16]) * 16 + x % 16 for i, n in enumerate(lens) for x in range(i % 3, n + i % 3)], device="cuda")
+    pool = _randn(1, (nb, 2, 16, 64), "bf16")
+    bounds = torch.stack([pool.amax(2), pool.amin(2)], 2) * 3  # of pages that begin before the run: to be extended
+    want = _bounds_ref(pool, slots, bounds)
+    ops.page_bounds(pool, slots, bounds)
+    _same(bounds, want)
+
+
 def test_bounds_of_keys_that_are_not_finite():
     from zealot_amd import ops
     pool = _randn(4, (4, 2, 16, 64), "bf16")

@@ -131,7 +131,12 @@ page_bounds_kernel(const char *__restrict__ k_pool, const int64_t *__restrict__ 
     constexpr int N = P::N, ES = KV == ZK_F32 ? 4 : KV == ZK_BF16 ? 2 : 1;
     const int lane = threadIdx.x & 63;
     const int ppr = head_dim / N, pieces = hkv * ppr;
-    const int64_t t0 = (int64_t)blockIdx.x * rows;
+    // Workgroups go to the 8 XCDs in turn, and of a prompt's only those work where a page
+    // begins: an XCD takes the rows of 16 tokens in a row (2000 rows of one prompt 7.5 us
+    // in order, which one XCD has alone, 6.2)
+    const int bx = blockIdx.x, per = 16 / rows, span = 8 * per;
+    const int group = (bx | (span - 1)) < (int)gridDim.x ? (bx & ~(span - 1)) | (bx & 7) * per | (bx >> 3 & (per - 1)) : bx;
+    const int64_t t0 = (int64_t)group * rows;
     // lane i: row t0 - 1 + i
     const int64_t t = t0 - 1 + lane;
     const int64_t slot = t >= 0 && t < num_tokens ? slots[t] : -2;
@@ -246,8 +251,10 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
     // Consecutive workgroups go to the XCDs in turn: the kv-heads first, so that a block's
     // rows are not asked for by one XCD at a time (256 contexts 56 us with the sequences
     // first, 54; 64 of f32 39, 34), chunks last, as a sequence's later ones are often
-    // behind its context
-    const int kvh = blockIdx.x * (blockDim.x >> 6) + wave, n = blockIdx.y;
+    // behind its context, and a sequence's chunks in other places of their turns, so that a
+    // long context has all XCDs
+    const int kvh = blockIdx.x * (blockDim.x >> 6) + wave;
+    const int n = (int)(gridDim.y & 1 ? blockIdx.y : (blockIdx.y + blockIdx.z) % gridDim.y);
     const int held = held_pages(a.seq_lens[n], a.block_size, a.max_blocks);
     const int32_t *row = a.tables + (size_t)n * a.max_blocks;
     const int p0 = blockIdx.z * 16 * a.tiles, p1 = min(p0 + 16 * a.tiles, a.max_blocks);
@@ -564,9 +571,10 @@ int zk_page_bounds(const void *k_pool, zk_dtype kv_dtype, const int64_t *slot_ma
     if (!k_pool || !slot_mapping || !bounds)
         return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_bounds: NULL pointer");
     const bool vec = ((size_t)head_dim * elt_size(kv_dtype)) % 16 == 0 && (((uintptr_t)k_pool | (uintptr_t)bounds) & 15u) == 0;
-    // a row a workgroup while that fills the chip no more than a few times, then
-    // four: 26000 rows of prompts 19.4, 12.8, 13.0 and 13.1 us with 1, 4, 8 and 16
-    const int64_t rows = num_tokens <= 4096 ? 1 : 4;
+    // a row a workgroup while that fills the chip no more than a few times, then two and
+    // four: us with 1, 2, 4 and 8, 26000 rows of prompts 19.4, 14.2, 12.9 and 13.1; 2000
+    // of one prompt 6.3, 4.7, 4.5; 1000 and 3000 single tokens 4.2, 5.0, 6.1 and 8.7, 8.0, 9.1
+    const int64_t rows = num_tokens <= 512 ? 1 : num_tokens <= 4096 ? 2 : 4;
     const int64_t groups = (num_tokens + rows - 1) / rows;
     if (groups > 0xffffff)
         return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_page_bounds: too many tokens for one launch");
