@@ -269,7 +269,8 @@ int zk_select_pages(const float *scores, const int32_t *seq_lens, int num_seqs, 
  * A negative entry, one past the table or the length and one whose block lies
  * outside the pool add nothing; a row without tokens is zero.  Operands as in
  * zk_paged_decode; head_dim <= 256, H / Hkv <= 16, num_seqs <= 65535; F32 queries
- * on BF16 and FP8 pools count with 8 bits on the matrix-core kernel's shapes.  workspace:
+ * keep their 24 bits on every pool (zk_paged_decode rounds them to 8 on BF16 and FP8
+ * ones).  workspace:
  * zk_paged_decode_sparse_workspace_size bytes (0: none needed), 256-B aligned. */
 size_t zk_paged_decode_sparse_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
                                              int num_pages);

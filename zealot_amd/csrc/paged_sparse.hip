@@ -11,8 +11,7 @@
 //
 // Bound by HBM: every listed page's K and V are read once for the G = H / Hkv
 // heads that share them.  Softmax in the log2 domain, statistics and sums in
-// f32; f32 queries are rounded to bf16 for the matrix cores on bf16 and fp8 pools,
-// as the decode over all pages does.
+// f32; f32 queries keep their 24 bits on every pool.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -159,9 +158,27 @@ __device__ __forceinline__ void load_words(const char *p, uint32_t *w) {
     }
 }
 
-template <int KV, int D>
+// A value as three bf16 of its sign that add up to it: the leading 8 bits, the next 8
+// and the last.  A part that would be zero is 2^-30 of the value instead (an infinite
+// key times 0 would be NaN), and an infinity or NaN is all three.
+__device__ __forceinline__ void three_parts(float x, float (&part)[3]) {
+    const bool finite = fabsf(x) < INFINITY;
+    const float tiny = x * 0x1p-30f;
+    part[0] = finite ? __uint_as_float(__float_as_uint(x) & 0xffff0000u) : x;
+    const float rest = x - part[0];
+    part[1] = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+    part[2] = rest - part[1];
+#pragma unroll
+    for (int i = 1; i < 3; ++i) part[i] = !finite ? x : part[i] == 0.0f ? tiny : part[i];
+}
+
+// PARTS: bf16 values that a query value is held in: 1, or 3 for f32 queries on bf16
+// and fp8 pools (exact: 24 bits).  256 lists of 64 pages with one part of 8 bits and with
+// three: bf16 pools 175 and 182 us, fp8 100 and 111; 128 of heads of 256 192 and 223.
+template <int KV, int D, int PARTS>
 __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) {
     constexpr bool F32 = KV == ZK_F32;
+    static_assert(!F32 || PARTS == 1, "f32 products take f32 values");
     constexpr int BS = 16, ELT = F32 ? 4 : KV == ZK_BF16 ? 2 : 1, RB = D * ELT;
     constexpr int PG = F32 ? 1 : 2;            // pages a step
     constexpr int CB = RB % 64 ? 8 : 16;       // bytes of a K row that a lane reads at once
@@ -181,25 +198,34 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
     // query pieces, as the lanes read K: bf16 rows (and fp8 ones read 8 bytes at
     // once): dims 32 kk + 8 grp .. + 7; fp8 rows (16 dims in 16 bytes): 64 (kk / 2) +
     // 16 grp + 8 (kk % 2) .. + 7; f32 rows: 16 kk + 4 grp .. + 3
-    u32x4 qf[KK];
+    u32x4 qf[PARTS][KK];
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
         const int d0 = F32 ? 16 * kk + 4 * grp : KV == ZK_BF16 || CB == 8 ? 32 * kk + 8 * grp : 64 * (kk / 2) + 16 * grp + 8 * (kk % 2);
-        u32x4 w = {0u, 0u, 0u, 0u};
+        u32x4 w[PARTS];
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) w[i] = u32x4{0u, 0u, 0u, 0u};
         if (col < G) {
             const size_t at = ((size_t)n * H + qhead_of(a, kvh, col, G)) * D + d0;
             if constexpr (F32) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(load_q(a, at + j));
-            } else if (a.q_f32) {
+                for (int j = 0; j < 4; ++j) w[0][j] = __float_as_uint(load_q(a, at + j));
+            } else if constexpr (PARTS == 3) {
                 const float *p = (const float *)a.q + at;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = bf16x2_rne(p[2 * j], p[2 * j + 1]);
+                for (int j = 0; j < 4; ++j) {
+                    float lo[3], hi[3];
+                    three_parts(p[2 * j], lo);
+                    three_parts(p[2 * j + 1], hi);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) w[i][j] = bf16x2_rne(lo[i], hi[i]);
+                }
             } else {
-                w = *reinterpret_cast<const u32x4 *>((const uint16_t *)a.q + at);
+                w[0] = *reinterpret_cast<const u32x4 *>((const uint16_t *)a.q + at);
             }
         }
-        qf[kk] = w;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) qf[i][kk] = w[i];
     }
     float sl2 = a.scale_log2, vscale = 1.0f;
     if constexpr (KV == ZK_FP8_E4M3) {
@@ -241,7 +267,7 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         f32x4 &t = e & 1 ? s2 : s;
-                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[h][c][e]), __uint_as_float(qf[c][e]), t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[h][c][e]), __uint_as_float(qf[0][c][e]), t, 0, 0, 0);
                     }
                 s += s2;
             } else {
@@ -255,8 +281,10 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
                         const u32x2 lo = e4m3x4_to_bf16x4(c8[0]), hi = e4m3x4_to_bf16x4(c8[1]);
                         w = u32x4{lo[0], lo[1], hi[0], hi[1]};
                     }
-                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w),
-                                                                __builtin_bit_cast(bf16x8, qf[kk]), s, 0, 0, 0);
+#pragma unroll
+                    for (int i = PARTS - 1; i >= 0; --i)
+                        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w),
+                                                                    __builtin_bit_cast(bf16x8, qf[i][kk]), s, 0, 0, 0);
                 }
             }
 #pragma unroll
@@ -578,12 +606,17 @@ int check_launch(const char *what) {
     return ZK_OK;
 }
 
+template <int KV, int PARTS>
+void launch_mfma(const SparseArgs &a, dim3 grid, hipStream_t s) {
+    if (a.head_dim == 64) sparse_mfma_kernel<KV, 64, PARTS><<<grid, 64 * kWaves, 0, s>>>(a);
+    else if (a.head_dim == 96) sparse_mfma_kernel<KV, 96, PARTS><<<grid, 64 * kWaves, 0, s>>>(a);
+    else if (a.head_dim == 128) sparse_mfma_kernel<KV, 128, PARTS><<<grid, 64 * kWaves, 0, s>>>(a);
+    else sparse_mfma_kernel<KV, 256, PARTS><<<grid, 64 * kWaves, 0, s>>>(a);
+}
 template <int KV>
 void launch(const SparseArgs &a, dim3 grid, int G, bool mfma, hipStream_t s) {
-    if (mfma && a.head_dim == 64) sparse_mfma_kernel<KV, 64><<<grid, 64 * kWaves, 0, s>>>(a);
-    else if (mfma && a.head_dim == 96) sparse_mfma_kernel<KV, 96><<<grid, 64 * kWaves, 0, s>>>(a);
-    else if (mfma && a.head_dim == 128) sparse_mfma_kernel<KV, 128><<<grid, 64 * kWaves, 0, s>>>(a);
-    else if (mfma) sparse_mfma_kernel<KV, 256><<<grid, 64 * kWaves, 0, s>>>(a);
+    if (mfma && a.q_f32 && KV != ZK_F32) launch_mfma<KV, KV == ZK_F32 ? 1 : 3>(a, grid, s);
+    else if (mfma) launch_mfma<KV, 1>(a, grid, s);
     else if (G <= 4) sparse_generic_kernel<KV, 4><<<grid, 64, 0, s>>>(a);
     else if (G <= 8) sparse_generic_kernel<KV, 8><<<grid, 64, 0, s>>>(a);
     else sparse_generic_kernel<KV, 16><<<grid, 64, 0, s>>>(a);
