@@ -1,0 +1,135 @@
+"""A row's norm and rotation is the same, bit for bit, whatever the call's other
+operands are: their alignment and strides, how many heads share the call, and
+whether K goes to a tensor or to a pool of the source's type."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+KINDS = [torch.float32, torch.bfloat16]
+# (heads, kv-heads, head size, rotated dimensions)
+SHAPES = [(32, 8, 128, 128), (6, 2, 64, 64), (20, 4, 96, 96), (4, 2, 128, 64), (3, 1, 256, 256), (70, 2, 64, 64), (2, 1, 17, 16), (3, 2, 34, 30)]
+
+
+def _problem(seed, T, H, Hkv, D, rot, dtype):
+    from zealot_amd import dense
+    g = torch.Generator().manual_seed(seed)
+    x = {"q": torch.randn(T, H, D, generator=g), "k": torch.randn(T, Hkv, D, generator=g), "v": torch.randn(T, Hkv, D, generator=g)}
+    x = {n: t.to(dtype).cuda() for n, t in x.items()}
+    x["q_weight"], x["k_weight"] = [(1 + 0.2 * torch.randn(D, generator=g)).to(dtype).cuda() for _ in range(2)]
+    x["rope"] = dense.rope_table(300, rot)
+    x["positions"] = torch.randint(0, 300, (T,), generator=g, dtype=torch.int32).cuda()
+    x["slots"] = torch.randperm((T // 16 + 2) * 16, generator=g)[:T].cuda()
+    x["k_pool"], x["v_pool"] = [torch.zeros(T // 16 + 2, Hkv, 16, D, dtype=dtype, device="cuda") for _ in range(2)]
+    return x
+
+
+def _off(t):
+    """The same values one element behind a vector's border."""
+    buf = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+    buf[1:] = t.flatten()
+    return buf[1:].view(t.shape)
+
+
+def _odd_rows(t):
+    """The same rows, an odd number of elements apart."""
+    buf = torch.empty(t.shape[0], t.shape[1] * t.shape[2] + 1, dtype=t.dtype, device="cuda")
+    buf[:, :-1] = t.flatten(1)
+    return buf[:, :-1].unflatten(1, t.shape[1:])
+
+
+def _fused(x, interleaved):
+    from zealot_amd import ops
+    kp, vp = x["k_pool"], x["v_pool"]
+    kp.zero_()
+    vp.zero_()
+    q = ops.qk_norm_rope_append(kp, vp, x["q"], x["k"], x["v"], x["positions"], x["slots"], x["rope"], x["q_weight"], x["k_weight"],
+                                interleaved=interleaved, q_out=x.get("q_out"))
+    return q.clone(), kp.clone(), vp.clone()
+
+
+def _separate(x, interleaved):
+    from zealot_amd import dense, ops
+    kp, vp = torch.zeros_like(x["k_pool"]), torch.zeros_like(x["v_pool"])
+    q, k = dense.qk_norm_rope(x["q"], x["k"], x["positions"], x["rope"], x["q_weight"], x["k_weight"], interleaved=interleaved,
+                              q_out=x.get("q_out"), k_out=x.get("k_out"))
+    ops.append(kp, vp, k.contiguous(), x["v"].contiguous(), x["slots"])
+    return q.clone(), kp, vp
+
+
+@pytest.mark.parametrize("dtype", KINDS)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("H,Hkv,D,rot", SHAPES)
+def test_alignment_and_strides(H, Hkv, D, rot, interleaved, dtype):
+    x = _problem(H + D, 37, H, Hkv, D, rot, dtype)
+    want = _fused(x, interleaved)
+    for got in (_separate(x, interleaved),):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for name in ("q", "k", "v", "q_weight", "k_weight", "rope", "k_pool", "v_pool", "q_out", "k_out", "q/", "k/", "v/", "q_out/"):
+        y = dict(x)
+        if name.startswith("q_out"):
+            y["q_out"] = torch.empty_like(x["q"])
+        if name == "k_out":
+            y["k_out"] = _off(torch.empty_like(x["k"]))
+        elif name.endswith("/"):
+            y[name[:-1]] = _odd_rows(y[name[:-1]])
+        else:
+            y[name] = _off(y[name])
+        for call in (_fused, _separate):
+            got = call(y, interleaved)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (name, call.__name__)
+
+
+@pytest.mark.parametrize("dtype", KINDS)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_other_heads_of_the_call(interleaved, dtype):
+    """One head's rows alone, and among enough heads and tokens for every number of heads a lane."""
+    from zealot_amd import dense
+    T = 2500
+    for H, Hkv in ((8, 2), (24, 8), (40, 8), (56, 8), (72, 8)):
+        x = _problem(H, T, H, Hkv, 128, 128, dtype)
+        how = dict(interleaved=interleaved)
+        q, k = dense.qk_norm_rope(x["q"], x["k"], x["positions"], x["rope"], x["q_weight"], x["k_weight"], **how)
+        one = dense.qk_norm_rope(x["q"][:, :1], x["k"][:, :1], x["positions"], x["rope"], x["q_weight"], x["k_weight"], **how)
+        assert torch.equal(q[:, :1], one[0]) and torch.equal(k[:, :1], one[1])
+        got = _fused(x, interleaved)
+        assert torch.equal(got[0], q) and torch.equal(got[1].transpose(1, 2).flatten(0, 1)[x["slots"]], k)
+
+
+@pytest.mark.parametrize("dtype", KINDS)
+@pytest.mark.parametrize("which", [(True, False), (False, True), (False, False)])
+def test_without_weights_or_a_table(which, dtype):
+    x = _problem(5, 30, 6, 2, 128, 128, dtype)
+    for name, on in zip(("q_weight", "k_weight"), which):
+        if not on:
+            x[name] = None
+    for table in (x["rope"], None):
+        x["rope"] = table
+        want = _fused(x, False)
+        for name in ("q", "v", "v_pool"):
+            y = dict(x)
+            y[name] = _off(y[name])
+            for call in (_fused, _separate):
+                assert all(torch.equal(a, b) for a, b in zip(call(y, False), want)), (name, call.__name__)
+
+
+@pytest.mark.parametrize("pool", ["f32", "bf16", "fp8"])
+@pytest.mark.parametrize("dtype", KINDS)
+def test_pools_of_other_types(dtype, pool):
+    """Off their alignment and on it: the same bytes."""
+    from zealot_amd import ops
+    T, H, Hkv, D = 50, 4, 2, 64
+    x = _problem(6, T, H, Hkv, D, D, dtype)
+    t = {"f32": torch.float32, "bf16": torch.bfloat16, "fp8": torch.float8_e4m3fn}[pool]
+    more = {}
+    if pool == "fp8":
+        more = dict(k_scales=torch.full((2, Hkv), 0.02, device="cuda"), v_scales=torch.full((2, Hkv), 0.03, device="cuda"),
+                    token_row=(torch.arange(T, dtype=torch.int32) % 2).cuda())
+    outs = []
+    for off in (False, True):
+        n = x["k_pool"].numel()
+        raw = [torch.zeros(n + 1, device="cuda").to(t) for _ in range(2)]
+        kp, vp = [r[int(off):n + int(off)].view(x["k_pool"].shape) for r in raw]
+        q = ops.qk_norm_rope_append(kp, vp, x["q"], x["k"], x["v"], x["positions"], x["slots"], x["rope"], x["q_weight"], x["k_weight"], **more)
+        outs.append((q, kp.contiguous().view(torch.uint8) if pool == "fp8" else kp, vp.contiguous().view(torch.uint8) if pool == "fp8" else vp))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))

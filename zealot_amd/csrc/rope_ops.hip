@@ -43,7 +43,7 @@ template <> struct Elt<float> {
     static __device__ __forceinline__ float squares(u32x4 v) {
         float s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s += __uint_as_float(v[e]) * __uint_as_float(v[e]);
+        for (int e = 0; e < 4; ++e) s = fmaf(__uint_as_float(v[e]), __uint_as_float(v[e]), s);
         return s;
     }
     static __device__ __forceinline__ float get(const float *p) { return *p; }
@@ -75,10 +75,38 @@ template <> struct Elt<uint16_t> {  // bf16 bits
     static __device__ __forceinline__ void put(uint16_t *p, float x) { *p = (uint16_t)f32_to_bf16_bits(x); }
 };
 
+// A vector of the element type T at p: one access at its own alignment (nontemporal
+// where NT), or accesses of T for operands off it (OFF).
+template <typename T, bool OFF, bool NT>
+__device__ __forceinline__ u32x4 load_vec(const T *p) {
+    if constexpr (OFF) {
+        u32x4 v;
+        __builtin_memcpy(&v, p, 16);
+        return v;
+    } else if constexpr (NT) {
+        return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+    } else {
+        return *reinterpret_cast<const u32x4 *>(p);
+    }
+}
+template <typename T, bool OFF>
+__device__ __forceinline__ void store_vec(T *p, u32x4 v) {
+    if constexpr (OFF) __builtin_memcpy(p, &v, 16);
+    else __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(p));
+}
+
+__device__ __forceinline__ void put_pool(void *pool, int dt, size_t at, float x, float inv) {
+    if (dt == ZK_BF16) ((uint16_t *)pool)[at] = (uint16_t)f32_to_bf16_bits(x);
+    else if (dt == ZK_F32) ((float *)pool)[at] = x;
+    else ((uint8_t *)pool)[at] = (uint8_t)(e4m3x4(x * inv, 0.f, 0.f, 0.f) & 0xffu);
+}
 // V values to element `at` of a pool of type `dt`, inv: 1 / scale of an fp8 pool.
-template <int V>
+template <int V, bool OFF>
 __device__ __forceinline__ void store_pool(void *pool, int dt, size_t at, const float *x, float inv) {
-    if (dt == ZK_BF16) {
+    if constexpr (OFF) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) put_pool(pool, dt, at + e, x[e], inv);
+    } else if (dt == ZK_BF16) {
         if constexpr (V == 8) {
             __builtin_nontemporal_store(Elt<uint16_t>::pack(x), reinterpret_cast<u32x4 *>((uint16_t *)pool + at));
         } else {
@@ -95,11 +123,6 @@ __device__ __forceinline__ void store_pool(void *pool, int dt, size_t at, const 
             reinterpret_cast<uint32_t *>((uint8_t *)pool + at)[j] =
                 e4m3x4(x[4 * j] * inv, x[4 * j + 1] * inv, x[4 * j + 2] * inv, x[4 * j + 3] * inv);
     }
-}
-__device__ __forceinline__ void put_pool(void *pool, int dt, size_t at, float x, float inv) {
-    if (dt == ZK_BF16) ((uint16_t *)pool)[at] = (uint16_t)f32_to_bf16_bits(x);
-    else if (dt == ZK_F32) ((float *)pool)[at] = x;
-    else ((uint8_t *)pool)[at] = (uint8_t)(e4m3x4(x * inv, 0.f, 0.f, 0.f) & 0xffu);
 }
 
 // Row index in the pools of a slot's token (of head 0; heads are block_size
@@ -136,7 +159,12 @@ __device__ __forceinline__ float lane_sum(float x, int lanes) {
 // plain loads and stores).  And its waves must be many (82 registers, six a
 // SIMD): workgroups that walk the tokens and load the next one ahead hold 180-200
 // registers, two waves a SIMD, and took 178-217 us.
-template <typename T, int NP, bool INTER>
+//
+// Sums and products are written out as they are to be rounded (fmaf), so that a row's
+// result is the same in every variant, whatever the call's other operands are: the
+// fused call's K is bit for bit the separate calls'.  OFF: operands off a vector's
+// alignment.
+template <typename T, int NP, bool INTER, bool OFF>
 __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
     constexpr int V = Elt<T>::V, TV = INTER ? V / 2 : V;  // cosines of a lane
     // read only: scalar loads, apart from the vector loads' order
@@ -162,12 +190,12 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
         for (int e = 0; e < V; ++e) one[e] = 1.0f;
         wq = wk = uq = uk = Elt<T>::pack(one);
         if (live && a.q_weight) {
-            wq = *reinterpret_cast<const u32x4 *>((const T *)a.q_weight + d0);
-            uq = *reinterpret_cast<const u32x4 *>((const T *)a.q_weight + d0 + away * V);
+            wq = load_vec<T, OFF, false>((const T *)a.q_weight + d0);
+            uq = load_vec<T, OFF, false>((const T *)a.q_weight + d0 + away * V);
         }
         if (live && a.k_weight) {
-            wk = *reinterpret_cast<const u32x4 *>((const T *)a.k_weight + d0);
-            uk = *reinterpret_cast<const u32x4 *>((const T *)a.k_weight + d0 + away * V);
+            wk = load_vec<T, OFF, false>((const T *)a.k_weight + d0);
+            uk = load_vec<T, OFF, false>((const T *)a.k_weight + d0 + away * V);
         }
     }
     // Workgroups go to the 8 XCDs in turn: of each 128 tokens an XCD takes 16 in a row,
@@ -183,8 +211,8 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
         const int64_t stride = q_row ? a.q_stride : vh < 0 ? a.k_stride : a.v_stride;
         const T *p = q_row ? (const T *)a.q : vh < 0 ? (const T *)a.k : (const T *)a.v;
         if (live && h < heads) p += (size_t)(kh < 0 ? h : vh < 0 ? kh : vh) * D + d0;
-        raw[j] = __builtin_nontemporal_load(
-            reinterpret_cast<const u32x4 *>((const char *)p + (uint64_t)(uint32_t)t * (uint32_t)(sizeof(T) * stride)));
+        if constexpr (OFF) raw[j] = load_vec<T, true, true>(p + t * stride);
+        else raw[j] = load_vec<T, false, true>((const T *)((const char *)p + (uint64_t)(uint32_t)t * (uint32_t)(sizeof(T) * stride)));
         has_q = has_q || kh < 0;
         has_k = has_k || (kh >= 0 && vh < 0);
     }
@@ -193,7 +221,13 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
     f32x4 cs[V / 4], sn[V / 4];  // cosines and sines of this lane's pairs
     if (rot) {
         const float *row = a.rope + (zero ? 0 : (size_t)pos * a.rot_dim) + at_table;
-        if constexpr (TV >= 4) {
+        if constexpr (OFF) {
+#pragma unroll
+            for (int e = 0; e < TV; ++e) {
+                cs[e / 4][e % 4] = row[e];
+                sn[e / 4][e % 4] = row[half + e];
+            }
+        } else if constexpr (TV >= 4) {
 #pragma unroll
             for (int e = 0; e < TV / 4; ++e) {
                 cs[e] = *reinterpret_cast<const f32x4 *>(row + 4 * e);
@@ -229,7 +263,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
         float inv = 1.0f;
         if (norm) {
             const float ss = Elt<T>::squares(v);
-            inv = rsqrtf(lane_sum(live ? ss : 0.0f, lanes) * a.inv_dim + a.eps);
+            inv = rsqrtf(fmaf(lane_sum(live ? ss : 0.0f, lanes), a.inv_dim, a.eps));
         }
         if (!rot) {
 #pragma unroll
@@ -250,7 +284,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
 #pragma unroll
             for (int e = 0; e < V; ++e) p[e] = rotated ? p[e] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) y[e] = (x[e] * m.c[e] + p[e] * m.s[e]) * inv;
+        for (int e = 0; e < V; ++e) y[e] = fmaf(x[e], m.c[e], p[e] * m.s[e]) * inv;
     };
     const int64_t prow = pool ? pool_row(a, ((clong_t)a.slots)[t]) : 0;
     auto to_pool = [&](bool is_v, int hd, const float *y) {
@@ -258,7 +292,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
         float f = 1.0f;
         if (a.cache_dtype == ZK_FP8_E4M3)
             f = 1.0f / (is_v ? a.v_scales : a.k_scales)[(size_t)((cint_t)a.token_row)[t] * a.num_kv_heads + hd];
-        store_pool<V>(is_v ? a.v_pool : a.k_pool, a.cache_dtype, ((size_t)prow + (size_t)hd * a.block_size) * D + d0, y, f);
+        store_pool<V, OFF>(is_v ? a.v_pool : a.k_pool, a.cache_dtype, ((size_t)prow + (size_t)hd * a.block_size) * D + d0, y, f);
     };
     // queries, keys, values: a wave skips what none of its lanes holds
     if (has_q) {
@@ -272,9 +306,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
             turn(raw[j], m, a.q_weight != nullptr, y);
             u32x4 w = Elt<T>::pack(y);
             if (zero) w = u32x4{0u, 0u, 0u, 0u};
-            if (live)
-                __builtin_nontemporal_store(
-                    w, reinterpret_cast<u32x4 *>((T *)a.q_out + t * a.q_out_stride + (size_t)h * D + d0));
+            if (live) store_vec<T, OFF>((T *)a.q_out + t * a.q_out_stride + (size_t)h * D + d0, w);
         }
     }
     if (has_k) {
@@ -291,9 +323,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
                 for (int e = 0; e < V; ++e) y[e] = 0.0f;
             if (!live) continue;
             if (pool) to_pool(false, kh, y);
-            else
-                __builtin_nontemporal_store(
-                    Elt<T>::pack(y), reinterpret_cast<u32x4 *>((T *)a.k_out + t * a.k_out_stride + (size_t)kh * D + d0));
+            else store_vec<T, OFF>((T *)a.k_out + t * a.k_out_stride + (size_t)kh * D + d0, Elt<T>::pack(y));
         }
     }
     if (pool)
@@ -307,8 +337,8 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
         }
 }
 
-// Any shape and alignment up to kMaxDim: one wave per (token, head), the row
-// in LDS.
+// Head sizes and rotations that are not whole vectors, up to kMaxDim: one wave per
+// (token, head), the row in LDS.
 template <typename T>
 __global__ void __launch_bounds__(64) qk_norm_rope_generic_kernel(RopeArgs a) {
     __shared__ float row[kMaxDim];
@@ -373,8 +403,10 @@ bool rows_overlap(const void *a, int64_t a_stride, int64_t a_width, const void *
     return d < a_width * elt || d + b_width * elt > s;
 }
 
+// vec: rows are whole vectors (by the shape alone); off: some operand is off their
+// alignment, or its rows are too far apart for 32-bit steps.
 template <typename T>
-void launch(const RopeArgs &a, bool vec, int heads, hipStream_t s) {
+void launch(const RopeArgs &a, bool vec, bool off, int heads, hipStream_t s) {
     if (!vec) {
         qk_norm_rope_generic_kernel<T><<<dim3((unsigned)a.num_tokens, heads), 64, 0, s>>>(a);
         return;
@@ -389,16 +421,21 @@ void launch(const RopeArgs &a, bool vec, int heads, hipStream_t s) {
     // 64 + 2 x 8 heads: 61 us as two workgroups of three, 57; six passes of f32 62.4 as
     // two of three, 63.2 as one).
     const int passes = (heads * a.lanes + threads - 1) / threads;
+    if (off) {  // one head a lane
+        const dim3 grid((unsigned)a.num_tokens, passes);
+        (a.interleaved ? qk_norm_rope_kernel<T, 1, true, true> : qk_norm_rope_kernel<T, 1, false, true>)<<<grid, threads, 0, s>>>(a);
+        return;
+    }
     const int64_t fill = 2048 / std::max<int64_t>(1, a.num_tokens);
     const int y = std::max((passes + 4) / 5, (int)std::max<int64_t>(1, std::min<int64_t>(passes, fill)));
     const int np = (passes + y - 1) / y;
     const dim3 grid((unsigned)a.num_tokens, y);
     auto go = [&](auto rotate_half, auto inter) { (a.interleaved ? inter : rotate_half)<<<grid, threads, 0, s>>>(a); };
-    if (np <= 1) go(qk_norm_rope_kernel<T, 1, false>, qk_norm_rope_kernel<T, 1, true>);
-    else if (np <= 2) go(qk_norm_rope_kernel<T, 2, false>, qk_norm_rope_kernel<T, 2, true>);
-    else if (np <= 3) go(qk_norm_rope_kernel<T, 3, false>, qk_norm_rope_kernel<T, 3, true>);
-    else if (np <= 4) go(qk_norm_rope_kernel<T, 4, false>, qk_norm_rope_kernel<T, 4, true>);
-    else go(qk_norm_rope_kernel<T, 5, false>, qk_norm_rope_kernel<T, 5, true>);
+    if (np <= 1) go(qk_norm_rope_kernel<T, 1, false, false>, qk_norm_rope_kernel<T, 1, true, false>);
+    else if (np <= 2) go(qk_norm_rope_kernel<T, 2, false, false>, qk_norm_rope_kernel<T, 2, true, false>);
+    else if (np <= 3) go(qk_norm_rope_kernel<T, 3, false, false>, qk_norm_rope_kernel<T, 3, true, false>);
+    else if (np <= 4) go(qk_norm_rope_kernel<T, 4, false, false>, qk_norm_rope_kernel<T, 4, true, false>);
+    else go(qk_norm_rope_kernel<T, 5, false, false>, qk_norm_rope_kernel<T, 5, true, false>);
 }
 
 }  // namespace
@@ -469,20 +506,20 @@ int zk::qk_norm_rope(const RopeArgs &in, hipStream_t s) {
     const int V = 16 / e, D = a.head_dim, half = a.rot_dim / 2;
     auto mult = [&](int64_t stride) { return stride % V == 0; };
     auto al = [](const void *p) { return ((uintptr_t)p & 15u) == 0; };
-    bool vec = D % V == 0 && D / V <= 64 && (a.interleaved ? a.rot_dim % V == 0 : half % V == 0) && mult(a.q_stride) &&
-               mult(a.k_stride) && mult(a.q_out_stride) && al(a.q) && al(a.k) && al(a.q_out) && al(a.q_weight) &&
-               al(a.k_weight) && (!a.rot_dim || al(a.rope));
-    if (pool) vec = vec && mult(a.v_stride) && al(a.v) && al(a.k_pool) && al(a.v_pool);
-    else vec = vec && mult(a.k_out_stride) && al(a.k_out);
-    vec = vec && std::max({a.q_stride, a.k_stride, pool ? a.v_stride : 0}) * e < (1ll << 32);  // (32-bit steps)
+    const bool vec = D % V == 0 && D / V <= 64 && (a.interleaved ? a.rot_dim % V == 0 : half % V == 0);
+    bool on = mult(a.q_stride) && mult(a.k_stride) && mult(a.q_out_stride) && al(a.q) && al(a.k) && al(a.q_out) &&
+              al(a.q_weight) && al(a.k_weight) && (!a.rot_dim || al(a.rope));
+    if (pool) on = on && mult(a.v_stride) && al(a.v) && al(a.k_pool) && al(a.v_pool);
+    else on = on && mult(a.k_out_stride) && al(a.k_out);
+    on = on && std::max({a.q_stride, a.k_stride, pool ? a.v_stride : 0}) * e < (1ll << 32);  // (32-bit steps)
     int lanes = 1;
     while (lanes * V < D) lanes *= 2;
     a.lanes = lanes;
     a.inv_dim = 1.0f / (float)D;
     const int heads = a.num_heads + (pool ? 2 : 1) * a.num_kv_heads;
     KernelTimer timer("qk_norm_rope", s);
-    if (a.dtype == ZK_BF16) launch<uint16_t>(a, vec, heads, s);
-    else launch<float>(a, vec, heads, s);
+    if (a.dtype == ZK_BF16) launch<uint16_t>(a, vec, !on, heads, s);
+    else launch<float>(a, vec, !on, heads, s);
     if (hipError_t er = hipGetLastError(); er != hipSuccess)
         return set_error(ZK_ERR_HIP, std::string("Internal error: zk_qk_norm_rope: ") + hipGetErrorString(er));
     return ZK_OK;
