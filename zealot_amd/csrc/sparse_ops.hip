@@ -313,6 +313,7 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
             const int slot = 64 * j + lane, r = slot / CPR, c = slot % CPR;
             *reinterpret_cast<u32x4 *>(lds + r * LDR + c * 16) = in[j];
         }
+        wave_sync();  // rows go to other lanes than loaded them
         f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int c = 0; c < CPR / 4; ++c) {
@@ -333,6 +334,7 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
                 }
             }
         }
+        wave_sync();  // the next tile's rows come behind these reads
         f32x4 s = acc[0] + acc[1];  // column col's scores of the tile's pages 4 grp + i
 #pragma unroll
         for (int i = 0; i < 4; ++i) {  // maximum over the 16 columns
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(64 * kScoreHeads) page_scores_mfma_kernel(Scor
         }
     }
     // in whole lines at the end: 64 bytes a tile as they come cost 2 us of 256 contexts' 54
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     for (int p = lane; p < live; p += 64) out[p] = found[wave][p];
 }
 
