@@ -463,14 +463,29 @@ select_pages_kernel(const float *__restrict__ scores, const int32_t *__restrict_
 #pragma unroll
         for (int r = 0; r < R; ++r) key[r] = __float_as_uint(row[min((w * R + r) * 64 + lane, held - 1)]);
     }
+    // What follows goes through a lane's keys four times.  With many of them the compiler
+    // must not keep the page numbers and masks of one pass for the next, nor a pass's
+    // masks to its end: they are more registers than there are, and keys spilt to memory
+    // (64 keys a lane: 92 bytes of them; 32 rows of 62000 pages 64 us, 48)
+    constexpr bool kMany = R > 16;
+    int page = w * R * 64 + lane;  // of key[0]
+    auto again = [&] {
+        if constexpr (kMany) asm volatile("" : "+v"(page));
+    };
+    auto settle = [](int r, int &sum) {  // the sum so far, every 8 keys
+        if constexpr (kMany)
+            if (r % 8 == 7) asm volatile("" : "+s"(sum));
+    };
+    again();
     uint32_t diff = 0;  // bits in which competing keys differ from the first one
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int p = (w * R + r) * 64 + lane;
+        const int p = page + r * 64;
         const bool competes = p >= free0 && p < free1;
         const uint32_t x = score_key(__uint_as_float(key[r]));
         diff |= competes ? x ^ base : 0u;
         key[r] = competes ? x : p < held ? kGiven : 0u;
+        if constexpr (kMany) asm volatile("" : "+v"(key[r]));  // here, not behind the barriers
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) diff |= (uint32_t)__shfl_xor((int)diff, o);
@@ -493,7 +508,10 @@ select_pages_kernel(const float *__restrict__ scores, const int32_t *__restrict_
         const uint32_t cand = t | 1u << bit;
         int c = 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] >= cand));
+        for (int r = 0; r < R; ++r) {
+            c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] >= cand));
+            settle(r, c);
+        }
         if constexpr (W > 1) {
             if (lane == 0) atomicAdd(&count_s[bit], c);
             __syncthreads();
@@ -509,6 +527,8 @@ select_pages_kernel(const float *__restrict__ scores, const int32_t *__restrict_
     for (int r = 0; r < R; ++r) {
         above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] > t));
         equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] == t));
+        settle(r, above);
+        settle(r, equal);
     }
     int above_at = 0, equal_at = 0, all_above = above;
     if constexpr (W > 1) {
@@ -528,11 +548,13 @@ select_pages_kernel(const float *__restrict__ scores, const int32_t *__restrict_
     }
     const int want = k - all_above;  // of the equal ones, the first (after a count of exactly k: all)
     const uint64_t below = (1ull << lane) - 1;
+    again();
+    if constexpr (kMany) asm volatile("" : "+v"(t));
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const uint64_t gt = __builtin_amdgcn_ballot_w64(key[r] > t), eq = __builtin_amdgcn_ballot_w64(key[r] == t);
         const int ga = above_at + __builtin_popcountll(gt & below), ea = equal_at + __builtin_popcountll(eq & below);
-        if (key[r] > t || (key[r] == t && ea < want)) out[ga + min(ea, want)] = (w * R + r) * 64 + lane;
+        if (key[r] > t || (key[r] == t && ea < want)) out[ga + min(ea, want)] = page + r * 64;
         above_at += __builtin_popcountll(gt);
         equal_at += __builtin_popcountll(eq);
     }
@@ -675,7 +697,7 @@ int zk_select_pages(const float *scores, const int32_t *seq_lens, int num_seqs, 
     };
     // the fewest waves that hold a row in a few registers a lane (2048 rows of up to 8192
     // pages with 16 waves of 8 registers 55 us, 8 of 16 43; 32 rows of 16250 with 16 of 32
-    // 24.5, 8 of 32 16.8, 16 of 16 15.1; 32 of 62000 with 8 of 128 114, 16 of 64 64)
+    // 24.5, 8 of 32 16.8, 16 of 16 15.1; 32 of 62000 with 16 of 64 48)
     if (width <= 64 * 8) go(select_pages_kernel<1, 8>, 1);
     else if (width <= 64 * 4 * 8) go(select_pages_kernel<4, 8>, 4);
     else if (width <= 64 * 8 * 16) go(select_pages_kernel<8, 16>, 8);
