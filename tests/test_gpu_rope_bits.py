@@ -133,3 +133,48 @@ def test_pools_of_other_types(dtype, pool):
         q = ops.qk_norm_rope_append(kp, vp, x["q"], x["k"], x["v"], x["positions"], x["slots"], x["rope"], x["q_weight"], x["k_weight"], **more)
         outs.append((q, kp.contiguous().view(torch.uint8) if pool == "fp8" else kp, vp.contiguous().view(torch.uint8) if pool == "fp8" else vp))
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dtype", KINDS)
+def test_norms_alone_through_the_cache(dtype, kind):
+    """Without a table the cache's call takes no positions: the two calls' bits, step after step, with a plain write between."""
+    import zealot_amd as ze
+    from zealot_amd import KVCache, dense
+    H, hkv, d, ids = 4, 2, 64, ["a", "b"]
+    caches, managers = [], []  # (a cache's blocks belong to its manager)
+    for _ in range(2):
+        bm, c = ze.BlockManager(32, 16), KVCache(32, 16, 1, hkv, d, dtype=kind, max_seqs=4, max_blocks_per_seq=16)
+        for rid in ids:
+            c.register_seq(rid, 16)
+            for _ in range(8):
+                c.alloc_block(rid, bm)
+            if kind == torch.float8_e4m3fn:
+                c.set_fp8_scales(rid, [0.02] * hkv, [0.03] * hkv)
+        caches.append(c)
+        managers.append(bm)
+    g = torch.Generator().manual_seed(3)
+    wq, wk = [(1 + 0.1 * torch.randn(d, generator=g)).to(dtype).cuda() for _ in range(2)]
+    for step, counts in enumerate([[20, 3], [1, 40], [1, 1], [5, 0], [1, 1]]):
+        T = sum(counts)
+        q, k, v = [torch.randn(T, h, d, generator=g).to(dtype).cuda() for h in (H, hkv, hkv)]
+        if step == 3:  # as projected
+            for c in caches:
+                c.write_batch(0, ids, counts, k, v)
+            continue
+        got = caches[0].write_batch_rope(0, ids, counts, q, k, v, None, wq, wk)
+        # K's one rounding is to the pool's type: equal where the separate calls' K is f32, or of the pool's type
+        if kind == dtype or dtype == torch.float32:
+            want_q, want_k = dense.qk_norm_rope(q, k, None, None, wq, wk)
+            caches[1].write_batch(0, ids, counts, want_k, v)
+            assert torch.equal(got, want_q)
+            torch.cuda.synchronize()
+            for a, b in ((caches[0].k_pool(0), caches[1].k_pool(0)), (caches[0].v_pool(0), caches[1].v_pool(0))):
+                for i, rid in enumerate(ids):
+                    rows = [c.seq_state(rid) for c in caches]
+                    assert rows[0].cached_tokens == rows[1].cached_tokens
+                    x, y = [p.view(torch.uint8)[torch.tensor(r.block_ids, device="cuda")].transpose(1, 2).flatten(0, 1)[:r.cached_tokens]
+                            for p, r in zip((a, b), rows)]
+                    assert torch.equal(x, y), (step, rid)
+        else:
+            torch.cuda.synchronize()

@@ -4,7 +4,7 @@ built library: none keeps registers in memory, and the waves a SIMD that their
 comments count on fit its 512 registers."""
 import pytest
 
-from test_kernel_resources import SIMD_VGPRS, _all, _alloc, _one, kernel_registers
+from tests.test_kernel_resources import SIMD_VGPRS, _all, _alloc, _one, kernel_registers
 
 OBJECTS = ["step_ops.o", "rope_ops.o", "sparse_ops.o", "paged_sparse.o"]
 

@@ -917,7 +917,7 @@ int zk_cache_write_batch_rope(zk_kv_cache *c, size_t layer, const char *const *i
     }
     WritePrep w;
     if (int rc = prepare_write(c, layer, ids, num_tokens, n, q && k && v && q_out, w, true,
-                               rot_dim > 0 ? max_positions : INT64_MAX))
+                               rot_dim > 0 ? max_positions : -1))
         return rc;
     if (w.T == 0) return ZK_OK;
     a.slots = w.d_slots;
