@@ -812,6 +812,7 @@ int zk_cache_write_batch(zk_kv_cache *c, size_t layer, const char *const *ids, c
     WritePrep w;
     if (int rc = prepare_write(c, layer, ids, num_tokens, n, k && v, w)) return rc;
     if (w.T == 0) return ZK_OK;
+    DeviceGuard g(c->device);
     if (int rc = zk::append(c->k_pool(layer), c->v_pool(layer), (zk_dtype)c->dtype, k, v, src_dtype,
                             src_token_stride, w.d_slots, (int64_t)w.T, (int)c->num_kv_heads, (int)c->head_dim,
                             (int)c->block_size, (int64_t)c->num_blocks, w.d_ks, w.d_vs, w.d_rows, c->stream))
@@ -838,6 +839,7 @@ int zk_cache_write_batch_qkv(zk_kv_cache *c, size_t layer, const char *const *id
     WritePrep w;
     if (int rc = prepare_write(c, layer, ids, num_tokens, n, x && w_qkv && qkv, w)) return rc;
     if (w.T == 0) return ZK_OK;
+    DeviceGuard g(c->device);
     const int64_t T = (int64_t)w.T;
     bool fused = false;
     if (c->dtype == ZK_BF16) {  // the projection's split-k sums, if its plan keeps them, go straight to the pools
@@ -925,6 +927,7 @@ int zk_cache_write_batch_rope(zk_kv_cache *c, size_t layer, const char *const *i
     a.k_scales = w.d_ks;
     a.v_scales = w.d_vs;
     a.token_row = w.d_rows;
+    DeviceGuard g(c->device);
     if (int rc = zk::qk_norm_rope(a, c->stream)) return rc;
     finish_write(c, layer, num_tokens, n, w);
     return ZK_OK;
