@@ -178,3 +178,23 @@ def test_norms_alone_through_the_cache(dtype, kind):
                     assert torch.equal(x, y), (step, rid)
         else:
             torch.cuda.synchronize()
+
+
+def test_a_sequence_without_new_tokens_may_lie_behind_the_table():
+    """Written as projected past the table's positions, then in a batch of rotated keys with no token of its own."""
+    import zealot_amd as ze
+    from zealot_amd import KVCache, ZealotError, dense
+    H, hkv, d = 4, 2, 64
+    bm, c = ze.BlockManager(16, 16), KVCache(16, 16, 1, hkv, d, dtype=torch.bfloat16, max_seqs=4, max_blocks_per_seq=8)
+    for rid in "ab":
+        c.register_seq(rid, 4)
+        for _ in range(4):
+            c.alloc_block(rid, bm)
+    rope = dense.rope_table(30, d)
+    q, k, v = [torch.randn(40, h, d, dtype=torch.bfloat16, device="cuda") for h in (H, hkv, hkv)]
+    c.write_batch(0, ["a"], [40], k, v)
+    got = c.write_batch_rope(0, ["a", "b"], [0, 5], q[:5], k[:5], v[:5], rope)
+    want = dense.qk_norm_rope(q[:5], k[:5], torch.arange(5, dtype=torch.int32, device="cuda"), rope)[0]
+    assert torch.equal(got, want) and c.seq_state("a").cached_tokens == 40 and c.seq_state("b").cached_tokens == 5
+    with pytest.raises(ZealotError):
+        c.write_batch_rope(0, ["a", "b"], [1, 5], q[:6], k[:6], v[:6], rope)

@@ -562,7 +562,7 @@ int prepare_write(zk_kv_cache *c, size_t layer, const char *const *ids, const in
         if (fp8 && s.k_scales.empty())
             return set_error(ZK_ERR_FAILED_PRECONDITION,
                              std::string("Failed precondition: fp8 scales not set for seq ") + ids[i]);
-        if (max_positions >= 0 && s.cached_tokens + (size_t)num_tokens[i] > (size_t)max_positions)
+        if (max_positions >= 0 && num_tokens[i] > 0 && s.cached_tokens + (size_t)num_tokens[i] > (size_t)max_positions)
             return set_error_typed(ZK_ERR_SEQUENCE_TOO_LONG, zk::ErrorKind::SequenceTooLong,
                                    s.cached_tokens + (size_t)num_tokens[i], (uint64_t)max_positions);
         T += (size_t)num_tokens[i];
