@@ -125,8 +125,9 @@ __device__ __forceinline__ int stage_list(const SparseArgs &a, int n, int kvh, i
 //
 // 256 contexts, 64 pages of each, 32 / 8 heads of 128 bf16 (1048 MB): 166 us, 6.3
 // TB/s (a read of one piece reaches 7.5, one of shuffled 4 KB pieces 7 % less).
-// One step ahead in registers needs 208 of them, two waves a SIMD, and took 179; the
-// 128 registers of four waves a SIMD spill, 215.
+// Three workgroups run on a CU, by LDS (42.5 KB at a head size of 128: the lists' and the
+// merge's) as by registers (134 to 158).  One step ahead in registers needs 208 of them,
+// two waves a SIMD, and took 179; held to 128 registers the kernel spills, 215.
 constexpr int kWaves = 4;
 constexpr float kSlack = 8.0f;
 
@@ -581,9 +582,10 @@ __global__ void __launch_bounds__(kReduceThreads) sparse_reduce_kernel(SparseArg
 
 bool mfma_dim(int head_dim) { return head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256; }
 
-// Parts of a list: enough workgroups to fill the CUs twice (one-wave ones of
-// the generic kernel: four waves a SIMD), of at least 8 (4) pages each and, from 16
-// parts on, 16, at most kMaxList.  us with parts of 8, 16 and 32 pages: 8 lists of
+// Parts of a list, by its capacity (what it holds is known on the device only): enough
+// workgroups to fill the CUs twice (one-wave ones of the generic kernel at head sizes
+// that are not the matrix cores': four waves a SIMD), of at least 8 (4) pages each and,
+// from 16 parts on, 16, at most kMaxList.  us with parts of 8, 16 and 32 pages: 8 lists of
 // 64 bf16 pages 9.6, 10.8, 13.3; 16 of 256 fp8 pages 13.3 (32 parts), 12.0, 13.7.
 int splits_for(int num_seqs, int num_kv_heads, int head_dim, int num_pages) {
     const int64_t rows = (int64_t)num_seqs * num_kv_heads;

@@ -156,7 +156,7 @@ __device__ __forceinline__ float lane_sum(float x, int lanes) {
 // needs is kept small: cosines and sines times the weights once a token, the
 // norm's factor applied to the rotated value, sums of squares by dot products of
 // packed pairs, partners exchanged packed, V copied (before: 187 us, and 233 with
-// plain loads and stores).  And its waves must be many (82 registers, six a
+// plain loads and stores).  And its waves must be many (83 registers, five a
 // SIMD): workgroups that walk the tokens and load the next one ahead hold 180-200
 // registers, two waves a SIMD, and took 178-217 us.
 //
