@@ -126,7 +126,7 @@ __device__ __forceinline__ int stage_list(const SparseArgs &a, int n, int kvh, i
 // 256 contexts, 64 pages of each, 32 / 8 heads of 128 bf16 (1048 MB): 166 us, 6.3
 // TB/s (a read of one piece reaches 7.5, one of shuffled 4 KB pieces 7 % less).
 // Three workgroups run on a CU, by LDS (42.5 KB at a head size of 128: the lists' and the
-// merge's) as by registers (134 to 158).  One step ahead in registers needs 208 of them,
+// merge's) as by registers (134 to 162).  One step ahead in registers needs 208 of them,
 // two waves a SIMD, and took 179; held to 128 registers the kernel spills, 215.
 constexpr int kWaves = 4;
 constexpr float kSlack = 8.0f;
@@ -175,7 +175,7 @@ __device__ __forceinline__ void three_parts(float x, float (&part)[3]) {
 
 // PARTS: bf16 values that a query value is held in: 1, or 3 for f32 queries on bf16
 // and fp8 pools (exact: 24 bits).  256 lists of 64 pages with one part of 8 bits and with
-// three: bf16 pools 175 and 182 us, fp8 100 and 111; 128 of heads of 256 192 and 223.
+// three: bf16 pools 176 and 184 us, fp8 100 and 112; 128 of heads of 256 192 and 227.
 template <int KV, int D, int PARTS>
 __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) {
     constexpr bool F32 = KV == ZK_F32;
@@ -344,18 +344,27 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
             // weights as two bf16 each, the leading 8 bits and what they leave (16 bits in
             // all): the matrix cores wait for memory anyway.  2^-20 of the weight is added
             // to the second, which is then never zero nor of the other sign: an infinity
-            // in V stays one.
-            u32x4 pw, rw;
+            // in V stays one.  In f32 results (queries of three parts) the weights are three
+            // parts as well, their 24 bits (184 us as with two).
+            constexpr int WP = PARTS == 3 ? 3 : 2;
+            u32x4 pw[WP];
 #pragma unroll
             for (int h = 0; h < PG; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
-                    const uint32_t w = __builtin_amdgcn_perm(__float_as_uint(pr[h][i + 1]), __float_as_uint(pr[h][i]), 0x07060302u);
-                    constexpr float kAll = 1.0f + 0x1p-20f;
-                    pw[2 * h + i / 2] = w;
-                    rw[2 * h + i / 2] = bf16x2_rne(fmaf(pr[h][i], kAll, -bf16lo(w)), fmaf(pr[h][i + 1], kAll, -bf16hi(w)));
+                    if constexpr (WP == 3) {
+                        float lo[3], hi[3];
+                        three_parts(pr[h][i], lo);
+                        three_parts(pr[h][i + 1], hi);
+#pragma unroll
+                        for (int j = 0; j < 3; ++j) pw[j][2 * h + i / 2] = bf16x2_rne(lo[j], hi[j]);
+                    } else {
+                        const uint32_t w = __builtin_amdgcn_perm(__float_as_uint(pr[h][i + 1]), __float_as_uint(pr[h][i]), 0x07060302u);
+                        constexpr float kAll = 1.0f + 0x1p-20f;
+                        pw[0][2 * h + i / 2] = w;
+                        pw[1][2 * h + i / 2] = bf16x2_rne(fmaf(pr[h][i], kAll, -bf16lo(w)), fmaf(pr[h][i + 1], kAll, -bf16hi(w)));
+                    }
                 }
-            const bf16x8 pb = __builtin_bit_cast(bf16x8, pw), rb = __builtin_bit_cast(bf16x8, rw);
 #pragma unroll
             for (int j = 0; j < DT / 2; ++j) {
                 u32x4 ev, od;
@@ -367,10 +376,12 @@ __global__ void __launch_bounds__(64 * kWaves) sparse_mfma_kernel(SparseArgs a) 
                     od[2 * h + 1] = __builtin_amdgcn_perm(vb[h][3][j], vb[h][2][j], 0x07060302u);
                 }
                 const bf16x8 e8 = __builtin_bit_cast(bf16x8, ev), o8 = __builtin_bit_cast(bf16x8, od);
-                o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e8, pb, o[2 * j], 0, 0, 0);
-                o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(o8, pb, o[2 * j + 1], 0, 0, 0);
-                o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e8, rb, o[2 * j], 0, 0, 0);
-                o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(o8, rb, o[2 * j + 1], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < WP; ++i) {
+                    const bf16x8 w8 = __builtin_bit_cast(bf16x8, pw[i]);
+                    o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e8, w8, o[2 * j], 0, 0, 0);
+                    o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(o8, w8, o[2 * j + 1], 0, 0, 0);
+                }
             }
         }
     }
