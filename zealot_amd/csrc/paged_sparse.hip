@@ -126,7 +126,7 @@ __device__ __forceinline__ int stage_list(const SparseArgs &a, int n, int kvh, i
 // 256 contexts, 64 pages of each, 32 / 8 heads of 128 bf16 (1048 MB): 166 us, 6.3
 // TB/s (a read of one piece reaches 7.5, one of shuffled 4 KB pieces 7 % less).
 // Three workgroups run on a CU, by LDS (42.5 KB at a head size of 128: the lists' and the
-// merge's) as by registers (134 to 162).  One step ahead in registers needs 208 of them,
+// merge's) as by registers (bf16 pools: 134 to 162).  One step ahead in registers needs 208 of them,
 // two waves a SIMD, and took 179; held to 128 registers the kernel spills, 215.
 constexpr int kWaves = 4;
 constexpr float kSlack = 8.0f;
