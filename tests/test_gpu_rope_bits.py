@@ -196,5 +196,7 @@ def test_a_sequence_without_new_tokens_may_lie_behind_the_table():
     got = c.write_batch_rope(0, ["a", "b"], [0, 5], q[:5], k[:5], v[:5], rope)
     want = dense.qk_norm_rope(q[:5], k[:5], torch.arange(5, dtype=torch.int32, device="cuda"), rope)[0]
     assert torch.equal(got, want) and c.seq_state("a").cached_tokens == 40 and c.seq_state("b").cached_tokens == 5
-    with pytest.raises(ZealotError):
+    with pytest.raises(ZealotError) as e:
         c.write_batch_rope(0, ["a", "b"], [1, 5], q[:6], k[:6], v[:6], rope)
+    assert e.value.fields == {"required": 41, "capacity": 30}
+    assert "seq a would hold 41 tokens" in str(e.value) and "30 rows" in str(e.value) and "blocks" not in str(e.value)

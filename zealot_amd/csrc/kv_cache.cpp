@@ -562,9 +562,12 @@ int prepare_write(zk_kv_cache *c, size_t layer, const char *const *ids, const in
         if (fp8 && s.k_scales.empty())
             return set_error(ZK_ERR_FAILED_PRECONDITION,
                              std::string("Failed precondition: fp8 scales not set for seq ") + ids[i]);
-        if (max_positions >= 0 && num_tokens[i] > 0 && s.cached_tokens + (size_t)num_tokens[i] > (size_t)max_positions)
-            return set_error_typed(ZK_ERR_SEQUENCE_TOO_LONG, zk::ErrorKind::SequenceTooLong,
-                                   s.cached_tokens + (size_t)num_tokens[i], (uint64_t)max_positions);
+        const size_t after = s.cached_tokens + (size_t)num_tokens[i];
+        if (max_positions >= 0 && num_tokens[i] > 0 && after > (size_t)max_positions) {
+            (void)set_error_typed(ZK_ERR_SEQUENCE_TOO_LONG, zk::ErrorKind::SequenceTooLong, after, (uint64_t)max_positions);
+            return zk::set_error_text(std::string("Sequence too long: seq ") + ids[i] + " would hold " + std::to_string(after) +
+                                      " tokens, the position table has " + std::to_string(max_positions) + " rows");
+        }
         T += (size_t)num_tokens[i];
     }
     if (T == 0) return ZK_OK;

@@ -46,6 +46,11 @@ int set_error_typed(int code, ErrorKind kind, uint64_t a, uint64_t b, uint64_t c
     g_err.built = false;
     return code;
 }
+int set_error_text(const std::string &msg) {
+    g_err.message = msg;
+    g_err.built = true;
+    return g_err.code;
+}
 void clear_error() { set_error(ZK_OK, ""); }
 ErrorSnapshot save_error() { return g_err; }
 int restore_error(const ErrorSnapshot &e) {

@@ -29,6 +29,9 @@ enum class ErrorKind {
     SequenceTooLong
 };
 int set_error_typed(int code, ErrorKind kind, uint64_t a, uint64_t b = 0, uint64_t c = 0);
+// Its own text for a typed error whose fields do not mean what the variant's text says;
+// returns the code.
+int set_error_text(const std::string &msg);
 void clear_error();
 // The whole last-error state, so a caller that must clean up (calling
 // functions that may fail in turn) can re-raise the original error unchanged.
