@@ -177,6 +177,79 @@ int zk_linear_tiled_choice(int64_t m, int64_t n, int64_t k, zk_dtype out_dtype, 
 int zk_linear_pin_split(int64_t m, int64_t n, int64_t k, zk_dtype in_dtype, zk_dtype out_dtype, int tiled,
                         int fused_splits, int fused_rows);
 
+/* ---- projections in 8 bits.  No reference counterpart (its projections are
+ * f32 sgemms, attention/cublas.rs:72-114).  8 bits are e4m3 (OCP; largest value
+ * 448); a row y is held as one f32 scale and 8-bit values,
+ *   scale = max(max |y| / 448, 2^-126),  q = e4m3(y / scale), nearest even;
+ * a row that holds a NaN has a NaN scale and NaN values.
+ *
+ * zk_rms_norm (as there: s = x + residual rounded to the tensors' type and
+ * written to residual_out) whose rows are written in 8 bits, from f32 and
+ * rounded once: q [num_rows, dim] bytes, scales [num_rows].  rows (device int64
+ * [num_rows], NULL: all, x_rows == num_rows) selects rows of x [x_rows, dim] and
+ * of the residual; one outside [0, x_rows) gives zeros.  residual_out may be x
+ * or the residual itself when rows is NULL; outputs overlap nothing else.
+ * dim <= 32768 (bf16) / 16384 (f32) for 16-byte rows, <= 4096 otherwise. */
+int zk_rms_norm_fp8(const void *x, const void *residual, const void *weight, void *q, float *scales,
+                    void *residual_out, const int64_t *rows, int64_t x_rows, int64_t num_rows, int64_t dim, float eps,
+                    zk_dtype dtype, void *stream);
+/* zk_silu_mul (rows gate_stride / up_stride elements apart, 0 = cols) whose rows
+ * are written in 8 bits.  cols as dim above. */
+int zk_silu_mul_fp8(const void *gate, const void *up, void *q, float *scales, int64_t rows, int64_t cols,
+                    int64_t gate_stride, int64_t up_stride, zk_dtype dtype, void *stream);
+/* A weight w [n, k] (nn.Linear layout) in 8 bits with one scale a row, packed
+ * once for zk_linear_fp8: [ceil(n / 64)][4 tiles][ceil(k / 128)][8 units][16
+ * rows][16 bytes], unit u of a chunk holding its columns 16 u .. 16 u + 15 and
+ * row i of tile t of group G being row 64 G + 16 (i / 4) + 4 t + i % 4; zeros
+ * behind n and k.  dtype F32 or BF16: scales [n] is written (as for the rows
+ * above); FP8_E4M3: w holds the 8-bit values, whose scales the caller has (scales
+ * is not touched and may be NULL).  packed: zk_fp8_weight_bytes(n, k) bytes,
+ * 16-byte aligned. */
+size_t zk_fp8_weight_bytes(int64_t n, int64_t k);
+int zk_fp8_weight(const void *w, zk_dtype dtype, void *packed, float *scales, int64_t n, int64_t k, void *stream);
+/* y[m, n] = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] for x [m, k] in 8 bits
+ * (packed rows; k % 16 == 0) and a packed weight, f32 sums, y F32 or BF16.  x,
+ * the weight and y 16-byte aligned.  Nothing is tuned: a call launches what its
+ * sizes say. */
+int zk_linear_fp8(const void *x, const float *x_scales, const void *packed, const float *w_scales, void *y, int64_t m,
+                  int64_t n, int64_t k, zk_dtype out_dtype, void *stream);
+
+/* ---- low-rank adapters of many requests beside a shared projection.  No
+ * reference counterpart (one set of weights, model_loader.rs:241).
+ *
+ * The plan of a step: row t belongs to a request with adapter adapter_ids[t]
+ * (device int32 [num_rows]; outside [0, num_adapters): none).
+ *   order [num_rows]            the rows with an adapter, sorted by it, in their
+ *                               order within one; then -1
+ *   offsets [num_adapters + 1]  where each adapter's rows begin in order
+ *   tiles [zk_lora_max_tiles][2]  runs of rows that zk_lora works on (its own)
+ * It holds for every projection of the step.  At most 2^24 rows and 2048
+ * adapters; outputs overlap nothing. */
+int64_t zk_lora_max_tiles(int64_t num_rows, int64_t num_adapters);
+int zk_lora_plan(const int32_t *adapter_ids, int64_t num_rows, int64_t num_adapters, int32_t *order, int32_t *offsets,
+                 int32_t *tiles, void *stream);
+/* y[t] += scales[a] b[a] (a_weights[a] x[t]) for the rows of a plan, a their
+ * adapter; other rows of y are left as they are.  x [num_rows, k] (rows x_stride
+ * elements apart, 0 = k), a_weights [num_adapters, num_parts * rank, k], b
+ * [num_adapters, n, rank], scales f32 [num_adapters] (NULL: 1), y [num_rows, n]
+ * (rows y_stride apart, 0 = n), all of `dtype` (F32, BF16); beside BF16 x may be
+ * FP8_E4M3 rows with x_scales [num_rows].  With num_parts > 1 the columns of y
+ * come in parts that have ranks of their own: part p (its columns: part_cols[p]
+ * behind those of the parts before it, host int64 [num_parts]) meets rows p rank
+ * .. of a_weights[a] alone.  part_block > 0 instead: the columns take their
+ * parts in turn, part_block at a time (the gate and up rows of
+ * zk_linear_silu_mul: 2 parts, blocks of 16).  f32 sums; the ranks' values keep
+ * 16 bits or more between the two products.  rank <= 256, num_parts <= 4, rank *
+ * num_parts <= 512.  workspace: zk_lora_workspace_size bytes, 16-byte aligned;
+ * calls that share one must not overlap in time.  y and the workspace overlap
+ * no operand. */
+size_t zk_lora_workspace_size(int64_t num_rows, int64_t num_adapters, int64_t k, int rank, int num_parts, zk_dtype dtype);
+int zk_lora(const void *x, const float *x_scales, int64_t x_stride, zk_dtype x_dtype, const void *a_weights,
+            const void *b_weights, const float *scales, zk_dtype dtype, const int32_t *order, const int32_t *offsets,
+            const int32_t *tiles, int64_t num_rows, int64_t num_adapters, int64_t k, int64_t n, int rank, int num_parts,
+            const int64_t *part_cols, int part_block, void *y, int64_t y_stride, void *workspace, size_t workspace_bytes,
+            void *stream);
+
 /* On (default): the first call of each (m, n, k, dtypes) times hipBLASLt's
  * candidate algorithms on its operands (synchronizing the stream once) and
  * keeps the fastest.  Off: the heuristic's first choice, no synchronization

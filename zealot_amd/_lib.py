@@ -163,6 +163,16 @@ SIGNATURES = {
     "zk_linear_skinny": (_I, [_P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _P]),
     "zk_linear_tuning": (_I, [_I]),
     "zk_linear_pin_split": (_I, [_I64, _I64, _I64, _I, _I, _I, _I, _I]),
+    "zk_rms_norm_fp8": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _F, _I, _P]),
+    "zk_silu_mul_fp8": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P]),
+    "zk_fp8_weight_bytes": (_SZ, [_I64, _I64]),
+    "zk_fp8_weight": (_I, [_P, _I, _P, _P, _I64, _I64, _P]),
+    "zk_linear_fp8": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P]),
+    "zk_lora_max_tiles": (_I64, [_I64, _I64]),
+    "zk_lora_plan": (_I, [_P, _I64, _I64, _P, _P, _P, _P]),
+    "zk_lora_workspace_size": (_SZ, [_I64, _I64, _I64, _I, _I, _I]),
+    "zk_lora": (_I, [_P, _P, _I64, _I, _P, _P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _P, _I, _P, _I64, _P, _SZ,
+                     _P]),
     "zk_sched_create": (_I, [ctypes.POINTER(SchedConfigC), _P, ctypes.POINTER(_P)]),
     "zk_sched_destroy": (None, [_P]),
     "zk_sched_block_manager": (_P, [_P]),

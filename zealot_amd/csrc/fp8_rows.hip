@@ -1,0 +1,319 @@
+// fp8_rows.hip -- rows in 8 bits for the 8-bit projections: RMSNorm (with the
+// residual add before it) and SiLU(gate) * up whose results are written as
+// e4m3 values and one f32 scale a row.
+//
+// A row y is held as s = max(max |y| / 448, 2^-126) and q = e4m3(y / s), to
+// nearest even (448: the largest e4m3 value; 2^-126 keeps 1 / s finite and a
+// row of zeros zero).  A row with a NaN has NaN for its scale and all values.
+//   norm: t = x (+ residual, rounded to the tensors' type and written),
+//         y = t * rsqrt(mean(t^2) + eps) * w
+//   SiLU: y = g / (1 + exp(-g)) * u
+// y itself is f32 and rounded once, to e4m3: the 16-bit row that the unfused
+// sequence writes and reads again never exists.  The reference has neither
+// (its projections are f32, src/attention/cublas.rs:72-114).
+//
+// Both are bound by HBM: a row is read once into registers, its sum of
+// squares and its largest |t w| (which is the largest |y| up to the factor of
+// the row) go through one reduction, and it is written from the registers.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+#include "zk_common.h"
+
+using namespace zk;
+
+namespace {
+
+constexpr float kTop = 448.0f;        // e4m3's largest value
+constexpr float kLeast = 0x1p-126f;   // smallest scale
+
+struct RowArgs {
+    const void *x, *other;  // norm: x and the residual (or null); SiLU: gate and up
+    const void *weight;     // norm
+    uint8_t *q;
+    float *scales;
+    void *sum_out;          // norm with a residual
+    const int64_t *rows;    // norm: the input row of each output row, or null
+    int64_t in_rows;        // rows of x; one outside them is a row of zeros
+    int64_t x_stride, other_stride;
+    int dim;
+    float eps;
+};
+
+template <typename T> struct Elems;
+template <> struct Elems<float> { static constexpr int N = 4; };
+template <> struct Elems<uint16_t> { static constexpr int N = 8; };
+
+template <int VEC>
+__device__ __forceinline__ void load(const float *p, float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        v[0] = *p;
+    } else {
+        const f32x4 w = *reinterpret_cast<const f32x4 *>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = w[e];
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void load(const uint16_t *p, float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        v[0] = __uint_as_float((uint32_t)*p << 16);
+    } else {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[2 * e] = bf16lo(w[e]);
+            v[2 * e + 1] = bf16hi(w[e]);
+        }
+    }
+}
+// v rounded to the tensor's type, and written there
+template <int VEC>
+__device__ __forceinline__ void store_sum(float *p, float (&v)[VEC]) {
+    if constexpr (VEC == 1) *p = v[0];
+    else *reinterpret_cast<f32x4 *>(p) = f32x4{v[0], v[1], v[2], v[3]};
+}
+template <int VEC>
+__device__ __forceinline__ void store_sum(uint16_t *p, float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        const uint32_t b = f32_to_bf16_bits(v[0]);
+        *p = (uint16_t)b;
+        v[0] = __uint_as_float(b << 16);
+    } else {
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            w[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+            v[2 * e] = bf16lo(w[e]);
+            v[2 * e + 1] = bf16hi(w[e]);
+        }
+        *reinterpret_cast<u32x4 *>(p) = w;
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void store_q(uint8_t *p, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        *p = (uint8_t)e4m3x4(v[0], 0.f, 0.f, 0.f);
+    } else if constexpr (VEC == 4) {
+        *reinterpret_cast<uint32_t *>(p) = e4m3x4(v[0], v[1], v[2], v[3]);
+    } else {
+        *reinterpret_cast<u32x2 *>(p) = u32x2{e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7])};
+    }
+}
+
+// One workgroup a row, MAXV vectors a thread.  A workgroup reads its whole row
+// before it writes any of it (two barriers apart from nothing else), so sum_out
+// may be the row's own x or residual.
+template <bool NORM, typename T, int VEC, int MAXV, int THREADS>
+__global__ void __launch_bounds__(THREADS) fp8_rows_kernel(RowArgs a) {
+    constexpr int W = THREADS / 64;
+    __shared__ float red_sum[W];
+    __shared__ uint32_t red_max[W];
+    const int64_t row = blockIdx.x;
+    int64_t in = row;
+    if (NORM && a.rows) {
+        in = a.rows[row];
+        if ((uint64_t)in >= (uint64_t)a.in_rows) {  // no such row: zeros
+            for (int i = threadIdx.x; i < a.dim; i += THREADS) {
+                a.q[(size_t)row * a.dim + i] = 0;
+                if (a.other) ((T *)a.sum_out)[(size_t)row * a.dim + i] = T(0);
+            }
+            if (threadIdx.x == 0) a.scales[row] = kLeast;
+            return;
+        }
+    }
+    const T *x = (const T *)a.x + (size_t)in * a.x_stride;
+    const T *o = a.other ? (const T *)a.other + (size_t)in * a.other_stride : nullptr;
+    float v[MAXV][VEC], w[MAXV][VEC];
+    float ss = 0.0f;
+    uint32_t top = 0;  // of |value| as bits: NaN above infinity above the numbers
+#pragma unroll
+    for (int j = 0; j < MAXV; ++j) {
+        const int i = (j * THREADS + (int)threadIdx.x) * VEC;
+        if (i < a.dim) {
+            load<VEC>(x + i, v[j]);
+            if (NORM) load<VEC>((const T *)a.weight + i, w[j]);
+            else load<VEC>(o + i, w[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < MAXV; ++j) {
+        const int i = (j * THREADS + (int)threadIdx.x) * VEC;
+        if (i < a.dim) {
+            if (NORM && o) {
+                float r[VEC];
+                load<VEC>(o + i, r);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[j][e] += r[e];
+                store_sum<VEC>((T *)a.sum_out + (size_t)row * a.dim + i, v[j]);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (NORM) {
+                    ss += v[j][e] * v[j][e];
+                    v[j][e] *= w[j][e];
+                } else {
+                    v[j][e] = v[j][e] / (1.0f + expf(-v[j][e])) * w[j][e];
+                }
+                top = max(top, __float_as_uint(v[j][e]) & 0x7fffffffu);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) {
+        if (NORM) ss += __shfl_xor(ss, k);
+        top = max(top, (uint32_t)__shfl_xor((int)top, k));
+    }
+    if (W > 1) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+            red_sum[wave] = ss;
+            red_max[wave] = top;
+        }
+        __syncthreads();
+        ss = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            ss += red_sum[k];
+            top = max(top, red_max[k]);
+        }
+    }
+    const float inv = NORM ? rsqrtf(ss / (float)a.dim + a.eps) : 1.0f;
+    const float most = __uint_as_float(top) * inv / kTop;
+    const float s = most < kLeast ? kLeast : most;  // (NaN stays)
+    const float r = 1.0f / s;
+    if (threadIdx.x == 0) a.scales[row] = s;
+#pragma unroll
+    for (int j = 0; j < MAXV; ++j) {
+        const int i = (j * THREADS + (int)threadIdx.x) * VEC;
+        if (i < a.dim) {
+            float y[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) y[e] = NORM ? v[j][e] * inv * r : v[j][e] * r;
+            store_q<VEC>(a.q + (size_t)row * a.dim + i, y);
+        }
+    }
+}
+
+bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+
+template <bool NORM, typename T, int VEC>
+bool launch_vec(const RowArgs &a, int rows, hipStream_t s) {
+    const int n = (a.dim + VEC - 1) / VEC;
+    auto go = [&](auto kernel, int threads) { kernel<<<(unsigned)rows, threads, 0, s>>>(a); };
+    if (n <= 64) go(fp8_rows_kernel<NORM, T, VEC, 1, 64>, 64);
+    else if (n <= 256) go(fp8_rows_kernel<NORM, T, VEC, 1, 256>, 256);
+    else if (n <= 512) go(fp8_rows_kernel<NORM, T, VEC, 2, 256>, 256);
+    else if (n <= 1024) go(fp8_rows_kernel<NORM, T, VEC, 4, 256>, 256);
+    else if (n <= 2048) go(fp8_rows_kernel<NORM, T, VEC, 8, 256>, 256);
+    else if (n <= 4096) go(fp8_rows_kernel<NORM, T, VEC, 4, 1024>, 1024);
+    else return false;
+    return true;
+}
+
+template <bool NORM>
+int launch(const RowArgs &a, int64_t rows, zk_dtype dtype, const char *name, hipStream_t s) {
+    const int V = dtype == ZK_BF16 ? 8 : 4;
+    const bool vec = a.dim % V == 0 && a.x_stride % V == 0 && a.other_stride % V == 0 && aligned(a.x, 16) &&
+                     aligned(a.other, 16) && aligned(a.weight, 16) && aligned(a.sum_out, 16) && aligned(a.q, V);
+    bool ok;
+    if (dtype == ZK_BF16)
+        ok = vec ? launch_vec<NORM, uint16_t, 8>(a, (int)rows, s) : launch_vec<NORM, uint16_t, 1>(a, (int)rows, s);
+    else
+        ok = vec ? launch_vec<NORM, float, 4>(a, (int)rows, s) : launch_vec<NORM, float, 1>(a, (int)rows, s);
+    if (!ok)
+        return set_error(ZK_ERR_INVALID_ARGUMENT,
+                         std::string("Internal error: ") + name + ": rows of " + std::to_string(a.dim) +
+                             " too long (at most 32768 bf16 / 16384 f32 elements with 16-byte rows, 4096 otherwise)");
+    if (hipError_t e = hipGetLastError(); e != hipSuccess)
+        return set_error(ZK_ERR_HIP, std::string("Internal error: ") + name + ": " + hipGetErrorString(e));
+    return ZK_OK;
+}
+
+struct Span {
+    const void *p;
+    int64_t bytes;
+};
+bool meet(const Span &u, const Span &v) {
+    const uintptr_t a = (uintptr_t)u.p, b = (uintptr_t)v.p;
+    return u.p && v.p && u.bytes > 0 && v.bytes > 0 && a < b + v.bytes && b < a + u.bytes;
+}
+
+}  // namespace
+
+extern "C" {
+
+int zk_rms_norm_fp8(const void *x, const void *residual, const void *weight, void *q, float *scales,
+                    void *residual_out, const int64_t *rows, int64_t x_rows, int64_t num_rows, int64_t dim, float eps,
+                    zk_dtype dtype, void *stream) {
+    if (dtype != ZK_F32 && dtype != ZK_BF16)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_rms_norm_fp8: dtype must be f32 or bf16");
+    if (num_rows < 0 || x_rows < 0 || dim <= 0 || dim > 32768 || num_rows > 0x7fffffff || x_rows > 0x7fffffff ||
+        (!rows && x_rows != num_rows))
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_rms_norm_fp8: bad shape");
+    if (num_rows == 0) return ZK_OK;
+    if (!x || !weight || !q || !scales || (residual && !residual_out))
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_rms_norm_fp8: NULL pointer");
+    const int64_t e = elt_size(dtype);
+    const Span in[] = {{x, x_rows * dim * e}, {residual, x_rows * dim * e}, {weight, dim * e}, {rows, 8 * num_rows}};
+    const Span out[] = {{q, num_rows * dim}, {scales, 4 * num_rows}, {residual ? residual_out : nullptr, num_rows * dim * e}};
+    for (int i = 0; i < 3; ++i) {
+        for (int j = 0; j < 4; ++j)  // (a row's own sum may take its place)
+            if (meet(out[i], in[j]) && !(i == 2 && j < 2 && !rows && out[i].p == in[j].p))
+                return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_rms_norm_fp8: an output overlaps an input");
+        for (int j = 0; j < i; ++j)
+            if (meet(out[i], out[j]))
+                return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_rms_norm_fp8: outputs overlap");
+    }
+    RowArgs a{};
+    a.x = x;
+    a.other = residual;
+    a.weight = weight;
+    a.q = (uint8_t *)q;
+    a.scales = scales;
+    a.sum_out = residual ? residual_out : nullptr;
+    a.rows = rows;
+    a.in_rows = x_rows;
+    a.x_stride = a.other_stride = dim;
+    a.dim = (int)dim;
+    a.eps = eps;
+    hipStream_t s = (hipStream_t)stream;
+    KernelTimer timer("rms_norm_fp8", s);
+    return launch<true>(a, num_rows, dtype, "zk_rms_norm_fp8", s);
+}
+
+int zk_silu_mul_fp8(const void *gate, const void *up, void *q, float *scales, int64_t rows, int64_t cols,
+                    int64_t gate_stride, int64_t up_stride, zk_dtype dtype, void *stream) {
+    if (dtype != ZK_F32 && dtype != ZK_BF16)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_silu_mul_fp8: dtype must be f32 or bf16");
+    if (rows < 0 || cols <= 0 || cols > 32768 || rows > 0x7fffffff)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_silu_mul_fp8: bad shape");
+    if (gate_stride == 0) gate_stride = cols;
+    if (up_stride == 0) up_stride = cols;
+    if (gate_stride < cols || up_stride < cols || gate_stride > (1ll << 31) || up_stride > (1ll << 31))
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_silu_mul_fp8: bad row stride");
+    if (rows == 0) return ZK_OK;
+    if (!gate || !up || !q || !scales)
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_silu_mul_fp8: NULL pointer");
+    const int64_t e = elt_size(dtype);
+    const Span in[] = {{gate, ((rows - 1) * gate_stride + cols) * e}, {up, ((rows - 1) * up_stride + cols) * e}};
+    const Span out[] = {{q, rows * cols}, {scales, 4 * rows}};
+    if (meet(out[0], in[0]) || meet(out[0], in[1]) || meet(out[1], in[0]) || meet(out[1], in[1]) || meet(out[0], out[1]))
+        return set_error(ZK_ERR_INVALID_ARGUMENT, "Internal error: zk_silu_mul_fp8: an output overlaps another operand");
+    RowArgs a{};
+    a.x = gate;
+    a.other = up;
+    a.q = (uint8_t *)q;
+    a.scales = scales;
+    a.x_stride = gate_stride;
+    a.other_stride = up_stride;
+    a.dim = (int)cols;
+    hipStream_t s = (hipStream_t)stream;
+    KernelTimer timer("silu_mul_fp8", s);
+    return launch<false>(a, rows, dtype, "zk_silu_mul_fp8", s);
+}
+
+}  // extern "C"

@@ -1,0 +1,587 @@
+// lora_ops.hip -- low-rank adapters of many requests beside a shared
+// projection: y[t] += c_a B_a (A_a x[t]) for every row t whose request brings
+// an adapter a = ids[t].  No counterpart in the reference (one model, one set
+// of weights, src/model_loader.rs:241).
+//
+// A step's plan groups its rows by adapter, once for all layers' projections:
+//   order    the rows, sorted by adapter, in order within one; then -1
+//   offsets  where each adapter's rows begin in it
+//   tiles    (adapter, first position) of runs of at most tile_rows rows of one
+//            adapter; (-1, 0) behind the last
+// A product is two launches over the tiles.  The shrink forms
+// v[p] = c_a A_a x[order[p]] (f32, R = parts * rank values a row) with A as the
+// first operand of the matrix instruction and the tile's rows as the second, k
+// split over the waves of a workgroup and, where there are few tiles, over
+// workgroups, whose sums the second launch adds in their order.  The expand
+// takes 64 columns of y a wave: B's rows as the first operand, v as the
+// second, so that a lane ends with 16 consecutive columns of a row and adds them
+// in place.
+// Columns of y may come in parts that have an A of their own each (query, key
+// and value columns of a fused projection): part p meets v[p rank ..] alone.
+//
+// Both launches read x, A, B and y once at most tile_rows rows a pass and are
+// bound by that traffic, and for a few rows by their latency.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+#include "zk_common.h"
+
+using namespace zk;
+
+namespace {
+
+constexpr int kMaxAdapters = 2048;
+constexpr int kMaxParts = 4;
+constexpr int kMaxRank = 256, kMaxRanks = 512;  // of one part, of all
+
+// Rows of a tile: 16 (one matrix instruction) for a decode step, where most
+// tiles have few rows; 64 for prompts, whose rows of one adapter are many: A and
+// B are then read once per 64 rows.
+int tile_rows_for(int64_t rows) { return rows <= 1024 ? 16 : 64; }
+int64_t max_tiles(int64_t rows, int64_t adapters) {
+    return rows / tile_rows_for(rows) + std::min(rows, adapters);
+}
+
+// ---------------------------------------------------------------------- plan
+struct PlanArgs {
+    const int32_t *ids;
+    int32_t *order, *offsets;
+    int2 *tiles;
+    int rows, adapters, bits, tile_rows, max_tiles;
+};
+
+// One workgroup: each wave counts the adapters of a stretch of rows (64 rows at
+// a time: lanes of the same adapter find each other bit by bit), the counts of
+// (adapter, wave) become positions, and each wave goes through its stretch
+// again.  The waves' counts are their own, so the order does not depend on
+// scheduling.
+__global__ void __launch_bounds__(1024) lora_plan_kernel(PlanArgs a) {
+    __shared__ int at[16 * kMaxAdapters];
+    __shared__ int first[kMaxAdapters], tile0[kMaxAdapters];
+    __shared__ int scan_rows[16], scan_tiles[16];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, A = a.adapters;
+    const int stretch = ((a.rows + 1023) / 1024) * 64;
+    const int r0 = min(wave * stretch, a.rows), r1 = min(r0 + stretch, a.rows);
+    for (int i = t; i < 16 * A; i += 1024) at[i] = 0;
+    __syncthreads();
+    // the lanes whose row has this lane's adapter (0: no row, no adapter)
+    auto peers = [&](int r, int &id) -> uint64_t {
+        id = r < r1 ? a.ids[r] : -1;
+        const bool has = (unsigned)id < (unsigned)A;
+        uint64_t same = __ballot(has);
+        for (int b = 0; b < a.bits; ++b) {
+            const uint64_t set = __ballot((id >> b) & 1);
+            same &= (id >> b) & 1 ? set : ~set;
+        }
+        return has ? same : 0;
+    };
+    for (int r = r0; r < r1; r += 64) {
+        int id;
+        const uint64_t same = peers(r + lane, id);
+        if (same && lane == __ffsll((unsigned long long)same) - 1) atomicAdd(&at[wave * A + id], __popcll(same));
+    }
+    __syncthreads();
+    const int per = (A + 1023) / 1024, a0 = min(t * per, A), a1 = min(a0 + per, A);
+    int mine = 0, my_tiles = 0;
+    for (int x = a0; x < a1; ++x) {
+        int n = 0;
+        for (int w = 0; w < 16; ++w) {
+            const int c = at[w * A + x];
+            at[w * A + x] = n;
+            n += c;
+        }
+        first[x] = n;  // (for now its rows)
+        mine += n;
+        my_tiles += (n + a.tile_rows - 1) / a.tile_rows;
+    }
+    int total, tiles;
+    int pos = block_exclusive_scan_1024(mine, scan_rows, &total);
+    int tile = block_exclusive_scan_1024(my_tiles, scan_tiles, &tiles);
+    for (int x = a0; x < a1; ++x) {
+        const int n = first[x];
+        a.offsets[x] = pos;
+        first[x] = pos;
+        tile0[x] = tile;
+        for (int w = 0; w < 16; ++w) at[w * A + x] += pos;
+        pos += n;
+        tile += (n + a.tile_rows - 1) / a.tile_rows;
+    }
+    if (t == 0) a.offsets[A] = total;
+    for (int i = total + t; i < a.rows; i += 1024) a.order[i] = -1;
+    for (int i = tiles + t; i < a.max_tiles; i += 1024) a.tiles[i] = make_int2(-1, 0);
+    __syncthreads();
+    for (int r = r0; r < r1; r += 64) {
+        int id, base = 0;
+        const uint64_t same = peers(r + lane, id);
+        const int leader = same ? __ffsll((unsigned long long)same) - 1 : lane;
+        if (same && lane == leader) base = atomicAdd(&at[wave * A + id], __popcll(same));
+        base = __shfl(base, leader);
+        if (same) {
+            const int p = base + __popcll(same & ((1ull << lane) - 1)), j = p - first[id];
+            a.order[p] = r + lane;
+            if (j % a.tile_rows == 0) a.tiles[tile0[id] + j / a.tile_rows] = make_int2(id, p);
+        }
+    }
+}
+
+// ------------------------------------------------------------------- products
+struct LoraArgs {
+    const void *x;
+    const float *x_scales;  // fp8 rows
+    int64_t x_stride;
+    const void *a, *b;
+    const float *scales;  // [adapters] or null
+    const int32_t *order, *offsets;
+    const int2 *tiles;
+    float *v;  // [splits][rows][ranks16]
+    void *y;
+    int64_t y_stride;
+    int rows, adapters, k, n, rank, parts, ranks, ranks16, splits;
+    int part_end[kMaxParts], part_block;
+};
+
+// E values of a row from column c on, as the matrix instruction's operand (16
+// bytes of T): whole where `whole` says that rows are aligned and E divides their
+// length, else one by one; zeros from `cols` on.
+template <typename T> struct Operand;
+template <> struct Operand<uint16_t> {
+    static constexpr int E = 8;  // values a lane, 32 a step
+    static __device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Operand<float> {
+    static constexpr int E = 4;  // values a lane, 16 a step
+    static __device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, f32x4 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+        return c;
+    }
+};
+template <bool WHOLE>
+__device__ __forceinline__ u32x4 take(const uint16_t *row, int c, int cols) {
+    u32x4 w = {0, 0, 0, 0};
+    if (WHOLE) {
+        if (c < cols) w = *reinterpret_cast<const u32x4 *>(row + c);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < cols) w[i / 2] |= (uint32_t)row[c + i] << (16 * (i & 1));
+    }
+    return w;
+}
+template <bool WHOLE>
+__device__ __forceinline__ u32x4 take(const float *row, int c, int cols) {
+    u32x4 w = {0, 0, 0, 0};
+    if (WHOLE) {
+        if (c < cols) w = *reinterpret_cast<const u32x4 *>(row + c);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < cols) w[i] = __float_as_uint(row[c + i]);
+    }
+    return w;
+}
+// eight e4m3 values as bf16 (exact)
+template <bool WHOLE>
+__device__ __forceinline__ u32x4 take(const uint8_t *row, int c, int cols) {
+    u32x2 q = {0, 0};
+    if (WHOLE) {
+        if (c < cols) q = *reinterpret_cast<const u32x2 *>(row + c);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < cols) q[i / 4] |= (uint32_t)row[c + i] << (8 * (i & 3));
+    }
+    const u32x2 lo = e4m3x4_to_bf16x4(q[0]), hi = e4m3x4_to_bf16x4(q[1]);
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// Rows of tile `i`: its adapter, first position and count (0: none).
+__device__ __forceinline__ int tile_at(const LoraArgs &a, int i, int rows, int &adapter, int &p0) {
+    const int2 t = a.tiles[i];
+    adapter = t.x;
+    p0 = t.y;
+    if ((unsigned)adapter >= (unsigned)a.adapters || (unsigned)p0 >= (unsigned)a.rows) return 0;
+    return max(0, min(rows, min(a.offsets[adapter + 1], a.rows) - p0));
+}
+
+// v of a tile: MT groups of 16 rows by RT groups of 16 ranks, four waves that
+// take every fourth step of four matrix instructions of the workgroup's k.
+template <typename X, typename T, int MT, int RT, bool WHOLE>
+__global__ void __launch_bounds__(256) lora_shrink_kernel(LoraArgs a) {
+    constexpr int E = Operand<T>::E, U = 4, kStep = 4 * E * U;
+    __shared__ f32x4 sums[4][RT * MT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    int adapter, p0;
+    const int count = tile_at(a, blockIdx.x, 16 * MT, adapter, p0);
+    if (count == 0) return;
+    const int rt0 = blockIdx.y * RT, split = blockIdx.z;
+    const X *xr[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = a.order[p0 + min(16 * m + r16, count - 1)];
+        xr[m] = (const X *)a.x + (size_t)min((unsigned)row, (unsigned)a.rows - 1) * a.x_stride;
+    }
+    const T *ar[RT];
+#pragma unroll
+    for (int f = 0; f < RT; ++f)
+        ar[f] = (const T *)a.a + ((size_t)adapter * a.ranks + min((rt0 + f) * 16 + r16, a.ranks - 1)) * a.k;
+    f32x4 acc[RT][MT];
+#pragma unroll
+    for (int f = 0; f < RT; ++f)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = (split * 4 + wave) * kStep; c < a.k; c += a.splits * 4 * kStep) {
+        u32x4 av[U][RT], xv[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = c + 4 * E * u + E * g;
+#pragma unroll
+            for (int f = 0; f < RT; ++f) av[u][f] = take<WHOLE>(ar[f], at, a.k);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) xv[u][m] = take<WHOLE>(xr[m], at, a.k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int f = 0; f < RT; ++f)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[f][m] = Operand<T>::mfma(av[u][f], xv[u][m], acc[f][m]);
+    }
+#pragma unroll
+    for (int f = 0; f < RT; ++f)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) sums[wave][f * MT + m][lane] = acc[f][m];
+    __syncthreads();
+    const float scale = a.scales ? a.scales[adapter] : 1.0f;
+    for (int j = wave; j < RT * MT; j += 4) {
+        const int f = j / MT, i = 16 * (j % MT) + r16, rk = (rt0 + f) * 16 + 4 * g;
+        if (i >= count || rk >= a.ranks16) continue;
+        f32x4 v = sums[0][j][lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += sums[w][j][lane];
+        float s = scale;
+        if (sizeof(X) == 1) s *= a.x_scales[min((unsigned)a.order[p0 + i], (unsigned)a.rows - 1)];
+        v *= s;
+        *reinterpret_cast<f32x4 *>(a.v + ((size_t)split * a.rows + p0 + i) * a.ranks16 + rk) = v;
+    }
+}
+
+__device__ __forceinline__ int part_of(const LoraArgs &a, int col) {
+    if (a.part_block) return (col / a.part_block) % a.parts;
+    int p = 0;
+#pragma unroll
+    for (int i = 0; i < kMaxParts - 1; ++i) p += i < a.parts - 1 && col >= a.part_end[i];
+    return p;
+}
+
+// y of a tile and 256 columns.  v comes to LDS first, a part's ranks padded with
+// zeros to whole steps: f32 as it is; for bf16 each value as two, which together
+// hold 16 bits of it, so the sum keeps what f32 v has over one rounding to 8.
+template <typename T, int MT, bool WHOLE>
+__global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
+    constexpr int E = Operand<T>::E, kStep = 4 * E, H = sizeof(T) == 2 ? 2 : 1;  // H: halves of a value
+    extern __shared__ u32x4 lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    int adapter, p0;
+    const int count = tile_at(a, blockIdx.x, 16 * MT, adapter, p0);
+    if (count == 0) return;
+    const int steps = (a.rank + kStep - 1) / kStep, rp = steps * kStep;
+    const int line = rp / E + 1;  // 16-byte units of a row of a part; one spare against bank conflicts
+    const int plane = a.parts * 16 * MT * line;
+    T *lt = reinterpret_cast<T *>(lds);
+    for (int i = threadIdx.x; i < a.parts * 16 * MT * rp; i += 256) {
+        const int r = i % rp, row = i / rp % (16 * MT), part = i / rp / (16 * MT);
+        float v = 0.0f;
+        if (r < a.rank && row < count) {
+            const float *src = a.v + (size_t)(p0 + row) * a.ranks16 + part * a.rank + r;
+            for (int s = 0; s < a.splits; ++s) v += src[(size_t)s * a.rows * a.ranks16];
+        }
+        const size_t to = (size_t)(part * 16 * MT + row) * line * E + r;
+        if constexpr (H == 2) {
+            const uint32_t hi = f32_to_bf16_bits(v), top = hi << 16;
+            // (nothing is left of a value that has no finite first half)
+            const float rest = (top & 0x7f800000u) == 0x7f800000u ? 0.0f : v - __uint_as_float(top);
+            lt[to] = (T)hi;
+            lt[(size_t)plane * E + to] = (T)f32_to_bf16_bits(rest);
+        } else {
+            lt[to] = v;
+        }
+    }
+    __syncthreads();
+    const int n0 = blockIdx.y * 256 + wave * 64;
+    if (n0 >= a.n) return;
+    // row r16 of B tile t: column n0 + 16 (r16 / 4) + 4 t + r16 % 4
+    const int c0 = n0 + 16 * (r16 >> 2) + (r16 & 3);
+    const T *bb = (const T *)a.b + (size_t)adapter * a.n * a.rank;
+    // the product of these columns with part p's values
+    auto product = [&](int p, f32x4 (&acc)[4][MT]) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < steps; ++s) {
+            u32x4 bv[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                bv[t] = take<WHOLE>(bb + (size_t)min(c0 + 4 * t, a.n - 1) * a.rank, s * kStep + E * g, a.rank);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const u32x4 vv = lds[h * plane + (p * 16 * MT + 16 * m + r16) * line + s * 4 + g];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) acc[t][m] = Operand<T>::mfma(bv[t], vv, acc[t][m]);
+                }
+        }
+    };
+    f32x4 acc[4][MT];
+    const int last = min(n0 + 63, a.n - 1), part = part_of(a, n0);
+    if (a.parts == 1 || (part_of(a, last) == part && (!a.part_block || a.part_block >= 64))) {
+        product(part, acc);
+    } else {  // columns of several parts: each takes its own part's product
+        f32x4 one[4][MT];
+        for (int p = 0; p < a.parts; ++p) {
+            product(p, one);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool mine = part_of(a, min(n0 + 16 * g + 4 * t + e, a.n - 1)) == p;
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) acc[t][m][e] = mine || p == 0 ? one[t][m][e] : acc[t][m][e];
+                }
+        }
+    }
+    // lane: columns n0 + 16 g .. + 15 of row r16 of each group
+    const int n1 = n0 + 16 * g;
+    if (n1 >= a.n) return;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int i = 16 * m + r16;
+        if (i >= count) continue;
+        const unsigned row = (unsigned)a.order[p0 + i];
+        if (row >= (unsigned)a.rows) continue;
+        T *y = (T *)a.y + (size_t)row * a.y_stride + n1;
+        if (n1 + 16 <= a.n && (((uintptr_t)y) & 15u) == 0) {
+            u32x4 *yw = reinterpret_cast<u32x4 *>(y);
+            u32x4 w[16 / E];
+#pragma unroll
+            for (int j = 0; j < 16 / E; ++j) w[j] = yw[j];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float d = acc[j / 4][m][j % 4];
+                if constexpr (H == 2) {
+                    const uint32_t o = w[j / 8][j % 8 / 2];
+                    if (j % 2 == 0) w[j / 8][j % 8 / 2] = (o & 0xffff0000u) | f32_to_bf16_bits(bf16lo(o) + d);
+                    else w[j / 8][j % 8 / 2] = (o & 0xffffu) | f32_to_bf16_bits(bf16hi(o) + d) << 16;
+                } else {
+                    w[j / 4][j % 4] = __float_as_uint(__uint_as_float(w[j / 4][j % 4]) + d);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 16 / E; ++j) yw[j] = w[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (n1 + j < a.n) {
+                    const float d = acc[j / 4][m][j % 4];
+                    if constexpr (H == 2) y[j] = (T)f32_to_bf16_bits(__uint_as_float((uint32_t)y[j] << 16) + d);
+                    else y[j] += d;
+                }
+        }
+    }
+}
+
+// Workgroups of k of one tile and rank group: enough of them for two a CU, a
+// wave at least two steps.
+int splits_for(int64_t rows, int64_t adapters, int groups, int64_t k, int step) {
+    const int64_t tiles = std::max<int64_t>(1, max_tiles(rows, adapters)) * groups;
+    const int64_t most = std::max<int64_t>(1, k / (8 * step)), want = std::max<int64_t>(1, 512 / tiles);
+    return (int)std::min<int64_t>({most, want, 16});
+}
+int rank_groups(int ranks) { return ranks <= 16 ? 1 : ranks <= 32 ? 2 : 4; }  // 16-rank tiles a workgroup
+
+bool meet(const void *p, int64_t pb, const void *q, int64_t qb) {
+    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+    return p && q && pb > 0 && qb > 0 && a < b + qb && b < a + pb;
+}
+int bad(const char *what) { return set_error(ZK_ERR_INVALID_ARGUMENT, std::string("Internal error: ") + what); }
+bool aligned(const void *p, int b) { return ((uintptr_t)p & (uintptr_t)(b - 1)) == 0; }
+
+bool shape_ok(int64_t rows, int64_t adapters, int64_t k, int rank, int parts) {
+    return rows >= 0 && rows <= (1 << 24) && adapters >= 1 && adapters <= kMaxAdapters && k >= 1 && k <= (1 << 23) && rank >= 1 &&
+           rank <= kMaxRank && parts >= 1 && parts <= kMaxParts && rank * parts <= kMaxRanks;
+}
+int step_of(zk_dtype dtype) { return dtype == ZK_F32 ? 64 : 128; }
+int splits_of(int64_t rows, int64_t adapters, int64_t k, int rank, int parts, zk_dtype dtype) {
+    const int rt = rank_groups(rank * parts), groups = ((rank * parts + 15) / 16 + rt - 1) / rt;
+    return splits_for(rows, adapters, groups, k, step_of(dtype));
+}
+
+template <typename X, typename T, int MT>
+void shrink(const LoraArgs &a, int tiles, bool whole, hipStream_t s) {
+    const int rt = rank_groups(a.ranks), groups = ((a.ranks + 15) / 16 + rt - 1) / rt;
+    const dim3 grid((unsigned)tiles, (unsigned)groups, (unsigned)a.splits);
+    auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(a); };
+    if (rt == 1) whole ? go(lora_shrink_kernel<X, T, MT, 1, true>) : go(lora_shrink_kernel<X, T, MT, 1, false>);
+    else if (rt == 2) whole ? go(lora_shrink_kernel<X, T, MT, 2, true>) : go(lora_shrink_kernel<X, T, MT, 2, false>);
+    else whole ? go(lora_shrink_kernel<X, T, MT, 4, true>) : go(lora_shrink_kernel<X, T, MT, 4, false>);
+}
+
+template <typename T, int MT>
+void expand(const LoraArgs &a, int tiles, hipStream_t s) {
+    constexpr int E = Operand<T>::E;
+    const int rp = (a.rank + 4 * E - 1) / (4 * E) * 4 * E;
+    const size_t bytes = (size_t)(sizeof(T) == 2 ? 2 : 1) * a.parts * 16 * MT * (rp / E + 1) * 16;
+    const bool whole = a.rank % E == 0 && aligned(a.b, 16);
+    const dim3 grid((unsigned)tiles, (unsigned)((a.n + 255) / 256));
+    auto go = [&](auto kernel) {
+        if (bytes > 65536) (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        kernel<<<grid, 256, bytes, s>>>(a);
+    };
+    whole ? go(lora_expand_kernel<T, MT, true>) : go(lora_expand_kernel<T, MT, false>);
+}
+
+template <typename X, typename T>
+void both(const LoraArgs &a, int tiles, hipStream_t s) {
+    constexpr int E = Operand<T>::E;
+    const bool whole = a.k % E == 0 && a.x_stride % E == 0 && aligned(a.x, E * (int)sizeof(X)) && aligned(a.a, 16);
+    if (tile_rows_for(a.rows) == 16) {
+        shrink<X, T, 1>(a, tiles, whole, s);
+        expand<T, 1>(a, tiles, s);
+    } else {
+        shrink<X, T, 4>(a, tiles, whole, s);
+        expand<T, 4>(a, tiles, s);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t zk_lora_max_tiles(int64_t num_rows, int64_t num_adapters) {
+    if (num_rows <= 0 || num_rows > (1 << 24) || num_adapters <= 0 || num_adapters > kMaxAdapters) return 0;
+    return max_tiles(num_rows, num_adapters);
+}
+
+int zk_lora_plan(const int32_t *adapter_ids, int64_t num_rows, int64_t num_adapters, int32_t *order, int32_t *offsets,
+                 int32_t *tiles, void *stream) {
+    if (num_rows < 0 || num_rows > (1 << 24) || num_adapters <= 0 || num_adapters > kMaxAdapters)
+        return bad("zk_lora_plan: bad shape (at most 2^24 rows and 2048 adapters)");
+    if (!offsets || (num_rows > 0 && (!adapter_ids || !order || !tiles))) return bad("zk_lora_plan: NULL pointer");
+    if (!aligned(tiles, 8)) return bad("zk_lora_plan: tiles must be 8-byte aligned");
+    const int64_t nt = num_rows ? max_tiles(num_rows, num_adapters) : 0;
+    const struct {
+        const void *p;
+        int64_t bytes;
+    } all[] = {{order, 4 * num_rows}, {offsets, 4 * (num_adapters + 1)}, {tiles, 8 * nt}, {adapter_ids, 4 * num_rows}};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 4; ++j)
+            if (meet(all[i].p, all[i].bytes, all[j].p, all[j].bytes)) return bad("zk_lora_plan: operands overlap");
+    PlanArgs a{};
+    a.ids = adapter_ids;
+    a.order = order;
+    a.offsets = offsets;
+    a.tiles = (int2 *)tiles;
+    a.rows = (int)num_rows;
+    a.adapters = (int)num_adapters;
+    while ((1 << a.bits) < num_adapters) ++a.bits;
+    a.tile_rows = tile_rows_for(num_rows);
+    a.max_tiles = (int)nt;
+    hipStream_t s = (hipStream_t)stream;
+    KernelTimer timer("lora_plan", s);
+    lora_plan_kernel<<<1, 1024, 0, s>>>(a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess)
+        return set_error(ZK_ERR_HIP, std::string("Internal error: zk_lora_plan: ") + hipGetErrorString(e));
+    return ZK_OK;
+}
+
+size_t zk_lora_workspace_size(int64_t num_rows, int64_t num_adapters, int64_t k, int rank, int num_parts, zk_dtype dtype) {
+    if (!shape_ok(num_rows, num_adapters, k, rank, num_parts) || num_rows == 0) return 0;
+    return (size_t)splits_of(num_rows, num_adapters, k, rank, num_parts, dtype) * num_rows * ((rank * num_parts + 15) / 16 * 16) * 4;
+}
+
+int zk_lora(const void *x, const float *x_scales, int64_t x_stride, zk_dtype x_dtype, const void *a_weights,
+            const void *b_weights, const float *scales, zk_dtype dtype, const int32_t *order, const int32_t *offsets,
+            const int32_t *tiles, int64_t num_rows, int64_t num_adapters, int64_t k, int64_t n, int rank, int num_parts,
+            const int64_t *part_cols, int part_block, void *y, int64_t y_stride, void *workspace, size_t workspace_bytes,
+            void *stream) {
+    if (dtype != ZK_F32 && dtype != ZK_BF16) return bad("zk_lora: the weights and y must be f32 or bf16");
+    if (x_dtype != dtype && !(x_dtype == ZK_FP8_E4M3 && dtype == ZK_BF16))
+        return bad("zk_lora: x must have the weights' type, or be fp8 beside bf16 weights");
+    if ((x_dtype == ZK_FP8_E4M3) != (x_scales != nullptr)) return bad("zk_lora: x_scales go with fp8 rows");
+    if (!shape_ok(num_rows, num_adapters, k, rank, num_parts) || n <= 0 || n > (1 << 23) || part_block < 0)
+        return bad("zk_lora: bad shape (ranks of a part at most 256, of all parts 512, at most 4 parts and 2048 adapters)");
+    if (x_stride == 0) x_stride = k;
+    if (y_stride == 0) y_stride = n;
+    if (x_stride < k || y_stride < n || x_stride > (1ll << 31) || y_stride > (1ll << 31)) return bad("zk_lora: bad row stride");
+    LoraArgs a{};
+    if (part_block) {
+        if (n % ((int64_t)part_block * num_parts)) return bad("zk_lora: the columns must be whole rounds of the parts' blocks");
+    } else if (num_parts > 1) {
+        if (!part_cols) return bad("zk_lora: part_cols missing");
+        int64_t end = 0;
+        for (int i = 0; i < num_parts; ++i) {
+            if (part_cols[i] <= 0 || part_cols[i] > n) return bad("zk_lora: parts must hold the columns of y");
+            end += part_cols[i];
+            a.part_end[i] = (int)std::min(end, n);
+        }
+        if (end != n) return bad("zk_lora: parts must hold the columns of y");
+    }
+    if (num_rows == 0) return ZK_OK;
+    if (!x || !a_weights || !b_weights || !order || !offsets || !tiles || !y) return bad("zk_lora: NULL pointer");
+    const size_t need = zk_lora_workspace_size(num_rows, num_adapters, k, rank, num_parts, dtype);
+    if (!workspace || workspace_bytes < need) return bad("zk_lora: workspace too small (zk_lora_workspace_size)");
+    if (!aligned(workspace, 16) || !aligned(tiles, 8)) return bad("zk_lora: the workspace must be 16-byte, tiles 8-byte aligned");
+    const int e = elt_size(dtype), ranks = rank * num_parts;
+    const int64_t nt = max_tiles(num_rows, num_adapters);
+    const int64_t xb = ((num_rows - 1) * x_stride + k) * elt_size(x_dtype), yb = ((num_rows - 1) * y_stride + n) * e;
+    const struct {
+        const void *p;
+        int64_t bytes;
+    } in[] = {{x, xb}, {x_scales, 4 * num_rows}, {a_weights, num_adapters * ranks * k * e}, {b_weights, num_adapters * n * rank * e},
+              {scales, 4 * num_adapters}, {order, 4 * num_rows}, {offsets, 4 * (num_adapters + 1)}, {tiles, 8 * nt}};
+    for (const auto &i : in)
+        if (meet(i.p, i.bytes, y, yb) || meet(i.p, i.bytes, workspace, (int64_t)need)) return bad("zk_lora: y or the workspace overlaps an input");
+    if (meet(y, yb, workspace, (int64_t)need)) return bad("zk_lora: y overlaps the workspace");
+    a.x = x;
+    a.x_scales = x_scales;
+    a.x_stride = x_stride;
+    a.a = a_weights;
+    a.b = b_weights;
+    a.scales = scales;
+    a.order = order;
+    a.offsets = offsets;
+    a.tiles = (const int2 *)tiles;
+    a.v = (float *)workspace;
+    a.y = y;
+    a.y_stride = y_stride;
+    a.rows = (int)num_rows;
+    a.adapters = (int)num_adapters;
+    a.k = (int)k;
+    a.n = (int)n;
+    a.rank = rank;
+    a.parts = num_parts;
+    a.ranks = ranks;
+    a.ranks16 = (ranks + 15) / 16 * 16;
+    a.splits = splits_of(num_rows, num_adapters, k, rank, num_parts, dtype);
+    a.part_block = part_block;
+    hipStream_t s = (hipStream_t)stream;
+    KernelTimer timer("lora", s);
+    if (dtype == ZK_F32) both<float, float>(a, (int)nt, s);
+    else if (x_dtype == ZK_BF16) both<uint16_t, uint16_t>(a, (int)nt, s);
+    else both<uint8_t, uint16_t>(a, (int)nt, s);
+    if (hipError_t er = hipGetLastError(); er != hipSuccess)
+        return set_error(ZK_ERR_HIP, std::string("Internal error: zk_lora: ") + hipGetErrorString(er));
+    return ZK_OK;
+}
+
+}  // extern "C"

@@ -1,15 +1,20 @@
 """Dense ops around the paged-KV path over the C ABI (include/zealot_dense.h):
 rms_norm (optionally fused with the residual add), silu_mul, add, embedding,
 qk_norm_rope (head norms and rotary embedding) and linear (hipBLASLt or the weight-streaming kernel; TiledWeight for weights
-kept in that kernel's tiled layout).  Torch device tensors in, launches on
+kept in that kernel's tiled layout); rms_norm_fp8, silu_mul_fp8 and linear_fp8
+(rows and weights in 8 bits); lora_plan and lora (low-rank adapters of the
+requests beside a shared projection).  Torch device tensors in, launches on
 torch's current stream; the kernels are in zealot_amd/csrc/dense_ops.hip,
-rope_ops.hip, gemm.cpp and skinny_gemm.hip."""
+rope_ops.hip, gemm.cpp, skinny_gemm.hip, fp8_rows.hip, fp8_gemm.hip and lora_ops.hip."""
 from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from .ops import _dev, _dims, _empty, _rope_operands, _rows, _stream, _target, zk_dtype
+from .ops import _dev, _dims, _empty, _need, _need_opt, _rope_operands, _rows, _stream, _target, zk_dtype
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -326,6 +331,245 @@ def linear_silu_mul(x, gate_up, out=None, gu=None, stream=None):
     _lib.check(_lib.lib().zk_linear_silu_mul(_dev(x, "x"), _dev(gate_up, "gate_up"), _dev(out, "out"), m, n // 2, k,
                                              _dev(gu, "gu"), _stream(stream)))
     return out
+
+
+# ------------------------------------------------------------------ projections in 8 bits
+
+class Fp8Rows(NamedTuple):
+    """Rows in 8 bits: e4m3 values [m, k] and one float32 scale a row [m]; a
+    row's values are data * scale."""
+    data: torch.Tensor
+    scales: torch.Tensor
+
+
+_FP8 = torch.float8_e4m3fn
+
+
+def _fp8_out(out, like, rows: int, cols: int, cur: int, stream):
+    """(the Fp8Rows to write, addresses of its values and scales)."""
+    if out is None:
+        out = Fp8Rows(_empty(like, (rows, cols), _FP8, stream), _empty(like, (rows,), torch.float32, stream))
+        return out, out.data.data_ptr(), out.scales.data_ptr()
+    return out, _need(out.data, "out.data", (rows, cols), _FP8, cur), _need(out.scales, "out.scales", (rows,), torch.float32, cur)
+
+
+def rms_norm_fp8(x, weight, eps: float = 1e-6, residual=None, out=None, residual_out=None, rows=None, stream=None):
+    """rms_norm with the rows written in 8 bits for linear_fp8
+    (zk_rms_norm_fp8): returns Fp8Rows, or (Fp8Rows, residual_out) with a
+    residual.  x [T, dim]; rows (device int64) selects some of them, one outside
+    x gives zeros; residual_out may be x or `residual` when rows is None."""
+    t, dim = _dims(x, "x", "[T, dim]")
+    dt = x.dtype
+    code = _dt(x)
+    cur, at_stream = _target(stream)
+    px, pw = _need(x, "x", (t, dim), dt, cur), _need(weight, "weight", (dim,), dt, cur)
+    pr, n, pi = _need_opt(residual, "residual", (t, dim), dt, cur), t, None
+    if rows is not None:
+        n, = _dims(rows, "rows", "[rows]")
+        pi = _need(rows, "rows", (n,), torch.int64, cur)
+    po = None
+    if residual is not None:
+        if residual_out is None:
+            residual_out = _empty(x, (n, dim), dt, stream)
+            po = residual_out.data_ptr()
+        else:
+            po = _need(residual_out, "residual_out", (n, dim), dt, cur)
+    out, pq, ps = _fp8_out(out, x, n, dim, cur, stream)
+    # (an empty selection has no address: NULL would mean all rows)
+    _lib.check(_lib.lib().zk_rms_norm_fp8(px, pr, pw, pq, ps, po, pi if n else px, t, n, dim, eps, code, at_stream))
+    return out if residual is None else (out, residual_out)
+
+
+def silu_mul_fp8(gate, up, out=None, stream=None):
+    """silu_mul with the rows written in 8 bits for linear_fp8
+    (zk_silu_mul_fp8): gate and up [rows, cols] may be column slices of one
+    tensor; returns Fp8Rows."""
+    rows, cols = _dims(gate, "gate", "[rows, cols]")
+    dt = gate.dtype
+    code = _dt(gate)
+    cur, at_stream = _target(stream)
+    gs, us = _rows2(gate, "gate", rows, cols, dt, cur), _rows2(up, "up", rows, cols, dt, cur)
+    out, pq, ps = _fp8_out(out, gate, rows, cols, cur, stream)
+    _lib.check(_lib.lib().zk_silu_mul_fp8(gate.data_ptr(), up.data_ptr(), pq, ps, rows, cols, gs, us, code, at_stream))
+    return out
+
+
+def _rows2(t, name: str, rows: int, cols: int, dtype, cur: int) -> int:
+    """Elements from one row of an operand [rows, cols] to the next; a row is packed."""
+    try:
+        ok = t.get_device() == cur and t.dtype is dtype and t.shape == (rows, cols)
+    except AttributeError:
+        ok = False
+    if not ok:
+        _need(t, name, (rows, cols), dtype, cur)
+    st = t.stride()
+    if rows and ((st[1] != 1 and cols > 1) or (st[0] < cols and rows > 1)):
+        raise ValueError(f"{name} must have packed rows that do not overlap")
+    return st[0] if rows > 1 else cols
+
+
+class Fp8Weight:
+    """A weight [n, k] in 8 bits with one float32 scale a row (`scales` [n]), in
+    the packed order that linear_fp8 reads (zk_fp8_weight; fp8_weight makes
+    one).  `data` is the flat device buffer."""
+
+    __slots__ = ("data", "scales", "n", "k")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, n: int, k: int):
+        if data.dtype != torch.uint8 or data.dim() != 1 or data.numel() != _lib.lib().zk_fp8_weight_bytes(n, k) or not data.is_contiguous():
+            raise ValueError("a packed weight is a flat uint8 buffer of zk_fp8_weight_bytes(n, k)")
+        if scales.dtype != torch.float32 or tuple(scales.shape) != (n,) or not scales.is_contiguous():
+            raise ValueError("scales must be float32 [n]")
+        if scales.device != data.device:
+            raise ValueError("scales must be on the packed weight's device")
+        self.data, self.scales, self.n, self.k = data, scales, n, k
+
+    @property
+    def shape(self):
+        return (self.n, self.k)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def numel(self) -> int:
+        return self.n * self.k
+
+    def rowmajor(self) -> torch.Tensor:
+        """The e4m3 values, row-major [n, k] (the inverse permutation, on the device)."""
+        groups, chunks = -(-self.n // 64), -(-self.k // 128)
+        # [G tile chunk unit 4 4 byte]: row 64 G + 16 i1 + 4 tile + i0, column 128 chunk + 16 unit + byte
+        t = self.data.view(groups, 4, chunks, 8, 4, 4, 16).permute(0, 4, 1, 5, 2, 3, 6)
+        return t.reshape(groups * 64, chunks * 128)[:self.n, :self.k].contiguous().view(_FP8)
+
+
+def fp8_weight(weight: torch.Tensor, scales: torch.Tensor | None = None, stream=None) -> Fp8Weight:
+    """The 8-bit packed form of a weight [n, k] (nn.Linear layout): float32 or
+    bfloat16 values, rounded with a scale a row, or float8_e4m3fn values with
+    their float32 `scales` [n]."""
+    n, k = _dims(weight, "weight", "[n, k]")
+    ready = weight.dtype == _FP8
+    if not ready:
+        _dt(weight)
+    if ready != (scales is not None):
+        raise ValueError("scales go with float8_e4m3fn weights")
+    cur, at_stream = _target(stream)
+    pw = _need(weight, "weight", (n, k), weight.dtype, cur)
+    if n == 0 or k == 0:
+        raise ValueError("weight must not be empty")
+    if ready:
+        _need(scales, "scales", (n,), torch.float32, cur)
+    else:
+        scales = _empty(weight, (n,), torch.float32, stream)
+    data = _empty(weight, (_lib.lib().zk_fp8_weight_bytes(n, k),), torch.uint8, stream)
+    _lib.check(_lib.lib().zk_fp8_weight(pw, zk_dtype(weight), data.data_ptr(), scales.data_ptr(), n, k, at_stream))
+    return Fp8Weight(data, scales, n, k)
+
+
+def linear_fp8(x: Fp8Rows, weight: Fp8Weight, out=None, out_dtype=torch.bfloat16, stream=None):
+    """x . weight^T for rows and a weight in 8 bits (zk_linear_fp8): y [m, n],
+    bfloat16 or float32 (`out_dtype`, or out's own).  k % 16 == 0."""
+    m, k = _dims(x.data, "x.data", "[m, k]")
+    if not isinstance(weight, Fp8Weight):
+        raise TypeError("weight must be an Fp8Weight (fp8_weight makes one)")
+    n = weight.n
+    if weight.k != k:
+        raise ValueError(f"x has {k} columns, the weight {weight.k}")
+    cur, at_stream = _target(stream)
+    px, ps = _need(x.data, "x.data", (m, k), _FP8, cur), _need(x.scales, "x.scales", (m,), torch.float32, cur)
+    pw, pws = _need(weight.data, "weight", weight.data.shape, torch.uint8, cur), _need(weight.scales, "weight.scales", (n,), torch.float32, cur)
+    if out is None:
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"out_dtype must be float32 or bfloat16, got {out_dtype}")
+        out = _empty(x.data, (m, n), out_dtype, stream)
+        py = out.data_ptr()
+    else:
+        py = _need(out, "out", (m, n), None, cur)
+        _dt(out)
+    _lib.check(_lib.lib().zk_linear_fp8(px, ps, pw, pws, py, m, n, k, zk_dtype(out), at_stream))
+    return out
+
+
+# ------------------------------------------------------------------ low-rank adapters
+
+class LoraPlan(NamedTuple):
+    """A step's rows grouped by adapter (lora_plan), for all its projections."""
+    order: torch.Tensor    # int32 [T]: the rows with an adapter, sorted by it; then -1
+    offsets: torch.Tensor  # int32 [adapters + 1]: where each adapter's rows begin in it
+    tiles: torch.Tensor    # int32 [tiles, 2]: the kernels' own
+
+
+def lora_plan(adapter_ids, num_adapters: int, out: LoraPlan | None = None, stream=None) -> LoraPlan:
+    """Group the rows of a step by adapter (zk_lora_plan): adapter_ids int32 [T],
+    outside [0, num_adapters): none."""
+    t, = _dims(adapter_ids, "adapter_ids", "[T]")
+    cur, at_stream = _target(stream)
+    i32 = torch.int32
+    ids = _need(adapter_ids, "adapter_ids", (t,), i32, cur)
+    if num_adapters <= 0:
+        raise ValueError("num_adapters must be positive")
+    tiles = _lib.lib().zk_lora_max_tiles(t, num_adapters)
+    if out is None:  # one buffer, the tiles first
+        buf = _empty(adapter_ids, (2 * tiles + t + num_adapters + 1,), i32, stream)
+        part = buf.split_with_sizes((2 * tiles, t, num_adapters + 1))
+        out = LoraPlan(part[1], part[2], part[0].view(tiles, 2))
+    _lib.check(_lib.lib().zk_lora_plan(ids, t, num_adapters, _need(out.order, "out.order", (t,), i32, cur),
+                                       _need(out.offsets, "out.offsets", (num_adapters + 1,), i32, cur),
+                                       _need(out.tiles, "out.tiles", (tiles, 2), i32, cur), at_stream))
+    return out
+
+
+def lora_workspace_bytes(num_rows: int, num_adapters: int, k: int, rank: int, num_parts: int, dtype) -> int:
+    return int(_lib.lib().zk_lora_workspace_size(num_rows, num_adapters, k, rank, num_parts, _LORA_CODES[dtype]))
+
+
+_LORA_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+def lora(x, a, b, scales, plan: LoraPlan, y, parts=None, part_block: int = 0, workspace=None, stream=None):
+    """y += scales[i] b[i] (a[i] x) row by row, i the row's adapter in `plan`
+    (zk_lora); rows without one stay as they are.  x [T, k] (rows may lie apart)
+    of the weights' type, or Fp8Rows beside bfloat16 weights; a [adapters, P * rank,
+    k], b [adapters, n, rank], scales float32 [adapters] or None; y [T, n], in
+    place (rows may lie apart: columns of a fused output).  parts: the columns of
+    y's P parts, each with ranks of its own (None: one), or, with part_block, how
+    many parts take turns of part_block columns.  Returns y."""
+    na, n, rank = _dims(b, "b", "[adapters, n, rank]")
+    dt = b.dtype
+    code = _dt(b)
+    rows = x.data if isinstance(x, Fp8Rows) else x
+    t, k = _dims(rows, "x", "[T, k]")
+    cur, at_stream = _target(stream)
+    cols, p = None, 1
+    if part_block:
+        if not isinstance(parts, int) or parts < 1:
+            raise ValueError("with part_block, parts is their number")
+        p = parts
+    elif parts is not None:
+        p = len(parts)
+        if p == 0 or sum(parts) != n:
+            raise ValueError(f"parts must add up to the {n} columns of y")
+        cols = (ctypes.c_int64 * p)(*parts)
+    if isinstance(x, Fp8Rows):
+        xc, xs = _lib.FP8_E4M3, _rows2(rows, "x.data", t, k, _FP8, cur)
+        sc = _need(x.scales, "x.scales", (t,), torch.float32, cur)
+    else:
+        xc, xs, sc = code, _rows2(rows, "x", t, k, dt, cur), None
+    ys = _rows2(y, "y", t, n, dt, cur)
+    lib = _lib.lib()
+    i32 = torch.int32
+    tiles = lib.zk_lora_max_tiles(t, na)
+    size = lib.zk_lora_workspace_size(t, na, k, rank, p, code)
+    if workspace is None:
+        ws = (_empty(y, (size,), torch.uint8, stream).data_ptr() if size else None, size)
+    else:
+        ws = (_need(workspace, "workspace", workspace.shape, None, cur), workspace.numel() * workspace.element_size())
+    _lib.check(lib.zk_lora(
+        rows.data_ptr(), sc, xs, xc, _need(a, "a", (na, p * rank, k), dt, cur), _need(b, "b", (na, n, rank), dt, cur),
+        _need_opt(scales, "scales", (na,), torch.float32, cur), code, _need(plan.order, "plan.order", (t,), i32, cur),
+        _need(plan.offsets, "plan.offsets", (na + 1,), i32, cur), _need(plan.tiles, "plan.tiles", (tiles, 2), i32, cur), t, na, k, n,
+        rank, p, cols, part_block, y.data_ptr(), ys, *ws, at_stream))
+    return y
 
 
 def linear_choice(m, n, k, in_dtype=torch.bfloat16, out_dtype=None, tiled=False) -> dict:
