@@ -208,11 +208,16 @@ int zk_silu_mul_fp8(const void *gate, const void *up, void *q, float *scales, in
 size_t zk_fp8_weight_bytes(int64_t n, int64_t k);
 int zk_fp8_weight(const void *w, zk_dtype dtype, void *packed, float *scales, int64_t n, int64_t k, void *stream);
 /* y[m, n] = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] for x [m, k] in 8 bits
- * (packed rows; k % 16 == 0) and a packed weight, f32 sums, y F32 or BF16.  x,
- * the weight and y 16-byte aligned.  Nothing is tuned: a call launches what its
- * sizes say. */
+ * (packed rows; k % 16 == 0) and a packed weight; y F32 or BF16.  Sums in f32; for
+ * BF16 each eight products are first cut to a multiple of 2^-13 of the largest
+ * one's power of two (the 8-bit matrix instruction's own rounding), F32 results
+ * keep their 24 bits.  x, the weight and y 16-byte aligned.  Nothing is tuned: a
+ * call launches what its sizes say, and values are added in a fixed order.
+ * workspace: zk_linear_fp8_workspace_size bytes (0: none needed), 16-byte aligned;
+ * calls that share one must not overlap in time. */
+size_t zk_linear_fp8_workspace_size(int64_t m, int64_t n, int64_t k, zk_dtype out_dtype);
 int zk_linear_fp8(const void *x, const float *x_scales, const void *packed, const float *w_scales, void *y, int64_t m,
-                  int64_t n, int64_t k, zk_dtype out_dtype, void *stream);
+                  int64_t n, int64_t k, zk_dtype out_dtype, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- low-rank adapters of many requests beside a shared projection.  No
  * reference counterpart (one set of weights, model_loader.rs:241).

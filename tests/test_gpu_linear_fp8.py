@@ -93,7 +93,10 @@ def test_products(m, n, k, out_dtype):
     _check(y, x, w, ws, out_dtype)
 
 
-@pytest.mark.parametrize("m,n,k", [(4100, 4200, 256), (2049, 8192, 144), (300, 28672, 512)])
+@pytest.mark.parametrize("m,n,k", [(4100, 4200, 256), (2049, 8192, 144), (300, 28672, 512), (1000, 9000, 16), (2300, 4100, 80), (700, 20000, 64),
+                                   (1025, 7000, 1040), (900, 4160, 1472), (64, 4096, 14336), (40, 1000, 8192), (130, 2000, 6000), (256, 70, 16384),
+                                   (2560, 4096, 208), (4000, 4030, 2000), (3900, 4030, 1040), (500, 28610, 2192),
+                                   (300, 30001, 1072), (500, 30000, 1088), (4000, 4096, 640), (8200, 4100, 528)])
 def test_large_products(m, n, k):
     from zealot_amd import dense
     x, w, ws = _rows(3, m, k), _randn(5, (n, k), 20.0).clamp(-448, 448).to(FP8), 0.01 + _randn(6, (n,)).abs()

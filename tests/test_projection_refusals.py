@@ -60,23 +60,31 @@ def test_silu_mul_fp8():
 def test_fp8_weight():
     size = _lib.lib().zk_fp8_weight_bytes
     assert size(64, 128) == 8192 and size(1, 1) == 8192 and size(65, 129) == 4 * 8192
-    assert size(0, 1) == 0 and size(1, 0) == 0 and size(1 << 25, 1) == 0
+    assert size(0, 1) == 0 and size(1, 0) == 0 and size((1 << 22) + 1, 1) == 0
     base = dict(w=_at(0), dt=_lib.BF16, p=_at(0x300000), s=_at(0x500000), n=100, k=300)
     call = lambda **kw: _rc(_lib.lib().zk_fp8_weight(*dict(base, **kw).values(), None))  # noqa: E731
-    for kw in (dict(dt=7), dict(n=0), dict(k=0), dict(n=1 << 25), dict(w=None), dict(p=None), dict(s=None), dict(p=_at(8)), dict(p=_at(0x300008)),
+    for kw in (dict(dt=7), dict(n=0), dict(k=0), dict(n=(1 << 22) + 1), dict(w=None), dict(p=None), dict(s=None), dict(p=_at(8)), dict(p=_at(0x300008)),
                dict(p=_at(1024)), dict(s=_at(100)), dict(s=_at(0x300100))):
         assert call(**kw)[0] == BAD, kw
 
 
 def test_linear_fp8():
-    base = dict(x=_at(0), xs=_at(0x100000), w=_at(0x200000), ws=_at(0x300000), y=_at(0x400000), m=10, n=100, k=256, dt=_lib.BF16)
+    base = dict(x=_at(0), xs=_at(0x100000), w=_at(0x200000), ws=_at(0x300000), y=_at(0x400000), m=10, n=100, k=256, dt=_lib.BF16, wk=None, wb=0)
     call = lambda **kw: _rc(_lib.lib().zk_linear_fp8(*dict(base, **kw).values(), None))  # noqa: E731
     for kw in (dict(dt=_lib.FP8_E4M3), dict(m=-1), dict(n=0), dict(k=0), dict(k=250), dict(k=8), dict(m=1 << 25), dict(n=1 << 25), dict(k=1 << 25),
                dict(x=None), dict(xs=None), dict(w=None), dict(ws=None), dict(y=None), dict(x=_at(8)), dict(w=_at(0x200008)), dict(y=_at(0x400004)),
-               dict(y=_at(0)), dict(y=_at(0x100000)), dict(y=_at(0x200100)), dict(y=_at(0x300000)), dict(m=1 << 24, n=1 << 24)):
+               dict(y=_at(0)), dict(y=_at(0x100000)), dict(y=_at(0x200100)), dict(y=_at(0x300000)), dict(m=1 << 24, n=1 << 22)):
         rc, msg = call(**kw)
         assert rc == BAD and "zk_linear_fp8" in msg, kw
     assert call(m=0, x=None)[0] == OK
+    # k split over workgroups: the sums need room
+    far = dict(m=64, n=4096, k=14336, x=_at(0), xs=_at(0x1000000), w=_at(0x2000000), ws=_at(0x9000000), y=_at(0xa000000), wk=_at(0xb000000), wb=1 << 26)
+    size = _lib.lib().zk_linear_fp8_workspace_size(64, 4096, 14336, _lib.BF16)
+    assert size > 0 and _lib.lib().zk_linear_fp8_workspace_size(16, 4096, 14336, _lib.BF16) == 0
+    assert _lib.lib().zk_linear_fp8_workspace_size(0, 4096, 14336, _lib.BF16) == 0 and _lib.lib().zk_linear_fp8_workspace_size(64, 4096, 14330, _lib.BF16) == 0
+    for kw in (dict(wk=None), dict(wb=size - 1), dict(wk=_at(0xb000008)), dict(wk=_at(0x2000000)), dict(wk=_at(0xa000000)), dict(wk=_at(0x1000000 - 16))):
+        rc, msg = call(**dict(far, **kw))
+        assert rc == BAD and "zk_linear_fp8" in msg, kw
 
 
 def _plan(**kw):

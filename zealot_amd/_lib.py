@@ -167,7 +167,8 @@ SIGNATURES = {
     "zk_silu_mul_fp8": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P]),
     "zk_fp8_weight_bytes": (_SZ, [_I64, _I64]),
     "zk_fp8_weight": (_I, [_P, _I, _P, _P, _I64, _I64, _P]),
-    "zk_linear_fp8": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P]),
+    "zk_linear_fp8_workspace_size": (_SZ, [_I64, _I64, _I64, _I]),
+    "zk_linear_fp8": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P, _SZ, _P]),
     "zk_lora_max_tiles": (_I64, [_I64, _I64]),
     "zk_lora_plan": (_I, [_P, _I64, _I64, _P, _P, _P, _P]),
     "zk_lora_workspace_size": (_SZ, [_I64, _I64, _I64, _I, _I, _I]),

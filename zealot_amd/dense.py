@@ -343,6 +343,7 @@ class Fp8Rows(NamedTuple):
 
 
 _FP8 = torch.float8_e4m3fn
+_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
 def _fp8_out(out, like, rows: int, cols: int, cur: int, stream):
@@ -466,7 +467,11 @@ def fp8_weight(weight: torch.Tensor, scales: torch.Tensor | None = None, stream=
     return Fp8Weight(data, scales, n, k)
 
 
-def linear_fp8(x: Fp8Rows, weight: Fp8Weight, out=None, out_dtype=torch.bfloat16, stream=None):
+def linear_fp8_workspace_bytes(m: int, n: int, k: int, out_dtype=torch.bfloat16) -> int:
+    return int(_lib.lib().zk_linear_fp8_workspace_size(m, n, k, _CODES[out_dtype]))
+
+
+def linear_fp8(x: Fp8Rows, weight: Fp8Weight, out=None, out_dtype=torch.bfloat16, workspace=None, stream=None):
     """x . weight^T for rows and a weight in 8 bits (zk_linear_fp8): y [m, n],
     bfloat16 or float32 (`out_dtype`, or out's own).  k % 16 == 0."""
     m, k = _dims(x.data, "x.data", "[m, k]")
@@ -486,7 +491,16 @@ def linear_fp8(x: Fp8Rows, weight: Fp8Weight, out=None, out_dtype=torch.bfloat16
     else:
         py = _need(out, "out", (m, n), None, cur)
         _dt(out)
-    _lib.check(_lib.lib().zk_linear_fp8(px, ps, pw, pws, py, m, n, k, zk_dtype(out), at_stream))
+    lib, code = _lib.lib(), zk_dtype(out)
+    ws = (None, 0)
+    if workspace is not None:  # (its size is checked by the call)
+        ws = (_need(workspace, "workspace", workspace.shape, None, cur), workspace.numel() * workspace.element_size())
+    elif m > 16:
+        size = lib.zk_linear_fp8_workspace_size(m, n, k, code)
+        if size:
+            workspace = _empty(out, (size,), torch.uint8, stream)  # (held until the launch is made)
+            ws = (workspace.data_ptr(), size)
+    _lib.check(lib.zk_linear_fp8(px, ps, pw, pws, py, m, n, k, code, *ws, at_stream))
     return out
 
 
@@ -520,10 +534,7 @@ def lora_plan(adapter_ids, num_adapters: int, out: LoraPlan | None = None, strea
 
 
 def lora_workspace_bytes(num_rows: int, num_adapters: int, k: int, rank: int, num_parts: int, dtype) -> int:
-    return int(_lib.lib().zk_lora_workspace_size(num_rows, num_adapters, k, rank, num_parts, _LORA_CODES[dtype]))
-
-
-_LORA_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+    return int(_lib.lib().zk_lora_workspace_size(num_rows, num_adapters, k, rank, num_parts, _CODES[dtype]))
 
 
 def lora(x, a, b, scales, plan: LoraPlan, y, parts=None, part_block: int = 0, workspace=None, stream=None):
@@ -561,7 +572,8 @@ def lora(x, a, b, scales, plan: LoraPlan, y, parts=None, part_block: int = 0, wo
     tiles = lib.zk_lora_max_tiles(t, na)
     size = lib.zk_lora_workspace_size(t, na, k, rank, p, code)
     if workspace is None:
-        ws = (_empty(y, (size,), torch.uint8, stream).data_ptr() if size else None, size)
+        workspace = _empty(y, (size,), torch.uint8, stream)  # (held until the launches are made)
+        ws = (workspace.data_ptr() if size else None, size)
     else:
         ws = (_need(workspace, "workspace", workspace.shape, None, cur), workspace.numel() * workspace.element_size())
     _lib.check(lib.zk_lora(
