@@ -250,9 +250,9 @@ int zk_lora_plan(const int32_t *adapter_ids, int64_t num_rows, int64_t num_adapt
  * no operand. */
 size_t zk_lora_workspace_size(int64_t num_rows, int64_t num_adapters, int64_t k, int rank, int num_parts, zk_dtype dtype);
 int zk_lora(const void *x, const float *x_scales, int64_t x_stride, zk_dtype x_dtype, const void *a_weights,
-            const void *b_weights, const float *scales, zk_dtype dtype, const int32_t *order, const int32_t *offsets,
-            const int32_t *tiles, int64_t num_rows, int64_t num_adapters, int64_t k, int64_t n, int rank, int num_parts,
-            const int64_t *part_cols, int part_block, void *y, int64_t y_stride, void *workspace, size_t workspace_bytes,
+            const void *b_weights, const float *scales, zk_dtype dtype, const int32_t *order, const int32_t *tiles,
+            int64_t num_rows, int64_t num_adapters, int64_t k, int64_t n, int rank, int num_parts, const int64_t *part_cols,
+            int part_block, void *y, int64_t y_stride, void *workspace, size_t workspace_bytes,
             void *stream);
 
 /* On (default): the first call of each (m, n, k, dtypes) times hipBLASLt's

@@ -45,8 +45,8 @@ def _check_plan(ids, adapters, plan):
     counts = np.bincount(ids[valid], minlength=adapters)
     offsets = np.concatenate([[0], counts.cumsum()])
     assert np.array_equal(plan.offsets.cpu().numpy(), offsets)
-    tr = 16 if len(ids) <= 1024 else 64
-    tiles = [(a, p) for a in range(adapters) for p in range(offsets[a], offsets[a + 1], tr)]
+    tr = 16 if len(ids) <= 1024 else 32
+    tiles = [(a | min(tr, offsets[a + 1] - p) << 16, p) for a in range(adapters) for p in range(offsets[a], offsets[a + 1], tr)]
     got = plan.tiles.cpu().numpy()
     assert len(tiles) <= len(got)
     assert got[:len(tiles)].tolist() == [list(t) for t in tiles] and (got[len(tiles):] == [-1, 0]).all()

@@ -104,7 +104,7 @@ def test_lora_plan():
 
 def _lora(**kw):
     a = dict(x=_at(0), xsc=None, xst=0, xd=_lib.BF16, a=_at(0x1000000), b=_at(0x2000000), sc=_at(0x3000000), dt=_lib.BF16, order=_at(0x3100000),
-             off=_at(0x3200000), tiles=_at(0x3300000), n=50, na=4, k=256, cols=192, rank=16, parts=1, pc=None, pb=0, y=_at(0x4000000), ys=0,
+             tiles=_at(0x3300000), n=50, na=4, k=256, cols=192, rank=16, parts=1, pc=None, pb=0, y=_at(0x4000000), ys=0,
              ws=_at(0x5000000), wb=1 << 24)
     a.update(kw)
     return _rc(_lib.lib().zk_lora(*a.values(), None))
@@ -115,13 +115,13 @@ def test_lora():
                dict(xsc=_at(0x3400000)), dict(n=-1), dict(n=(1 << 24) + 1), dict(na=0), dict(na=2049), dict(k=0), dict(cols=0), dict(rank=0), dict(rank=257),
                dict(parts=0), dict(parts=5), dict(parts=3, rank=171, pc=(I64 * 3)(64, 64, 64)), dict(parts=2), dict(parts=2, pc=(I64 * 2)(100, 93)),
                dict(parts=2, pc=(I64 * 2)(192, 0)), dict(parts=2, pc=(I64 * 2)(-10, 202)), dict(parts=2, pc=(I64 * 2)(1 << 40, 1 << 40)), dict(pb=-1),
-               dict(parts=2, pb=64), dict(xst=255), dict(ys=100), dict(x=None), dict(a=None), dict(b=None), dict(order=None), dict(off=None),
+               dict(parts=2, pb=64), dict(xst=255), dict(ys=100), dict(x=None), dict(a=None), dict(b=None), dict(order=None),
                dict(tiles=None), dict(y=None), dict(ws=None), dict(wb=100), dict(ws=_at(0x5000008)), dict(tiles=_at(0x3300004)), dict(cols=1 << 24),
                dict(k=1 << 24)):
         rc, msg = _lora(**kw)
         assert rc == BAD and "zk_lora" in msg, kw
     for kw in (dict(y=_at(0x100)), dict(y=_at(0x1000000)), dict(y=_at(0x2000000)), dict(y=_at(0x3000000)), dict(y=_at(0x3100000)), dict(ws=_at(0)),
-               dict(ws=_at(0x2000000)), dict(ws=_at(0x4000000)), dict(ws=_at(0x3200000))):
+               dict(ws=_at(0x2000000)), dict(ws=_at(0x4000000)), dict(ws=_at(0x3300000))):
         rc, msg = _lora(**kw)
         assert rc == BAD and "overlaps" in msg, kw
     assert _lora(n=0, x=None, y=None, ws=None)[0] == OK

@@ -172,7 +172,7 @@ SIGNATURES = {
     "zk_lora_max_tiles": (_I64, [_I64, _I64]),
     "zk_lora_plan": (_I, [_P, _I64, _I64, _P, _P, _P, _P]),
     "zk_lora_workspace_size": (_SZ, [_I64, _I64, _I64, _I, _I, _I]),
-    "zk_lora": (_I, [_P, _P, _I64, _I, _P, _P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _P, _I, _P, _I64, _P, _SZ,
+    "zk_lora": (_I, [_P, _P, _I64, _I, _P, _P, _P, _I, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _P, _I, _P, _I64, _P, _SZ,
                      _P]),
     "zk_sched_create": (_I, [ctypes.POINTER(SchedConfigC), _P, ctypes.POINTER(_P)]),
     "zk_sched_destroy": (None, [_P]),

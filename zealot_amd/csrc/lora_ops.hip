@@ -6,16 +6,16 @@
 // A step's plan groups its rows by adapter, once for all layers' projections:
 //   order    the rows, sorted by adapter, in order within one; then -1
 //   offsets  where each adapter's rows begin in it
-//   tiles    (adapter, first position) of runs of at most tile_rows rows of one
-//            adapter; (-1, 0) behind the last
+//   tiles    (adapter + 2^16 rows, first position) of runs of at most tile_rows
+//            rows of one adapter; (-1, 0) behind the last
 // A product is two launches over the tiles.  The shrink forms
-// v[p] = c_a A_a x[order[p]] (f32, R = parts * rank values a row) with A as the
-// first operand of the matrix instruction and the tile's rows as the second, k
-// split over the waves of a workgroup and, where there are few tiles, over
-// workgroups, whose sums the second launch adds in their order.  The expand
-// takes 64 columns of y a wave: B's rows as the first operand, v as the
-// second, so that a lane ends with 16 consecutive columns of a row and adds them
-// in place.
+// v[p] = c_a A_a x[order[p]] (f32, parts * rank values a row) with A as the first
+// operand of the matrix instruction and the tile's rows as the second, k split
+// over the waves of a workgroup and, where there are few tiles, over workgroups,
+// whose sums the second launch adds in their order.  The expand takes 64 columns
+// of y a wave: B's rows as the first operand, v as the second, straight from
+// memory into registers; a lane ends with two runs of eight columns of a row and
+// adds them in place.
 // Columns of y may come in parts that have an A of their own each (query, key
 // and value columns of a fused projection): part p meets v[p rank ..] alone.
 //
@@ -38,9 +38,9 @@ constexpr int kMaxParts = 4;
 constexpr int kMaxRank = 256, kMaxRanks = 512;  // of one part, of all
 
 // Rows of a tile: 16 (one matrix instruction) for a decode step, where most
-// tiles have few rows; 64 for prompts, whose rows of one adapter are many: A and
-// B are then read once per 64 rows.
-int tile_rows_for(int64_t rows) { return rows <= 1024 ? 16 : 64; }
+// tiles have few rows; 32 for prompts, whose rows of one adapter are many: A and
+// B are read once per 32 rows, and 8192 rows are a workgroup a CU.
+int tile_rows_for(int64_t rows) { return rows <= 1024 ? 16 : 32; }
 int64_t max_tiles(int64_t rows, int64_t adapters) {
     return rows / tile_rows_for(rows) + std::min(rows, adapters);
 }
@@ -60,7 +60,7 @@ struct PlanArgs {
 // scheduling.
 __global__ void __launch_bounds__(1024) lora_plan_kernel(PlanArgs a) {
     __shared__ int at[16 * kMaxAdapters];
-    __shared__ int first[kMaxAdapters], tile0[kMaxAdapters];
+    __shared__ int first[kMaxAdapters], tile0[kMaxAdapters], count[kMaxAdapters];
     __shared__ int scan_rows[16], scan_tiles[16];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, A = a.adapters;
     const int stretch = ((a.rows + 1023) / 1024) * 64;
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(PlanArgs a) {
             at[w * A + x] = n;
             n += c;
         }
-        first[x] = n;  // (for now its rows)
+        count[x] = n;
         mine += n;
         my_tiles += (n + a.tile_rows - 1) / a.tile_rows;
     }
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(PlanArgs a) {
     int pos = block_exclusive_scan_1024(mine, scan_rows, &total);
     int tile = block_exclusive_scan_1024(my_tiles, scan_tiles, &tiles);
     for (int x = a0; x < a1; ++x) {
-        const int n = first[x];
+        const int n = count[x];
         a.offsets[x] = pos;
         first[x] = pos;
         tile0[x] = tile;
@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(PlanArgs a) {
         if (same) {
             const int p = base + __popcll(same & ((1ull << lane) - 1)), j = p - first[id];
             a.order[p] = r + lane;
-            if (j % a.tile_rows == 0) a.tiles[tile0[id] + j / a.tile_rows] = make_int2(id, p);
+            if (j % a.tile_rows == 0)
+                a.tiles[tile0[id] + j / a.tile_rows] = make_int2(id | min(a.tile_rows, count[id] - j) << 16, p);
         }
     }
 }
@@ -134,12 +135,12 @@ struct LoraArgs {
     int64_t x_stride;
     const void *a, *b;
     const float *scales;  // [adapters] or null
-    const int32_t *order, *offsets;
+    const int32_t *order;
     const int2 *tiles;
-    float *v;  // [splits][rows][ranks16]
+    float *v;  // [splits][rows][v_stride]: part p from p * part_stride on
     void *y;
     int64_t y_stride;
-    int rows, adapters, k, n, rank, parts, ranks, ranks16, splits;
+    int rows, adapters, k, n, rank, parts, part_stride, v_stride, splits, blocks;  // blocks: of 64 columns a wave
     int part_end[kMaxParts], part_block;
 };
 
@@ -204,40 +205,43 @@ __device__ __forceinline__ u32x4 take(const uint8_t *row, int c, int cols) {
 // Rows of tile `i`: its adapter, first position and count (0: none).
 __device__ __forceinline__ int tile_at(const LoraArgs &a, int i, int rows, int &adapter, int &p0) {
     const int2 t = a.tiles[i];
-    adapter = t.x;
+    adapter = t.x & 0xffff;
     p0 = t.y;
-    if ((unsigned)adapter >= (unsigned)a.adapters || (unsigned)p0 >= (unsigned)a.rows) return 0;
-    return max(0, min(rows, min(a.offsets[adapter + 1], a.rows) - p0));
+    if (t.x < 0 || adapter >= a.adapters || (unsigned)p0 >= (unsigned)a.rows) return 0;
+    return min(min(t.x >> 16, rows), a.rows - p0);
 }
 
-// v of a tile: MT groups of 16 rows by RT groups of 16 ranks, four waves that
-// take every fourth step of four matrix instructions of the workgroup's k.
-template <typename X, typename T, int MT, int RT, bool WHOLE>
-__global__ void __launch_bounds__(256) lora_shrink_kernel(LoraArgs a) {
+// v of a tile: MT groups of 16 rows by RT groups of 16 ranks, each wave of the
+// workgroup every W-th step of four matrix instructions of its stretch of k.
+template <typename X, typename T, int MT, int RT, int W, bool WHOLE>
+__global__ void __launch_bounds__(64 * W) lora_shrink_kernel(LoraArgs a) {
     constexpr int E = Operand<T>::E, U = 4, kStep = 4 * E * U;
-    __shared__ f32x4 sums[4][RT * MT][64];
+    __shared__ f32x4 sums[W][RT * MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     int adapter, p0;
     const int count = tile_at(a, blockIdx.x, 16 * MT, adapter, p0);
     if (count == 0) return;
-    const int rt0 = blockIdx.y * RT, split = blockIdx.z;
+    const int i0 = blockIdx.y * RT * 16, split = blockIdx.z;
     const X *xr[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const int row = a.order[p0 + min(16 * m + r16, count - 1)];
         xr[m] = (const X *)a.x + (size_t)min((unsigned)row, (unsigned)a.rows - 1) * a.x_stride;
     }
+    // row i of v's values: rank i % part_stride of part i / part_stride (what is behind a part's ranks is not kept)
     const T *ar[RT];
 #pragma unroll
-    for (int f = 0; f < RT; ++f)
-        ar[f] = (const T *)a.a + ((size_t)adapter * a.ranks + min((rt0 + f) * 16 + r16, a.ranks - 1)) * a.k;
+    for (int f = 0; f < RT; ++f) {
+        const int i = min(i0 + 16 * f + r16, a.parts * a.part_stride - 1), part = i / a.part_stride;
+        ar[f] = (const T *)a.a + ((size_t)adapter * a.parts * a.rank + part * a.rank + min(i - part * a.part_stride, a.rank - 1)) * a.k;
+    }
     f32x4 acc[RT][MT];
 #pragma unroll
     for (int f = 0; f < RT; ++f)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int c = (split * 4 + wave) * kStep; c < a.k; c += a.splits * 4 * kStep) {
+    for (int c = (split * W + wave) * kStep; c < a.k; c += a.splits * W * kStep) {
         u32x4 av[U][RT], xv[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -260,16 +264,16 @@ __global__ void __launch_bounds__(256) lora_shrink_kernel(LoraArgs a) {
         for (int m = 0; m < MT; ++m) sums[wave][f * MT + m][lane] = acc[f][m];
     __syncthreads();
     const float scale = a.scales ? a.scales[adapter] : 1.0f;
-    for (int j = wave; j < RT * MT; j += 4) {
-        const int f = j / MT, i = 16 * (j % MT) + r16, rk = (rt0 + f) * 16 + 4 * g;
-        if (i >= count || rk >= a.ranks16) continue;
+    for (int j = wave; j < RT * MT; j += W) {
+        const int f = j / MT, row = 16 * (j % MT) + r16, i = i0 + 16 * f + 4 * g;
+        if (row >= count || i >= a.v_stride) continue;
         f32x4 v = sums[0][j][lane];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) v += sums[w][j][lane];
+        for (int w = 1; w < W; ++w) v += sums[w][j][lane];
         float s = scale;
-        if (sizeof(X) == 1) s *= a.x_scales[min((unsigned)a.order[p0 + i], (unsigned)a.rows - 1)];
+        if (sizeof(X) == 1) s *= a.x_scales[min((unsigned)a.order[p0 + row], (unsigned)a.rows - 1)];
         v *= s;
-        *reinterpret_cast<f32x4 *>(a.v + ((size_t)split * a.rows + p0 + i) * a.ranks16 + rk) = v;
+        *reinterpret_cast<f32x4 *>(a.v + ((size_t)split * a.rows + p0 + row) * a.v_stride + i) = v;
     }
 }
 
@@ -281,133 +285,180 @@ __device__ __forceinline__ int part_of(const LoraArgs &a, int col) {
     return p;
 }
 
-// y of a tile and 256 columns.  v comes to LDS first, a part's ranks padded with
-// zeros to whole steps: f32 as it is; for bf16 each value as two, which together
-// hold 16 bits of it, so the sum keeps what f32 v has over one rounding to 8.
+// two values as bf16, to nearest even (one instruction)
+__device__ __forceinline__ uint32_t two(float lo, float hi) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2_t));
+}
+
+// E values of v's row from rank r on, as operands: f32 as they are; for bf16 each
+// as two, which together hold 16 bits of it, so that the sum keeps what f32 v has
+// over one rounding to 8.
+template <typename T> struct Values;
+template <> struct Values<float> {
+    static constexpr int H = 1;
+    static __device__ __forceinline__ void split(const float (&v)[4], u32x4 (&o)[1]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[0][i] = __float_as_uint(v[i]);
+    }
+};
+template <> struct Values<uint16_t> {
+    static constexpr int H = 2;
+    static __device__ __forceinline__ void split(const float (&v)[8], u32x4 (&o)[2]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = two(v[2 * i], v[2 * i + 1]);
+            o[0][i] = w;
+            // (nothing is left of a value that has no finite first half)
+            const float a = bf16lo(w), b = bf16hi(w);
+            o[1][i] = two((w & 0x7f80u) == 0x7f80u ? 0.0f : v[2 * i] - a, (w & 0x7f800000u) == 0x7f800000u ? 0.0f : v[2 * i + 1] - b);
+        }
+    }
+};
+
+// y of a tile and a wave's blocks of 64 columns.
 template <typename T, int MT, bool WHOLE>
 __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
-    constexpr int E = Operand<T>::E, kStep = 4 * E, H = sizeof(T) == 2 ? 2 : 1;  // H: halves of a value
-    extern __shared__ u32x4 lds[];
+    constexpr int E = Operand<T>::E, kStep = 4 * E, H = Values<T>::H;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     int adapter, p0;
     const int count = tile_at(a, blockIdx.x, 16 * MT, adapter, p0);
     if (count == 0) return;
-    const int steps = (a.rank + kStep - 1) / kStep, rp = steps * kStep;
-    const int line = rp / E + 1;  // 16-byte units of a row of a part; one spare against bank conflicts
-    const int plane = a.parts * 16 * MT * line;
-    T *lt = reinterpret_cast<T *>(lds);
-    for (int i = threadIdx.x; i < a.parts * 16 * MT * rp; i += 256) {
-        const int r = i % rp, row = i / rp % (16 * MT), part = i / rp / (16 * MT);
-        float v = 0.0f;
-        if (r < a.rank && row < count) {
-            const float *src = a.v + (size_t)(p0 + row) * a.ranks16 + part * a.rank + r;
-            for (int s = 0; s < a.splits; ++s) v += src[(size_t)s * a.rows * a.ranks16];
-        }
-        const size_t to = (size_t)(part * 16 * MT + row) * line * E + r;
-        if constexpr (H == 2) {
-            const uint32_t hi = f32_to_bf16_bits(v), top = hi << 16;
-            // (nothing is left of a value that has no finite first half)
-            const float rest = (top & 0x7f800000u) == 0x7f800000u ? 0.0f : v - __uint_as_float(top);
-            lt[to] = (T)hi;
-            lt[(size_t)plane * E + to] = (T)f32_to_bf16_bits(rest);
-        } else {
-            lt[to] = v;
-        }
-    }
-    __syncthreads();
-    const int n0 = blockIdx.y * 256 + wave * 64;
-    if (n0 >= a.n) return;
-    // row r16 of B tile t: column n0 + 16 (r16 / 4) + 4 t + r16 % 4
-    const int c0 = n0 + 16 * (r16 >> 2) + (r16 & 3);
-    const T *bb = (const T *)a.b + (size_t)adapter * a.n * a.rank;
-    // the product of these columns with part p's values
-    auto product = [&](int p, f32x4 (&acc)[4][MT]) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) acc[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < steps; ++s) {
-            u32x4 bv[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                bv[t] = take<WHOLE>(bb + (size_t)min(c0 + 4 * t, a.n - 1) * a.rank, s * kStep + E * g, a.rank);
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    const u32x4 vv = lds[h * plane + (p * 16 * MT + 16 * m + r16) * line + s * 4 + g];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) acc[t][m] = Operand<T>::mfma(bv[t], vv, acc[t][m]);
-                }
-        }
-    };
-    f32x4 acc[4][MT];
-    const int last = min(n0 + 63, a.n - 1), part = part_of(a, n0);
-    if (a.parts == 1 || (part_of(a, last) == part && (!a.part_block || a.part_block >= 64))) {
-        product(part, acc);
-    } else {  // columns of several parts: each takes its own part's product
-        f32x4 one[4][MT];
-        for (int p = 0; p < a.parts; ++p) {
-            product(p, one);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool mine = part_of(a, min(n0 + 16 * g + 4 * t + e, a.n - 1)) == p;
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) acc[t][m][e] = mine || p == 0 ? one[t][m][e] : acc[t][m][e];
-                }
-        }
-    }
-    // lane: columns n0 + 16 g .. + 15 of row r16 of each group
-    const int n1 = n0 + 16 * g;
-    if (n1 >= a.n) return;
+    const int steps = (a.rank + kStep - 1) / kStep;
+    const int first = (blockIdx.y * 4 + wave) * a.blocks * 64, end = min(first + a.blocks * 64, a.n);
+    if (first >= end) return;
+    // rows of y (from a.rows on: none), rows of v
+    unsigned row[MT];
+    const float *vr[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const int i = 16 * m + r16;
-        if (i >= count) continue;
-        const unsigned row = (unsigned)a.order[p0 + i];
-        if (row >= (unsigned)a.rows) continue;
-        T *y = (T *)a.y + (size_t)row * a.y_stride + n1;
-        if (n1 + 16 <= a.n && (((uintptr_t)y) & 15u) == 0) {
-            u32x4 *yw = reinterpret_cast<u32x4 *>(y);
-            u32x4 w[16 / E];
+        row[m] = i < count ? (unsigned)a.order[p0 + i] : ~0u;
+        vr[m] = a.v + (size_t)(p0 + min(i, count - 1)) * a.v_stride;
+    }
+    auto values = [&](int part, int s, u32x4 (&o)[MT][H]) {
+        const int r = s * kStep + E * g;
 #pragma unroll
-            for (int j = 0; j < 16 / E; ++j) w[j] = yw[j];
+        for (int m = 0; m < MT; ++m) {
+            float v[E];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float d = acc[j / 4][m][j % 4];
-                if constexpr (H == 2) {
-                    const uint32_t o = w[j / 8][j % 8 / 2];
-                    if (j % 2 == 0) w[j / 8][j % 8 / 2] = (o & 0xffff0000u) | f32_to_bf16_bits(bf16lo(o) + d);
-                    else w[j / 8][j % 8 / 2] = (o & 0xffffu) | f32_to_bf16_bits(bf16hi(o) + d) << 16;
+            for (int i = 0; i < E; ++i) v[i] = 0.0f;
+            if (r < a.rank) {
+                const float *src = vr[m] + part * a.part_stride + r;
+                for (int q = 0; q < a.splits; ++q, src += (size_t)a.rows * a.v_stride)
+#pragma unroll
+                    for (int i = 0; i < E; i += 4)
+                        if (WHOLE || r + i < a.rank) {
+                            const f32x4 w = *reinterpret_cast<const f32x4 *>(src + i);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[i + e] += w[e];
+                        }
+                if (!WHOLE)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) v[i] = r + i < a.rank ? v[i] : 0.0f;
+            }
+            Values<T>::split(v, o[m]);
+        }
+    };
+    u32x4 kept[MT][H];  // of one step's ranks, over the blocks of a part
+    int kept_part = -1;
+    for (int n0 = first; n0 < end; n0 += 64) {
+        // row r16 of B tile t: column n0 + 32 (t / 2) + 8 (r16 / 4) + 4 (t % 2) + r16 % 4
+        const T *bb[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            bb[t] = (const T *)a.b + ((size_t)adapter * a.n + min(n0 + 32 * (t >> 1) + 8 * (r16 >> 2) + 4 * (t & 1) + (r16 & 3), a.n - 1)) * a.rank;
+        // the product of these columns with part p's values
+        auto product = [&](int p, f32x4 (&acc)[4][MT]) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < steps; ++s) {
+                u32x4 bv[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) bv[t] = take<WHOLE>(bb[t], s * kStep + E * g, a.rank);
+                if (steps > 1 || kept_part != p) {
+                    values(p, s, kept);
+                    kept_part = p;
+                }
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) acc[t][m] = Operand<T>::mfma(bv[t], kept[m][h], acc[t][m]);
+            }
+        };
+        f32x4 acc[4][MT];
+        const int last = min(n0 + 63, a.n - 1), part = part_of(a, n0);
+        if (a.parts == 1 || (part_of(a, last) == part && (!a.part_block || a.part_block >= 64))) {
+            product(part, acc);
+        } else {  // columns of several parts: each takes its own part's product
+            f32x4 one[4][MT];
+            for (int p = 0; p < a.parts; ++p) {
+                product(p, one);
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool mine = part_of(a, min(n0 + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + e, a.n - 1)) == p;
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) acc[t][m][e] = mine || p == 0 ? one[t][m][e] : acc[t][m][e];
+                    }
+            }
+        }
+        // lane: columns n0 + 32 q + 8 g .. + 7 of row r16 of each group
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (row[m] >= (unsigned)a.rows) continue;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int n1 = n0 + 32 * q + 8 * g;
+                T *y = (T *)a.y + (size_t)row[m] * a.y_stride + n1;
+                float d[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] = acc[2 * q + i / 4][m][i % 4];
+                if (n1 + 8 <= a.n && (((uintptr_t)y) & 15u) == 0) {
+                    u32x4 *yw = reinterpret_cast<u32x4 *>(y);
+                    if constexpr (H == 2) {
+                        u32x4 w = *yw;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = two(bf16lo(w[i]) + d[2 * i], bf16hi(w[i]) + d[2 * i + 1]);
+                        *yw = w;
+                    } else {
+                        u32x4 w[2] = {yw[0], yw[1]};
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = __float_as_uint(__uint_as_float(w[i / 4][i % 4]) + d[i]);
+                        yw[0] = w[0];
+                        yw[1] = w[1];
+                    }
                 } else {
-                    w[j / 4][j % 4] = __float_as_uint(__uint_as_float(w[j / 4][j % 4]) + d);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (n1 + i < a.n) {
+                            if constexpr (H == 2) y[i] = (T)two(__uint_as_float((uint32_t)y[i] << 16) + d[i], 0.0f);
+                            else y[i] += d[i];
+                        }
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 16 / E; ++j) yw[j] = w[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (n1 + j < a.n) {
-                    const float d = acc[j / 4][m][j % 4];
-                    if constexpr (H == 2) y[j] = (T)f32_to_bf16_bits(__uint_as_float((uint32_t)y[j] << 16) + d);
-                    else y[j] += d;
-                }
         }
     }
 }
 
-// Workgroups of k of one tile and rank group: enough of them for two a CU, a
-// wave at least two steps.
-int splits_for(int64_t rows, int64_t adapters, int groups, int64_t k, int step) {
-    const int64_t tiles = std::max<int64_t>(1, max_tiles(rows, adapters)) * groups;
-    const int64_t most = std::max<int64_t>(1, k / (8 * step)), want = std::max<int64_t>(1, 512 / tiles);
+int part_stride_of(int rank) { return (rank + 3) / 4 * 4; }
+int v_stride_of(int rank, int parts) { return (part_stride_of(rank) * parts + 15) / 16 * 16; }
+int rank_groups(int v_stride) { return v_stride <= 64 ? v_stride / 16 : 4; }  // of 16, a workgroup
+// Workgroups of k of one tile and rank group: enough of them for two a CU (prompts:
+// one, of twice the waves), a wave at least one step.
+int splits_of(int64_t rows, int64_t adapters, int64_t k, int rank, int parts, zk_dtype dtype) {
+    const int vs = v_stride_of(rank, parts), rt = rank_groups(vs), waves = tile_rows_for(rows) == 16 ? 4 : 8;
+    const int64_t tiles = std::max<int64_t>(1, max_tiles(rows, adapters)) * ((vs / 16 + rt - 1) / rt);
+    const int64_t most = std::max<int64_t>(1, k / (waves * (dtype == ZK_F32 ? 64 : 128)));
+    const int64_t want = ((waves == 4 ? 512 : 256) + tiles - 1) / tiles;
     return (int)std::min<int64_t>({most, want, 16});
 }
-int rank_groups(int ranks) { return ranks <= 16 ? 1 : ranks <= 32 ? 2 : 4; }  // 16-rank tiles a workgroup
 
 bool meet(const void *p, int64_t pb, const void *q, int64_t qb) {
     const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
@@ -420,33 +471,27 @@ bool shape_ok(int64_t rows, int64_t adapters, int64_t k, int rank, int parts) {
     return rows >= 0 && rows <= (1 << 24) && adapters >= 1 && adapters <= kMaxAdapters && k >= 1 && k <= (1 << 23) && rank >= 1 &&
            rank <= kMaxRank && parts >= 1 && parts <= kMaxParts && rank * parts <= kMaxRanks;
 }
-int step_of(zk_dtype dtype) { return dtype == ZK_F32 ? 64 : 128; }
-int splits_of(int64_t rows, int64_t adapters, int64_t k, int rank, int parts, zk_dtype dtype) {
-    const int rt = rank_groups(rank * parts), groups = ((rank * parts + 15) / 16 + rt - 1) / rt;
-    return splits_for(rows, adapters, groups, k, step_of(dtype));
-}
 
 template <typename X, typename T, int MT>
 void shrink(const LoraArgs &a, int tiles, bool whole, hipStream_t s) {
-    const int rt = rank_groups(a.ranks), groups = ((a.ranks + 15) / 16 + rt - 1) / rt;
+    constexpr int W = MT == 1 ? 4 : 8;
+    const int rt = rank_groups(a.v_stride), groups = (a.v_stride / 16 + rt - 1) / rt;
     const dim3 grid((unsigned)tiles, (unsigned)groups, (unsigned)a.splits);
-    auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(a); };
-    if (rt == 1) whole ? go(lora_shrink_kernel<X, T, MT, 1, true>) : go(lora_shrink_kernel<X, T, MT, 1, false>);
-    else if (rt == 2) whole ? go(lora_shrink_kernel<X, T, MT, 2, true>) : go(lora_shrink_kernel<X, T, MT, 2, false>);
-    else whole ? go(lora_shrink_kernel<X, T, MT, 4, true>) : go(lora_shrink_kernel<X, T, MT, 4, false>);
+    auto go = [&](auto kernel) { kernel<<<grid, 64 * W, 0, s>>>(a); };
+    if (rt == 1) whole ? go(lora_shrink_kernel<X, T, MT, 1, W, true>) : go(lora_shrink_kernel<X, T, MT, 1, W, false>);
+    else if (rt == 2) whole ? go(lora_shrink_kernel<X, T, MT, 2, W, true>) : go(lora_shrink_kernel<X, T, MT, 2, W, false>);
+    else if (rt == 3) whole ? go(lora_shrink_kernel<X, T, MT, 3, W, true>) : go(lora_shrink_kernel<X, T, MT, 3, W, false>);
+    else whole ? go(lora_shrink_kernel<X, T, MT, 4, W, true>) : go(lora_shrink_kernel<X, T, MT, 4, W, false>);
 }
 
 template <typename T, int MT>
-void expand(const LoraArgs &a, int tiles, hipStream_t s) {
-    constexpr int E = Operand<T>::E;
-    const int rp = (a.rank + 4 * E - 1) / (4 * E) * 4 * E;
-    const size_t bytes = (size_t)(sizeof(T) == 2 ? 2 : 1) * a.parts * 16 * MT * (rp / E + 1) * 16;
-    const bool whole = a.rank % E == 0 && aligned(a.b, 16);
-    const dim3 grid((unsigned)tiles, (unsigned)((a.n + 255) / 256));
-    auto go = [&](auto kernel) {
-        if (bytes > 65536) (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        kernel<<<grid, 256, bytes, s>>>(a);
-    };
+void expand(LoraArgs a, int tiles, hipStream_t s) {
+    const bool whole = a.rank % Operand<T>::E == 0 && aligned(a.b, 16);
+    // blocks of 64 columns a wave: v and its halves are formed once for them, as long as 4096 waves are left
+    const int all = (a.n + 63) / 64;
+    a.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(8, (int64_t)tiles * all / 4096));
+    const dim3 grid((unsigned)tiles, (unsigned)((all + 4 * a.blocks - 1) / (4 * a.blocks)));
+    auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(a); };
     whole ? go(lora_expand_kernel<T, MT, true>) : go(lora_expand_kernel<T, MT, false>);
 }
 
@@ -458,8 +503,8 @@ void both(const LoraArgs &a, int tiles, hipStream_t s) {
         shrink<X, T, 1>(a, tiles, whole, s);
         expand<T, 1>(a, tiles, s);
     } else {
-        shrink<X, T, 4>(a, tiles, whole, s);
-        expand<T, 4>(a, tiles, s);
+        shrink<X, T, 2>(a, tiles, whole, s);
+        expand<T, 2>(a, tiles, s);
     }
 }
 
@@ -506,11 +551,11 @@ int zk_lora_plan(const int32_t *adapter_ids, int64_t num_rows, int64_t num_adapt
 
 size_t zk_lora_workspace_size(int64_t num_rows, int64_t num_adapters, int64_t k, int rank, int num_parts, zk_dtype dtype) {
     if (!shape_ok(num_rows, num_adapters, k, rank, num_parts) || num_rows == 0) return 0;
-    return (size_t)splits_of(num_rows, num_adapters, k, rank, num_parts, dtype) * num_rows * ((rank * num_parts + 15) / 16 * 16) * 4;
+    return (size_t)splits_of(num_rows, num_adapters, k, rank, num_parts, dtype) * num_rows * v_stride_of(rank, num_parts) * 4;
 }
 
 int zk_lora(const void *x, const float *x_scales, int64_t x_stride, zk_dtype x_dtype, const void *a_weights,
-            const void *b_weights, const float *scales, zk_dtype dtype, const int32_t *order, const int32_t *offsets,
+            const void *b_weights, const float *scales, zk_dtype dtype, const int32_t *order,
             const int32_t *tiles, int64_t num_rows, int64_t num_adapters, int64_t k, int64_t n, int rank, int num_parts,
             const int64_t *part_cols, int part_block, void *y, int64_t y_stride, void *workspace, size_t workspace_bytes,
             void *stream) {
@@ -537,7 +582,7 @@ int zk_lora(const void *x, const float *x_scales, int64_t x_stride, zk_dtype x_d
         if (end != n) return bad("zk_lora: parts must hold the columns of y");
     }
     if (num_rows == 0) return ZK_OK;
-    if (!x || !a_weights || !b_weights || !order || !offsets || !tiles || !y) return bad("zk_lora: NULL pointer");
+    if (!x || !a_weights || !b_weights || !order || !tiles || !y) return bad("zk_lora: NULL pointer");
     const size_t need = zk_lora_workspace_size(num_rows, num_adapters, k, rank, num_parts, dtype);
     if (!workspace || workspace_bytes < need) return bad("zk_lora: workspace too small (zk_lora_workspace_size)");
     if (!aligned(workspace, 16) || !aligned(tiles, 8)) return bad("zk_lora: the workspace must be 16-byte, tiles 8-byte aligned");
@@ -548,7 +593,7 @@ int zk_lora(const void *x, const float *x_scales, int64_t x_stride, zk_dtype x_d
         const void *p;
         int64_t bytes;
     } in[] = {{x, xb}, {x_scales, 4 * num_rows}, {a_weights, num_adapters * ranks * k * e}, {b_weights, num_adapters * n * rank * e},
-              {scales, 4 * num_adapters}, {order, 4 * num_rows}, {offsets, 4 * (num_adapters + 1)}, {tiles, 8 * nt}};
+              {scales, 4 * num_adapters}, {order, 4 * num_rows}, {tiles, 8 * nt}};
     for (const auto &i : in)
         if (meet(i.p, i.bytes, y, yb) || meet(i.p, i.bytes, workspace, (int64_t)need)) return bad("zk_lora: y or the workspace overlaps an input");
     if (meet(y, yb, workspace, (int64_t)need)) return bad("zk_lora: y overlaps the workspace");
@@ -559,7 +604,6 @@ int zk_lora(const void *x, const float *x_scales, int64_t x_stride, zk_dtype x_d
     a.b = b_weights;
     a.scales = scales;
     a.order = order;
-    a.offsets = offsets;
     a.tiles = (const int2 *)tiles;
     a.v = (float *)workspace;
     a.y = y;
@@ -570,8 +614,8 @@ int zk_lora(const void *x, const float *x_scales, int64_t x_stride, zk_dtype x_d
     a.n = (int)n;
     a.rank = rank;
     a.parts = num_parts;
-    a.ranks = ranks;
-    a.ranks16 = (ranks + 15) / 16 * 16;
+    a.part_stride = part_stride_of(rank);
+    a.v_stride = v_stride_of(rank, num_parts);
     a.splits = splits_of(num_rows, num_adapters, k, rank, num_parts, dtype);
     a.part_block = part_block;
     hipStream_t s = (hipStream_t)stream;

@@ -579,7 +579,7 @@ def lora(x, a, b, scales, plan: LoraPlan, y, parts=None, part_block: int = 0, wo
     _lib.check(lib.zk_lora(
         rows.data_ptr(), sc, xs, xc, _need(a, "a", (na, p * rank, k), dt, cur), _need(b, "b", (na, n, rank), dt, cur),
         _need_opt(scales, "scales", (na,), torch.float32, cur), code, _need(plan.order, "plan.order", (t,), i32, cur),
-        _need(plan.offsets, "plan.offsets", (na + 1,), i32, cur), _need(plan.tiles, "plan.tiles", (tiles, 2), i32, cur), t, na, k, n,
+        _need(plan.tiles, "plan.tiles", (tiles, 2), i32, cur), t, na, k, n,
         rank, p, cols, part_block, y.data_ptr(), ys, *ws, at_stream))
     return y
 
