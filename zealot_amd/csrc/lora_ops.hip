@@ -50,80 +50,110 @@ struct PlanArgs {
     const int32_t *ids;
     int32_t *order, *offsets;
     int2 *tiles;
-    int rows, adapters, bits, tile_rows, max_tiles;
+    int rows, adapters, bits, tile_shift, max_tiles;  // tiles of 2^tile_shift rows
 };
 
 // One workgroup: each wave counts the adapters of a stretch of rows (64 rows at
-// a time: lanes of the same adapter find each other bit by bit), the counts of
-// (adapter, wave) become positions, and each wave goes through its stretch
-// again.  The waves' counts are their own, so the order does not depend on
-// scheduling.
+// a time: lanes of the same adapter find each other bit by bit, or at once where
+// all have one, as in a prompt), the counts of (adapter, wave) become positions,
+// and each wave goes through its stretch again.  The waves' counts are their own,
+// so the order does not depend on scheduling.  What bounds it is the latency of a
+// decode step (64 rows 4.5 us) and the one CU of a long one; ids and positions are
+// asked for kBatch groups of 64 at a time (32768 rows 30 us, one at a time 56).
+constexpr int kBatch = 8;
 __global__ void __launch_bounds__(1024) lora_plan_kernel(PlanArgs a) {
     __shared__ int at[16 * kMaxAdapters];
     __shared__ int first[kMaxAdapters], tile0[kMaxAdapters], count[kMaxAdapters];
     __shared__ int scan_rows[16], scan_tiles[16];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, A = a.adapters;
-    const int stretch = ((a.rows + 1023) / 1024) * 64;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), A = a.adapters;
+    const int tile_rows = 1 << a.tile_shift, stretch = ((a.rows + 1023) / 1024) * 64;
     const int r0 = min(wave * stretch, a.rows), r1 = min(r0 + stretch, a.rows);
-    for (int i = t; i < 16 * A; i += 1024) at[i] = 0;
-    __syncthreads();
+    auto ids_of = [&](int r, int (&id)[kBatch]) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) id[i] = a.ids[min(r + 64 * i + lane, a.rows - 1)];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) id[i] = r + 64 * i + lane < r1 ? id[i] : -1;
+    };
     // the lanes whose row has this lane's adapter (0: no row, no adapter)
-    auto peers = [&](int r, int &id) -> uint64_t {
-        id = r < r1 ? a.ids[r] : -1;
+    auto peers = [&](int id) -> uint64_t {
         const bool has = (unsigned)id < (unsigned)A;
         uint64_t same = __ballot(has);
+        if (same == 0 || __ballot(id == __builtin_amdgcn_readfirstlane(id)) == ~0ull) return same;
         for (int b = 0; b < a.bits; ++b) {
             const uint64_t set = __ballot((id >> b) & 1);
             same &= (id >> b) & 1 ? set : ~set;
         }
         return has ? same : 0;
     };
-    for (int r = r0; r < r1; r += 64) {
-        int id;
-        const uint64_t same = peers(r + lane, id);
-        if (same && lane == __ffsll((unsigned long long)same) - 1) atomicAdd(&at[wave * A + id], __popcll(same));
+    auto rank_of = [](uint64_t same) {   // how many of them come before this lane
+        return __builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0));
+    };
+    int id[kBatch];
+    if (r0 < r1) ids_of(r0, id);
+    for (int i = t; i < 16 * A; i += 1024) at[i] = 0;
+    __syncthreads();
+    for (int r = r0; r < r1; r += 64 * kBatch) {
+        if (r > r0) ids_of(r, id);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (r + 64 * i >= r1) break;
+            const uint64_t same = peers(id[i]);
+            if (same && rank_of(same) == 0) atomicAdd(&at[wave * A + id[i]], __popcll(same));
+        }
     }
     __syncthreads();
     const int per = (A + 1023) / 1024, a0 = min(t * per, A), a1 = min(a0 + per, A);
     int mine = 0, my_tiles = 0;
     for (int x = a0; x < a1; ++x) {
         int n = 0;
-        for (int w = 0; w < 16; ++w) {
-            const int c = at[w * A + x];
-            at[w * A + x] = n;
-            n += c;
-        }
+#pragma unroll
+        for (int w = 0; w < 16; ++w) n += at[w * A + x];
         count[x] = n;
         mine += n;
-        my_tiles += (n + a.tile_rows - 1) / a.tile_rows;
+        my_tiles += (n + tile_rows - 1) >> a.tile_shift;
     }
     int total, tiles;
     int pos = block_exclusive_scan_1024(mine, scan_rows, &total);
     int tile = block_exclusive_scan_1024(my_tiles, scan_tiles, &tiles);
     for (int x = a0; x < a1; ++x) {
-        const int n = count[x];
+        int c[16], n = pos;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) c[w] = at[w * A + x];
         a.offsets[x] = pos;
         first[x] = pos;
         tile0[x] = tile;
-        for (int w = 0; w < 16; ++w) at[w * A + x] += pos;
-        pos += n;
-        tile += (n + a.tile_rows - 1) / a.tile_rows;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            at[w * A + x] = n;
+            n += c[w];
+        }
+        tile += (n - pos + tile_rows - 1) >> a.tile_shift;
+        pos = n;
     }
     if (t == 0) a.offsets[A] = total;
     for (int i = total + t; i < a.rows; i += 1024) a.order[i] = -1;
     for (int i = tiles + t; i < a.max_tiles; i += 1024) a.tiles[i] = make_int2(-1, 0);
     __syncthreads();
-    for (int r = r0; r < r1; r += 64) {
-        int id, base = 0;
-        const uint64_t same = peers(r + lane, id);
-        const int leader = same ? __ffsll((unsigned long long)same) - 1 : lane;
-        if (same && lane == leader) base = atomicAdd(&at[wave * A + id], __popcll(same));
-        base = __shfl(base, leader);
-        if (same) {
-            const int p = base + __popcll(same & ((1ull << lane) - 1)), j = p - first[id];
-            a.order[p] = r + lane;
-            if (j % a.tile_rows == 0)
-                a.tiles[tile0[id] + j / a.tile_rows] = make_int2(id | min(a.tile_rows, count[id] - j) << 16, p);
+    const bool again = r1 - r0 > 64 * kBatch;
+    for (int r = r0; r < r1; r += 64 * kBatch) {
+        if (again) ids_of(r, id);
+        uint64_t same[kBatch];
+        int base[kBatch];   // asked for all groups first: the answers come in order
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            same[i] = r + 64 * i < r1 ? peers(id[i]) : 0;
+            base[i] = 0;
+            if (same[i] && rank_of(same[i]) == 0)
+                base[i] = atomicAdd(&at[wave * A + id[i]], __popcll(same[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int from = __shfl(base[i], same[i] ? __ffsll((unsigned long long)same[i]) - 1 : lane);
+            if (same[i] == 0) continue;
+            const int p = from + (int)rank_of(same[i]), j = p - first[id[i]];
+            a.order[p] = r + 64 * i + lane;
+            if ((j & (tile_rows - 1)) == 0)
+                a.tiles[tile0[id[i]] + (j >> a.tile_shift)] = make_int2(id[i] | min(tile_rows, count[id[i]] - j) << 16, p);
         }
     }
 }
@@ -140,13 +170,16 @@ struct LoraArgs {
     float *v;  // [splits][rows][v_stride]: part p from p * part_stride on
     void *y;
     int64_t y_stride;
-    int rows, adapters, k, n, rank, parts, part_stride, v_stride, splits, blocks;  // blocks: of 64 columns a wave
+    int rows, adapters, k, n, rank, parts, part_stride, v_stride, splits, blocks, groups;  // blocks: of 64 columns a wave; groups: of workgroups' columns
     int part_end[kMaxParts], part_block;
+    int y_whole;  // 16-byte pieces of y are aligned
 };
 
 // E values of a row from column c on, as the matrix instruction's operand (16
-// bytes of T): whole where `whole` says that rows are aligned and E divides their
-// length, else one by one; zeros from `cols` on.
+// bytes of T), zeros from `cols` on: whole where WHOLE says that rows are aligned
+// and E divides their length, else one by one.  No branch around a load (it would
+// be waited for before the next): what lies behind the row is read at its end and
+// not used.
 template <typename T> struct Operand;
 template <> struct Operand<uint16_t> {
     static constexpr int E = 8;  // values a lane, 32 a step
@@ -167,11 +200,13 @@ template <bool WHOLE>
 __device__ __forceinline__ u32x4 take(const uint16_t *row, int c, int cols) {
     u32x4 w = {0, 0, 0, 0};
     if (WHOLE) {
-        if (c < cols) w = *reinterpret_cast<const u32x4 *>(row + c);
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(row + min(c, cols - 8));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = c < cols ? v[i] : 0;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (c + i < cols) w[i / 2] |= (uint32_t)row[c + i] << (16 * (i & 1));
+            w[i / 2] |= (c + i < cols ? (uint32_t)row[min(c + i, cols - 1)] : 0u) << (16 * (i & 1));
     }
     return w;
 }
@@ -179,11 +214,13 @@ template <bool WHOLE>
 __device__ __forceinline__ u32x4 take(const float *row, int c, int cols) {
     u32x4 w = {0, 0, 0, 0};
     if (WHOLE) {
-        if (c < cols) w = *reinterpret_cast<const u32x4 *>(row + c);
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(row + min(c, cols - 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = c < cols ? v[i] : 0;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (c + i < cols) w[i] = __float_as_uint(row[c + i]);
+            w[i] = c + i < cols ? __float_as_uint(row[min(c + i, cols - 1)]) : 0u;
     }
     return w;
 }
@@ -192,11 +229,13 @@ template <bool WHOLE>
 __device__ __forceinline__ u32x4 take(const uint8_t *row, int c, int cols) {
     u32x2 q = {0, 0};
     if (WHOLE) {
-        if (c < cols) q = *reinterpret_cast<const u32x2 *>(row + c);
+        const u32x2 v = *reinterpret_cast<const u32x2 *>(row + min(c, cols - 8));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) q[i] = c < cols ? v[i] : 0;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (c + i < cols) q[i / 4] |= (uint32_t)row[c + i] << (8 * (i & 3));
+            q[i / 4] |= (c + i < cols ? (uint32_t)row[min(c + i, cols - 1)] : 0u) << (8 * (i & 3));
     }
     const u32x2 lo = e4m3x4_to_bf16x4(q[0]), hi = e4m3x4_to_bf16x4(q[1]);
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
@@ -215,7 +254,8 @@ __device__ __forceinline__ int tile_at(const LoraArgs &a, int i, int rows, int &
 // workgroup every W-th step of four matrix instructions of its stretch of k.
 template <typename X, typename T, int MT, int RT, int W, bool WHOLE>
 __global__ void __launch_bounds__(64 * W) lora_shrink_kernel(LoraArgs a) {
-    constexpr int E = Operand<T>::E, U = 4, kStep = 4 * E * U;
+    // (more under way a wave where registers allow it: 8192 x 4096 of rank 32 24 us with four)
+    constexpr int E = Operand<T>::E, U = !WHOLE ? 2 : MT == 2 && RT <= 2 ? 8 : 4, kStep = 4 * E * U;
     __shared__ f32x4 sums[W][RT * MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
@@ -251,6 +291,7 @@ __global__ void __launch_bounds__(64 * W) lora_shrink_kernel(LoraArgs a) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) xv[u][m] = take<WHOLE>(xr[m], at, a.k);
         }
+        __builtin_amdgcn_sched_barrier(0);  // (every load before the first product)
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -316,54 +357,121 @@ template <> struct Values<uint16_t> {
     }
 };
 
-// y of a tile and a wave's blocks of 64 columns.
-template <typename T, int MT, bool WHOLE>
+// y of a tile and a workgroup's columns, 64 of every 256 a wave: workgroups that
+// follow one another, and the waves of one, write the same rows side by side.  The values of the parts that these columns meet are summed over
+// the splits into LDS first, then each wave works alone: a block of y is asked
+// for before the product that is added to it.  ONE: no block of 64 columns meets two
+// parts.
+template <typename T, int MT, bool WHOLE, bool ONE>
 __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
     constexpr int E = Operand<T>::E, kStep = 4 * E, H = Values<T>::H;
+    extern __shared__ f32x4 lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     int adapter, p0;
-    const int count = tile_at(a, blockIdx.x, 16 * MT, adapter, p0);
+    const int count = tile_at(a, blockIdx.x / a.groups, 16 * MT, adapter, p0);
     if (count == 0) return;
     const int steps = (a.rank + kStep - 1) / kStep;
-    const int first = (blockIdx.y * 4 + wave) * a.blocks * 64, end = min(first + a.blocks * 64, a.n);
-    if (first >= end) return;
-    // rows of y (from a.rows on: none), rows of v
+    const int begin = blockIdx.x % a.groups * a.blocks * 256, end = min(begin + a.blocks * 256, a.n);
+    // rows of y (from a.rows on: none)
     unsigned row[MT];
-    const float *vr[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int i = 16 * m + r16;
-        row[m] = i < count ? (unsigned)a.order[p0 + i] : ~0u;
-        vr[m] = a.v + (size_t)(p0 + min(i, count - 1)) * a.v_stride;
+    for (int m = 0; m < MT; ++m) row[m] = 16 * m + r16 < count ? (unsigned)a.order[p0 + 16 * m + r16] : ~0u;
+    // values: rows of `line` 16-byte units, one spare against bank conflicts
+    int part0 = 0, part1 = a.parts - 1;
+    if (!a.part_block) {
+        part0 = part_of(a, begin);
+        part1 = part_of(a, end - 1);
     }
+    const int units = (part1 + 1 - part0) * (a.part_stride / 4), line = units + 1;
+    {
+        const float *src = a.v + (size_t)p0 * a.v_stride + part0 * a.part_stride;
+        const size_t plane = (size_t)a.rows * a.v_stride;
+        for (int i = threadIdx.x; i < 16 * MT * units; i += 256) {
+            const int r = i / units, u = i - r * units;
+            if (r >= count) break;
+            const float *at = src + (size_t)r * a.v_stride + 4 * u;
+            f32x4 v = *reinterpret_cast<const f32x4 *>(at);
+#pragma unroll 4
+            for (int q = 1; q < a.splits; ++q) v += *reinterpret_cast<const f32x4 *>(at + q * plane);
+            lds[r * line + u] = v;
+        }
+    }
+    __syncthreads();
     auto values = [&](int part, int s, u32x4 (&o)[MT][H]) {
         const int r = s * kStep + E * g;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             float v[E];
+            const f32x4 *src = lds + min(16 * m + r16, count - 1) * line + (part - part0) * (a.part_stride / 4);
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = 0.0f;
-            if (r < a.rank) {
-                const float *src = vr[m] + part * a.part_stride + r;
-                for (int q = 0; q < a.splits; ++q, src += (size_t)a.rows * a.v_stride)
+            for (int i = 0; i < E; i += 4) {
+                const f32x4 w = src[min(r + i, a.part_stride - 4) / 4];
 #pragma unroll
-                    for (int i = 0; i < E; i += 4)
-                        if (WHOLE || r + i < a.rank) {
-                            const f32x4 w = *reinterpret_cast<const f32x4 *>(src + i);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v[i + e] += w[e];
-                        }
-                if (!WHOLE)
-#pragma unroll
-                    for (int i = 0; i < E; ++i) v[i] = r + i < a.rank ? v[i] : 0.0f;
+                for (int e = 0; e < 4; ++e) v[i + e] = r + i + e < a.rank ? w[e] : 0.0f;
             }
             Values<T>::split(v, o[m]);
         }
     };
+    // columns n1 = n0 + 32 q + 8 g .. + 7 of row r16 of each group, whole pieces.  (No branch around a load: lanes that have
+    // none read another.)
+    typedef u32x4 Pieces[MT][2][H == 2 ? 1 : 2];
+    const bool pieces = a.y_whole && a.n >= 8;
+    const unsigned any = (unsigned)min((unsigned)a.order[p0], (unsigned)a.rows - 1);
+    auto ask = [&](int n0, Pieces &had) {
+        if (!pieces) return;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const T *y = (const T *)a.y + (size_t)(row[m] < (unsigned)a.rows ? row[m] : any) * a.y_stride + min(n0 + 32 * q + 8 * g, (a.n - 8) & ~7);
+#pragma unroll
+                for (int i = 0; i < (H == 2 ? 1 : 2); ++i) had[m][q][i] = reinterpret_cast<const u32x4 *>(y)[i];
+            }
+    };
+    auto give = [&](int n0, const Pieces &had, const f32x4 (&acc)[4][MT]) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (row[m] >= (unsigned)a.rows) continue;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int n1 = n0 + 32 * q + 8 * g;
+                T *y = (T *)a.y + (size_t)row[m] * a.y_stride + n1;
+                float d[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] = acc[2 * q + i / 4][m][i % 4];
+                if (n1 + 8 <= a.n && pieces) {
+                    u32x4 *yw = reinterpret_cast<u32x4 *>(y);
+                    if constexpr (H == 2) {
+                        u32x4 w = had[m][q][0];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = two(bf16lo(w[i]) + d[2 * i], bf16hi(w[i]) + d[2 * i + 1]);
+                        yw[0] = w;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            u32x4 w = had[m][q][i];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) + d[4 * i + e]);
+                            yw[i] = w;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (n1 + i < a.n) {
+                            if constexpr (H == 2) y[i] = (T)two(__uint_as_float((uint32_t)y[i] << 16) + d[i], 0.0f);
+                            else y[i] += d[i];
+                        }
+                }
+            }
+        }
+    };
     u32x4 kept[MT][H];  // of one step's ranks, over the blocks of a part
     int kept_part = -1;
-    for (int n0 = first; n0 < end; n0 += 64) {
+    for (int n0 = begin + wave * 64; n0 < end; n0 += 256) {
+        Pieces had;
+        ask(n0, had);
         // row r16 of B tile t: column n0 + 32 (t / 2) + 8 (r16 / 4) + 4 (t % 2) + r16 % 4
         const T *bb[4];
 #pragma unroll
@@ -392,12 +500,13 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
             }
         };
         f32x4 acc[4][MT];
-        const int last = min(n0 + 63, a.n - 1), part = part_of(a, n0);
-        if (a.parts == 1 || (part_of(a, last) == part && (!a.part_block || a.part_block >= 64))) {
-            product(part, acc);
+        if (ONE) {
+            product(part_of(a, n0), acc);
         } else {  // columns of several parts: each takes its own part's product
+            const int lo = a.part_block ? 0 : part_of(a, n0), hi = a.part_block ? a.parts - 1 : part_of(a, min(n0 + 63, a.n - 1));
+            product(lo, acc);
             f32x4 one[4][MT];
-            for (int p = 0; p < a.parts; ++p) {
+            for (int p = lo + 1; p <= hi; ++p) {
                 product(p, one);
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
@@ -405,45 +514,11 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
                     for (int e = 0; e < 4; ++e) {
                         const bool mine = part_of(a, min(n0 + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + e, a.n - 1)) == p;
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) acc[t][m][e] = mine || p == 0 ? one[t][m][e] : acc[t][m][e];
+                        for (int m = 0; m < MT; ++m) acc[t][m][e] = mine ? one[t][m][e] : acc[t][m][e];
                     }
             }
         }
-        // lane: columns n0 + 32 q + 8 g .. + 7 of row r16 of each group
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if (row[m] >= (unsigned)a.rows) continue;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int n1 = n0 + 32 * q + 8 * g;
-                T *y = (T *)a.y + (size_t)row[m] * a.y_stride + n1;
-                float d[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = acc[2 * q + i / 4][m][i % 4];
-                if (n1 + 8 <= a.n && (((uintptr_t)y) & 15u) == 0) {
-                    u32x4 *yw = reinterpret_cast<u32x4 *>(y);
-                    if constexpr (H == 2) {
-                        u32x4 w = *yw;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = two(bf16lo(w[i]) + d[2 * i], bf16hi(w[i]) + d[2 * i + 1]);
-                        *yw = w;
-                    } else {
-                        u32x4 w[2] = {yw[0], yw[1]};
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = __float_as_uint(__uint_as_float(w[i / 4][i % 4]) + d[i]);
-                        yw[0] = w[0];
-                        yw[1] = w[1];
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (n1 + i < a.n) {
-                            if constexpr (H == 2) y[i] = (T)two(__uint_as_float((uint32_t)y[i] << 16) + d[i], 0.0f);
-                            else y[i] += d[i];
-                        }
-                }
-            }
-        }
+        give(n0, had, acc);
     }
 }
 
@@ -486,13 +561,24 @@ void shrink(const LoraArgs &a, int tiles, bool whole, hipStream_t s) {
 
 template <typename T, int MT>
 void expand(LoraArgs a, int tiles, hipStream_t s) {
-    const bool whole = a.rank % Operand<T>::E == 0 && aligned(a.b, 16);
-    // blocks of 64 columns a wave: v and its halves are formed once for them, as long as 4096 waves are left
+    constexpr int E = Operand<T>::E;
+    const bool whole = a.rank % E == 0 && aligned(a.b, 16);
+    a.y_whole = a.y_stride % E == 0 && aligned(a.y, 16);
+    bool one = a.part_block % 64 == 0;
+    for (int i = 0; i < a.parts - 1 && !a.part_block; ++i) one = one && a.part_end[i] % 64 == 0;
+    // Blocks of 64 columns a wave: values are summed and split once for them, as long as
+    // 16384 waves are left (with 4096: 32768 rows x 4096 223 us for 199, 8192 x 28672 262 for 235).
     const int all = (a.n + 63) / 64;
-    a.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(8, (int64_t)tiles * all / 4096));
-    const dim3 grid((unsigned)tiles, (unsigned)((all + 4 * a.blocks - 1) / (4 * a.blocks)));
-    auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(a); };
-    whole ? go(lora_expand_kernel<T, MT, true>) : go(lora_expand_kernel<T, MT, false>);
+    a.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(4, (int64_t)tiles * all / 16384));
+    a.groups = (all + 4 * a.blocks - 1) / (4 * a.blocks);
+    const dim3 grid((unsigned)tiles * (unsigned)a.groups);
+    const size_t bytes = (size_t)16 * MT * (a.parts * (a.part_stride / 4) + 1) * 16;
+    auto go = [&](auto kernel) {
+        if (bytes > 65536) (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        kernel<<<grid, 256, bytes, s>>>(a);
+    };
+    if (one) whole ? go(lora_expand_kernel<T, MT, true, true>) : go(lora_expand_kernel<T, MT, false, true>);
+    else whole ? go(lora_expand_kernel<T, MT, true, false>) : go(lora_expand_kernel<T, MT, false, false>);
 }
 
 template <typename X, typename T>
@@ -539,7 +625,7 @@ int zk_lora_plan(const int32_t *adapter_ids, int64_t num_rows, int64_t num_adapt
     a.rows = (int)num_rows;
     a.adapters = (int)num_adapters;
     while ((1 << a.bits) < num_adapters) ++a.bits;
-    a.tile_rows = tile_rows_for(num_rows);
+    a.tile_shift = tile_rows_for(num_rows) == 16 ? 4 : 5;
     a.max_tiles = (int)nt;
     hipStream_t s = (hipStream_t)stream;
     KernelTimer timer("lora_plan", s);
@@ -588,6 +674,7 @@ int zk_lora(const void *x, const float *x_scales, int64_t x_stride, zk_dtype x_d
     if (!aligned(workspace, 16) || !aligned(tiles, 8)) return bad("zk_lora: the workspace must be 16-byte, tiles 8-byte aligned");
     const int e = elt_size(dtype), ranks = rank * num_parts;
     const int64_t nt = max_tiles(num_rows, num_adapters);
+    if (nt * ((n + 1023) / 1024) > 0x7fffffff) return bad("zk_lora: more rows of y than a launch takes");
     const int64_t xb = ((num_rows - 1) * x_stride + k) * elt_size(x_dtype), yb = ((num_rows - 1) * y_stride + n) * e;
     const struct {
         const void *p;
