@@ -9,8 +9,9 @@ of rounded squares: off by 87 steps of 2^-24 of itself, its root by half of that
 division, addition of eps, reciprocal root (4), the product with w, with the root
 and the division by 448: 10 more.  So y and the scale are off by at most 60 x
 2^-24 < 2^-18; a value lies between the roundings of y / s (1 - e) and (1 + e) with e
-= 2^-17 (both of them move it).  SiLU: expf, sum, division and product, 8 steps:
-less than that."""
+= 2^-17 (both of them move it).  SiLU: exp2
+of a product off by 2^-24 of itself (|g| <= 6 here: 9 x 2^-24 in the exponent, 6 of the
+result), 2 of its own, sum, reciprocal (2) and products, 13 steps: less than that."""
 import pytest
 import torch
 

@@ -12,9 +12,11 @@
 // sequence writes and reads again never exists.  The reference has neither
 // (its projections are f32, src/attention/cublas.rs:72-114).
 //
-// Both are bound by HBM: a row is read once into registers, its sum of
-// squares and its largest |t w| (which is the largest |y| up to the factor of
-// the row) go through one reduction, and it is written from the registers.
+// Both are bound by HBM (32768 rows of 4096 with a residual 158 us, 6.0 TB/s; SiLU of
+// 8192 rows of 14336 100 us, 5.85 TB/s), a few rows by latency: a row is read once
+// into registers, its sum of squares and its largest |t w| (which is the largest
+// |y| up to the factor of the row) go through one reduction, and it is written from
+// the registers.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -38,60 +40,41 @@ struct RowArgs {
     void *sum_out;          // norm with a residual
     const int64_t *rows;    // norm: the input row of each output row, or null
     int64_t in_rows;        // rows of x; one outside them is a row of zeros
-    int64_t x_stride, other_stride;
+    int64_t x_stride, other_stride, num_rows;
     int dim;
     float eps;
 };
 
-template <typename T> struct Elems;
-template <> struct Elems<float> { static constexpr int N = 4; };
-template <> struct Elems<uint16_t> { static constexpr int N = 8; };
+// What a thread loads at once: VEC values, as they are in memory.
+template <typename T, int VEC> struct Raw { T v; };
+template <> struct Raw<float, 4> { f32x4 v; };
+template <> struct Raw<uint16_t, 8> { u32x4 v; };
 
-template <int VEC>
-__device__ __forceinline__ void load(const float *p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        v[0] = *p;
-    } else {
-        const f32x4 w = *reinterpret_cast<const f32x4 *>(p);
+template <typename T, int VEC>
+__device__ __forceinline__ Raw<T, VEC> load(const T *p) { return *reinterpret_cast<const Raw<T, VEC> *>(p); }
+__device__ __forceinline__ void values(const Raw<float, 1> &r, float (&v)[1]) { v[0] = r.v; }
+__device__ __forceinline__ void values(const Raw<float, 4> &r, float (&v)[4]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = w[e];
+    for (int e = 0; e < 4; ++e) v[e] = r.v[e];
+}
+__device__ __forceinline__ void values(const Raw<uint16_t, 1> &r, float (&v)[1]) { v[0] = __uint_as_float((uint32_t)r.v << 16); }
+__device__ __forceinline__ void values(const Raw<uint16_t, 8> &r, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        v[2 * e] = bf16lo(r.v[e]);
+        v[2 * e + 1] = bf16hi(r.v[e]);
     }
 }
-template <int VEC>
-__device__ __forceinline__ void load(const uint16_t *p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        v[0] = __uint_as_float((uint32_t)*p << 16);
-    } else {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[2 * e] = bf16lo(w[e]);
-            v[2 * e + 1] = bf16hi(w[e]);
-        }
-    }
+// v rounded to the tensor's type (to nearest even, the machine's conversion)
+__device__ __forceinline__ Raw<float, 1> rounded(const float (&v)[1], float) { return {v[0]}; }
+__device__ __forceinline__ Raw<float, 4> rounded(const float (&v)[4], float) { return {f32x4{v[0], v[1], v[2], v[3]}}; }
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2_t));
 }
-// v rounded to the tensor's type, and written there
-template <int VEC>
-__device__ __forceinline__ void store_sum(float *p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) *p = v[0];
-    else *reinterpret_cast<f32x4 *>(p) = f32x4{v[0], v[1], v[2], v[3]};
-}
-template <int VEC>
-__device__ __forceinline__ void store_sum(uint16_t *p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        const uint32_t b = f32_to_bf16_bits(v[0]);
-        *p = (uint16_t)b;
-        v[0] = __uint_as_float(b << 16);
-    } else {
-        u32x4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            w[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
-            v[2 * e] = bf16lo(w[e]);
-            v[2 * e + 1] = bf16hi(w[e]);
-        }
-        *reinterpret_cast<u32x4 *>(p) = w;
-    }
+__device__ __forceinline__ Raw<uint16_t, 1> rounded(const float (&v)[1], uint16_t) { return {(uint16_t)bf16_pair(v[0], v[0])}; }
+__device__ __forceinline__ Raw<uint16_t, 8> rounded(const float (&v)[8], uint16_t) {
+    return {u32x4{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])}};
 }
 template <int VEC>
 __device__ __forceinline__ void store_q(uint8_t *p, const float (&v)[VEC]) {
@@ -103,64 +86,87 @@ __device__ __forceinline__ void store_q(uint8_t *p, const float (&v)[VEC]) {
         *reinterpret_cast<u32x2 *>(p) = u32x2{e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7])};
     }
 }
+// g / (1 + exp(-g)) with the machine's exp2 and reciprocal: off by 2^-24 |g| log2(e)
+// at most (the product's rounding) and 3 steps of 2^-24; 0 below -87, where 1 / (1 + exp(-g)) is
+// no normal number.  With expf and a division the instructions bind, not memory (8192 rows of
+// 14336 129 us).
+__device__ __forceinline__ float silu(float g) {
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f));
+}
 
-// One workgroup a row, MAXV vectors a thread.  A workgroup reads its whole row
-// before it writes any of it (two barriers apart from nothing else), so sum_out
-// may be the row's own x or residual.
-template <bool NORM, typename T, int VEC, int MAXV, int THREADS>
-__global__ void __launch_bounds__(THREADS) fp8_rows_kernel(RowArgs a) {
-    constexpr int W = THREADS / 64;
+// W waves a row, MAXV vectors a thread, R rows a workgroup (more than one where a
+// row is one wave's).  Each sum is written by the thread that read its terms, so
+// sum_out may be x or residual.  Loads past the row's end repeat its last vector,
+// so that none waits for a branch; what they give (in place: the vector or its sum)
+// is not used.
+template <bool NORM, typename T, int VEC, int MAXV, int W, int R>
+__global__ void __launch_bounds__(64 * W * R) fp8_rows_kernel(RowArgs a) {
+    static_assert(W == 1 || R == 1, "rows of several waves meet at barriers");
+    constexpr int THREADS = 64 * W;
     __shared__ float red_sum[W];
     __shared__ uint32_t red_max[W];
-    const int64_t row = blockIdx.x;
+    const int t = R > 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int64_t row = (int64_t)blockIdx.x * R + (R > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+    if (R > 1 && row >= a.num_rows) return;
     int64_t in = row;
     if (NORM && a.rows) {
         in = a.rows[row];
         if ((uint64_t)in >= (uint64_t)a.in_rows) {  // no such row: zeros
-            for (int i = threadIdx.x; i < a.dim; i += THREADS) {
+            for (int i = t; i < a.dim; i += THREADS) {
                 a.q[(size_t)row * a.dim + i] = 0;
                 if (a.other) ((T *)a.sum_out)[(size_t)row * a.dim + i] = T(0);
             }
-            if (threadIdx.x == 0) a.scales[row] = kLeast;
+            if (t == 0) a.scales[row] = kLeast;
             return;
         }
     }
     const T *x = (const T *)a.x + (size_t)in * a.x_stride;
     const T *o = a.other ? (const T *)a.other + (size_t)in * a.other_stride : nullptr;
-    float v[MAXV][VEC], w[MAXV][VEC];
+    Raw<T, VEC> rx[MAXV], ro[MAXV], rw[MAXV];
+    const int last = a.dim - VEC;
+#pragma unroll
+    for (int j = 0; j < MAXV; ++j) rx[j] = load<T, VEC>(x + min((j * THREADS + t) * VEC, last));
+    if (!NORM || o) {
+#pragma unroll
+        for (int j = 0; j < MAXV; ++j) ro[j] = load<T, VEC>(o + min((j * THREADS + t) * VEC, last));
+    }
+    if (NORM) {
+#pragma unroll
+        for (int j = 0; j < MAXV; ++j) rw[j] = load<T, VEC>((const T *)a.weight + min((j * THREADS + t) * VEC, last));
+    }
+    float v[MAXV][VEC];
     float ss = 0.0f;
     uint32_t top = 0;  // of |value| as bits: NaN above infinity above the numbers
 #pragma unroll
     for (int j = 0; j < MAXV; ++j) {
-        const int i = (j * THREADS + (int)threadIdx.x) * VEC;
-        if (i < a.dim) {
-            load<VEC>(x + i, v[j]);
-            if (NORM) load<VEC>((const T *)a.weight + i, w[j]);
-            else load<VEC>(o + i, w[j]);
-        }
-    }
+        const int i = (j * THREADS + t) * VEC;
+        values(rx[j], v[j]);
+        float other[VEC];
+        if (NORM) {
+            if (o) {
+                values(ro[j], other);
 #pragma unroll
-    for (int j = 0; j < MAXV; ++j) {
-        const int i = (j * THREADS + (int)threadIdx.x) * VEC;
-        if (i < a.dim) {
-            if (NORM && o) {
-                float r[VEC];
-                load<VEC>(o + i, r);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[j][e] += r[e];
-                store_sum<VEC>((T *)a.sum_out + (size_t)row * a.dim + i, v[j]);
+                for (int e = 0; e < VEC; ++e) v[j][e] += other[e];
+                const Raw<T, VEC> sum = rounded(v[j], T());
+                values(sum, v[j]);
+                if (i < a.dim) *reinterpret_cast<Raw<T, VEC> *>((T *)a.sum_out + (size_t)row * a.dim + i) = sum;
             }
+            float part = 0.0f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                if (NORM) {
-                    ss += v[j][e] * v[j][e];
-                    v[j][e] *= w[j][e];
-                } else {
-                    v[j][e] = v[j][e] / (1.0f + expf(-v[j][e])) * w[j][e];
-                }
-                top = max(top, __float_as_uint(v[j][e]) & 0x7fffffffu);
-            }
+            for (int e = 0; e < VEC; ++e) part += v[j][e] * v[j][e];
+            ss += i < a.dim ? part : 0.0f;
+            values(rw[j], other);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[j][e] *= other[e];
+        } else {
+            values(ro[j], other);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[j][e] = silu(v[j][e]) * other[e];
         }
+        uint32_t most = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) most = max(most, __float_as_uint(v[j][e]) & 0x7fffffffu);
+        top = max(top, i < a.dim ? most : 0u);
     }
 #pragma unroll
     for (int k = 32; k > 0; k >>= 1) {
@@ -185,10 +191,10 @@ __global__ void __launch_bounds__(THREADS) fp8_rows_kernel(RowArgs a) {
     const float most = __uint_as_float(top) * inv / kTop;
     const float s = most < kLeast ? kLeast : most;  // (NaN stays)
     const float r = 1.0f / s;
-    if (threadIdx.x == 0) a.scales[row] = s;
+    if (t == 0) a.scales[row] = s;
 #pragma unroll
     for (int j = 0; j < MAXV; ++j) {
-        const int i = (j * THREADS + (int)threadIdx.x) * VEC;
+        const int i = (j * THREADS + t) * VEC;
         if (i < a.dim) {
             float y[VEC];
 #pragma unroll
@@ -200,30 +206,53 @@ __global__ void __launch_bounds__(THREADS) fp8_rows_kernel(RowArgs a) {
 
 bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
 
+// Waves a row: a wave for short rows, four rows a workgroup (32768 rows of 1024,
+// two vectors a thread 43 us, a workgroup a row 51).  Longer rows of the norm take two to four
+// vectors a thread (8192 rows of 16384: eight 163 us, four 160, two 164; 32768 of
+// 4096: two 158, one 160), SiLU, whose threads compute more between two loads, as few
+// as 16 waves allow (8192 of 14336: eight 110, four 109, two 100; 16384 of 4096: two
+// 60.5, one 57.7).  Rows off their alignment go value by value: eight a thread
+// (8192 of 2001: 31 us, four 36, two 49).
 template <bool NORM, typename T, int VEC>
-bool launch_vec(const RowArgs &a, int rows, hipStream_t s) {
+bool launch_vec(const RowArgs &a, hipStream_t s) {
     const int n = (a.dim + VEC - 1) / VEC;
-    auto go = [&](auto kernel, int threads) { kernel<<<(unsigned)rows, threads, 0, s>>>(a); };
-    if (n <= 64) go(fp8_rows_kernel<NORM, T, VEC, 1, 64>, 64);
-    else if (n <= 256) go(fp8_rows_kernel<NORM, T, VEC, 1, 256>, 256);
-    else if (n <= 512) go(fp8_rows_kernel<NORM, T, VEC, 2, 256>, 256);
-    else if (n <= 1024) go(fp8_rows_kernel<NORM, T, VEC, 4, 256>, 256);
-    else if (n <= 2048) go(fp8_rows_kernel<NORM, T, VEC, 8, 256>, 256);
-    else if (n <= 4096) go(fp8_rows_kernel<NORM, T, VEC, 4, 1024>, 1024);
-    else return false;
+    auto go = [&](auto kernel, int threads, int rows) {
+        kernel<<<(unsigned)((a.num_rows + rows - 1) / rows), threads, 0, s>>>(a);
+    };
+    if (n <= 64) go(fp8_rows_kernel<NORM, T, VEC, 1, 1, 4>, 256, 4);
+    else if (n <= 128) go(fp8_rows_kernel<NORM, T, VEC, 2, 1, 4>, 256, 4);
+    else if (n <= 256) go(fp8_rows_kernel<NORM, T, VEC, 1, 4, 1>, 256, 1);
+    else if constexpr (VEC == 1) {
+        if (n <= 512) go(fp8_rows_kernel<NORM, T, VEC, 2, 4, 1>, 256, 1);
+        else if (n <= 2048) go(fp8_rows_kernel<NORM, T, VEC, 8, 4, 1>, 256, 1);
+        else if (n <= 4096) go(fp8_rows_kernel<NORM, T, VEC, 8, 8, 1>, 512, 1);
+        else return false;
+    } else if constexpr (NORM) {
+        if (n <= 512) go(fp8_rows_kernel<NORM, T, VEC, 2, 4, 1>, 256, 1);
+        else if (n <= 1024) go(fp8_rows_kernel<NORM, T, VEC, 2, 8, 1>, 512, 1);
+        else if (n <= 2048) go(fp8_rows_kernel<NORM, T, VEC, 4, 8, 1>, 512, 1);
+        else if (n <= 4096) go(fp8_rows_kernel<NORM, T, VEC, 4, 16, 1>, 1024, 1);
+        else return false;
+    } else {
+        if (n <= 512) go(fp8_rows_kernel<NORM, T, VEC, 1, 8, 1>, 512, 1);
+        else if (n <= 1024) go(fp8_rows_kernel<NORM, T, VEC, 1, 16, 1>, 1024, 1);
+        else if (n <= 2048) go(fp8_rows_kernel<NORM, T, VEC, 2, 16, 1>, 1024, 1);
+        else if (n <= 4096) go(fp8_rows_kernel<NORM, T, VEC, 4, 16, 1>, 1024, 1);
+        else return false;
+    }
     return true;
 }
 
 template <bool NORM>
-int launch(const RowArgs &a, int64_t rows, zk_dtype dtype, const char *name, hipStream_t s) {
+int launch(const RowArgs &a, zk_dtype dtype, const char *name, hipStream_t s) {
     const int V = dtype == ZK_BF16 ? 8 : 4;
     const bool vec = a.dim % V == 0 && a.x_stride % V == 0 && a.other_stride % V == 0 && aligned(a.x, 16) &&
                      aligned(a.other, 16) && aligned(a.weight, 16) && aligned(a.sum_out, 16) && aligned(a.q, V);
     bool ok;
     if (dtype == ZK_BF16)
-        ok = vec ? launch_vec<NORM, uint16_t, 8>(a, (int)rows, s) : launch_vec<NORM, uint16_t, 1>(a, (int)rows, s);
+        ok = vec ? launch_vec<NORM, uint16_t, 8>(a, s) : launch_vec<NORM, uint16_t, 1>(a, s);
     else
-        ok = vec ? launch_vec<NORM, float, 4>(a, (int)rows, s) : launch_vec<NORM, float, 1>(a, (int)rows, s);
+        ok = vec ? launch_vec<NORM, float, 4>(a, s) : launch_vec<NORM, float, 1>(a, s);
     if (!ok)
         return set_error(ZK_ERR_INVALID_ARGUMENT,
                          std::string("Internal error: ") + name + ": rows of " + std::to_string(a.dim) +
@@ -277,12 +306,13 @@ int zk_rms_norm_fp8(const void *x, const void *residual, const void *weight, voi
     a.sum_out = residual ? residual_out : nullptr;
     a.rows = rows;
     a.in_rows = x_rows;
+    a.num_rows = num_rows;
     a.x_stride = a.other_stride = dim;
     a.dim = (int)dim;
     a.eps = eps;
     hipStream_t s = (hipStream_t)stream;
     KernelTimer timer("rms_norm_fp8", s);
-    return launch<true>(a, num_rows, dtype, "zk_rms_norm_fp8", s);
+    return launch<true>(a, dtype, "zk_rms_norm_fp8", s);
 }
 
 int zk_silu_mul_fp8(const void *gate, const void *up, void *q, float *scales, int64_t rows, int64_t cols,
@@ -306,6 +336,7 @@ int zk_silu_mul_fp8(const void *gate, const void *up, void *q, float *scales, in
     RowArgs a{};
     a.x = gate;
     a.other = up;
+    a.num_rows = rows;
     a.q = (uint8_t *)q;
     a.scales = scales;
     a.x_stride = gate_stride;
@@ -313,7 +344,7 @@ int zk_silu_mul_fp8(const void *gate, const void *up, void *q, float *scales, in
     a.dim = (int)cols;
     hipStream_t s = (hipStream_t)stream;
     KernelTimer timer("silu_mul_fp8", s);
-    return launch<false>(a, rows, dtype, "zk_silu_mul_fp8", s);
+    return launch<false>(a, dtype, "zk_silu_mul_fp8", s);
 }
 
 }  // extern "C"
