@@ -9,6 +9,7 @@ rope_ops.hip, gemm.cpp, skinny_gemm.hip, fp8_rows.hip, fp8_gemm.hip and lora_ops
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -467,6 +468,11 @@ def fp8_weight(weight: torch.Tensor, scales: torch.Tensor | None = None, stream=
     return Fp8Weight(data, scales, n, k)
 
 
+@functools.lru_cache(1024)
+def _fp8_ws(m: int, n: int, k: int, code: int) -> int:
+    return _lib.lib().zk_linear_fp8_workspace_size(m, n, k, code)
+
+
 def linear_fp8_workspace_bytes(m: int, n: int, k: int, out_dtype=torch.bfloat16) -> int:
     return int(_lib.lib().zk_linear_fp8_workspace_size(m, n, k, _CODES[out_dtype]))
 
@@ -496,7 +502,7 @@ def linear_fp8(x: Fp8Rows, weight: Fp8Weight, out=None, out_dtype=torch.bfloat16
     if workspace is not None:  # (its size is checked by the call)
         ws = (_need(workspace, "workspace", workspace.shape, None, cur), workspace.numel() * workspace.element_size())
     elif m > 16:
-        size = lib.zk_linear_fp8_workspace_size(m, n, k, code)
+        size = _fp8_ws(m, n, k, code)
         if size:
             workspace = _empty(out, (size,), torch.uint8, stream)  # (held until the launch is made)
             ws = (workspace.data_ptr(), size)
@@ -522,7 +528,7 @@ def lora_plan(adapter_ids, num_adapters: int, out: LoraPlan | None = None, strea
     ids = _need(adapter_ids, "adapter_ids", (t,), i32, cur)
     if num_adapters <= 0:
         raise ValueError("num_adapters must be positive")
-    tiles = _lib.lib().zk_lora_max_tiles(t, num_adapters)
+    tiles = _lora_tiles(t, num_adapters)
     if out is None:  # one buffer, the tiles first
         buf = _empty(adapter_ids, (2 * tiles + t + num_adapters + 1,), i32, stream)
         part = buf.split_with_sizes((2 * tiles, t, num_adapters + 1))
@@ -531,6 +537,23 @@ def lora_plan(adapter_ids, num_adapters: int, out: LoraPlan | None = None, strea
                                        _need(out.offsets, "out.offsets", (num_adapters + 1,), i32, cur),
                                        _need(out.tiles, "out.tiles", (tiles, 2), i32, cur), at_stream))
     return out
+
+
+# Sizes depend on a call's numbers alone: asked for once each (0.6 us a question, of a
+# call's 10).
+@functools.lru_cache(1024)
+def _lora_tiles(rows: int, adapters: int) -> int:
+    return _lib.lib().zk_lora_max_tiles(rows, adapters)
+
+
+@functools.lru_cache(1024)
+def _lora_sizes(rows: int, adapters: int, k: int, rank: int, parts: int, code: int):
+    return _lora_tiles(rows, adapters), _lib.lib().zk_lora_workspace_size(rows, adapters, k, rank, parts, code)
+
+
+@functools.lru_cache(1024)
+def _columns(parts: tuple):
+    return (ctypes.c_int64 * len(parts))(*parts), sum(parts)
 
 
 def lora_workspace_bytes(num_rows: int, num_adapters: int, k: int, rank: int, num_parts: int, dtype) -> int:
@@ -558,9 +581,9 @@ def lora(x, a, b, scales, plan: LoraPlan, y, parts=None, part_block: int = 0, wo
         p = parts
     elif parts is not None:
         p = len(parts)
-        if p == 0 or sum(parts) != n:
+        cols, total = _columns(tuple(parts))
+        if p == 0 or total != n:
             raise ValueError(f"parts must add up to the {n} columns of y")
-        cols = (ctypes.c_int64 * p)(*parts)
     if isinstance(x, Fp8Rows):
         xc, xs = _lib.FP8_E4M3, _rows2(rows, "x.data", t, k, _FP8, cur)
         sc = _need(x.scales, "x.scales", (t,), torch.float32, cur)
@@ -569,8 +592,7 @@ def lora(x, a, b, scales, plan: LoraPlan, y, parts=None, part_block: int = 0, wo
     ys = _rows2(y, "y", t, n, dt, cur)
     lib = _lib.lib()
     i32 = torch.int32
-    tiles = lib.zk_lora_max_tiles(t, na)
-    size = lib.zk_lora_workspace_size(t, na, k, rank, p, code)
+    tiles, size = _lora_sizes(t, na, k, rank, p, code)
     if workspace is None:
         workspace = _empty(y, (size,), torch.uint8, stream)  # (held until the launches are made)
         ws = (workspace.data_ptr() if size else None, size)

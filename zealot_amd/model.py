@@ -30,13 +30,21 @@ rope_theta or qk_norm set, both run in the KV write's launch
     contiguous 1 KiB loads; their row-major copies serve steps of more than
     64 rows (prefill, mixed) on the GEMM plan, since the weight-streaming
     kernel reads a weight once per 64 rows;
+  - with projections in 8 bits (LlamaWeights.in_8_bits: qkv, gate|up and down) the
+    norms and SiLU * up write the rows that the 8-bit products read (rms_norm_fp8,
+    silu_mul_fp8, linear_fp8); the o projection, whose rows attention writes, and
+    lm_head stay in bf16;
+  - requests may bring low-rank adapters (LlamaAdapters, step's `adapters`): the
+    rows of a step are grouped by adapter once (lora_plan) and each projection
+    adds its rows' adapters to its output (lora).  A step without any runs as
+    before;
   - weights are random-initialised here (there is no checkpoint loader in
     this build; the reference loads HF weights, model_loader.rs:241).
 """
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 
@@ -84,6 +92,23 @@ class LlamaWeights:
     final_norm: torch.Tensor  # [hidden]
     lm_head: object           # [vocab, hidden] (a dense.TiledWeight for bf16 models)
 
+    def in_8_bits(self) -> "LlamaWeights":
+        """The model with qkv, gate|up and down as dense.Fp8Weight (bf16 models):
+        gate|up holds the gate rows, then the up rows.  The rest is shared."""
+        if self.embedding.dtype != torch.bfloat16:
+            raise TypeError("8-bit projections are for bf16 models")
+        if any(isinstance(lw.gate_up, dense.Fp8Weight) for lw in self.layers):
+            raise ValueError("the projections are in 8 bits already")
+
+        def full(t):
+            return t if isinstance(t, torch.Tensor) else t.rowmajor() if t.full is None else t.full
+
+        def layer(lw):
+            gate_up = torch.cat(dense.split_gate_up(full(lw.gate_up)))
+            return replace(lw, qkv=dense.fp8_weight(full(lw.qkv)), gate_up=dense.fp8_weight(gate_up),
+                           down=dense.fp8_weight(full(lw.down)))
+        return replace(self, layers=[layer(lw) for lw in self.layers])
+
     @staticmethod
     def random(cfg: LlamaConfig, dtype=torch.bfloat16, device="cuda", seed: int = 0,
                tiled: bool = True, keep_full: bool = True) -> "LlamaWeights":
@@ -113,11 +138,52 @@ class LlamaWeights:
         return LlamaWeights(emb, layers, norm(hid), tile(lin(cfg.vocab_size, hid)))
 
 
+@dataclass
+class LayerAdapters:
+    """One layer's adapters for dense.lora: (a, b) of each projection, or None."""
+    qkv: tuple | None = None      # a [A, 3 r, hidden] (q, k and v ranks), b [A, (H + 2 Hkv) D, r]
+    o: tuple | None = None        # a [A, r, H D], b [A, hidden, r]
+    gate_up: tuple | None = None  # a [A, 2 r, hidden], b [A, 2 I, r] in the rows' order of the model's gate_up
+    down: tuple | None = None     # a [A, r, I], b [A, hidden, r]
+
+
+@dataclass
+class LlamaAdapters:
+    """The low-rank adapters that requests may name, of the model's type."""
+    count: int
+    layers: list
+    scales: torch.Tensor | None = None  # float32 [count]; None: 1
+
+    @staticmethod
+    def random(cfg: LlamaConfig, count: int, rank: int, dtype=torch.bfloat16, device="cuda", seed: int = 0,
+               in_8_bits: bool = False) -> "LlamaAdapters":
+        """N(0, 1/fan_in) a and b, for every projection (seeded); in_8_bits: for
+        a model of LlamaWeights.in_8_bits, whose gate and up rows do not alternate."""
+        g = torch.Generator(device=device).manual_seed(seed)
+
+        def mat(n, k):
+            return (torch.randn((count, n, k), generator=g, device=device) / math.sqrt(k)).to(dtype)
+
+        def pair(n, k, parts=1):
+            return mat(parts * rank, k), mat(n, rank)
+
+        def gate_up(n, k):
+            a, b = pair(2 * n, k, 2)
+            if not in_8_bits:
+                b = torch.stack([dense.interleave_gate_up(t[:n], t[n:]) for t in b])
+            return a, b
+
+        H, Hkv, D, hid, I = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.hidden_size, cfg.intermediate_size
+        layers = [LayerAdapters(pair((H + 2 * Hkv) * D, hid, 3), pair(hid, H * D), gate_up(I, hid), pair(hid, I))
+                  for _ in range(cfg.num_layers)]
+        return LlamaAdapters(count, layers, 0.5 + torch.rand((count,), generator=g, device=device))
+
+
 class HipModelRunner:
     """ModelRunner::step (engine.rs:15-37) for a schedule() batch: returns the
     f32 logits [len(batch), vocab] of each sequence's last step token."""
 
-    def __init__(self, cfg: LlamaConfig, weights: LlamaWeights, kv: PagedKVRunner):
+    def __init__(self, cfg: LlamaConfig, weights: LlamaWeights, kv: PagedKVRunner, adapters: LlamaAdapters | None = None):
         c = kv.cache
         if (c.num_layers, c.num_kv_heads, c.head_dim) != (cfg.num_layers, cfg.num_kv_heads, cfg.head_dim):
             raise ValueError("KV cache shape does not match the model")
@@ -127,12 +193,18 @@ class HipModelRunner:
             self.rope = dense.rope_table(cfg.max_positions, cfg.head_dim, cfg.rope_theta, weights.embedding.device)
         if cfg.qk_norm and any(lw.q_norm is None or lw.k_norm is None for lw in weights.layers):
             raise ValueError("a model with qk_norm needs the layers' q_norm and k_norm")
+        if adapters is not None and len(adapters.layers) != len(weights.layers):
+            raise ValueError("adapters must have the model's layers")
+        self.adapters = adapters
+        self.in_8_bits = isinstance(weights.layers[0].gate_up, dense.Fp8Weight)
 
     def drop_state(self, request_id: str) -> None:
         self.kv.drop_state(request_id)
 
-    def step(self, out) -> torch.Tensor:
-        """One step over ScheduleOutput `out` (zealot_amd.scheduler)."""
+    def step(self, out, adapters: dict | None = None) -> torch.Tensor:
+        """One step over ScheduleOutput `out` (zealot_amd.scheduler); adapters:
+        the adapter of each request id that brings one, the same at all its steps."""
+        per_row = self._adapter_rows(out, adapters)
         plan = self.kv.begin_step(out)
         if not out.batch:
             return torch.empty((0, self.cfg.vocab_size), dtype=torch.float32, device=self.w.embedding.device)
@@ -141,14 +213,78 @@ class HipModelRunner:
         ids = [t for e in out.batch for t in e.step_input()]
         both = torch.tensor(ids + plan_last_rows(plan), dtype=torch.int64, pin_memory=True)
         both = both.to(self.w.embedding.device, non_blocking=True)
-        return self.forward(plan, both[:len(ids)], both[len(ids):])
+        lora = None
+        if per_row is not None:
+            rows = torch.tensor(per_row, dtype=torch.int32, pin_memory=True)
+            lora = dense.lora_plan(rows.to(both.device, non_blocking=True), self.adapters.count)
+        return self.forward(plan, both[:len(ids)], both[len(ids):], lora)
 
-    def forward(self, plan: StepPlan, ids: torch.Tensor, last_rows: torch.Tensor) -> torch.Tensor:
+    def _adapter_rows(self, out, adapters: dict | None):
+        """The adapter of every step row (-1: none), or None where no row has one."""
+        mine = {e.request_id: adapters[e.request_id] for e in out.batch if e.request_id in adapters} if adapters else {}
+        if not mine:
+            return None
+        if self.adapters is None:
+            raise ValueError("the runner has no adapters")
+        for rid, a in mine.items():
+            if not 0 <= a < self.adapters.count:
+                raise ValueError(f"request {rid} names adapter {a} of {self.adapters.count}")
+        return [mine.get(e.request_id, -1) for e in out.batch for _ in range(e.num_tokens)]
+
+    def _norm(self, x, weight, resid=None):
+        """The norm of x, or of resid += x, as the next projection reads it."""
+        eps = self.cfg.rms_eps
+        norm = dense.rms_norm_fp8 if self.in_8_bits else dense.rms_norm
+        return norm(x, weight, eps) if resid is None else norm(x, weight, eps, residual=resid, residual_out=resid)[0]
+
+    def _forward_apart(self, plan: StepPlan, ids: torch.Tensor, last_rows: torch.Tensor, lora) -> torch.Tensor:
+        """forward with each projection on its own: in 8 bits, or with the rows'
+        adapters added before its output is used."""
+        cfg, w, T = self.cfg, self.w, plan.total_tokens
+        H, Hkv, D, I = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.intermediate_size
+        qd, kd = H * D, Hkv * D
+
+        def project(x, weight, adapters, **parts):
+            y = dense.linear_fp8(x, weight) if isinstance(weight, dense.Fp8Weight) else dense.linear(x, weight)
+            if adapters is not None:
+                dense.lora(x, *adapters, self.adapters.scales, lora, y, **parts)
+            return y
+
+        resid = dense.embedding(ids, w.embedding)
+        normed = self._norm(resid, w.layers[0].attn_norm)
+        for layer, lw in enumerate(w.layers):
+            ad = LayerAdapters() if lora is None else self.adapters.layers[layer]
+            qkv = project(normed, lw.qkv, ad.qkv, parts=(qd, kd, kd))
+            q, k, v = (t.view(T, -1, D) for t in qkv.split((qd, kd, kd), 1))
+            if self.rope is not None or cfg.qk_norm:
+                self.kv.write_rope(layer, plan, q, k, v, self.rope, lw.q_norm if cfg.qk_norm else None,
+                                   lw.k_norm if cfg.qk_norm else None, cfg.rms_eps, cfg.rope_interleaved, q_out=q)
+            else:
+                self.kv.write(layer, plan, k, v)
+            attn = self.kv.attention(layer, plan, q)
+            normed = self._norm(project(attn.view(T, qd), lw.o, ad.o), lw.ffn_norm, resid)
+            if self.in_8_bits:
+                gu = project(normed, lw.gate_up, ad.gate_up, parts=(I, I))
+                act = dense.silu_mul_fp8(gu[:, :I], gu[:, I:])
+            else:  # gate and up columns alternate in blocks: a block is a row of SiLU's
+                b = dense.GATE_UP_BLOCK
+                gu = project(normed, lw.gate_up, ad.gate_up, parts=2, part_block=b).view(-1, 2 * b)
+                act = dense.silu_mul(gu[:, :b], gu[:, b:]).view(T, I)
+            delta = project(act, lw.down, ad.down)
+            if layer + 1 < len(w.layers):
+                normed = self._norm(delta, w.layers[layer + 1].attn_norm, resid)
+        final, _ = dense.rms_norm(delta, w.final_norm, cfg.rms_eps, residual=resid, rows=last_rows)
+        return dense.linear(final, w.lm_head, out_dtype=torch.float32)
+
+    def forward(self, plan: StepPlan, ids: torch.Tensor, last_rows: torch.Tensor, lora=None) -> torch.Tensor:
+        """The step's logits; lora: the dense.lora_plan of its rows' adapters."""
         cfg, w = self.cfg, self.w
+        if ids.numel() != plan.total_tokens:
+            raise ValueError("one token id per step row")
+        if lora is not None or self.in_8_bits:
+            return self._forward_apart(plan, ids, last_rows, lora)
         H, Hkv, D = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
         T = plan.total_tokens
-        if ids.numel() != T:
-            raise ValueError("one token id per step row")
         qd, kd = H * D, Hkv * D
         resid = dense.embedding(ids, w.embedding)  # the residual stream [T, hidden]
         normed = torch.empty_like(resid)
