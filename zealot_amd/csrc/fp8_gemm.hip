@@ -554,35 +554,62 @@ __global__ void __launch_bounds__(256) fp8_sum_kernel(GemmArgs a) {
 }
 
 // ----------------------------------------------------------------- packing
-// One workgroup a packed row: its largest value, then its values in order.
-__global__ void __launch_bounds__(256) fp8_pack_kernel(const void *w, int dtype, uint8_t *out, float *scales, int n, int k,
-                                                       int chunks) {
-    __shared__ uint32_t red[4];
-    const int T = blockIdx.x >> 4, i = blockIdx.x & 15, row = row_of(T, i);
+// One workgroup a tile of 16 rows, 16 threads a row: the rows' largest values, then
+// their values in order, a unit of 16 a thread (28672 x 4096 from e4m3 values 38 us, byte by byte 112;
+// from bf16 91 us, 323).
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_pack_kernel(const T *w, uint8_t *out, float *scales, int n, int k, int chunks, bool vec) {
+    constexpr bool kReady = sizeof(T) == 1;  // values and scales are there
+    __shared__ uint32_t red[4][16];
+    const int tile = blockIdx.x, i = threadIdx.x & 15, row = row_of(tile, i), units = chunks * (kChunk / 16);
     const bool real = row < n;
-    auto value = [&](int c) {
-        return dtype == ZK_F32 ? ((const float *)w)[(size_t)row * k + c]
-                               : __uint_as_float((uint32_t)((const uint16_t *)w)[(size_t)row * k + c] << 16);
+    const T *from = w + (size_t)min(row, n - 1) * k;
+    // the 16 values of a unit, zeros from column k on
+    auto unit = [&](int u, T (&v)[16]) {
+        if (vec && 16 * u + 16 <= k) {
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T); ++j)
+                reinterpret_cast<u32x4 *>(v)[j] = reinterpret_cast<const u32x4 *>(from + 16 * u)[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = 16 * u + j < k ? from[16 * u + j] : T(0);
+        }
+    };
+    auto f32_of = [](T v) {
+        if constexpr (sizeof(T) == 4) return v;
+        else return __uint_as_float((uint32_t)v << 16);
     };
     float r = 0.0f;
-    if (dtype != ZK_FP8_E4M3 && real) {
+    if constexpr (!kReady) {
         uint32_t top = 0;  // as bits: NaN above infinity above the numbers
-        for (int c = threadIdx.x; c < k; c += 256) top = max(top, __float_as_uint(value(c)) & 0x7fffffffu);
-        for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+        for (int u = threadIdx.x >> 4; u < units; u += 16) {
+            alignas(16) T v[16];
+            unit(u, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(f32_of(v[j])) & 0x7fffffffu);
+        }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        if ((threadIdx.x & 63) < 16) red[threadIdx.x >> 6][i] = top;
         __syncthreads();
-        top = max(max(red[0], red[1]), max(red[2], red[3]));
+        top = max(max(red[0][i], red[1][i]), max(red[2][i], red[3][i]));
         const float most = __uint_as_float(top) / 448.0f, s = most < 0x1p-126f ? 0x1p-126f : most;
-        if (threadIdx.x == 0) scales[row] = s;
+        if (threadIdx.x < 16 && real) scales[row] = s;
         r = 1.0f / s;
     }
-    uint8_t *to = out + (size_t)T * chunks * kTile + i * 16;
-    for (int c = threadIdx.x; c < chunks * kChunk; c += 256) {
-        uint8_t q = 0;
-        if (real && c < k)
-            q = dtype == ZK_FP8_E4M3 ? ((const uint8_t *)w)[(size_t)row * k + c]
-                                     : (uint8_t)e4m3x4(value(c) * r, 0.f, 0.f, 0.f);
-        to[(size_t)(c / kChunk) * kTile + (c % kChunk) / 16 * 256 + c % 16] = q;
+    u32x4 *to = reinterpret_cast<u32x4 *>(out + (size_t)tile * chunks * kTile) + i;
+    for (int u = threadIdx.x >> 4; u < units; u += 16) {
+        alignas(16) T v[16];
+        unit(u, v);
+        u32x4 q;
+        if constexpr (kReady) {
+            q = *reinterpret_cast<const u32x4 *>(v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                q[j] = e4m3x4(f32_of(v[4 * j]) * r, f32_of(v[4 * j + 1]) * r, f32_of(v[4 * j + 2]) * r, f32_of(v[4 * j + 3]) * r);
+        }
+        to[u * 16] = real ? q : u32x4{0, 0, 0, 0};
     }
 }
 
@@ -703,7 +730,12 @@ int zk_fp8_weight(const void *w, zk_dtype dtype, void *packed, float *scales, in
         return bad("zk_fp8_weight: operands overlap");
     hipStream_t s = (hipStream_t)stream;
     const int chunks = (int)((k + kChunk - 1) / kChunk);
-    fp8_pack_kernel<<<(unsigned)((n + 63) / 64 * 64), 256, 0, s>>>(w, dtype, (uint8_t *)packed, scales, (int)n, (int)k, chunks);
+    const unsigned grid = (unsigned)((n + 63) / 64 * 4);
+    const bool vec = k % 16 == 0 && aligned16(w);
+    auto go = [&](auto *from) { fp8_pack_kernel<<<grid, 256, 0, s>>>(from, (uint8_t *)packed, scales, (int)n, (int)k, chunks, vec); };
+    if (dtype == ZK_F32) go((const float *)w);
+    else if (dtype == ZK_BF16) go((const uint16_t *)w);
+    else go((const uint8_t *)w);
     if (hipError_t e = hipGetLastError(); e != hipSuccess)
         return set_error(ZK_ERR_HIP, std::string("Internal error: zk_fp8_weight: ") + hipGetErrorString(e));
     return ZK_OK;
