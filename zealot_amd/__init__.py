@@ -18,6 +18,9 @@ zealot_amd/csrc with `python -m zealot_amd.build`):
                               head norms and rotary embedding, with the KV write
   ops.page_bounds / page_scores / select_pages / paged_decode_sparse
                               decode over the pages that bounds of their keys select
+  dense.rms_norm_fp8 / silu_mul_fp8 / fp8_weight / linear_fp8
+                              rows, weights and products in 8 bits
+  dense.lora_plan / lora      low-rank adapters of many requests beside a projection
 """
 from ._lib import ZealotError, lib  # noqa: F401
 from .block_manager import BlockHandle, BlockManager  # noqa: F401
