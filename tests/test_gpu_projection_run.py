@@ -264,6 +264,8 @@ def test_adapters_that_are_not_there():
     ad = LlamaAdapters.random(cfg, 2, 4, F32)
     with pytest.raises(ValueError):
         HipModelRunner(cfg, w, kv, LlamaAdapters(2, []))
+    with pytest.raises(ValueError):  # gate and up rows in the other order
+        HipModelRunner(cfg, w, kv, LlamaAdapters.random(cfg, 2, 4, F32, in_8_bits=True))
     sched.add(sched.make_sequence("a", [1, 2, 3], 2, Priority.Medium))
     out = sched.schedule()
     with pytest.raises(ValueError):
@@ -273,3 +275,7 @@ def test_adapters_that_are_not_there():
         with pytest.raises(ValueError):
             runner.step(out, {"a": bad})
     assert runner.step(out, {"a": 1, "other": 9}).shape == (1, 64)
+    kv.drop_state("a")
+    none = runner.step(out, {"a": None}).clone()
+    kv.drop_state("a")
+    assert torch.equal(none, HipModelRunner(cfg, w, kv).step(out))

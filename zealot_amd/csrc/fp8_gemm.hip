@@ -344,7 +344,10 @@ __global__ void __launch_bounds__(64 * WM * WN) fp8_gemm_kernel(GemmArgs a) {
 // 32 / 16) and units 2 (l / 32), 2 (l / 32) + 1 of the step's four, and ends with
 // columns 16 (l / 32) + 32 (j % 2) + 8 a + 4 (j / 2) + i of its 64 in element 4 j + i
 // of tile a: two runs of 16.  x lies in rows of 64 bytes, unit u at u ^ (row / 4 %
-// 4): the reads of a unit of 16 rows hit every bank once.
+// 4): the reads of a unit of 16 rows hit every bank once.  8192 x 28672 x 4096: 790
+// us, 658 without y's stores; the card's clock is 1.7 GHz under it and the matrix
+// cores are busy 68 % of that.  (Workgroups that stay for several tiles, with the next
+// tile's first stages ahead of the stores, took as long.)
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 __device__ __forceinline__ rsrc_t buffer_of(const uint8_t *p, uint32_t bytes) {
@@ -568,8 +571,10 @@ __global__ void __launch_bounds__(256) fp8_pack_kernel(const T *w, uint8_t *out,
     auto unit = [&](int u, T (&v)[16]) {
         if (vec && 16 * u + 16 <= k) {
 #pragma unroll
-            for (int j = 0; j < (int)sizeof(T); ++j)
-                reinterpret_cast<u32x4 *>(v)[j] = reinterpret_cast<const u32x4 *>(from + 16 * u)[j];
+            for (int j = 0; j < (int)sizeof(T); ++j) {
+                const u32x4 piece = reinterpret_cast<const u32x4 *>(from + 16 * u)[j];
+                __builtin_memcpy(reinterpret_cast<char *>(v) + 16 * j, &piece, 16);
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = 16 * u + j < k ? from[16 * u + j] : T(0);
@@ -603,7 +608,7 @@ __global__ void __launch_bounds__(256) fp8_pack_kernel(const T *w, uint8_t *out,
         unit(u, v);
         u32x4 q;
         if constexpr (kReady) {
-            q = *reinterpret_cast<const u32x4 *>(v);
+            __builtin_memcpy(&q, v, 16);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)

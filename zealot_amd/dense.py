@@ -480,6 +480,8 @@ def linear_fp8_workspace_bytes(m: int, n: int, k: int, out_dtype=torch.bfloat16)
 def linear_fp8(x: Fp8Rows, weight: Fp8Weight, out=None, out_dtype=torch.bfloat16, workspace=None, stream=None):
     """x . weight^T for rows and a weight in 8 bits (zk_linear_fp8): y [m, n],
     bfloat16 or float32 (`out_dtype`, or out's own).  k % 16 == 0."""
+    if not isinstance(x, Fp8Rows):
+        raise TypeError("x must be Fp8Rows (rms_norm_fp8 and silu_mul_fp8 give them)")
     m, k = _dims(x.data, "x.data", "[m, k]")
     if not isinstance(weight, Fp8Weight):
         raise TypeError("weight must be an Fp8Weight (fp8_weight makes one)")

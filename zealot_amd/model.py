@@ -153,12 +153,12 @@ class LlamaAdapters:
     count: int
     layers: list
     scales: torch.Tensor | None = None  # float32 [count]; None: 1
+    in_8_bits: bool = False  # for a model of LlamaWeights.in_8_bits, whose gate and up rows do not alternate
 
     @staticmethod
     def random(cfg: LlamaConfig, count: int, rank: int, dtype=torch.bfloat16, device="cuda", seed: int = 0,
                in_8_bits: bool = False) -> "LlamaAdapters":
-        """N(0, 1/fan_in) a and b, for every projection (seeded); in_8_bits: for
-        a model of LlamaWeights.in_8_bits, whose gate and up rows do not alternate."""
+        """N(0, 1/fan_in) a and b, for every projection (seeded)."""
         g = torch.Generator(device=device).manual_seed(seed)
 
         def mat(n, k):
@@ -176,7 +176,7 @@ class LlamaAdapters:
         H, Hkv, D, hid, I = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.hidden_size, cfg.intermediate_size
         layers = [LayerAdapters(pair((H + 2 * Hkv) * D, hid, 3), pair(hid, H * D), gate_up(I, hid), pair(hid, I))
                   for _ in range(cfg.num_layers)]
-        return LlamaAdapters(count, layers, 0.5 + torch.rand((count,), generator=g, device=device))
+        return LlamaAdapters(count, layers, 0.5 + torch.rand((count,), generator=g, device=device), in_8_bits)
 
 
 class HipModelRunner:
@@ -193,17 +193,18 @@ class HipModelRunner:
             self.rope = dense.rope_table(cfg.max_positions, cfg.head_dim, cfg.rope_theta, weights.embedding.device)
         if cfg.qk_norm and any(lw.q_norm is None or lw.k_norm is None for lw in weights.layers):
             raise ValueError("a model with qk_norm needs the layers' q_norm and k_norm")
-        if adapters is not None and len(adapters.layers) != len(weights.layers):
-            raise ValueError("adapters must have the model's layers")
-        self.adapters = adapters
         self.in_8_bits = isinstance(weights.layers[0].gate_up, dense.Fp8Weight)
+        if adapters is not None and (len(adapters.layers) != len(weights.layers) or adapters.in_8_bits != self.in_8_bits):
+            raise ValueError("adapters must have the model's layers, and gate and up rows in its order (in_8_bits)")
+        self.adapters = adapters
 
     def drop_state(self, request_id: str) -> None:
         self.kv.drop_state(request_id)
 
     def step(self, out, adapters: dict | None = None) -> torch.Tensor:
         """One step over ScheduleOutput `out` (zealot_amd.scheduler); adapters:
-        the adapter of each request id that brings one, the same at all its steps."""
+        the adapter of each request id that brings one (others: none, or None), the
+        same at all its steps."""
         per_row = self._adapter_rows(out, adapters)
         plan = self.kv.begin_step(out)
         if not out.batch:
@@ -221,7 +222,8 @@ class HipModelRunner:
 
     def _adapter_rows(self, out, adapters: dict | None):
         """The adapter of every step row (-1: none), or None where no row has one."""
-        mine = {e.request_id: adapters[e.request_id] for e in out.batch if e.request_id in adapters} if adapters else {}
+        ids = [e.request_id for e in out.batch] if adapters else []
+        mine = {rid: adapters[rid] for rid in ids if adapters.get(rid) is not None}
         if not mine:
             return None
         if self.adapters is None:
