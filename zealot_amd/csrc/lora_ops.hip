@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "zk_common.h"
 
@@ -176,8 +177,8 @@ struct LoraArgs {
 };
 
 // E values of a row from column c on, as the matrix instruction's operand (16
-// bytes of T), zeros from `cols` on: whole where WHOLE says that rows are aligned
-// and E divides their length, else one by one.  No branch around a load (it would
+// bytes of T), zeros from `cols` on: one by one (`take`), or whole (`piece`) where
+// rows are aligned and E divides their length.  No branch around a load (it would
 // be waited for before the next): what lies behind the row is read at its end and
 // not used.
 template <typename T> struct Operand;
@@ -196,49 +197,56 @@ template <> struct Operand<float> {
         return c;
     }
 };
-template <bool WHOLE>
 __device__ __forceinline__ u32x4 take(const uint16_t *row, int c, int cols) {
     u32x4 w = {0, 0, 0, 0};
-    if (WHOLE) {
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(row + min(c, cols - 8));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = c < cols ? v[i] : 0;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            w[i / 2] |= (c + i < cols ? (uint32_t)row[min(c + i, cols - 1)] : 0u) << (16 * (i & 1));
-    }
+    for (int i = 0; i < 8; ++i) w[i / 2] |= (c + i < cols ? (uint32_t)row[min(c + i, cols - 1)] : 0u) << (16 * (i & 1));
     return w;
 }
-template <bool WHOLE>
 __device__ __forceinline__ u32x4 take(const float *row, int c, int cols) {
     u32x4 w = {0, 0, 0, 0};
-    if (WHOLE) {
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(row + min(c, cols - 4));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = c < cols ? v[i] : 0;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = c + i < cols ? __float_as_uint(row[min(c + i, cols - 1)]) : 0u;
-    }
+    for (int i = 0; i < 4; ++i) w[i] = c + i < cols ? __float_as_uint(row[min(c + i, cols - 1)]) : 0u;
     return w;
 }
 // eight e4m3 values as bf16 (exact)
-template <bool WHOLE>
+__device__ __forceinline__ u32x4 operand(const u32x4 &v) { return v; }
+__device__ __forceinline__ u32x4 operand(const u32x2 &v) {
+    const u32x2 lo = e4m3x4_to_bf16x4(v[0]), hi = e4m3x4_to_bf16x4(v[1]);
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
 __device__ __forceinline__ u32x4 take(const uint8_t *row, int c, int cols) {
     u32x2 q = {0, 0};
-    if (WHOLE) {
-        const u32x2 v = *reinterpret_cast<const u32x2 *>(row + min(c, cols - 8));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) q[i] = c < cols ? v[i] : 0;
-    } else {
+    for (int i = 0; i < 8; ++i) q[i / 4] |= (c + i < cols ? (uint32_t)row[min(c + i, cols - 1)] : 0u) << (8 * (i & 3));
+    return operand(q);
+}
+// As they are in memory, for `operand`.  Four lanes of a row ask for 64 bytes of it, half a line, and an
+// instruction for halves of 16 lines; so two steps are loaded together, lanes r and r +
+// 8 taking the line's pieces of row r in the first and of row r + 8 in the second, and
+// change places after (swap8).  Any order of k does as long as A and x share it.
+// (8192 x 4096 of rank 32: 21.5 us, 26 with half lines; 32768 rows 79, 93.)
+template <typename X> struct RawOf { typedef u32x4 type; };
+template <> struct RawOf<uint8_t> { typedef u32x2 type; };
+template <typename X>
+__device__ __forceinline__ typename RawOf<X>::type piece(const X *row, int c, int cols) {
+    typedef typename RawOf<X>::type Raw;
+    constexpr int E = sizeof(Raw) / sizeof(X), N = sizeof(Raw) / 4;
+    Raw v = *reinterpret_cast<const Raw *>(row + min(c, cols - E));
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            q[i / 4] |= (c + i < cols ? (uint32_t)row[min(c + i, cols - 1)] : 0u) << (8 * (i & 3));
+    for (int i = 0; i < N; ++i) v[i] = c < cols ? v[i] : 0;
+    return v;
+}
+// Lanes 8 .. 15 of u change places with lanes 0 .. 7 of v, in every row of 16 lanes.
+template <typename V>
+__device__ __forceinline__ void swap8(V &u, V &v) {
+    constexpr int kRotate8 = 0x128;  // row_ror:8
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(V) / 4); ++i) {
+        const uint32_t a = u[i], b = v[i];
+        u[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)a, (int)b, kRotate8, 0xf, 0xc, false);
+        v[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)b, (int)a, kRotate8, 0xf, 0x3, false);
     }
-    const u32x2 lo = e4m3x4_to_bf16x4(q[0]), hi = e4m3x4_to_bf16x4(q[1]);
-    return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
 // Rows of tile `i`: its adapter, first position and count (0: none).
@@ -254,8 +262,7 @@ __device__ __forceinline__ int tile_at(const LoraArgs &a, int i, int rows, int &
 // workgroup every W-th step of four matrix instructions of its stretch of k.
 template <typename X, typename T, int MT, int RT, int W, bool WHOLE>
 __global__ void __launch_bounds__(64 * W) lora_shrink_kernel(LoraArgs a) {
-    // (more under way a wave where registers allow it: 8192 x 4096 of rank 32 24 us with four)
-    constexpr int E = Operand<T>::E, U = !WHOLE ? 2 : MT == 2 && RT <= 2 ? 8 : 4, kStep = 4 * E * U;
+    constexpr int E = Operand<T>::E, U = WHOLE ? 4 : 2, kStep = 4 * E * U;
     __shared__ f32x4 sums[W][RT * MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
@@ -263,41 +270,66 @@ __global__ void __launch_bounds__(64 * W) lora_shrink_kernel(LoraArgs a) {
     const int count = tile_at(a, blockIdx.x, 16 * MT, adapter, p0);
     if (count == 0) return;
     const int i0 = blockIdx.y * RT * 16, split = blockIdx.z;
-    const X *xr[MT];
+    // rows of x and of A: two for a lane's pieces of two steps, or its own
+    constexpr int P = WHOLE ? 2 : 1;
+    const int r8 = WHOLE ? r16 & 7 : r16;
+    const X *xr[MT][P];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int row = a.order[p0 + min(16 * m + r16, count - 1)];
-        xr[m] = (const X *)a.x + (size_t)min((unsigned)row, (unsigned)a.rows - 1) * a.x_stride;
-    }
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < P; ++h) {
+            const int row = a.order[p0 + min(16 * m + 8 * h + r8, count - 1)];
+            xr[m][h] = (const X *)a.x + (size_t)min((unsigned)row, (unsigned)a.rows - 1) * a.x_stride;
+        }
     // row i of v's values: rank i % part_stride of part i / part_stride (what is behind a part's ranks is not kept)
-    const T *ar[RT];
+    const T *ar[RT][P];
 #pragma unroll
-    for (int f = 0; f < RT; ++f) {
-        const int i = min(i0 + 16 * f + r16, a.parts * a.part_stride - 1), part = i / a.part_stride;
-        ar[f] = (const T *)a.a + ((size_t)adapter * a.parts * a.rank + part * a.rank + min(i - part * a.part_stride, a.rank - 1)) * a.k;
-    }
+    for (int f = 0; f < RT; ++f)
+#pragma unroll
+        for (int h = 0; h < P; ++h) {
+            const int i = min(i0 + 16 * f + 8 * h + r8, a.parts * a.part_stride - 1);
+            const int part = (i >= a.part_stride) + (i >= 2 * a.part_stride) + (i >= 3 * a.part_stride);  // (of at most 4)
+            ar[f][h] = (const T *)a.a + ((size_t)adapter * a.parts * a.rank + part * a.rank + min(i - part * a.part_stride, a.rank - 1)) * a.k;
+        }
     f32x4 acc[RT][MT];
 #pragma unroll
     for (int f = 0; f < RT; ++f)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int c = (split * W + wave) * kStep; c < a.k; c += a.splits * W * kStep) {
-        u32x4 av[U][RT], xv[U][MT];
+        typedef typename RawOf<X>::type Raw;
+        u32x4 av[U][RT];
+        std::conditional_t<WHOLE, Raw, u32x4> xv[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int at = c + 4 * E * u + E * g;
+            if constexpr (WHOLE) {
+                const int at = c + 4 * E * (u & ~1) + E * (2 * g + (r16 >> 3));
 #pragma unroll
-            for (int f = 0; f < RT; ++f) av[u][f] = take<WHOLE>(ar[f], at, a.k);
+                for (int f = 0; f < RT; ++f) av[u][f] = piece(ar[f][u & 1], at, a.k);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) xv[u][m] = take<WHOLE>(xr[m], at, a.k);
+                for (int m = 0; m < MT; ++m) xv[u][m] = piece(xr[m][u & 1], at, a.k);
+            } else {
+                const int at = c + 4 * E * u + E * g;
+#pragma unroll
+                for (int f = 0; f < RT; ++f) av[u][f] = take(ar[f][0], at, a.k);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) xv[u][m] = take(xr[m][0], at, a.k);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);  // (every load before the first product)
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            if (WHOLE && u % 2 == 0) {
+#pragma unroll
+                for (int f = 0; f < RT; ++f) swap8(av[u][f], av[u + 1][f]);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) swap8(xv[u][m], xv[u + 1][m]);
+            }
 #pragma unroll
             for (int f = 0; f < RT; ++f)
 #pragma unroll
-                for (int m = 0; m < MT; ++m) acc[f][m] = Operand<T>::mfma(av[u][f], xv[u][m], acc[f][m]);
+                for (int m = 0; m < MT; ++m) acc[f][m] = Operand<T>::mfma(av[u][f], operand(xv[u][m]), acc[f][m]);
+        }
     }
 #pragma unroll
     for (int f = 0; f < RT; ++f)
@@ -373,10 +405,15 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
     if (count == 0) return;
     const int steps = (a.rank + kStep - 1) / kStep;
     const int begin = blockIdx.x % a.groups * a.blocks * 256, end = min(begin + a.blocks * 256, a.n);
-    // rows of y (from a.rows on: none)
-    unsigned row[MT];
+    // rows of y (from a.rows on: none), a lane's own and those whose lines it asks for
+    unsigned row[MT], line_row[MT][2];
+    const int r8 = r16 & 7, half = r16 >> 3;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) row[m] = 16 * m + r16 < count ? (unsigned)a.order[p0 + 16 * m + r16] : ~0u;
+    for (int m = 0; m < MT; ++m) {
+        row[m] = 16 * m + r16 < count ? (unsigned)a.order[p0 + 16 * m + r16] : ~0u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) line_row[m][h] = 16 * m + 8 * h + r8 < count ? (unsigned)a.order[p0 + 16 * m + 8 * h + r8] : ~0u;
+    }
     // values: rows of `line` 16-byte units, one spare against bank conflicts
     int part0 = 0, part1 = a.parts - 1;
     if (!a.part_block) {
@@ -413,23 +450,46 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
             Values<T>::split(v, o[m]);
         }
     };
-    // columns n1 = n0 + 32 q + 8 g .. + 7 of row r16 of each group, whole pieces.  (No branch around a load: lanes that have
-    // none read another.)
+    // Columns n1 = n0 + 32 q + 8 g .. + 7 of row r16 of each group, whole pieces.  (No branch around a load: lanes that have
+    // none read another.)  bf16: of 64 columns that y has, eight lanes ask for a row's line and give it back, as the shrink's
+    // do; between, a lane has its row's pieces (32768 x 4096 of rank 32: 102 us, 110 with half lines).
     typedef u32x4 Pieces[MT][2][H == 2 ? 1 : 2];
     const bool pieces = a.y_whole && a.n >= 8;
     const unsigned any = (unsigned)min((unsigned)a.order[p0], (unsigned)a.rows - 1);
+    auto lines = [&](int n0) { return H == 2 && pieces && n0 + 64 <= a.n; };
     auto ask = [&](int n0, Pieces &had) {
         if (!pieces) return;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const T *y = (const T *)a.y + (size_t)(row[m] < (unsigned)a.rows ? row[m] : any) * a.y_stride + min(n0 + 32 * q + 8 * g, (a.n - 8) & ~7);
+                const unsigned r = lines(n0) ? line_row[m][q] : row[m];
+                const int n1 = lines(n0) ? n0 + 8 * g + 32 * half : min(n0 + 32 * q + 8 * g, (a.n - 8) & ~7);
+                const T *y = (const T *)a.y + (size_t)(r < (unsigned)a.rows ? r : any) * a.y_stride + n1;
 #pragma unroll
                 for (int i = 0; i < (H == 2 ? 1 : 2); ++i) had[m][q][i] = reinterpret_cast<const u32x4 *>(y)[i];
             }
     };
-    auto give = [&](int n0, const Pieces &had, const f32x4 (&acc)[4][MT]) {
+    auto give = [&](int n0, Pieces &had, const f32x4 (&acc)[4][MT]) {
+        auto d = [&](int m, int q, int i) { return acc[2 * q + i / 4][m][i % 4]; };
+        auto add = [&](u32x4 &w, int m, int q) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = two(bf16lo(w[i]) + d(m, q, 2 * i), bf16hi(w[i]) + d(m, q, 2 * i + 1));
+        };
+        if (lines(n0)) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                swap8(had[m][0][0], had[m][1][0]);
+                add(had[m][0][0], m, 0);
+                add(had[m][1][0], m, 1);
+                swap8(had[m][0][0], had[m][1][0]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (line_row[m][h] < (unsigned)a.rows)
+                        *reinterpret_cast<u32x4 *>((T *)a.y + (size_t)line_row[m][h] * a.y_stride + n0 + 8 * g + 32 * half) = had[m][h][0];
+            }
+            return;
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             if (row[m] >= (unsigned)a.rows) continue;
@@ -437,22 +497,17 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
             for (int q = 0; q < 2; ++q) {
                 const int n1 = n0 + 32 * q + 8 * g;
                 T *y = (T *)a.y + (size_t)row[m] * a.y_stride + n1;
-                float d[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = acc[2 * q + i / 4][m][i % 4];
                 if (n1 + 8 <= a.n && pieces) {
                     u32x4 *yw = reinterpret_cast<u32x4 *>(y);
                     if constexpr (H == 2) {
-                        u32x4 w = had[m][q][0];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = two(bf16lo(w[i]) + d[2 * i], bf16hi(w[i]) + d[2 * i + 1]);
-                        yw[0] = w;
+                        add(had[m][q][0], m, q);
+                        yw[0] = had[m][q][0];
                     } else {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             u32x4 w = had[m][q][i];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) + d[4 * i + e]);
+                            for (int e = 0; e < 4; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) + d(m, q, 4 * i + e));
                             yw[i] = w;
                         }
                     }
@@ -460,8 +515,8 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         if (n1 + i < a.n) {
-                            if constexpr (H == 2) y[i] = (T)two(__uint_as_float((uint32_t)y[i] << 16) + d[i], 0.0f);
-                            else y[i] += d[i];
+                            if constexpr (H == 2) y[i] = (T)two(__uint_as_float((uint32_t)y[i] << 16) + d(m, q, i), 0.0f);
+                            else y[i] += d(m, q, i);
                         }
                 }
             }
@@ -486,7 +541,10 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
             for (int s = 0; s < steps; ++s) {
                 u32x4 bv[4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) bv[t] = take<WHOLE>(bb[t], s * kStep + E * g, a.rank);
+                for (int t = 0; t < 4; ++t) {
+                    if constexpr (WHOLE) bv[t] = piece(bb[t], s * kStep + E * g, a.rank);
+                    else bv[t] = take(bb[t], s * kStep + E * g, a.rank);
+                }
                 if (steps > 1 || kept_part != p) {
                     values(p, s, kept);
                     kept_part = p;
