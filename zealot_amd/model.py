@@ -193,7 +193,7 @@ class HipModelRunner:
             self.rope = dense.rope_table(cfg.max_positions, cfg.head_dim, cfg.rope_theta, weights.embedding.device)
         if cfg.qk_norm and any(lw.q_norm is None or lw.k_norm is None for lw in weights.layers):
             raise ValueError("a model with qk_norm needs the layers' q_norm and k_norm")
-        self.in_8_bits = isinstance(weights.layers[0].gate_up, dense.Fp8Weight)
+        self.in_8_bits = any(isinstance(lw.gate_up, dense.Fp8Weight) for lw in weights.layers)
         if adapters is not None and (len(adapters.layers) != len(weights.layers) or adapters.in_8_bits != self.in_8_bits):
             raise ValueError("adapters must have the model's layers, and gate and up rows in its order (in_8_bits)")
         self.adapters = adapters
@@ -283,6 +283,8 @@ class HipModelRunner:
         cfg, w = self.cfg, self.w
         if ids.numel() != plan.total_tokens:
             raise ValueError("one token id per step row")
+        if lora is not None and self.adapters is None:
+            raise ValueError("the runner has no adapters")
         if lora is not None or self.in_8_bits:
             return self._forward_apart(plan, ids, last_rows, lora)
         H, Hkv, D = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
