@@ -109,29 +109,32 @@ __device__ __forceinline__ void column_scales(const GemmArgs &a, int n0, float (
         for (int i = 0; i < N; ++i) ws[i] = a.ws[min(n0 + i, a.n - 1)];
     }
 }
-// y[row, n0 .. n0 + N) = v * xs * ws, N a multiple of 4; y's rows are 16-byte aligned
-// where n allows it
+// pieces of y's rows, which lie at their elements' alignment only where n is no multiple of 8
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+typedef u32x2 __attribute__((aligned(2))) u32x2_any;
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+// y[row, n0 .. n0 + N) = v * xs * ws, N a multiple of 4
 template <bool F32, int N>
 __device__ __forceinline__ void store_row(const GemmArgs &a, int row, int n0, const float (&v)[N], const float (&ws)[N], float xs) {
     float o[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = v[i] * xs * ws[i];
     const size_t at = (size_t)row * a.n + n0;
-    if (n0 + N <= a.n && a.n % 8 == 0) {
+    if (n0 + N <= a.n) {
         if constexpr (F32) {
 #pragma unroll
             for (int i = 0; i < N; i += 4)
-                *reinterpret_cast<f32x4 *>((float *)a.y + at + i) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+                *reinterpret_cast<f32x4_any *>((float *)a.y + at + i) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
         } else if constexpr (N % 8 == 0) {
 #pragma unroll
             for (int i = 0; i < N; i += 8)
-                *reinterpret_cast<u32x4 *>((uint16_t *)a.y + at + i) =
+                *reinterpret_cast<u32x4_any *>((uint16_t *)a.y + at + i) =
                     u32x4{two(o[i], o[i + 1]), two(o[i + 2], o[i + 3]), two(o[i + 4], o[i + 5]),
                           two(o[i + 6], o[i + 7])};
         } else {
 #pragma unroll
             for (int i = 0; i < N; i += 4)
-                *reinterpret_cast<u32x2 *>((uint16_t *)a.y + at + i) = u32x2{two(o[i], o[i + 1]), two(o[i + 2], o[i + 3])};
+                *reinterpret_cast<u32x2_any *>((uint16_t *)a.y + at + i) = u32x2{two(o[i], o[i + 1]), two(o[i + 2], o[i + 3])};
         }
     } else {
 #pragma unroll
