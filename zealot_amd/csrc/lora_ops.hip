@@ -175,12 +175,11 @@ struct LoraArgs {
     int64_t y_stride;
     int rows, adapters, k, n, rank, parts, part_stride, v_stride, splits, blocks, groups;  // blocks: of 64 columns a wave; groups: of workgroups' columns
     int part_end[kMaxParts], part_block;
-    int y_whole;  // 16-byte pieces of y are aligned
 };
 
 // E values of a row from column c on, as the matrix instruction's operand (16
 // bytes of T), zeros from `cols` on: one by one (`take`), or whole (`piece`) where
-// rows are aligned and E divides their length.  No branch around a load (it would
+// E divides the row's length.  No branch around a load (it would
 // be waited for before the next): what lies behind the row is read at its end and
 // not used.
 template <typename T> struct Operand;
@@ -228,13 +227,25 @@ __device__ __forceinline__ u32x4 take(const uint8_t *row, int c, int cols) {
 // 8 taking the line's pieces of row r in the first and of row r + 8 in the second, and
 // change places after (swap8).  Any order of k does as long as A and x share it.
 // (8192 x 4096 of rank 32: 21.5 us, 26 with half lines; 32768 rows 79, 93.)
-template <typename X> struct RawOf { typedef u32x4 type; };
-template <> struct RawOf<uint8_t> { typedef u32x2 type; };
+// (Any: at the elements' own alignment, in one instruction all the same.)
+template <typename X> struct RawOf;
+template <> struct RawOf<uint16_t> {
+    typedef u32x4 type;
+    typedef u32x4 __attribute__((aligned(2))) Any;
+};
+template <> struct RawOf<float> {
+    typedef u32x4 type;
+    typedef u32x4 __attribute__((aligned(4))) Any;
+};
+template <> struct RawOf<uint8_t> {
+    typedef u32x2 type;
+    typedef u32x2 __attribute__((aligned(1))) Any;
+};
 template <typename X>
 __device__ __forceinline__ typename RawOf<X>::type piece(const X *row, int c, int cols) {
     typedef typename RawOf<X>::type Raw;
     constexpr int E = sizeof(Raw) / sizeof(X), N = sizeof(Raw) / 4;
-    Raw v = *reinterpret_cast<const Raw *>(row + min(c, cols - E));
+    Raw v = *reinterpret_cast<const typename RawOf<X>::Any *>(row + min(c, cols - E));
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = c < cols ? v[i] : 0;
     return v;
@@ -457,7 +468,8 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
     // none read another.)  bf16: of 64 columns that y has, eight lanes ask for a row's line and give it back, as the shrink's
     // do; between, a lane has its row's pieces (32768 x 4096 of rank 32: 102 us, 110 with half lines).
     typedef u32x4 Pieces[MT][2][H == 2 ? 1 : 2];
-    const bool pieces = a.y_whole && a.n >= 8;
+    typedef typename RawOf<T>::Any Any;
+    const bool pieces = a.n >= 8;
     const unsigned any = (unsigned)min((unsigned)a.order[p0], (unsigned)a.rows - 1);
     auto lines = [&](int n0) { return H == 2 && pieces && n0 + 64 <= a.n; };
     auto ask = [&](int n0, Pieces &had) {
@@ -470,7 +482,7 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
                 const int n1 = lines(n0) ? n0 + 8 * g + 32 * half : min(n0 + 32 * q + 8 * g, (a.n - 8) & ~7);
                 const T *y = (const T *)a.y + (size_t)(r < (unsigned)a.rows ? r : any) * a.y_stride + n1;
 #pragma unroll
-                for (int i = 0; i < (H == 2 ? 1 : 2); ++i) had[m][q][i] = reinterpret_cast<const u32x4 *>(y)[i];
+                for (int i = 0; i < (H == 2 ? 1 : 2); ++i) had[m][q][i] = reinterpret_cast<const Any *>(y)[i];
             }
     };
     auto give = [&](int n0, Pieces &had, const f32x4 (&acc)[4][MT]) {
@@ -489,7 +501,7 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
                     if (line_row[m][h] < (unsigned)a.rows)
-                        *reinterpret_cast<u32x4 *>((T *)a.y + (size_t)line_row[m][h] * a.y_stride + n0 + 8 * g + 32 * half) = had[m][h][0];
+                        *reinterpret_cast<Any *>((T *)a.y + (size_t)line_row[m][h] * a.y_stride + n0 + 8 * g + 32 * half) = had[m][h][0];
             }
             return;
         }
@@ -501,7 +513,7 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
                 const int n1 = n0 + 32 * q + 8 * g;
                 T *y = (T *)a.y + (size_t)row[m] * a.y_stride + n1;
                 if (n1 + 8 <= a.n && pieces) {
-                    u32x4 *yw = reinterpret_cast<u32x4 *>(y);
+                    Any *yw = reinterpret_cast<Any *>(y);
                     if constexpr (H == 2) {
                         add(had[m][q][0], m, q);
                         yw[0] = had[m][q][0];
@@ -624,8 +636,7 @@ void shrink(const LoraArgs &a, int tiles, bool whole, hipStream_t s) {
 template <typename T, int MT>
 void expand(LoraArgs a, int tiles, hipStream_t s) {
     constexpr int E = Operand<T>::E;
-    const bool whole = a.rank % E == 0 && aligned(a.b, 16);
-    a.y_whole = a.y_stride % E == 0 && aligned(a.y, 16);
+    const bool whole = a.rank % E == 0;
     bool one = a.part_block % 64 == 0;
     for (int i = 0; i < a.parts - 1 && !a.part_block; ++i) one = one && a.part_end[i] % 64 == 0;
     // Blocks of 64 columns a wave: values are summed and split once for them, as long as
@@ -646,7 +657,7 @@ void expand(LoraArgs a, int tiles, hipStream_t s) {
 template <typename X, typename T>
 void both(const LoraArgs &a, int tiles, hipStream_t s) {
     constexpr int E = Operand<T>::E;
-    const bool whole = a.k % E == 0 && a.x_stride % E == 0 && aligned(a.x, E * (int)sizeof(X)) && aligned(a.a, 16);
+    const bool whole = a.k % E == 0;
     if (tile_rows_for(a.rows) == 16) {
         shrink<X, T, 1>(a, tiles, whole, s);
         expand<T, 1>(a, tiles, s);
