@@ -189,7 +189,8 @@ int zk_linear_pin_split(int64_t m, int64_t n, int64_t k, zk_dtype in_dtype, zk_d
  * [num_rows], NULL: all, x_rows == num_rows) selects rows of x [x_rows, dim] and
  * of the residual; one outside [0, x_rows) gives zeros.  residual_out may be x
  * or the residual itself when rows is NULL; outputs overlap nothing else.
- * dim <= 32768 (bf16) / 16384 (f32) for 16-byte rows, <= 4096 otherwise. */
+ * dim <= 32768 (bf16) / 16384 (f32) where it is a multiple of 8 / 4, <= 4096
+ * otherwise. */
 int zk_rms_norm_fp8(const void *x, const void *residual, const void *weight, void *q, float *scales,
                     void *residual_out, const int64_t *rows, int64_t x_rows, int64_t num_rows, int64_t dim, float eps,
                     zk_dtype dtype, void *stream);

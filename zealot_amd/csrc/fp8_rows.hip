@@ -45,10 +45,11 @@ struct RowArgs {
     float eps;
 };
 
-// What a thread loads at once: VEC values, as they are in memory.
-template <typename T, int VEC> struct Raw { T v; };
-template <> struct Raw<float, 4> { f32x4 v; };
-template <> struct Raw<uint16_t, 8> { u32x4 v; };
+// What a thread loads at once: VEC values, as they are in memory, at their own
+// alignment (one instruction all the same).
+template <typename T, int VEC> struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v; };
+template <> struct __attribute__((packed, aligned(4))) Raw<float, 4> { f32x4 v; };
+template <> struct __attribute__((packed, aligned(2))) Raw<uint16_t, 8> { u32x4 v; };
 
 template <typename T, int VEC>
 __device__ __forceinline__ Raw<T, VEC> load(const T *p) { return *reinterpret_cast<const Raw<T, VEC> *>(p); }
@@ -76,14 +77,16 @@ __device__ __forceinline__ Raw<uint16_t, 1> rounded(const float (&v)[1], uint16_
 __device__ __forceinline__ Raw<uint16_t, 8> rounded(const float (&v)[8], uint16_t) {
     return {u32x4{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])}};
 }
+typedef uint32_t __attribute__((aligned(1))) u32_any;
+typedef u32x2 __attribute__((aligned(1))) u32x2_any;
 template <int VEC>
 __device__ __forceinline__ void store_q(uint8_t *p, const float (&v)[VEC]) {
     if constexpr (VEC == 1) {
         *p = (uint8_t)e4m3x4(v[0], 0.f, 0.f, 0.f);
     } else if constexpr (VEC == 4) {
-        *reinterpret_cast<uint32_t *>(p) = e4m3x4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<u32_any *>(p) = e4m3x4(v[0], v[1], v[2], v[3]);
     } else {
-        *reinterpret_cast<u32x2 *>(p) = u32x2{e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7])};
+        *reinterpret_cast<u32x2_any *>(p) = u32x2{e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7])};
     }
 }
 // g / (1 + exp(-g)) with the machine's exp2 and reciprocal: off by 2^-24 |g| log2(e)
@@ -204,14 +207,12 @@ __global__ void __launch_bounds__(64 * W * R) fp8_rows_kernel(RowArgs a) {
     }
 }
 
-bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
-
 // Waves a row: a wave for short rows, four rows a workgroup (32768 rows of 1024,
 // two vectors a thread 43 us, a workgroup a row 51).  Longer rows of the norm take two to four
 // vectors a thread (8192 rows of 16384: eight 163 us, four 160, two 164; 32768 of
 // 4096: two 158, one 160), SiLU, whose threads compute more between two loads, as few
 // as 16 waves allow (8192 of 14336: eight 110, four 109, two 100; 16384 of 4096: two
-// 60.5, one 57.7).  Rows off their alignment go value by value: eight a thread
+// 60.5, one 57.7).  Rows that are no whole vectors go value by value: eight a thread
 // (8192 of 2001: 31 us, four 36, two 49).
 template <bool NORM, typename T, int VEC>
 bool launch_vec(const RowArgs &a, hipStream_t s) {
@@ -245,9 +246,7 @@ bool launch_vec(const RowArgs &a, hipStream_t s) {
 
 template <bool NORM>
 int launch(const RowArgs &a, zk_dtype dtype, const char *name, hipStream_t s) {
-    const int V = dtype == ZK_BF16 ? 8 : 4;
-    const bool vec = a.dim % V == 0 && a.x_stride % V == 0 && a.other_stride % V == 0 && aligned(a.x, 16) &&
-                     aligned(a.other, 16) && aligned(a.weight, 16) && aligned(a.sum_out, 16) && aligned(a.q, V);
+    const bool vec = a.dim % (dtype == ZK_BF16 ? 8 : 4) == 0;
     bool ok;
     if (dtype == ZK_BF16)
         ok = vec ? launch_vec<NORM, uint16_t, 8>(a, s) : launch_vec<NORM, uint16_t, 1>(a, s);
@@ -256,7 +255,7 @@ int launch(const RowArgs &a, zk_dtype dtype, const char *name, hipStream_t s) {
     if (!ok)
         return set_error(ZK_ERR_INVALID_ARGUMENT,
                          std::string("Internal error: ") + name + ": rows of " + std::to_string(a.dim) +
-                             " too long (at most 32768 bf16 / 16384 f32 elements with 16-byte rows, 4096 otherwise)");
+                             " too long (at most 32768 bf16 / 16384 f32 elements in whole vectors of 16 bytes, 4096 otherwise)");
     if (hipError_t e = hipGetLastError(); e != hipSuccess)
         return set_error(ZK_ERR_HIP, std::string("Internal error: ") + name + ": " + hipGetErrorString(e));
     return ZK_OK;
