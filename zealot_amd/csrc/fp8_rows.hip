@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "zk_common.h"
 
@@ -79,14 +80,16 @@ __device__ __forceinline__ Raw<uint16_t, 8> rounded(const float (&v)[8], uint16_
 }
 typedef uint32_t __attribute__((aligned(1))) u32_any;
 typedef u32x2 __attribute__((aligned(1))) u32x2_any;
-template <int VEC>
+// (FINITE: every value is, and at most 448 before its rounding)
+template <bool FINITE, int VEC>
 __device__ __forceinline__ void store_q(uint8_t *p, const float (&v)[VEC]) {
+    auto four = [](float a, float b, float c, float d) { return FINITE ? e4m3x4_in_range(a, b, c, d) : e4m3x4(a, b, c, d); };
     if constexpr (VEC == 1) {
-        *p = (uint8_t)e4m3x4(v[0], 0.f, 0.f, 0.f);
+        *p = (uint8_t)four(v[0], 0.f, 0.f, 0.f);
     } else if constexpr (VEC == 4) {
-        *reinterpret_cast<u32_any *>(p) = e4m3x4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<u32_any *>(p) = four(v[0], v[1], v[2], v[3]);
     } else {
-        *reinterpret_cast<u32x2_any *>(p) = u32x2{e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7])};
+        *reinterpret_cast<u32x2_any *>(p) = u32x2{four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7])};
     }
 }
 // g / (1 + exp(-g)) with the machine's exp2 and reciprocal: off by 2^-24 |g| log2(e)
@@ -195,16 +198,25 @@ __global__ void __launch_bounds__(64 * W * R) fp8_rows_kernel(RowArgs a) {
     const float s = most < kLeast ? kLeast : most;  // (NaN stays)
     const float r = 1.0f / s;
     if (t == 0) a.scales[row] = s;
+    auto write = [&](auto finite) {
+        constexpr bool kFinite = decltype(finite)::value;
 #pragma unroll
-    for (int j = 0; j < MAXV; ++j) {
-        const int i = (j * THREADS + t) * VEC;
-        if (i < a.dim) {
-            float y[VEC];
+        for (int j = 0; j < MAXV; ++j) {
+            const int i = (j * THREADS + t) * VEC;
+            if (i < a.dim) {
+                float q[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) y[e] = NORM ? v[j][e] * inv * r : v[j][e] * r;
-            store_q<VEC>(a.q + (size_t)row * a.dim + i, y);
+                for (int e = 0; e < VEC; ++e) {
+                    const float y = NORM ? v[j][e] * inv : v[j][e];
+                    q[e] = kFinite ? quotient(y, s, r) : y * r;
+                }
+                store_q<kFinite>(a.q + (size_t)row * a.dim + i, q);
+            }
         }
-    }
+    };
+    // A row whose scale is infinite or NaN (the same over the row) has no quotients to round: NaN, and zeros beside an infinity.
+    if (__builtin_amdgcn_readfirstlane(__float_as_uint(s)) < 0x7f800000u) write(std::true_type{});
+    else write(std::false_type{});
 }
 
 // Waves a row: a wave for short rows, four rows a workgroup (32768 rows of 1024,

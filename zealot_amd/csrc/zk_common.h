@@ -305,6 +305,19 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     }
     return r;
 }
+// y / s to nearest for finite y and finite normal s, r = 1 / s to nearest: the product y r
+// and one step on its exact remainder (Markstein, IBM J. Res. Dev. 34, 1990), which a
+// quotient that is representable meets exactly: y r alone is a step beside it for one in
+// three.  A zero keeps its sign.
+__device__ __forceinline__ float quotient(float y, float s, float r) {
+    const float q = y * r;
+    return fmaf(-fmaf(q, s, -y), r, q);
+}
+// Four finite f32 of magnitude < 464 (nearest to 448 at most) -> four e4m3 bytes.
+__device__ __forceinline__ uint32_t e4m3x4_in_range(float a, float b, float c, float d) {
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
 // Four e4m3 bytes -> four f32 (exact).
 __device__ __forceinline__ void e4m3x4_to_f32(uint32_t w, float *o) {
     f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
