@@ -1,8 +1,9 @@
-"""q = e4m3(y / scale), to nearest even, bit for bit: what dense.silu_mul_fp8 and
-rms_norm_fp8 write for rows y that they compute exactly.
+"""q = e4m3(y / scale), to nearest even, bit for bit: what dense.fp8_weight,
+silu_mul_fp8 and rms_norm_fp8 write for rows y that they compute exactly.
 
-SiLU(64) = 64 in f32 (exp(-64) is far below a step of 1), so up = y / 64; rows of 2s
-have the root 1 / 2 without an epsilon, so weight = y.  The rows hold every
+y is a power of two's worth of work away from the inputs in all three: a weight is
+y itself; SiLU(64) = 64 in f32 (exp(-64) is far below a step of 1), so up = y / 64;
+rows of 2s have the root 1 / 2 without an epsilon, so weight = y.  The rows hold every
 value halfway between two of e4m3, times scales whose reciprocal f32 does not
 have: y / scale is that halfway value and goes to the even neighbour, while y times
 a rounded reciprocal may lie on either side of it."""
@@ -44,6 +45,24 @@ def _rows_of(dtype):
     y = v[None, :] * s[:, None]
     assert torch.equal(y.to(dtype).float(), y) and torch.equal(y / s[:, None], v.expand_as(y))
     return y.to(dtype), _codes(v.expand_as(y)), s
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_weights(dtype):
+    from zealot_amd import dense
+    y, codes, s = _rows_of(dtype)
+    p = dense.fp8_weight(y.cuda())
+    _equal(dense.Fp8Rows(p.rowmajor(), p.scales), codes, s)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_any_weights(dtype):
+    """Rows of any values: the host's quotients (f32, to nearest), rounded."""
+    from zealot_amd import dense
+    y = torch.randn((4000, 500), generator=torch.Generator().manual_seed(1)).to(dtype)
+    s = y.float().abs().amax(1) / 448
+    p = dense.fp8_weight(y.cuda())
+    _equal(dense.Fp8Rows(p.rowmajor(), p.scales), _codes(y.float() / s[:, None]), s)
 
 
 @pytest.mark.parametrize("cols", [256, 255])

@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(256) fp8_pack_kernel(const T *w, uint8_t *out,
         if constexpr (sizeof(T) == 4) return v;
         else return __uint_as_float((uint32_t)v << 16);
     };
-    float r = 0.0f;
+    float s = 1.0f, r = 1.0f;
     if constexpr (!kReady) {
         uint32_t top = 0;  // as bits: NaN above infinity above the numbers
         for (int u = threadIdx.x >> 4; u < units; u += 16) {
@@ -601,7 +601,8 @@ __global__ void __launch_bounds__(256) fp8_pack_kernel(const T *w, uint8_t *out,
         if ((threadIdx.x & 63) < 16) red[threadIdx.x >> 6][i] = top;
         __syncthreads();
         top = max(max(red[0][i], red[1][i]), max(red[2][i], red[3][i]));
-        const float most = __uint_as_float(top) / 448.0f, s = most < 0x1p-126f ? 0x1p-126f : most;
+        const float most = __uint_as_float(top) / 448.0f;
+        s = most < 0x1p-126f ? 0x1p-126f : most;  // (NaN stays)
         if (threadIdx.x < 16 && real) scales[row] = s;
         r = 1.0f / s;
     }
@@ -612,7 +613,11 @@ __global__ void __launch_bounds__(256) fp8_pack_kernel(const T *w, uint8_t *out,
         u32x4 q;
         if constexpr (kReady) {
             __builtin_memcpy(&q, v, 16);
-        } else {
+        } else if (s < __builtin_inff()) {
+            auto over = [&](T y) { return quotient(f32_of(y), s, r); };
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[j] = e4m3x4_in_range(over(v[4 * j]), over(v[4 * j + 1]), over(v[4 * j + 2]), over(v[4 * j + 3]));
+        } else {  // no quotients: NaN, and zeros beside an infinity
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 q[j] = e4m3x4(f32_of(v[4 * j]) * r, f32_of(v[4 * j + 1]) * r, f32_of(v[4 * j + 2]) * r, f32_of(v[4 * j + 3]) * r);
