@@ -195,7 +195,8 @@ int zk_rms_norm_fp8(const void *x, const void *residual, const void *weight, voi
                     void *residual_out, const int64_t *rows, int64_t x_rows, int64_t num_rows, int64_t dim, float eps,
                     zk_dtype dtype, void *stream);
 /* zk_silu_mul (rows gate_stride / up_stride elements apart, 0 = cols) whose rows
- * are written in 8 bits.  cols as dim above. */
+ * are written in 8 bits; as there a gate below -88.72, whose exp(-g) is no f32,
+ * gives 0.  cols as dim above. */
 int zk_silu_mul_fp8(const void *gate, const void *up, void *q, float *scales, int64_t rows, int64_t cols,
                     int64_t gate_stride, int64_t up_stride, zk_dtype dtype, void *stream);
 /* A weight w [n, k] (nn.Linear layout) in 8 bits with one scale a row, packed
