@@ -344,6 +344,7 @@ class Fp8Rows(NamedTuple):
 
 
 _FP8 = torch.float8_e4m3fn
+FP8_LONGEST_ROW = 32768  # columns of bfloat16 rows that rms_norm_fp8 and silu_mul_fp8 write (whole vectors of 8)
 _CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 

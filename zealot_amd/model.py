@@ -85,6 +85,13 @@ class LayerWeights:
     k_norm: torch.Tensor | None = None
 
 
+def _check_8_bits(lw: LayerWeights) -> None:
+    """The rows that the layer's 8-bit projections read can be written."""
+    for what, k in (("hidden", lw.qkv.shape[1]), ("hidden", lw.gate_up.shape[1]), ("intermediate", lw.down.shape[1])):
+        if k % 16 or k > dense.FP8_LONGEST_ROW:
+            raise ValueError(f"8-bit projections need a {what} size that is a multiple of 16 up to {dense.FP8_LONGEST_ROW}, not {k}")
+
+
 @dataclass
 class LlamaWeights:
     embedding: torch.Tensor  # [vocab, hidden]
@@ -93,12 +100,16 @@ class LlamaWeights:
     lm_head: object           # [vocab, hidden] (a dense.TiledWeight for bf16 models)
 
     def in_8_bits(self) -> "LlamaWeights":
-        """The model with qkv, gate|up and down as dense.Fp8Weight (bf16 models):
-        gate|up holds the gate rows, then the up rows.  The rest is shared."""
+        """The model with qkv, gate|up and down as dense.Fp8Weight (bf16 models
+        whose hidden and intermediate sizes are multiples of 16 up to
+        dense.FP8_LONGEST_ROW): gate|up holds the gate rows, then the up rows.
+        The rest is shared."""
         if self.embedding.dtype != torch.bfloat16:
             raise TypeError("8-bit projections are for bf16 models")
         if any(isinstance(lw.gate_up, dense.Fp8Weight) for lw in self.layers):
             raise ValueError("the projections are in 8 bits already")
+        for lw in self.layers:
+            _check_8_bits(lw)
 
         def full(t):
             return t if isinstance(t, torch.Tensor) else t.rowmajor() if t.full is None else t.full
@@ -155,6 +166,32 @@ class LlamaAdapters:
     scales: torch.Tensor | None = None  # float32 [count]; None: 1
     in_8_bits: bool = False  # for a model of LlamaWeights.in_8_bits, whose gate and up rows do not alternate
 
+    def check(self, cfg: LlamaConfig, like: torch.Tensor) -> None:
+        """Raises unless dense.lora takes these adapters beside the projections of a
+        model of this shape and of `like`'s type and device."""
+        H, Hkv, D, hid, I = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.hidden_size, cfg.intermediate_size
+        shapes = {"qkv": (3, (H + 2 * Hkv) * D, hid), "o": (1, hid, H * D), "gate_up": (2, 2 * I, hid), "down": (1, hid, I)}
+
+        def need(t, name, shape, dtype):
+            if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+                raise TypeError(f"{name} of the adapters must be {dtype}")
+            if tuple(t.shape) != shape or not t.is_contiguous() or t.device != like.device:
+                raise ValueError(f"{name} of the adapters must be a contiguous {list(shape)} on {like.device}")
+
+        if self.scales is not None:
+            need(self.scales, "scales", (self.count,), torch.float32)
+        for i, layer in enumerate(self.layers):
+            for name, (parts, n, k) in shapes.items():
+                pair = getattr(layer, name)
+                if pair is None:
+                    continue
+                a, b = pair
+                rank = b.shape[-1]
+                need(a, f"layer {i}: a of {name}", (self.count, parts * rank, k), like.dtype)
+                need(b, f"layer {i}: b of {name}", (self.count, n, rank), like.dtype)
+                if dense.lora_workspace_bytes(1, self.count, k, rank, parts, like.dtype) == 0:
+                    raise ValueError(f"layer {i}: {self.count} adapters of rank {rank} for {name} ({parts} parts) are more than dense.lora takes")
+
     @staticmethod
     def random(cfg: LlamaConfig, count: int, rank: int, dtype=torch.bfloat16, device="cuda", seed: int = 0,
                in_8_bits: bool = False) -> "LlamaAdapters":
@@ -193,9 +230,18 @@ class HipModelRunner:
             self.rope = dense.rope_table(cfg.max_positions, cfg.head_dim, cfg.rope_theta, weights.embedding.device)
         if cfg.qk_norm and any(lw.q_norm is None or lw.k_norm is None for lw in weights.layers):
             raise ValueError("a model with qk_norm needs the layers' q_norm and k_norm")
-        self.in_8_bits = any(isinstance(lw.gate_up, dense.Fp8Weight) for lw in weights.layers)
+        # what a step would refuse is refused here: a step that fails half way has written to the cache
+        eight = [isinstance(t, dense.Fp8Weight) for lw in weights.layers for t in (lw.qkv, lw.gate_up, lw.down)]
+        self.in_8_bits = any(eight)
+        if self.in_8_bits:
+            if not all(eight):
+                raise ValueError("qkv, gate_up and down of every layer must be in 8 bits, or none")
+            for lw in weights.layers:
+                _check_8_bits(lw)
         if adapters is not None and (len(adapters.layers) != len(weights.layers) or adapters.in_8_bits != self.in_8_bits):
             raise ValueError("adapters must have the model's layers, and gate and up rows in its order (in_8_bits)")
+        if adapters is not None:
+            adapters.check(cfg, weights.embedding)
         self.adapters = adapters
 
     def drop_state(self, request_id: str) -> None:
