@@ -565,7 +565,7 @@ def lora_workspace_bytes(num_rows: int, num_adapters: int, k: int, rank: int, nu
 
 def lora(x, a, b, scales, plan: LoraPlan, y, parts=None, part_block: int = 0, workspace=None, stream=None):
     """y += scales[i] b[i] (a[i] x) row by row, i the row's adapter in `plan`
-    (zk_lora); rows without one stay as they are.  x [T, k] (rows may lie apart)
+    (zk_lora; of as many adapters); rows without one stay as they are.  x [T, k] (rows may lie apart)
     of the weights' type, or Fp8Rows beside bfloat16 weights; a [adapters, P * rank,
     k], b [adapters, n, rank], scales float32 [adapters] or None; y [T, n], in
     place (rows may lie apart: columns of a fused output).  parts: the columns of
@@ -587,6 +587,8 @@ def lora(x, a, b, scales, plan: LoraPlan, y, parts=None, part_block: int = 0, wo
         cols, total = _columns(tuple(parts))
         if p == 0 or total != n:
             raise ValueError(f"parts must add up to the {n} columns of y")
+    if plan.offsets.shape[0] != na + 1:  # (rows of an adapter that is not there would be left out without a word)
+        raise ValueError(f"the plan is of {plan.offsets.shape[0] - 1} adapters, the weights of {na}")
     if isinstance(x, Fp8Rows):
         xc, xs = _lib.FP8_E4M3, _rows2(rows, "x.data", t, k, _FP8, cur)
         sc = _need(x.scales, "x.scales", (t,), torch.float32, cur)
