@@ -108,3 +108,20 @@ def test_adapters_of_another_model():
     ad.scales = torch.ones(3, dtype=torch.float64)
     with pytest.raises(TypeError, match="scales"):
         _runner(cfg, w, ad)
+
+
+def test_adapters_are_named_by_whole_numbers():
+    """A step's rows take the adapter that its request names, and nothing near it."""
+    import numpy as np
+    cfg = _cfg()
+    runner = _runner(cfg, _weights(cfg, F32), _adapters(cfg))
+    out = SimpleNamespace(batch=[SimpleNamespace(request_id="a", num_tokens=2), SimpleNamespace(request_id="b", num_tokens=1)])
+    assert runner._adapter_rows(out, {"a": 1}) == [1, 1, -1]
+    assert runner._adapter_rows(out, {"a": np.int64(2), "b": torch.tensor(0)}) == [2, 2, 0]
+    assert runner._adapter_rows(out, {"b": None, "c": 7}) is None
+    for bad in (0.5, 1.0, "1", np.float32(1)):
+        with pytest.raises(TypeError):
+            runner._adapter_rows(out, {"a": bad})
+    for bad in (-1, 3):
+        with pytest.raises(ValueError):
+            runner._adapter_rows(out, {"a": bad})

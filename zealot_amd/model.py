@@ -44,6 +44,7 @@ rope_theta or qk_norm set, both run in the KV write's launch
 from __future__ import annotations
 
 import math
+import operator
 from dataclasses import dataclass, replace
 
 import torch
@@ -269,7 +270,8 @@ class HipModelRunner:
     def _adapter_rows(self, out, adapters: dict | None):
         """The adapter of every step row (-1: none), or None where no row has one."""
         ids = [e.request_id for e in out.batch] if adapters else []
-        mine = {rid: adapters[rid] for rid in ids if adapters.get(rid) is not None}
+        # (operator.index: a whole number, or TypeError)
+        mine = {rid: operator.index(adapters[rid]) for rid in ids if adapters.get(rid) is not None}
         if not mine:
             return None
         if self.adapters is None:
