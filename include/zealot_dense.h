@@ -235,8 +235,9 @@ int zk_linear_fp8(const void *x, const float *x_scales, const void *packed, cons
 int64_t zk_lora_max_tiles(int64_t num_rows, int64_t num_adapters);
 int zk_lora_plan(const int32_t *adapter_ids, int64_t num_rows, int64_t num_adapters, int32_t *order, int32_t *offsets,
                  int32_t *tiles, void *stream);
-/* y[t] += scales[a] b[a] (a_weights[a] x[t]) for the rows of a plan, a their
- * adapter; other rows of y are left as they are.  x [num_rows, k] (rows x_stride
+/* y[t] += scales[a] b[a] (a_weights[a] x[t]) for the rows of a plan (made for the
+ * same num_rows and num_adapters), a their adapter; other rows of y are left as
+ * they are.  x [num_rows, k] (rows x_stride
  * elements apart, 0 = k), a_weights [num_adapters, num_parts * rank, k], b
  * [num_adapters, n, rank], scales f32 [num_adapters] (NULL: 1), y [num_rows, n]
  * (rows y_stride apart, 0 = n), all of `dtype` (F32, BF16); beside BF16 x may be

@@ -13,7 +13,7 @@
 // (its projections are f32, src/attention/cublas.rs:72-114).
 //
 // Both are bound by HBM (32768 rows of 4096 with a residual 158 us, 6.0 TB/s; SiLU of
-// 8192 rows of 14336 100 us, 5.85 TB/s), a few rows by latency: a row is read once
+// 8192 rows of 14336 102 us, 5.8 TB/s), a few rows by latency: a row is read once
 // into registers, its sum of squares and its largest |t w| (which is the largest
 // |y| up to the factor of the row) go through one reduction, and it is written from
 // the registers.

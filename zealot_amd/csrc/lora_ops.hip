@@ -19,8 +19,10 @@
 // Columns of y may come in parts that have an A of their own each (query, key
 // and value columns of a fused projection): part p meets v[p rank ..] alone.
 //
-// Both launches read x, A, B and y once at most tile_rows rows a pass and are
-// bound by that traffic, and for a few rows by their latency.
+// Every tile reads all of its adapter's A and B, from L2 after the first, and x
+// once for every 64 ranks of all parts; y is read and written once.  A few rows are
+// bound by the launches' latency, prompts of ranks above 32 by A and B (8192 rows of 4096
+// columns: rank 32 53 us, 64 71, 128 112; the last asks L2 for 1 GB, x and y are 0.2).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -412,7 +414,9 @@ template <> struct Values<uint16_t> {
 // follow one another, and the waves of one, write the same rows side by side.  The
 // values of the parts that these columns meet are summed over the splits into LDS
 // first, then each wave works alone: a block of y is asked for before the product
-// that is added to it.  ONE: no block of 64 columns meets two parts.  What bounds it
+// that is added to it.  ONE: no block of 64 columns meets two parts; else each gets the
+// product of every part that it meets, and keeps its columns' (8192 x 28672 in two parts by
+// 16 columns in turn, rank 16, 362 us for both launches, in two halves 198).  What bounds it
 // is y's way there and back (8192 x 4096 of rank 32: 34 us, 3.9 TB/s; 28672 columns 4.6).
 template <typename T, int MT, bool WHOLE, bool ONE>
 __global__ void __launch_bounds__(256) lora_expand_kernel(LoraArgs a) {
