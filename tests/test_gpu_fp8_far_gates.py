@@ -1,10 +1,11 @@
 """dense.silu_mul_fp8 of gates whose exp(-g) is near the end of f32's range: from -87.3
 (there 1 / (1 + exp(-g)) is no normal number any more) to -88.7 the product is one, and
-silu_mul has it; a row of such gates must not become zeros.
+silu_mul has it; a row of such gates must not become zeros.  And gates near f32's smallest.
 
 Tolerance: g log2(e) is between 126 and 128: its constant is off by 2^-25 of
 itself and its rounding by half a step of 2^-17, 2^-18 each, times log(2); exp2, sum,
-reciprocal and three products 8 steps of 2^-24: below 2^-17.  A value lies between the
+reciprocal and products 8 steps of 2^-24, and the reciprocal's quarter half a step of
+2^-149, 2^-21 of itself at most (it is above 2^-129): below 2^-17.  A value lies between the
 roundings of y / s (1 -+ 2^-16), since both y and s move."""
 import pytest
 import torch
@@ -62,3 +63,15 @@ def test_gates_beyond():
     got = dense.silu_mul_fp8(g, u)
     assert (got.data[0].view(torch.uint8) == 0x80).all() and (dense.silu_mul(g, u)[0] == 0).all()
     _check(dense.Fp8Rows(got.data[1:], got.scales[1:]), g[1:].double())
+
+
+def test_gates_of_the_smallest_numbers():
+    """Even multiples of 2^-149: half of one is a number, and what comes of it with an up of 2^126."""
+    from zealot_amd import dense
+    g = (2.0 * torch.arange(1, 257, dtype=torch.float64) * 2.0 ** -149).float()[None]
+    u = torch.full_like(g, 2.0 ** 126)
+    y = g.double() / 2 * 2.0 ** 126
+    got = dense.silu_mul_fp8(g.cuda(), u.cuda())
+    s = (y.amax() / 448).float()
+    assert got.scales.item() == s.item()
+    assert torch.equal(got.data.view(torch.uint8).cpu(), (y / s.double()).float().to(FP8).view(torch.uint8))

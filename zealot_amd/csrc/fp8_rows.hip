@@ -92,16 +92,17 @@ __device__ __forceinline__ void store_q(uint8_t *p, const float (&v)[VEC]) {
         *reinterpret_cast<u32x2_any *>(p) = u32x2{four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7])};
     }
 }
-// g / (1 + exp(-g)) with the machine's exp2 and reciprocal, as (g / 4) / (1 / 4 + exp(-g) /
-// 4): the machine's reciprocal gives no numbers below 2^-126, exp(-g) may be up to 2^128.
-// 0 below -88.72, where exp(-g) is no f32.  The exponent -g log2(e) - 2 is off by 2^-25 of
+// g / (1 + exp(-g)) with the machine's exp2 and reciprocal, as g (1 / (1 / 4 + exp(-g) / 4)
+// / 4): the machine's reciprocal gives no numbers below 2^-126, exp(-g) may be up to 2^128.
+// (Below -87.3 the last quarter loses two bits; a quarter of g would lose them of gates
+// near 2^-149.)  0 below -88.72, where exp(-g) is no f32.  The exponent -g log2(e) - 2 is off by 2^-25 of
 // its first term at most (the constant's) and 2^-24 of the whole (its rounding): 2^-24 (2.2 |g| + 2),
 // and the value by log(2) of that where g is far below zero, by half and less of it above;
 // beside it exp2 and the reciprocal 2 steps of 2^-24 each, the sum and the product one: 6.
 // With expf and a division the instructions bind, not memory (8192 rows of 14336 129 us).
 __device__ __forceinline__ float silu(float g) {
     const float e = __builtin_amdgcn_exp2f(fmaf(g, -1.44269504088896341f, -2.0f));
-    return 0.25f * g * __builtin_amdgcn_rcpf(0.25f + e);
+    return g * (0.25f * __builtin_amdgcn_rcpf(0.25f + e));
 }
 
 // W waves a row, MAXV vectors a thread, R rows a workgroup (more than one where a

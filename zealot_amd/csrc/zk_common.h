@@ -308,7 +308,7 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 // y / s to nearest for finite y and finite normal s, r = 1 / s to nearest: the product y r
 // and one step on its exact remainder (Markstein, IBM J. Res. Dev. 34, 1990), which a
 // quotient that is representable meets exactly: y r alone is a step beside it for one in
-// three.  A zero keeps its sign.
+// four.  A zero keeps its sign.
 __device__ __forceinline__ float quotient(float y, float s, float r) {
     const float q = y * r;
     return fmaf(-fmaf(q, s, -y), r, q);
